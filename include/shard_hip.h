@@ -488,6 +488,111 @@ size_t shard_eigh_top_workspace(int32_t n);
 int shard_eigh_top(double* a, int32_t n, int32_t top, double* evals, double* evecs,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged KV cache held in 4 bits (no counterpart in the reference, whose cache
+ * is compressed once, after prompts of one length; this one takes tokens of a
+ * ragged batch as they come)
+ * ------------------------------------------------------------------------ */
+
+/* A page holds SHARD_KV4_PAGE tokens of every kv head, 68 * head_dim bytes a
+ * head, contiguous: E2M1 codes with an E5M2 scale for 32 channels of a token
+ * (the smallest scale >= amax / 6.5, from 2^-16 to 10240; codes to the
+ * nearest, ties to the even code, saturating; NaN is stored as 0), in the
+ * order that the header of csrc/kv4.hip lays down.
+ *
+ * A batch: sequence b's new tokens are rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 of q, k, v and the outputs (cu_seqlens null: row b
+ * alone), and the last ones of its seq_lens[b] tokens; its token t lives in
+ * page block_table[b * table_stride + t / 64], slot t % 64.  The three arrays
+ * are int32 in device memory and checked where they are used: rows are
+ * clamped to n_tokens, negative lengths to 0; tokens at positions before 0,
+ * past the table or (append) past the phases and tokens of pages outside
+ * 0 .. n_pages - 1 are left out: not stored, not attended to, read as zeros.
+ * Rows behind the last sequence's are neither read nor written.
+ *
+ * head_dim 64 or 128, any number of query heads per kv head; dtype of q, k, v
+ * and the outputs.  Strides are in elements, multiples of 8; rows of a head
+ * are contiguous; pointers 16-byte aligned; page_stride (bytes) a multiple of
+ * 16; q_out, k_out, v_out and out are contiguous (n_tokens, heads, head_dim).
+ * max_new and max_len (0: unknown) are the largest numbers of new tokens and
+ * of tokens of a sequence: they size launches, the results do not depend on
+ * them beyond the order of fp32 sums. */
+#define SHARD_KV4_PAGE 64
+#define SHARD_FP16 0
+#define SHARD_BF16 1
+#define SHARD_FP32 2
+
+typedef struct shard_kv4_args {
+  int32_t batch, n_tokens;          /* sequences; rows of q, k, v */
+  int32_t n_q_heads, n_kv_heads, head_dim;
+  int32_t dtype;                    /* SHARD_FP16 or SHARD_BF16 */
+  int32_t n_pages, table_width;
+  int32_t max_new, max_len;
+  uint8_t* cache;
+  int64_t page_stride;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;        /* (batch + 1) or null */
+  const void* q;
+  int64_t q_stride, q_head_stride;
+  const void* k;
+  int64_t k_stride, k_head_stride;
+  const void* v;
+  int64_t v_stride, v_head_stride;
+  const float* phases;              /* (n_phases, head_dim / 2, 2) cos, sin */
+  int32_t n_phases;
+  float scale;                      /* of the scores */
+  void* q_out;
+  void* k_out;
+  void* v_out;
+  void* out;
+} shard_kv4_args;
+
+size_t shard_kv4_args_size(void);
+/* Bytes of a page (0: unsupported). */
+int64_t shard_kv4_page_bytes(int32_t n_kv_heads, int32_t head_dim);
+
+/* New tokens into the cache: k rotated at its position by phases (x_i c -
+ * x_{i + D/2} s, x_{i + D/2} c + x_i s, in 64 bits) and v, rounded to 4 bits;
+ * with q, its rows rotated into q_out as well, rounded once.  One launch.
+ * A page that two sequences of the call append to is a race. */
+int shard_kv4_append(const shard_kv4_args* args, void* stream);
+
+/* K and V that the cache holds for the rows' tokens, exact in both types. */
+int shard_kv4_read(const shard_kv4_args* args, void* stream);
+
+/* Causal attention of the rows' tokens over their sequences: out =
+ * sum_t softmax_t(scale q . k_t) v_t over tokens t up to the row's own; rows
+ * that see none are zeros.  Scores, softmax statistics and sums in 32 bits,
+ * the weights of V in fp16.  Workspace: shard_kv4_attn_workspace(args) bytes,
+ * 16-byte aligned (0: none needed); nothing in it needs clearing. */
+size_t shard_kv4_attn_workspace(const shard_kv4_args* args);
+int shard_kv4_attn(const shard_kv4_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Log probabilities of a model's answers
+ * ------------------------------------------------------------------------ */
+
+/* For each row of logits (rows, vocab; row stride in elements; dtype
+ * SHARD_FP16, SHARD_BF16 or SHARD_FP32, aligned to its elements), in one pass
+ * over it, with lse = log sum_j exp(x_j):
+ *   logprob[r] = x[tokens[r]] - lse; 0 where tokens[r] < 0 (no token), NaN
+ *     where it is >= vocab; tokens may be null, then logprob is not written;
+ *   entropy[r] = lse - sum_j p_j x_j;
+ *   top_ids[r, i], top_logprobs[r, i] for i < top: the largest logits, equal
+ *     ones by index; NaN logits are not among them (-1 and NaN where a row has
+ *     fewer others).
+ * Sums in 32 bits.  A row without a logit above -inf, or with +inf or NaN,
+ * has NaN results.  top <= 64 and <= vocab.  Workspace:
+ * shard_token_logprobs_workspace bytes, 16-byte aligned (0: none needed);
+ * nothing in it needs clearing. */
+size_t shard_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top);
+int shard_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                         const int64_t* tokens, int32_t top, float* logprob, float* entropy,
+                         float* top_logprobs, int64_t* top_ids, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

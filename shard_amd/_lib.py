@@ -49,6 +49,22 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+class KV4Args(ctypes.Structure):
+    """Mirror of shard_kv4_args (include/shard_hip.h)."""
+    _fields_ = [
+        ("batch", c_int32), ("n_tokens", c_int32), ("n_q_heads", c_int32), ("n_kv_heads", c_int32),
+        ("head_dim", c_int32), ("dtype", c_int32), ("n_pages", c_int32), ("table_width", c_int32),
+        ("max_new", c_int32), ("max_len", c_int32),
+        ("cache", c_void_p), ("page_stride", c_int64), ("block_table", c_void_p), ("table_stride", c_int64),
+        ("seq_lens", c_void_p), ("cu_seqlens", c_void_p),
+        ("q", c_void_p), ("q_stride", c_int64), ("q_head_stride", c_int64),
+        ("k", c_void_p), ("k_stride", c_int64), ("k_head_stride", c_int64),
+        ("v", c_void_p), ("v_stride", c_int64), ("v_head_stride", c_int64),
+        ("phases", c_void_p), ("n_phases", c_int32), ("scale", c_float),
+        ("q_out", c_void_p), ("k_out", c_void_p), ("v_out", c_void_p), ("out", c_void_p),
+    ]
+
+
 # (name, restype, argtypes) of every exported symbol
 SIGNATURES = [
     ("shard_version", ctypes.c_char_p, []),
@@ -101,6 +117,14 @@ SIGNATURES = [
     ("shard_stream_quant_kv", c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32] + [c_void_p] * 10 + [c_void_p]),
     ("shard_rope_stream_append", c_int32, [c_void_p] * 5 + [c_int64] + [c_int32] * 4 + [c_void_p] * 3 + [c_int32] + [c_void_p] * 10 + [c_void_p]),
     ("shard_rope_stream_append_dev", c_int32, [c_void_p] * 5 + [c_int64] + [c_int32] * 4 + [c_void_p] * 3 + [c_int32] + [c_void_p] * 10 + [c_void_p, c_int32] + [c_void_p]),
+    ("shard_kv4_args_size", c_size_t, []),
+    ("shard_kv4_page_bytes", c_int64, [c_int32, c_int32]),
+    ("shard_kv4_append", c_int32, [ctypes.POINTER(KV4Args), c_void_p]),
+    ("shard_kv4_read", c_int32, [ctypes.POINTER(KV4Args), c_void_p]),
+    ("shard_kv4_attn_workspace", c_size_t, [ctypes.POINTER(KV4Args)]),
+    ("shard_kv4_attn", c_int32, [ctypes.POINTER(KV4Args), c_void_p, c_size_t, c_void_p]),
+    ("shard_token_logprobs_workspace", c_size_t, [c_int64, c_int64, c_int32]),
+    ("shard_token_logprobs", c_int32, [c_void_p, c_int32] + [c_int64] * 3 + [c_void_p, c_int32] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     ("shard_stream_dequant_qjl", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
 ]
 
@@ -129,6 +153,8 @@ def load():
         fn.argtypes = args
     if lib.shard_decode_args_size() != ctypes.sizeof(DecodeArgs):
         raise ShardHipUnavailable("shard_decode_args layout mismatch between header and binding")
+    if lib.shard_kv4_args_size() != ctypes.sizeof(KV4Args):
+        raise ShardHipUnavailable("shard_kv4_args layout mismatch between header and binding")
     _lib = lib
     return lib
 

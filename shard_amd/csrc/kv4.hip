@@ -1,0 +1,847 @@
+// Paged KV cache held in 4 bits: append (with RoPE), read back, attention.
+//
+// Format.  A page holds 64 tokens of every kv head, 68 * D bytes a head
+// (D = head_dim 64 or 128): an element is an E2M1 code, 32 channels of a token
+// share an E5M2 scale (its byte is the upper half of the fp16 number of the
+// same value).  value = e2m1(code) * scale has at most 5 significant bits and
+// a magnitude in {0} or 2^-17 .. 61440, so it is exact in fp16: the attention
+// multiplies fp16 operands and rounds nothing of the cache.
+// scale = the smallest E5M2 number >= amax / 6.5 (6.5 rather than 6: magnitudes
+// in (6, 6.5] scales saturate by at most half a scale, and the finer scale
+// pays elsewhere: relative rms error of Gaussian blocks 10.4% against 11.2%),
+// from 2^-16 to 10240.  Codes round to the nearest, ties to the even code;
+// magnitudes above 6 scales and infinities saturate, NaN is stored as 0.
+//
+// Within a page a head's bytes are laid out as the attention's MFMA operands
+// (16x16x32, fp16) take them, so that a wave reads them as contiguous 16-byte
+// lanes and nothing is transposed on the way:
+//   K codes   [0, 32 D): lane (kq, r) of token group sub = t / 16, r = t % 16,
+//             holds the D / 4 channels kq * D/4 .. of its token: 16 (D = 128) or
+//             8 bytes (D = 64, two token groups side by side), even channel low.
+//   K scales  [32 D, 34 D): [block][r][sub].
+//   V codes   [34 D, 66 D): a 32-bit word holds one channel of 8 tokens, the
+//             two runs of four that a lane's score registers hold: token
+//             32 s + 16 (e / 4) + 4 kq + e % 4 in nibble e; words
+//             [s][n / 4][kq][channel % 16][n % 4], n = channel / 16.
+//   V scales  [66 D, 68 D): [kq][s][block][e].
+//
+// Batch: sequence b's new tokens are rows cu[b] .. cu[b + 1] - 1 (or row b
+// alone) and the last of its seq_lens[b] tokens; token t of it lives in page
+// block_table[b][t / 64], slot t % 64.  Everything read from device memory is
+// checked where it is used: rows and lengths are clamped, positions outside
+// the table or the phases and page numbers outside the cache are left out.
+#include <stdio.h>
+
+#include "common.h"
+
+namespace shard {
+namespace {
+
+constexpr int kPage = 64;
+
+typedef __bf16 bf16_t;
+
+struct Seq {
+  int row0, n;      // its rows of q, k, v
+  int len;          // tokens, as given
+  int cap;          // tokens its block table can hold
+};
+
+__device__ __forceinline__ Seq seq_of(const shard_kv4_args& a, int b) {
+  Seq s;
+  int c0 = b, c1 = b + 1;
+  if (a.cu_seqlens) {
+    c0 = a.cu_seqlens[b];
+    c1 = a.cu_seqlens[b + 1];
+  }
+  c0 = min(max(c0, 0), a.n_tokens);
+  c1 = min(max(c1, c0), a.n_tokens);
+  s.row0 = c0;
+  s.n = c1 - c0;
+  s.len = max(a.seq_lens[b], 0);
+  s.cap = a.table_width * kPage;
+  return s;
+}
+
+// The page that holds token t of sequence b (t < cap), -1 if the table names none.
+__device__ __forceinline__ int page_of(const shard_kv4_args& a, int b, int t) {
+  const int p = a.block_table[(int64_t)b * a.table_stride + (t >> 6)];
+  return (unsigned)p < (unsigned)a.n_pages ? p : -1;
+}
+
+template <int D>
+__device__ __forceinline__ uint8_t* head_of(const shard_kv4_args& a, int page, int g) {
+  return a.cache + (int64_t)page * a.page_stride + (int64_t)g * (68 * D);
+}
+
+// Byte offsets within a head's part of a page.
+template <int D>
+__device__ __forceinline__ int k_code_at(int slot, int kq) {  // of D / 8 bytes
+  const int sub = slot >> 4, r = slot & 15;
+  return D == 128 ? (sub * 64 + kq * 16 + r) * 16 : ((sub >> 1) * 64 + kq * 16 + r) * 16 + (sub & 1) * 8;
+}
+template <int D>
+__device__ __forceinline__ int k_scale_at(int slot, int blk) {
+  return 32 * D + (blk * 16 + (slot & 15)) * 4 + (slot >> 4);
+}
+template <int D>
+__device__ __forceinline__ int v_word_at(int s, int kq, int ch) {  // of 4 bytes
+  const int n = ch >> 4;
+  return 34 * D + (((s * (D / 64) + (n >> 2)) * 64 + kq * 16 + (ch & 15)) * 4 + (n & 3)) * 4;
+}
+template <int D>
+__device__ __forceinline__ int v_scale_at(int slot, int blk) {
+  const int s = slot >> 5, u = slot & 31, e = ((u >> 4) << 2) | (u & 3), kq = (u >> 2) & 3;
+  return 66 * D + ((kq * 2 + s) * (D / 32) + blk) * 8 + e;
+}
+
+__device__ __forceinline__ float e5m2(unsigned byte) { return h2f((uint16_t)(byte << 8)); }
+
+// The scale byte of a block whose largest magnitude is `amax` (not NaN).
+__device__ __forceinline__ unsigned scale_byte(float amax) {
+  const unsigned c = f2h(amax * (1.0f / 6.5f)) >> 8;  // within one of the answer, from below
+  unsigned b = c > 1u ? min(c, 113u) : 1u;
+  b += 6.5f * e5m2(b) < amax ? 1u : 0u;               // 6.5 scale is exact: 7 significant bits
+  b += 6.5f * e5m2(b) < amax ? 1u : 0u;
+  return min(b, 113u);
+}
+
+// E2M1 code of x at scale s: nearest, ties to the even code.  s times a border
+// has at most 6 significant bits, so every comparison is exact.
+__device__ __forceinline__ unsigned code4(float x, float s) {
+  const float a = fabsf(x);
+  const unsigned b2 = a >= 1.75f * s;
+  const unsigned b1 = a >= (b2 ? 3.5f : 0.75f) * s;
+  const float t = b2 ? (b1 ? 5.0f : 2.5f) : (b1 ? 1.25f : 0.25f);
+  const unsigned b0 = a > t * s;
+  return (x < 0.f ? 8u : 0u) | b2 << 2 | b1 << 1 | b0;
+}
+
+// d in 32 bits, rounded to odd where it does not fit: compares with every
+// number of fewer bits as d does.
+__device__ __forceinline__ float to_odd(double d) {
+  const float f = (float)d;
+  uint32_t u = __float_as_uint(f);
+  const double back = (double)f;
+  if (back != d) {
+    if (fabs(back) > fabs(d)) u -= 1u;
+    u |= 1u;
+  }
+  return __uint_as_float(u);
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, dpp_mov<kDppXor1>(v));
+  return fmaxf(v, dpp_mov<kDppXor2>(v));
+}
+
+// 8 elements of a row at p (16-byte aligned) as floats.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  const vec8 v = *(const vec8*)p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  vec8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (T)x[i];
+  *(vec8*)p = v;
+}
+
+// --------------------------------------------------------------------------
+// Append: rotation of q and k, 4-bit rounding of k and v, scatter into pages.
+//
+// A workgroup owns 32 aligned tokens of a sequence for one kv head (blockIdx.y
+// < G): no other workgroup writes a word of its V codes, so words shared with
+// earlier tokens are read, merged and written without atomics.  Further y
+// rotate kHeadsQ query heads for the same tokens.
+// k is rotated in 64 bits, (c, s) being fp32 inputs: codes next to a border
+// come out as the formula's.  The products are exact there and the sum rounds
+// once, so nothing depends on contraction.
+// --------------------------------------------------------------------------
+constexpr int kHeadsQ = 4;
+
+template <class T, int D>
+__global__ __launch_bounds__(256)
+void k_kv4_append(const shard_kv4_args a) {
+  constexpr int PB = D / 64;  // pairs of 32-channel blocks: (pb, pb + PB)
+  __shared__ uint8_t codes[32][D + 4];
+  const int tid = threadIdx.x, b = blockIdx.z;
+  const Seq s = seq_of(a, b);
+  if (s.n == 0) return;
+  const int start = s.len - s.n;                    // position of the first new token
+  const bool is_q = blockIdx.y >= (unsigned)a.n_kv_heads;
+  const int g0 = (is_q ? start : max(start, 0)) >> 5, g1 = (s.len - 1) >> 5;
+  const int lq = tid & 3, pb = PB == 2 ? (tid >> 2) & 1 : 0;
+  const int tok = PB == 2 ? tid >> 3 : tid >> 2;    // of the 32 (D = 64: threads 0..127)
+  const int ch = pb * 32 + lq * 8;
+  for (int grp = g0 + blockIdx.x; grp <= g1; grp += gridDim.x) {
+    const int t0 = grp * 32;
+    const int pos = t0 + tok, i = pos - start;
+    const bool mine = tok < 32 && i >= 0 && i < s.n;
+    const bool there = mine && pos >= 0 && pos < s.cap && pos < a.n_phases;
+    float c[8], sn[8];
+    if (there) {
+      const float4* ph = (const float4*)(a.phases + ((int64_t)pos * (D / 2) + ch) * 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 f = ph[j];
+        c[2 * j] = f.x; sn[2 * j] = f.y; c[2 * j + 1] = f.z; sn[2 * j + 1] = f.w;
+      }
+    }
+    if (is_q) {                                     // query heads; zeros where a token has no place
+      if (!mine) continue;
+      const int h0 = (blockIdx.y - a.n_kv_heads) * kHeadsQ, h1 = min(h0 + kHeadsQ, a.n_q_heads);
+      for (int h = h0; h < h1; ++h) {
+        float lo[8] = {}, hi[8] = {};
+        if (there) {
+          const T* q = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)h * a.q_head_stride + ch;
+          float x[8], y[8];
+          load8(q, x);
+          load8(q + D / 2, y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            lo[j] = x[j] * c[j] - y[j] * sn[j];
+            hi[j] = y[j] * c[j] + x[j] * sn[j];
+          }
+        }
+        T* o = (T*)a.q_out + ((int64_t)(s.row0 + i) * a.n_q_heads + h) * D + ch;
+        store8(o, lo);
+        store8(o + D / 2, hi);
+      }
+      continue;
+    }
+    if (t0 >= s.cap) return;                        // cap is a multiple of 32
+    const int g = blockIdx.y;
+    const int page = page_of(a, b, t0);
+    if (page < 0) continue;
+    uint8_t* base = head_of<D>(a, page, g);
+    const int slot = (t0 & 63) + tok;
+    if (there) {
+      const T* k = (const T*)a.k + (int64_t)(s.row0 + i) * a.k_stride + (int64_t)g * a.k_head_stride + ch;
+      float x[8], y[8], r[2][8];
+      load8(k, x);
+      load8(k + D / 2, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double dl = (double)x[j] * c[j] - (double)y[j] * sn[j];
+        const double dh = (double)y[j] * c[j] + (double)x[j] * sn[j];
+        r[0][j] = dl == dl ? to_odd(dl) : 0.f;
+        r[1][j] = dh == dh ? to_odd(dh) : 0.f;
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(r[half][j]));
+        const unsigned sb = scale_byte(quad_max(m));
+        const float sc = e5m2(sb);
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w |= code4(r[half][j], sc) << (4 * j);
+        const int cc = half * (D / 2) + ch;
+        *(uint32_t*)(base + k_code_at<D>(slot, cc / (D / 4)) + (cc % (D / 4)) / 2) = w;
+        if (lq == 0) base[k_scale_at<D>(slot, cc / 32)] = (uint8_t)sb;
+      }
+    }
+    // V: codes into LDS by token, words of 8 tokens out
+    for (int u = tid; u < 32 * (D / 8); u += 256) {  // quads of lanes share a block of 32 channels
+      const int vt = u / (D / 8), vc = (u % (D / 8)) * 8;
+      const int vi = t0 + vt - start;
+      if (vi >= 0 && vi < s.n && t0 + vt < a.n_phases) {
+        const T* v = (const T*)a.v + (int64_t)(s.row0 + vi) * a.v_stride + (int64_t)g * a.v_head_stride + vc;
+        float x[8], m = 0.f;
+        load8(v, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = x[j] == x[j] ? x[j] : 0.f;
+          m = fmaxf(m, fabsf(x[j]));
+        }
+        const unsigned sb = scale_byte(quad_max(m));
+        const float sc = e5m2(sb);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) codes[vt][vc + j] = (uint8_t)code4(x[j], sc);
+        if ((vc & 31) == 0) base[v_scale_at<D>((t0 & 63) + vt, vc / 32)] = (uint8_t)sb;
+      }
+    }
+    __syncthreads();
+    for (int u = tid; u < 4 * D; u += 256) {
+      const int kq = u / D, vc = u % D;
+      uint32_t w = 0, keep = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int vt = 16 * (e >> 2) + 4 * kq + (e & 3), vi = t0 + vt - start;
+        if (vi >= 0 && vi < s.n && t0 + vt < a.n_phases) w |= (uint32_t)codes[vt][vc] << (4 * e);
+        else keep |= 15u << (4 * e);
+      }
+      uint32_t* at = (uint32_t*)(base + v_word_at<D>((t0 & 63) >> 5, kq, vc));
+      if (keep == 0) *at = w;
+      else if (keep != ~0u) *at = (*at & keep) | w;
+    }
+    __syncthreads();
+  }
+}
+
+// --------------------------------------------------------------------------
+// Read: the K and V that the cache holds for the new tokens' positions.
+// --------------------------------------------------------------------------
+__device__ __forceinline__ half2v fp4_pair(uint32_t w, int byte) {
+  switch (byte) {
+    case 0: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0);
+    case 1: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1);
+    case 2: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2);
+    default: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3);
+  }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256)
+void k_kv4_read(const shard_kv4_args a) {
+  __shared__ half_t rows[32][D + 2];
+  const int tid = threadIdx.x, b = blockIdx.z, g = blockIdx.y;
+  const Seq s = seq_of(a, b);
+  if (s.n == 0) return;
+  // rows that no token of the cache stands for (positions before 0 or past the table) are zero
+  const int start = s.len - s.n;
+  const int g0 = start >> 5, g1 = (s.len - 1) >> 5;  // floor, also below 0
+  for (int grp = g0 + blockIdx.x; grp <= g1; grp += gridDim.x) {
+    const int t0 = grp * 32;
+    const int page = t0 >= 0 && t0 < s.cap ? page_of(a, b, t0) : -1;
+    const uint8_t* base = page >= 0 ? head_of<D>(a, page, g) : nullptr;
+    for (int u = tid; u < 32 * (D / 8); u += 256) {
+      const int t = u / (D / 8), ch = (u % (D / 8)) * 8, i = t0 + t - start;
+      if (i < 0 || i >= s.n) continue;
+      float x[8] = {};
+      if (base) {
+        const int slot = (t0 & 63) + t;
+        const uint32_t w = *(const uint32_t*)(base + k_code_at<D>(slot, ch / (D / 4)) + (ch % (D / 4)) / 2);
+        const float sc = e5m2(base[k_scale_at<D>(slot, ch / 32)]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const half2v p = fp4_pair(w, j);
+          x[2 * j] = (float)p[0] * sc;
+          x[2 * j + 1] = (float)p[1] * sc;
+        }
+      }
+      store8((T*)a.k_out + ((int64_t)(s.row0 + i) * a.n_kv_heads + g) * D + ch, x);
+    }
+    __syncthreads();
+    if (base) {
+      for (int u = tid; u < 4 * D; u += 256) {
+        const int kq = u / D, vc = u % D;
+        const uint32_t w = *(const uint32_t*)(base + v_word_at<D>((t0 & 63) >> 5, kq, vc));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const half2v p = fp4_pair(w, j);
+          const int vt = 16 * (j >> 1) + 4 * kq + 2 * (j & 1);
+          rows[vt][vc] = p[0];
+          rows[vt + 1][vc] = p[1];
+        }
+      }
+    }
+    __syncthreads();
+    for (int u = tid; u < 32 * (D / 8); u += 256) {
+      const int t = u / (D / 8), ch = (u % (D / 8)) * 8, i = t0 + t - start;
+      if (i < 0 || i >= s.n) continue;
+      float x[8] = {};
+      if (base) {
+        const float sc = e5m2(base[v_scale_at<D>((t0 & 63) + t, ch / 32)]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)rows[t][ch + j] * sc;
+      }
+      store8((T*)a.v_out + ((int64_t)(s.row0 + i) * a.n_kv_heads + g) * D + ch, x);
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
+// Attention.
+//
+// Rows of (sequence, kv head): r = i * group + h for new token i and query
+// head h of the group; row r sees the keys up to its own position.
+// Scores are taken transposed, S^T = K Q^T (16 tokens x 16 rows an MFMA), so
+// that a lane's score registers hold four tokens of ONE row, and after the
+// softmax they are the right operand of O^T = V^T P^T as they stand.
+// P is rounded to fp16 (2^-11 of each weight; the sums are fp32); the cache's
+// values are exact.  bf16 queries are scaled by a power of two a row (their
+// largest below 2) and are then exact in fp16 down to 2^-17 of that largest
+// (below it they lose bits, 2^-26 of the largest at most); the power goes back
+// in through the softmax scale.
+// --------------------------------------------------------------------------
+struct AttnWork {
+  float* m;      // [row][split], rows (token, query head)
+  float* l;
+  float* acc;    // [row][split][D]
+  int n_splits;
+  int row_tiles; // workgroups along a sequence's rows
+};
+
+// Tiles (pages) a split of a sequence of `tiles` takes: at least kMinTiles, one
+// for each wave of the workgroup.
+constexpr int kMinTiles = 4;
+__device__ __forceinline__ int tiles_per_split(int tiles, int n_splits) {
+  return max(kMinTiles, (tiles + n_splits - 1) / n_splits);
+}
+
+// A page's operands for one wave.
+template <int D>
+struct PageRegs {
+  uint4 k[D / 32], v[D / 32], vs[D / 32];
+  uint32_t ks;
+  __device__ __forceinline__ void load(const uint8_t* base, int lane) {
+    const uint4* pk = (const uint4*)base + lane;
+    const uint4* pv = (const uint4*)(base + 34 * D) + lane;
+    const uint4* ps = (const uint4*)(base + 66 * D + (lane >> 4) * (D / 2));
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) k[j] = pk[64 * j];
+    ks = *(const uint32_t*)(base + 32 * D + ((D == 128 ? lane : (lane >> 5) * 16 + (lane & 15)) * 4));
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) v[j] = pv[64 * j];
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) { vs[2 * j] = ps[2 * j]; vs[2 * j + 1] = ps[2 * j + 1]; }
+  }
+};
+
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+__device__ __forceinline__ half8 dequant(uint32_t w, half2v s01, half2v s23, half2v s45, half2v s67) {
+  const half2v a = fp4_pair(w, 0) * s01, b = fp4_pair(w, 1) * s23;
+  const half2v c = fp4_pair(w, 2) * s45, d = fp4_pair(w, 3) * s67;
+  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Scales of tokens (or of one token twice) from the bytes of w: fp16 pairs.
+__device__ __forceinline__ half2v scale_pair(uint32_t w, int lo, int hi) {
+  const uint32_t sel = 0x0c | (uint32_t)lo << 8 | 0x0c0000u | (uint32_t)hi << 24;
+  return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0u, w, sel));
+}
+
+__device__ __forceinline__ float across_quarters_max(float v) {
+  float a, b;
+  perm16_swap(v, a, b);
+  v = fmaxf(a, b);
+  perm32_swap(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float across_quarters_sum(float v) {
+  float a, b;
+  perm16_swap(v, a, b);
+  v = a + b;
+  perm32_swap(v, a, b);
+  return a + b;
+}
+
+// Few rows: a workgroup of 4 waves takes 16 NQ rows and a split of the pages;
+// every wave walks its own pages (registers only) and the four are joined in
+// LDS at the end.
+template <class T, int D, int NQ>
+__global__ __launch_bounds__(256)
+void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
+  constexpr int ST = D / 32;  // k-steps of a score, 32-channel blocks
+  constexpr int NT = D / 16;  // channel tiles of the output
+  __shared__ float sh_acc[4][16 * NQ][D + 4];
+  __shared__ float sh_m[4][16 * NQ], sh_l[4][16 * NQ];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, kq = lane >> 4;
+  const int g = blockIdx.y, b = blockIdx.z;
+  const int split = blockIdx.x % w.n_splits;
+  const Seq s = seq_of(a, b);
+  const int group = a.n_q_heads / a.n_kv_heads;
+  const int n_rows = s.n * group;
+  const int keys = min(s.len, s.cap);
+  const int tiles = (keys + kPage - 1) / kPage;
+  const int per = tiles_per_split(tiles, w.n_splits);
+  const int first = split * per, last = min(first + per, tiles);
+  // a split past the sequence's end has no part that the merge reads
+  if (w.n_splits > 1 && first >= tiles) return;
+  const float scale2 = a.scale * 1.4426950408889634f;
+
+  for (int rt = blockIdx.x / w.n_splits; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
+    half8 q[NQ][ST];
+    float sc[NQ], m[NQ], l[NQ];
+    int lim[NQ];                      // keys that the lane's row sees
+    float4v acc[NQ][NT];
+    int lim_min = keys, lim_max = 0;  // of the tile's rows (uniform)
+    {
+      const int r0 = rt * 16 * NQ, r1 = min(r0 + 16 * NQ, n_rows) - 1;
+      lim_min = min(max(s.len - s.n + r0 / group + 1, 0), keys);
+      lim_max = min(max(s.len - s.n + r1 / group + 1, 0), keys);
+    }
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      const int r = (rt * NQ + t) * 16 + col;
+      const bool live = r < n_rows;
+      const int i = live ? r / group : 0, h = live ? r - i * group : 0;
+      lim[t] = live ? min(max(s.len - s.n + i + 1, 0), keys) : 0;
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+      sc[t] = scale2;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[t][n] = float4v{0.f, 0.f, 0.f, 0.f};
+      const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
+      if constexpr (__is_same(T, half_t)) {
+#pragma unroll
+        for (int j = 0; j < ST; ++j) q[t][j] = live ? *(const half8*)(qp + 8 * j) : half8{};
+      } else {
+        float x[ST][8], mx = 0.f;
+#pragma unroll
+        for (int j = 0; j < ST; ++j) {
+          if (live) load8(qp + 8 * j, x[j]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (!live) x[j][e] = 0.f;
+            mx = fmaxf(mx, fabsf(x[j][e]));
+          }
+        }
+        mx = across_quarters_max(mx);
+        const int ex = mx > 0.f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
+#pragma unroll
+        for (int j = 0; j < ST; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[t][j][e] = (half_t)ldexpf(x[j][e], -ex);
+        sc[t] = ldexpf(scale2, ex);
+      }
+    }
+
+    for (int tile = first + wave; tile < last; tile += 4) {
+      if (tile * kPage >= lim_max) break;
+      const int page = page_of(a, b, tile * kPage);
+      if (page < 0) continue;         // keys of no page: not seen
+      PageRegs<D> pg;
+      pg.load(head_of<D>(a, page, g), lane);
+      const int left = lim_max - tile * kPage;
+      if (left < kPage) {
+        // tokens behind the last key: whatever their bytes are, their V is finite
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int run = 0; run < 2; ++run) {
+            const int t0 = 32 * s2 + 16 * run + 4 * kq;
+            const int live = min(max(left - t0, 0), 4);
+            const uint32_t msk = live == 4 ? ~0u : (1u << (8 * live)) - 1u;
+#pragma unroll
+            for (int bk = 0; bk < ST; ++bk) {
+              const int at = (s2 * ST + bk) * 2 + run;   // word of the lane's scales
+              uint32_t* p = (uint32_t*)&pg.vs[at >> 2] + (at & 3);
+              *p &= msk;
+            }
+          }
+      }
+      float4v S[NQ][4];
+#pragma unroll
+      for (int sub = 0; sub < 4; ++sub) {
+        const half2v ks = scale_pair(pg.ks, sub, sub);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) S[t][sub] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < ST; ++j) {
+          const uint32_t kw = D == 128 ? word(pg.k[sub], j) : word(pg.k[sub >> 1], (sub & 1) * 2 + j);
+          const half8 kk = dequant(kw, ks, ks, ks, ks);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) S[t][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[t][j], S[t][sub], 0, 0, 0);
+        }
+      }
+      half8 P[NQ][2];
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) {
+        const bool masked = (tile + 1) * kPage > lim_min;  // or a row of the tile has no tokens
+        float mx = -INFINITY;
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v = S[t][sub][i] * sc[t];
+            if (masked) v = tile * kPage + 16 * sub + 4 * kq + i < lim[t] ? v : -INFINITY;
+            S[t][sub][i] = v;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(m[t], across_quarters_max(mx));
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float alpha = exp2f(m[t] - base);
+        m[t] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = exp2f(S[t][sub][i] - base);
+            sum += p;
+            P[t][sub >> 1][(sub & 1) * 4 + i] = (half_t)p;
+          }
+        l[t] = l[t] * alpha + sum;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[t][n] *= alpha;
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int bk = 0; bk < ST; ++bk) {
+          const int at = (s2 * ST + bk) * 2;
+          const uint32_t w0 = word(pg.vs[at >> 2], at & 3), w1 = word(pg.vs[at >> 2], (at & 3) + 1);
+          const half2v s01 = scale_pair(w0, 0, 1), s23 = scale_pair(w0, 2, 3);
+          const half2v s45 = scale_pair(w1, 0, 1), s67 = scale_pair(w1, 2, 3);
+#pragma unroll
+          for (int n = 2 * bk; n < 2 * bk + 2; ++n) {
+            const half8 vv = dequant(word(pg.v[s2 * (D / 64) + (n >> 2)], n & 3), s01, s23, s45, s67);
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, P[t][s2], acc[t][n], 0, 0, 0);
+          }
+        }
+    }
+
+    // join the four waves
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      const float lt = across_quarters_sum(l[t]);
+      if (kq == 0) {
+        sh_m[wave][16 * t + col] = m[t];
+        sh_l[wave][16 * t + col] = lt;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) *(float4v*)&sh_acc[wave][16 * t + col][16 * n + 4 * kq] = acc[t][n];
+    }
+    __syncthreads();
+    for (int u = tid; u < 16 * NQ * (D / 8); u += 256) {
+      const int rr = u / (D / 8), ch = (u % (D / 8)) * 8;
+      const int r = rt * 16 * NQ + rr;
+      if (r >= n_rows) continue;
+      const int i = r / group, h = g * group + r % group;
+      const float M = fmaxf(fmaxf(sh_m[0][rr], sh_m[1][rr]), fmaxf(sh_m[2][rr], sh_m[3][rr]));
+      const float base = M == -INFINITY ? 0.f : M;
+      float x[8] = {}, lt = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float f = exp2f(sh_m[v][rr] - base);
+        lt += f * sh_l[v][rr];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += f * sh_acc[v][rr][ch + j];
+      }
+      const int64_t row = (int64_t)(s.row0 + i) * a.n_q_heads + h;
+      if (w.n_splits == 1) {
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;   // a row that sees no key: zeros
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= inv;
+        store8((T*)a.out + row * D + ch, x);
+      } else {
+        const int64_t part = row * w.n_splits + split;
+        float4v* o = (float4v*)(w.acc + part * D + ch);
+        o[0] = float4v{x[0], x[1], x[2], x[3]};
+        o[1] = float4v{x[4], x[5], x[6], x[7]};
+        if (ch == 0) {
+          w.m[part] = M;
+          w.l[part] = lt;
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: a wave a row, each lane D / 64 channels.
+template <class T, int D>
+__global__ __launch_bounds__(256)
+void k_kv4_merge(const shard_kv4_args a, const AttnWork w) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.y;
+  const Seq s = seq_of(a, b);
+  const int tiles = (min(s.len, s.cap) + kPage - 1) / kPage;
+  const int n = (tiles + tiles_per_split(tiles, w.n_splits) - 1) / tiles_per_split(tiles, w.n_splits);
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < (int64_t)s.n * a.n_q_heads; r += (int64_t)gridDim.x * 4) {
+    const int64_t row = (int64_t)s.row0 * a.n_q_heads + r;
+    const float* pm = w.m + row * w.n_splits;
+    const float* pl = w.l + row * w.n_splits;
+    const float* pa = w.acc + row * w.n_splits * D;
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 64) M = fmaxf(M, pm[i]);
+    M = wave64_reduce(M, OpMax());
+    const float base = M == -INFINITY ? 0.f : M;
+    float x[D / 64] = {}, lt = 0.f;
+    for (int i = 0; i < n; ++i) {
+      const float f = exp2f(pm[i] - base);
+      lt += f * pl[i];
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) x[j] += f * pa[(int64_t)i * D + lane * (D / 64) + j];
+    }
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    T* o = (T*)a.out + row * D + lane * (D / 64);
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) o[j] = (T)(x[j] * inv);
+  }
+}
+
+// --------------------------------------------------------------------------
+// host side
+// --------------------------------------------------------------------------
+int check_batch(const shard_kv4_args* a) {
+  if (!a || !a->cache || !a->block_table || !a->seq_lens) return SHARD_ERR_ARG;
+  if (a->batch <= 0 || a->n_tokens < 0 || a->n_kv_heads <= 0 || a->n_pages <= 0 || a->table_width <= 0)
+    return SHARD_ERR_ARG;
+  if (!a->cu_seqlens && a->n_tokens != a->batch) return SHARD_ERR_ARG;
+  if (a->head_dim != 64 && a->head_dim != 128) return SHARD_ERR_SHAPE;
+  if (a->dtype != SHARD_FP16 && a->dtype != SHARD_BF16) return SHARD_ERR_SHAPE;
+  // positions are int32 and the grid's y and z 16 bits
+  if (a->table_width > (INT32_MAX - 64) / kPage || a->batch > 65535 || a->n_kv_heads > 1024) return SHARD_ERR_SHAPE;
+  if (a->page_stride < (int64_t)a->n_kv_heads * 68 * a->head_dim || a->page_stride % 16 || a->table_stride < a->table_width)
+    return SHARD_ERR_ARG;
+  if ((uintptr_t)a->cache % 16) return SHARD_ERR_ARG;
+  return SHARD_OK;
+}
+
+bool rows_ok(const void* p, int64_t stride, int64_t head_stride) {
+  return p && (uintptr_t)p % 16 == 0 && stride >= 0 && head_stride >= 0 && stride % 8 == 0 && head_stride % 8 == 0;
+}
+
+int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens can touch
+  const int n = a->max_new > 0 ? a->max_new : a->n_tokens;
+  return n <= 1 ? 1 : (int)(((int64_t)n + 30) / 32 + 1);
+}
+
+// Row tiles and splits of an attention call.  Enough workgroups to fill 256
+// CUs four times over (a split takes 4 tiles at least), and at most 32 tiles
+// (2,048 tokens) a split, so that a batch of uneven lengths ends together.
+struct AttnPlan {
+  int nq, row_tiles, n_splits;
+};
+AttnPlan plan_of(const shard_kv4_args* a) {
+  AttnPlan p;
+  const int group = a->n_q_heads / a->n_kv_heads;
+  const int64_t n = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
+  const int64_t rows = (a->cu_seqlens ? n : 1) * group;
+  p.nq = rows <= 16 ? 1 : 2;
+  p.row_tiles = (int)((rows + 16 * p.nq - 1) / (16 * p.nq));
+  const int64_t cap = (int64_t)a->table_width * kPage;
+  const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
+  const int64_t tiles = (len + kPage - 1) / kPage;
+  const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
+  int64_t sp = (1024 + wg - 1) / wg;
+  const int64_t even = (tiles + 31) / 32;
+  if (rows <= 32 && even > sp) sp = even;
+  if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
+  if (sp > 128) sp = 128;
+  p.n_splits = sp < 1 ? 1 : (int)sp;
+  return p;
+}
+
+int check_attn(const shard_kv4_args* a) {
+  const int rc = check_batch(a);
+  if (rc) return rc;
+  if (a->n_q_heads <= 0 || a->n_q_heads % a->n_kv_heads) return SHARD_ERR_SHAPE;
+  return SHARD_OK;
+}
+
+}  // namespace
+}  // namespace shard
+
+using namespace shard;
+
+#define KV4_DISPATCH(KERNEL, grid, s, ...)                                                                      \
+  do {                                                                                                          \
+    if (a->dtype == SHARD_FP16) {                                                                               \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<half_t, 128>), grid, dim3(256), 0, s, __VA_ARGS__);    \
+      else hipLaunchKernelGGL((KERNEL<half_t, 64>), grid, dim3(256), 0, s, __VA_ARGS__);                        \
+    } else {                                                                                                    \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16_t, 128>), grid, dim3(256), 0, s, __VA_ARGS__);    \
+      else hipLaunchKernelGGL((KERNEL<bf16_t, 64>), grid, dim3(256), 0, s, __VA_ARGS__);                        \
+    }                                                                                                           \
+  } while (0)
+
+template <int NQ>
+static void launch_rows(const shard_kv4_args* a, const AttnWork& w, hipStream_t s) {
+  const dim3 grid((unsigned)(w.n_splits * w.row_tiles), a->n_kv_heads, a->batch);
+  if (a->dtype == SHARD_FP16) {
+    if (a->head_dim == 128) hipLaunchKernelGGL((k_kv4_attn_rows<half_t, 128, NQ>), grid, dim3(256), 0, s, *a, w);
+    else hipLaunchKernelGGL((k_kv4_attn_rows<half_t, 64, NQ>), grid, dim3(256), 0, s, *a, w);
+  } else {
+    if (a->head_dim == 128) hipLaunchKernelGGL((k_kv4_attn_rows<bf16_t, 128, NQ>), grid, dim3(256), 0, s, *a, w);
+    else hipLaunchKernelGGL((k_kv4_attn_rows<bf16_t, 64, NQ>), grid, dim3(256), 0, s, *a, w);
+  }
+}
+
+extern "C" {
+
+size_t shard_kv4_args_size(void) { return sizeof(shard_kv4_args); }
+
+int64_t shard_kv4_page_bytes(int32_t n_kv_heads, int32_t head_dim) {
+  if (n_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return (int64_t)n_kv_heads * 68 * head_dim;
+}
+
+int shard_kv4_append(const shard_kv4_args* a, void* stream) {
+  const int rc = check_batch(a);
+  if (rc) return rc;
+  if (!a->phases || (uintptr_t)a->phases % 16 || a->n_phases <= 0) return SHARD_ERR_ARG;
+  if (!rows_ok(a->k, a->k_stride, a->k_head_stride) || !rows_ok(a->v, a->v_stride, a->v_head_stride)) return SHARD_ERR_ARG;
+  int q_groups = 0;
+  if (a->q) {
+    if (!rows_ok(a->q, a->q_stride, a->q_head_stride) || !a->q_out || (uintptr_t)a->q_out % 16 || a->n_q_heads <= 0)
+      return SHARD_ERR_ARG;
+    q_groups = (a->n_q_heads + kHeadsQ - 1) / kHeadsQ;
+    if (a->n_kv_heads + q_groups > 65535) return SHARD_ERR_SHAPE;
+  }
+  if (a->n_tokens == 0) return SHARD_OK;
+  const dim3 grid(groups_of(a), a->n_kv_heads + q_groups, a->batch);
+  KV4_DISPATCH(k_kv4_append, grid, (hipStream_t)stream, *a);
+  SHARD_LAUNCH_CHECK("shard_kv4_append");
+  return SHARD_OK;
+}
+
+int shard_kv4_read(const shard_kv4_args* a, void* stream) {
+  const int rc = check_batch(a);
+  if (rc) return rc;
+  if (!a->k_out || !a->v_out || (uintptr_t)a->k_out % 16 || (uintptr_t)a->v_out % 16) return SHARD_ERR_ARG;
+  if (a->n_tokens == 0) return SHARD_OK;
+  const dim3 grid(groups_of(a), a->n_kv_heads, a->batch);
+  KV4_DISPATCH(k_kv4_read, grid, (hipStream_t)stream, *a);
+  SHARD_LAUNCH_CHECK("shard_kv4_read");
+  return SHARD_OK;
+}
+
+size_t shard_kv4_attn_workspace(const shard_kv4_args* a) {
+  if (check_attn(a) || a->n_tokens == 0) return 0;
+  const AttnPlan p = plan_of(a);
+  if (p.n_splits == 1) return 0;
+  return (size_t)a->n_tokens * a->n_q_heads * p.n_splits * (a->head_dim + 2) * sizeof(float);
+}
+
+int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_attn(a);
+  if (rc) return rc;
+  if (!rows_ok(a->q, a->q_stride, a->q_head_stride) || !a->out || (uintptr_t)a->out % 16) return SHARD_ERR_ARG;
+  if (a->n_tokens == 0) return SHARD_OK;
+  const AttnPlan p = plan_of(a);
+  const int64_t rows = (int64_t)a->n_tokens * a->n_q_heads;
+  AttnWork w{};
+  w.n_splits = p.n_splits;
+  w.row_tiles = p.row_tiles;
+  if ((int64_t)w.n_splits * w.row_tiles > INT32_MAX) return SHARD_ERR_SHAPE;
+  if (p.n_splits > 1) {
+    const size_t need = shard_kv4_attn_workspace(a);
+    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) {
+      char text[96];
+      snprintf(text, sizeof(text), "shard_kv4_attn needs %zu bytes of workspace, 16-byte aligned", need);
+      set_last_text(text);
+      return SHARD_ERR_WORKSPACE;
+    }
+    w.acc = (float*)workspace;
+    w.m = w.acc + rows * p.n_splits * a->head_dim;
+    w.l = w.m + rows * p.n_splits;
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  if (p.nq == 1) launch_rows<1>(a, w, s);
+  else launch_rows<2>(a, w, s);
+  SHARD_LAUNCH_CHECK("shard_kv4_attn");
+  if (p.n_splits > 1) {
+    const int64_t per_seq = (a->cu_seqlens ? (a->max_new > 0 ? a->max_new : a->n_tokens) : 1) * (int64_t)a->n_q_heads;
+    const int64_t blocks = (per_seq + 3) / 4;
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), a->batch);
+    KV4_DISPATCH(k_kv4_merge, grid, s, *a, w);
+    SHARD_LAUNCH_CHECK("shard_kv4_attn merge");
+  }
+  return SHARD_OK;
+}
+
+}  // extern "C"

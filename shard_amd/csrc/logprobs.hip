@@ -1,0 +1,370 @@
+// Log probabilities of given tokens, entropy and the most probable tokens of
+// each row of logits, in one pass over the row.
+//
+// A workgroup takes a part of a row.  Every thread keeps its own running
+// maximum M with l = sum 2^d and t = sum d 2^d, d = (x - M) log2 e, and the
+// place of its best element; then
+//   lse = M + ln l,  logprob = x - lse,  entropy = ln l - ln2 t / l
+// after the threads' (and the parts') sums are joined at a common maximum.
+// The difference x - M is taken first, so that its rounding is relative to
+// itself and a row of equal logits far from 0 loses nothing.
+//
+// Top k: the k-th largest of the threads' best elements bounds the row's k-th
+// largest from below, so only the threads whose best reaches it (k of 256,
+// mostly) look through their elements once more and put those that reach it
+// into a list in LDS; an element's rank there is the number of larger ones.
+// Elements are compared as (value, lower index first) in 64 bits, so no two
+// are equal.  Where more than the list holds reach the bound (many equal
+// logits), the list's own k-th largest is the next bound.
+#include <stdio.h>
+
+#include "common.h"
+
+namespace shard {
+namespace {
+
+typedef __bf16 bf16_t;
+typedef unsigned long long u64;
+
+constexpr int kMaxTop = 64;
+constexpr int kMaxParts = 64;
+constexpr int kList = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e38f;
+
+struct LogprobArgs {
+  const void* logits;
+  int64_t vocab, stride;
+  const int64_t* tokens;
+  int top, parts;
+  int64_t granules;    // 16-byte granules of a part
+  float* logprob;
+  float* entropy;
+  float* top_logprobs;
+  int64_t* top_ids;
+  u64* ws_keys;        // [row][part][top], descending, 0 = none
+  float4* ws_stats;    // [row][part]: M, l, t
+};
+
+// Larger for larger values, for equal ones larger for lower indices; 0 for NaN.
+__device__ __forceinline__ u64 key_of(float x, int64_t i) {
+  return x == x ? (u64)f2ord(x + 0.f) << 32 | (uint32_t)(~(uint32_t)i) : 0;  // -0 counts as 0
+}
+__device__ __forceinline__ float value_of(u64 key) { return ord2f((uint32_t)(key >> 32)); }
+__device__ __forceinline__ int64_t index_of(u64 key) { return (int64_t)(uint32_t)~(uint32_t)key; }
+
+// A row seen as 16-byte granules from the aligned address at or before it.
+template <class T>
+struct Row {
+  static constexpr int VEC = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  const T* p;
+  int64_t n;
+  int mis;       // elements of the first granule that lie before the row
+  int64_t count; // granules
+  __device__ Row(const T* row, int64_t vocab) : p(row), n(vocab) {
+    mis = (int)(((uintptr_t)row & 15) / sizeof(T));
+    count = (n + mis + VEC - 1) / VEC;
+  }
+  // Elements outside the row are -inf.  Returns the index of x[0].
+  __device__ __forceinline__ int64_t load(int64_t j, float (&x)[VEC]) const {
+    const int64_t e0 = j * VEC - mis;
+    if (e0 >= 0 && e0 + VEC <= n) {
+      const vec v = *(const vec*)(p + e0);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = (float)v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = e0 + i >= 0 && e0 + i < n ? (float)p[e0 + i] : -INFINITY;
+    }
+    return e0;
+  }
+};
+
+struct Stats {
+  float M, l, t;
+};
+// the sums at another maximum (no smaller than s.M)
+__device__ __forceinline__ void move_to(Stats& s, float M) {
+  const float d = fmaxf((s.M - M) * kLog2e, -1e4f);
+  const float f = exp2f(d);
+  s.t = f * (s.t + d * s.l);
+  s.l *= f;
+  s.M = M;
+}
+
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, const Stats& s, float token_logit,
+                                          int64_t token) {
+  const float ln = logf(s.l);
+  a.entropy[row] = ln - kLn2 * s.t / s.l;
+  if (a.tokens)
+    a.logprob[row] = token < 0 ? 0.f : token < a.vocab ? token_logit - s.M - ln : NAN;
+}
+
+template <class T>
+__global__ __launch_bounds__(256)
+void k_logprobs(const LogprobArgs a) {
+  constexpr int VEC = Row<T>::VEC;
+  __shared__ u64 best[256];
+  __shared__ u64 list[kList];
+  __shared__ float sh_M[4], sh_l[4], sh_t[4];
+  __shared__ u64 bound;
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
+  const int part = blockIdx.y;
+  const Row<T> r((const T*)a.logits + row * a.stride, a.vocab);
+  const int64_t g0 = part * a.granules, g1 = g0 + a.granules < r.count ? g0 + a.granules : r.count;
+
+  Stats s{kLowest, 0.f, 0.f};
+  float bv = -INFINITY;
+  int64_t bi = -1;
+  for (int64_t j = g0 + tid; j < g1; j += 256) {
+    float x[VEC];
+    const int64_t e0 = r.load(j, x);
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < VEC; ++i) m = fmaxf(m, x[i]);
+    if (m > bv || bi < 0) {
+#pragma unroll
+      for (int i = VEC - 1; i >= 0; --i)
+        if (x[i] == m && e0 + i >= 0 && e0 + i < a.vocab) {
+          bi = e0 + i;
+          bv = m;
+        }
+      if (m > s.M) move_to(s, m);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float d = (x[i] - s.M) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(d);
+      s.l += e;
+      s.t += e * fmaxf(d, -1e4f);
+    }
+  }
+
+  // the row's (part's) sums
+  float M = wave64_reduce(s.M, OpMax());
+  if (lane == 0) sh_M[wave] = M;
+  const u64 mine = bi >= 0 ? key_of(bv, bi) : 0;
+  best[tid] = mine;
+  if (tid == 0) bound = 1;
+  __syncthreads();
+  M = fmaxf(fmaxf(sh_M[0], sh_M[1]), fmaxf(sh_M[2], sh_M[3]));
+  move_to(s, M);
+  const float l = wave64_reduce(s.l, OpAdd()), t = wave64_reduce(s.t, OpAdd());
+  if (lane == 0) {
+    sh_l[wave] = l;
+    sh_t[wave] = t;
+  }
+  if (a.top && mine) {
+    int rank = 0;
+    for (int i = 0; i < 256; ++i) rank += best[i] > mine;
+    if (rank == a.top - 1) bound = mine;
+  }
+  __syncthreads();
+  const Stats all{M, (sh_l[0] + sh_l[1]) + (sh_l[2] + sh_l[3]), (sh_t[0] + sh_t[1]) + (sh_t[2] + sh_t[3])};
+  if (tid == 0) {
+    if (a.parts == 1) {
+      const int64_t tok = a.tokens ? a.tokens[row] : -1;
+      write_row(a, row, all, tok >= 0 && tok < a.vocab ? (float)r.p[tok] : 0.f, tok);
+    } else {
+      a.ws_stats[row * a.parts + part] = make_float4(all.M, all.l, all.t, 0.f);
+    }
+  }
+  if (a.top == 0) return;
+
+  int n;
+  for (;;) {
+    if (tid == 0) found = 0;
+    __syncthreads();
+    const u64 need = bound;
+    if (mine >= need) {
+      for (int64_t j = g0 + tid; j < g1; j += 256) {
+        float x[VEC];
+        const int64_t e0 = r.load(j, x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (e0 + i < 0 || e0 + i >= a.vocab) continue;
+          const u64 key = key_of(x[i], e0 + i);
+          if (key >= need) {
+            const int at = atomicAdd(&found, 1);
+            if (at < kList) list[at] = key;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    n = found;
+    if (n <= kList) break;
+    // more than fit: kList of them are in the list; its k-th largest is at
+    // least the present bound's successor, as kList > top
+    for (int u = tid; u < kList; u += 256) {
+      const u64 key = list[u];
+      int rank = 0;
+      for (int i = 0; i < kList; ++i) rank += list[i] > key;
+      if (rank == a.top - 1) bound = key;
+    }
+    __syncthreads();
+  }
+  // ranks of the list's elements; what a row does not have is 0
+  const float ln = logf(all.l);
+  for (int u = tid; u < n + a.top; u += 256) {
+    u64 key = 0;
+    int rank = u;  // u >= n: the empty places behind the n elements
+    if (u < n) {
+      key = list[u];
+      rank = 0;
+      for (int i = 0; i < n; ++i) rank += list[i] > key;
+    }
+    if (rank >= a.top) continue;
+    if (a.parts > 1) {
+      a.ws_keys[(row * a.parts + part) * a.top + rank] = key;
+    } else {
+      a.top_ids[row * a.top + rank] = key ? index_of(key) : -1;
+      a.top_logprobs[row * a.top + rank] = key ? value_of(key) - all.M - ln : NAN;
+    }
+  }
+}
+
+// Joins the parts of a row.  A part's keys are in descending order, so an
+// element's rank is found by one binary search in every other part's; elements
+// below some part's k-th cannot be among the k largest.
+template <class T>
+__global__ __launch_bounds__(256)
+void k_logprobs_join(const LogprobArgs a) {
+  extern __shared__ u64 keys[];  // parts * top
+  __shared__ float sh[3];
+  __shared__ u64 bound;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int k = a.top, n = a.parts * k;
+  for (int u = tid; u < n; u += 256) keys[u] = a.ws_keys[row * n + u];
+  if (tid < 64) {
+    float4 f = make_float4(kLowest, 0.f, 0.f, 0.f);
+    if (tid < a.parts) f = a.ws_stats[row * a.parts + tid];
+    Stats s{f.x, f.y, f.z};
+    const float M = wave64_reduce(s.M, OpMax());
+    move_to(s, M);
+    const Stats all{M, wave64_reduce(s.l, OpAdd()), wave64_reduce(s.t, OpAdd())};
+    if (tid == 0) {
+      const int64_t tok = a.tokens ? a.tokens[row] : -1;
+      const T* p = (const T*)a.logits + row * a.stride;
+      write_row(a, row, all, tok >= 0 && tok < a.vocab ? (float)p[tok] : 0.f, tok);
+      sh[0] = all.M;
+      sh[1] = all.l;
+      bound = 0;
+    }
+  }
+  if (k == 0) return;
+  __syncthreads();
+  if (tid < a.parts) atomicMax(&bound, keys[tid * k + k - 1]);
+  __syncthreads();
+  const u64 need = bound;
+  const float M = sh[0], ln = logf(sh[1]);
+  // places that no key takes: the k-th and later of a row with fewer
+  int have = 0;
+  if (need == 0) {
+    for (int u = 0; u < n; ++u) have += keys[u] != 0;
+    for (int i = have + tid; i < k; i += 256) {
+      a.top_ids[row * k + i] = -1;
+      a.top_logprobs[row * k + i] = NAN;
+    }
+  }
+  for (int u = tid; u < n; u += 256) {
+    const u64 key = keys[u];
+    if (key == 0 || key < need) continue;
+    int rank = 0;
+    for (int p = 0; p < a.parts && rank < k; ++p) {
+      int lo = 0, hi = k;  // elements of part p above key
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (keys[p * k + mid] > key) lo = mid + 1;
+        else hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < k) {
+      a.top_ids[row * k + rank] = index_of(key);
+      a.top_logprobs[row * k + rank] = value_of(key) - M - ln;
+    }
+  }
+}
+
+// Parts of a row: about 1,024 workgroups in all, a granule a thread at least.
+int parts_of(int64_t rows, int64_t vocab) {
+  const int64_t most = (vocab / 8 + 255) / 256;
+  int64_t p = 1024 / rows;
+  if (p > kMaxParts) p = kMaxParts;
+  if (p > most) p = most;
+  return p < 1 ? 1 : (int)p;
+}
+
+bool sizes_ok(int64_t rows, int64_t vocab, int32_t top) {
+  return rows > 0 && rows <= INT32_MAX && vocab > 0 && vocab <= INT32_MAX && top >= 0 && top <= kMaxTop && top <= vocab;
+}
+
+}  // namespace
+}  // namespace shard
+
+using namespace shard;
+
+template <class T>
+static void launch_logprobs(const LogprobArgs& a, int64_t rows, hipStream_t s) {
+  hipLaunchKernelGGL(k_logprobs<T>, dim3((unsigned)rows, a.parts), dim3(256), 0, s, a);
+  if (a.parts > 1)
+    hipLaunchKernelGGL(k_logprobs_join<T>, dim3((unsigned)rows), dim3(256), a.parts * a.top * sizeof(u64), s, a);
+}
+
+extern "C" {
+
+size_t shard_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top) {
+  if (!sizes_ok(rows, vocab, top)) return 0;
+  const int parts = parts_of(rows, vocab);
+  return parts == 1 ? 0 : (size_t)rows * parts * (sizeof(float4) + top * sizeof(u64));
+}
+
+int shard_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                         const int64_t* tokens, int32_t top, float* logprob, float* entropy, float* top_logprobs,
+                         int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+  if (rows == 0) return SHARD_OK;
+  if (!logits || !entropy || (tokens && !logprob) || (top > 0 && (!top_logprobs || !top_ids))) return SHARD_ERR_ARG;
+  if (rows < 0 || vocab <= 0 || top < 0 || row_stride < 0) return SHARD_ERR_ARG;
+  if (!sizes_ok(rows, vocab, top)) return SHARD_ERR_SHAPE;
+  if (dtype != SHARD_FP16 && dtype != SHARD_BF16 && dtype != SHARD_FP32) return SHARD_ERR_SHAPE;
+  if ((uintptr_t)logits % (dtype == SHARD_FP32 ? 4 : 2)) return SHARD_ERR_ARG;
+  LogprobArgs a{};
+  a.logits = logits;
+  a.vocab = vocab;
+  a.stride = row_stride;
+  a.tokens = tokens;
+  a.top = top;
+  a.parts = parts_of(rows, vocab);
+  const int vec = dtype == SHARD_FP32 ? 4 : 8;
+  const int64_t granules = (vocab + 2 * vec - 2) / vec;  // of the worst aligned row
+  a.granules = (granules + a.parts - 1) / a.parts;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.top_logprobs = top_logprobs;
+  a.top_ids = top_ids;
+  if (a.parts > 1) {
+    const size_t need = shard_token_logprobs_workspace(rows, vocab, top);
+    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) {
+      char text[96];
+      snprintf(text, sizeof(text), "shard_token_logprobs needs %zu bytes of workspace, 16-byte aligned", need);
+      set_last_text(text);
+      return SHARD_ERR_WORKSPACE;
+    }
+    a.ws_stats = (float4*)workspace;
+    a.ws_keys = (u64*)(a.ws_stats + rows * a.parts);
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype == SHARD_FP16) launch_logprobs<half_t>(a, rows, s);
+  else if (dtype == SHARD_BF16) launch_logprobs<bf16_t>(a, rows, s);
+  else launch_logprobs<float>(a, rows, s);
+  SHARD_LAUNCH_CHECK("shard_token_logprobs");
+  return SHARD_OK;
+}
+
+}  // extern "C"

@@ -938,3 +938,235 @@ def kv_rebuild(fmt, batch: int, stream_n: int = 0):
     _lib.check("shard_kv_rebuild", _lib.load().shard_kv_rebuild(
         ctypes.byref(a), _p(k_out), _p(v_out), _stream(k_out)))
     return k_out, v_out
+
+
+# ---------------------------------------------------------------------------
+# paged cache held in 4 bits
+# ---------------------------------------------------------------------------
+KV4_PAGE = 64  # SHARD_KV4_PAGE: tokens of a page
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _same_device(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the call runs on {dev}")
+
+
+def kv4_cache(n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Empty pages, (n_pages, n_kv_heads, 68 * head_dim) uint8: 64 tokens a page,
+    4.25 bits an element.  head_dim 64 or 128."""
+    if n_pages <= 0 or n_kv_heads <= 0 or head_dim not in (64, 128):
+        raise ValueError(f"kv4_cache: {n_pages} pages of {n_kv_heads} heads of {head_dim}: "
+                         "head_dim is 64 or 128, the counts positive")
+    return torch.zeros(n_pages, n_kv_heads, 68 * head_dim, dtype=torch.uint8, device=device)
+
+
+def _kv4_args(cache, block_table, seq_lens, n_tokens, cu_seqlens, max_new, max_len=None) -> _lib.KV4Args:
+    """The batch's part of a call's argument block, checked."""
+    _require_gpu(cache, block_table, seq_lens, cu_seqlens)
+    dev = cache.device
+    _same_device(dev, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens)
+    if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[2] not in (68 * 64, 68 * 128):
+        raise TypeError("cache: expected the (pages, kv heads, 68 * head_dim) uint8 of kv4_cache")
+    n_pages, G, width = cache.shape
+    if cache.stride(2) != 1 or (G > 1 and cache.stride(1) != width):
+        raise ValueError("cache: the bytes of a page must be contiguous")
+    page_stride = cache.stride(0) if n_pages > 1 else G * width
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise TypeError("block_table: expected (batch, pages a sequence) int32 with contiguous rows")
+    B, W = block_table.shape
+    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,) or not seq_lens.is_contiguous():
+        raise TypeError(f"seq_lens: expected ({B},) contiguous int32")
+    if cu_seqlens is None:
+        if n_tokens != B:
+            raise ValueError(f"{n_tokens} tokens for {B} sequences: more than one each needs cu_seqlens")
+    elif cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (B + 1,) or not cu_seqlens.is_contiguous():
+        raise TypeError(f"cu_seqlens: expected ({B + 1},) contiguous int32")
+    if page_stride < G * width or W == 0 or n_pages == 0 or G == 0:
+        raise ValueError("cache and block_table must hold pages, and pages must not overlap")
+    a = _lib.KV4Args()
+    a.batch, a.n_tokens, a.n_kv_heads, a.head_dim = B, n_tokens, G, width // 68
+    a.n_pages, a.table_width = n_pages, W
+    a.max_new, a.max_len = max_new or 0, max_len or 0
+    a.cache, a.page_stride = cache.data_ptr(), page_stride
+    a.block_table, a.table_stride = block_table.data_ptr(), block_table.stride(0) if B > 1 else W
+    a.seq_lens = seq_lens.data_ptr()
+    a.cu_seqlens = None if cu_seqlens is None else cu_seqlens.data_ptr()
+    return a
+
+
+def _kv4_rows(t, name, a, heads=None):
+    """A (tokens, heads, head_dim) operand as the kernels take it: rows of a
+    head contiguous, strides multiples of 8 and 16-byte aligned (copied where
+    it is not), with its strides."""
+    if t.dim() != 3 or t.shape[0] != a.n_tokens or t.shape[2] != a.head_dim or heads not in (None, t.shape[1]):
+        raise ValueError(f"{name}: expected ({a.n_tokens}, {heads or 'heads'}, {a.head_dim}), got {tuple(t.shape)}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s0 | s1) & 7 or t.data_ptr() & 15:
+        t = t.contiguous()
+        if t.data_ptr() & 15:  # contiguous at an odd place of its storage
+            t = t.clone()
+        s0, s1, s2 = t.stride()
+        if (s0 | s1) & 7:      # strides of dimensions of size 1
+            s0, s1 = t.shape[1] * a.head_dim, a.head_dim
+    return t, s0, s1
+
+
+def _half_type(t, name):
+    code = _DTYPES.get(t.dtype, 2)
+    if code == 2:
+        raise TypeError(f"{name}: expected float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _kv4_launch(fn, name, a, t, *more):
+    """fn on t's device and its current stream."""
+    if torch.cuda.current_device() == t.get_device():
+        _lib.check(name, fn(ctypes.byref(a), *more, _stream(t)))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.check(name, fn(ctypes.byref(a), *more, _stream(t)))
+
+
+def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=None, max_new=None):
+    """Write new tokens into a paged 4-bit cache, k rotated at its position.
+
+    k, v (T, G, D) fp16 or bf16, before RoPE; cache from kv4_cache; block_table
+    (B, W) int32, the pages of each sequence; seq_lens (B,) int32, its tokens
+    with the new ones; cu_seqlens (B + 1,) int32, where each sequence's rows
+    begin (None: one new token each); phases (P, D / 2, 2) fp32 from
+    rope_phases(0, P, inv_freq), P at least 64 W.  With q (T, H, D) its rotated
+    rows are returned.  max_new, the most new tokens of a sequence, sizes the
+    launch where the caller knows it.  Lengths and pages are read on the
+    device: tokens at positions outside the table or in pages outside the cache
+    are left out; rows behind the last sequence's are not read, and their
+    rotated q not written.  Two sequences of one call must not append to the
+    same page."""
+    _require_gpu(k, v, phases, q)
+    lib = _lib.load()
+    a = _kv4_args(cache, block_table, seq_lens, k.shape[0], cu_seqlens, max_new)
+    _same_device(cache.device, k=k, v=v, phases=phases, q=q)
+    a.dtype = _half_type(k, "k")
+    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise TypeError("q, k and v must have one type")
+    if (phases.dtype != torch.float32 or phases.dim() != 3 or tuple(phases.shape[1:]) != (a.head_dim // 2, 2)
+            or not phases.is_contiguous() or phases.data_ptr() & 15):
+        raise TypeError(f"phases: expected (positions, {a.head_dim // 2}, 2) contiguous float32, 16-byte aligned")
+    if phases.shape[0] < KV4_PAGE * a.table_width:
+        raise ValueError(f"phases cover {phases.shape[0]} positions, the block table {KV4_PAGE * a.table_width}")
+    k, a.k_stride, a.k_head_stride = _kv4_rows(k, "k", a, a.n_kv_heads)
+    v, a.v_stride, a.v_head_stride = _kv4_rows(v, "v", a, a.n_kv_heads)
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.phases, a.n_phases = phases.data_ptr(), phases.shape[0]
+    q_out = None
+    if q is not None:
+        q, a.q_stride, a.q_head_stride = _kv4_rows(q, "q", a)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        a.n_q_heads = q.shape[1]
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if a.n_tokens:
+        _kv4_launch(lib.shard_kv4_append, "shard_kv4_append", a, cache)
+    return q_out
+
+
+def kv4_read(cache, block_table, seq_lens, n_tokens, dtype=torch.float16, cu_seqlens=None, max_new=None):
+    """K and V, (n_tokens, G, D) each, that the cache holds for the last tokens
+    of every sequence (rows as in kv4_append; seq_lens' cumulative sum as
+    cu_seqlens reads whole sequences).  Exact in fp16; bf16 is exact too.  Rows
+    of tokens that the table or the cache does not hold are zeros; rows behind
+    the last sequence's are not written."""
+    lib = _lib.load()
+    a = _kv4_args(cache, block_table, seq_lens, int(n_tokens), cu_seqlens, max_new)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"dtype: expected float16 or bfloat16, got {dtype}")
+    a.dtype = _DTYPES[dtype]
+    k = torch.empty(a.n_tokens, a.n_kv_heads, a.head_dim, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
+    if a.n_tokens:
+        _kv4_launch(lib.shard_kv4_read, "shard_kv4_read", a, cache)
+    return k, v
+
+
+def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=None, max_new=None, max_len=None):
+    """Causal attention of new tokens over their sequences in a paged 4-bit cache.
+
+    q (T, H, D) fp16 or bf16, rotated (kv4_append's), H a multiple of the
+    cache's kv heads; rows, block_table, seq_lens and cu_seqlens as in
+    kv4_append: new token i of a sequence of n tokens, m of them new, sees its
+    first n - m + i + 1.  scale: 1 / sqrt(D) where None.  Returns out (T, H, D),
+    the given contiguous one or a new one: rows that see no token are zeros,
+    rows behind the last sequence's are not written.  max_new and max_len, the
+    most new tokens and tokens of a sequence, size the launch where the caller
+    knows them (a captured graph must be given what its replays reach)."""
+    _require_gpu(q)
+    lib = _lib.load()
+    a = _kv4_args(cache, block_table, seq_lens, q.shape[0], cu_seqlens, max_new, max_len)
+    _same_device(cache.device, q=q, out=out)
+    a.dtype = _half_type(q, "q")
+    q, a.q_stride, a.q_head_stride = _kv4_rows(q, "q", a)
+    a.n_q_heads = H = q.shape[1]
+    if H == 0 or H % a.n_kv_heads:
+        raise ValueError(f"{H} query heads do not divide among {a.n_kv_heads} kv heads")
+    a.q = q.data_ptr()
+    a.scale = a.head_dim ** -0.5 if scale is None else float(scale)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
+        raise TypeError(f"out: expected {tuple(q.shape)} contiguous {q.dtype}, 16-byte aligned")
+    a.out = out.data_ptr()
+    if a.n_tokens == 0:
+        return out
+    need = lib.shard_kv4_attn_workspace(ctypes.byref(a))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _kv4_launch(lib.shard_kv4_attn, "shard_kv4_attn", a, cache, None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# log probabilities
+# ---------------------------------------------------------------------------
+TOP_LOGPROBS_MAX = 64
+
+
+def token_logprobs(logits, tokens=None, top=0):
+    """Log probabilities of a model's answers: logits (..., V) fp16, bf16 or
+    fp32, rows contiguous; tokens (...) int64.  Returns (logprob (...), entropy
+    (...), top_logprobs (..., top), top_ids (..., top) int64), fp32: of the
+    given tokens (0 where a token is negative, none given; NaN where it is not
+    below V; None without tokens), of the rows' distributions, and of their
+    most probable tokens, equal ones by index (top up to 64).  A row without a
+    logit above -inf, or with +inf or NaN, has NaN log probabilities; NaN
+    logits are never among the top (id -1 where a row has too few others)."""
+    _require_gpu(logits, tokens)
+    lib = _lib.load()
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"logits: expected float16, bfloat16 or float32, got {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError("logits: expected (..., vocabulary)")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if not 0 <= top <= min(TOP_LOGPROBS_MAX, V):
+        raise ValueError(f"top: 0 .. {min(TOP_LOGPROBS_MAX, V)}, got {top}")
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V > 1 or x.stride(0) < 0:
+        x = x.contiguous()
+    n, dev = x.shape[0], x.device
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.shape != lead:
+            raise TypeError(f"tokens: expected {tuple(lead)} int64, got {tuple(tokens.shape)} {tokens.dtype}")
+        _same_device(dev, tokens=tokens)
+        tokens = tokens.contiguous()
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
+    top_lp = torch.empty(*lead, top, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+    if n:
+        need = lib.shard_token_logprobs_workspace(n, V, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        with torch.cuda.device(dev):
+            _lib.check("shard_token_logprobs", lib.shard_token_logprobs(
+                x.data_ptr(), _DTYPES[x.dtype], n, V, x.stride(0), _p(tokens), top, _p(logprob), _p(entropy),
+                _p(top_lp), _p(top_ids), _p(ws), need, _stream(x)))
+    return logprob, entropy, top_lp, top_ids

@@ -1,0 +1,141 @@
+"""The paged 4-bit cache and the log probabilities on the CPU: the oracle
+against the formats' definitions, argument blocks, and every refusal of the C
+entry points (placeholder pointers: nothing is launched)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from oracle import kv4 as plain
+
+P = 4096  # a placeholder address, 16-byte aligned
+
+
+def test_formats():
+    assert plain.SCALES[0] == 2.0 ** -16 and plain.SCALES[-1] == 10240.0 and len(plain.SCALES) == 113
+    assert (np.diff(plain.SCALES) > 0).all()
+    # every value fits fp16
+    v = np.outer(plain.SCALES, plain.LEVELS)
+    assert (v.astype(np.float16).astype(np.float64) == v).all()
+
+
+def test_round4_ties_saturation_and_specials():
+    row = np.zeros(32)
+    row[:8] = [6.5, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]          # scale 1, every border
+    assert plain.round4(row)[:8].tolist() == [6, 0, 1, 1, 2, 2, 4, 4]
+    assert plain.round4(-row)[:8].tolist() == [-6, 0, -1, -1, -2, -2, -4, -4]
+    row[:] = 0
+    row[:3] = [np.nan, np.inf, 1e6]
+    assert plain.round4(row)[:3].tolist() == [0, 61440, 61440]
+    assert (plain.round4(np.full(32, 1e-9)) == 0).all()
+
+
+def _args(**kw):
+    from shard_amd import _lib
+    a = _lib.KV4Args()
+    base = dict(batch=2, n_tokens=2, n_q_heads=32, n_kv_heads=8, head_dim=128, dtype=0, n_pages=10, table_width=4,
+                cache=P, page_stride=8 * 68 * 128, block_table=P, table_stride=4, seq_lens=P,
+                q=P, q_stride=4096, q_head_stride=128, k=P, k_stride=1024, k_head_stride=128,
+                v=P, v_stride=1024, v_head_stride=128, phases=P, n_phases=256, scale=1.0,
+                q_out=P, k_out=P, v_out=P, out=P)
+    base.update(kw)
+    for name, value in base.items():
+        setattr(a, name, value)
+    return ctypes.byref(a)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(cache=None), -1), (dict(block_table=None), -1), (dict(seq_lens=None), -1), (dict(batch=0), -1),
+    (dict(n_tokens=-1), -1), (dict(n_tokens=3), -1), (dict(n_pages=0), -1), (dict(table_width=0), -1),
+    (dict(head_dim=96), -2), (dict(head_dim=256), -2), (dict(dtype=2), -2), (dict(dtype=-1), -2),
+    (dict(batch=70000, n_tokens=70000), -2), (dict(table_width=1 << 26, table_stride=1 << 26), -2),
+    (dict(page_stride=8 * 68 * 128 - 16), -1), (dict(page_stride=8 * 68 * 128 + 8), -1), (dict(table_stride=3), -1),
+    (dict(cache=P + 8), -1),
+], ids=str)
+def test_batch_refusals(kw, code):
+    from shard_amd import _lib
+    lib = _lib.load()
+    assert lib.shard_kv4_append(_args(**kw), None) == code
+    assert lib.shard_kv4_read(_args(**kw), None) == code
+    assert lib.shard_kv4_attn(_args(**kw), None, 0, None) == code
+    assert lib.shard_kv4_attn_workspace(_args(**kw)) == 0
+
+
+def test_operand_refusals():
+    from shard_amd import _lib
+    lib = _lib.load()
+    for fn in (lib.shard_kv4_append, lib.shard_kv4_read):
+        assert fn(None, None) == -1
+    assert lib.shard_kv4_attn(None, None, 0, None) == -1
+    for kw in (dict(k=None), dict(v=None), dict(k=P + 2), dict(k_stride=4), dict(v_head_stride=-8), dict(phases=None),
+               dict(phases=P + 8), dict(n_phases=0), dict(q_out=None), dict(q=P + 4), dict(n_q_heads=0), dict(q_out=P + 2)):
+        assert lib.shard_kv4_append(_args(**kw), None) == -1, kw
+    for kw in (dict(k_out=None), dict(v_out=None), dict(k_out=P + 8)):
+        assert lib.shard_kv4_read(_args(**kw), None) == -1, kw
+    for kw, code in ((dict(q=None), -1), (dict(out=None), -1), (dict(out=P + 8), -1), (dict(q_stride=3), -1),
+                     (dict(n_q_heads=12), -2), (dict(n_q_heads=0), -2)):
+        assert lib.shard_kv4_attn(_args(**kw), None, 0, None) == code, kw
+    # nothing to do is no error
+    assert lib.shard_kv4_append(_args(n_tokens=0, cu_seqlens=P), None) == 0
+    assert lib.shard_kv4_attn(_args(n_tokens=0, cu_seqlens=P), None, 0, None) == 0
+
+
+def test_workspace_is_checked_before_any_launch():
+    from shard_amd import _lib
+    lib = _lib.load()
+    a = _args(table_width=512, table_stride=512)
+    need = lib.shard_kv4_attn_workspace(a)
+    assert need > 0 and need % (130 * 4) == 0
+    assert lib.shard_kv4_attn(a, None, need, None) == -4
+    assert lib.shard_kv4_attn(a, P, need - 1, None) == -4
+    assert str(need).encode() in lib.shard_last_error()
+    assert lib.shard_kv4_attn(a, P + 4, need, None) == -4
+    assert lib.shard_kv4_attn_workspace(_args(max_len=64)) == 0   # one split
+
+
+def test_page_bytes():
+    from shard_amd import _lib
+    lib = _lib.load()
+    assert lib.shard_kv4_page_bytes(8, 128) == 8 * (64 * 128 + 64 * 8)   # 4 bits an element, a byte for 32
+    assert lib.shard_kv4_page_bytes(8, 64) == 8 * (64 * 64 + 64 * 4)
+    assert lib.shard_kv4_page_bytes(8, 96) == 0 and lib.shard_kv4_page_bytes(0, 128) == 0
+
+
+def test_cpu_tensors_are_refused():
+    import torch
+    from shard_amd import ops
+    c = ops.kv4_cache(2, 2, 64, device="cpu")
+    assert c.shape == (2, 2, 68 * 64)
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    k = torch.zeros(1, 2, 64, dtype=torch.float16)
+    with pytest.raises(ops.ShardHipUnavailable):
+        ops.kv4_append(k, k, c, t, n, torch.zeros(128, 32, 2))
+    with pytest.raises(ops.ShardHipUnavailable):
+        ops.kv4_read(c, t, n, 1)
+    with pytest.raises(ops.ShardHipUnavailable):
+        ops.kv4_attn(k, c, t, n)
+    with pytest.raises(ops.ShardHipUnavailable):
+        ops.token_logprobs(torch.zeros(2, 5))
+    for bad in ((0, 2, 64), (2, 0, 64), (2, 2, 96)):
+        with pytest.raises(ValueError):
+            ops.kv4_cache(*bad, device="cpu")
+
+
+def test_logprobs_refusals():
+    from shard_amd import _lib
+    lib = _lib.load()
+    call = lambda logits=P, dtype=0, rows=4, vocab=1000, stride=1000, tokens=P, top=5, lp=P, ent=P, tl=P, ti=P, ws=P, n=1 << 30: \
+        lib.shard_token_logprobs(logits, dtype, rows, vocab, stride, tokens, top, lp, ent, tl, ti, ws, n, None)
+    for kw in (dict(logits=None), dict(ent=None), dict(lp=None), dict(tl=None), dict(ti=None), dict(rows=-1), dict(vocab=0),
+               dict(top=-1), dict(stride=-1), dict(logits=P + 1), dict(dtype=2, logits=P + 2)):
+        assert call(**kw) == -1, kw
+    for kw in (dict(top=65), dict(top=5, vocab=4), dict(vocab=1 << 31), dict(dtype=3)):
+        assert call(**kw) == -2, kw
+    assert call(rows=0) == 0
+    need = lib.shard_token_logprobs_workspace(4, 128256, 5)
+    assert need > 0
+    big = dict(vocab=128256, stride=128256)
+    assert call(**big, ws=None) == -4 and call(**big, n=need - 1) == -4 and call(**big, ws=P + 8) == -4
+    assert str(need).encode() in lib.shard_last_error()
+    assert lib.shard_token_logprobs_workspace(4096, 128256, 5) == 0    # a workgroup a row
+    assert lib.shard_token_logprobs_workspace(4, 128256, 65) == 0
