@@ -641,6 +641,272 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   }
 }
 
+// Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and walks a
+// split of the pages.  A page is dequantized once for all of them into LDS
+// (fp16, two buffers: the next page is written while this one is multiplied,
+// and the one after it is on its way from memory), and read from there as
+// 32x32x16 operands.  Rows of 16-byte chunks, chunk ^ row: 8 lanes that read or
+// write one chunk of 8 rows use every bank once.
+// The maximum a row's weights refer to moves only where a score exceeds it by
+// 2^8 (weights stay below fp16's range by far): most pages rescale nothing.
+template <int D>
+struct TileRegs {  // a thread's part of a page
+  uint4 k, v, vs;
+  uint32_t ks;
+  __device__ __forceinline__ void load(const uint8_t* base, int tid) {
+    const int lane = tid & 63;
+    ks = base[k_scale_at<D>((tid >> 6) * 16 + (lane & 15), D == 128 ? lane >> 4 : lane >> 5)];
+    if constexpr (D == 128) {
+      k = *((const uint4*)base + tid);
+      v = *((const uint4*)(base + 34 * D) + tid);
+      vs = *(const uint4*)(base + 66 * D + ((lane >> 4) * 2 + (tid >> 7)) * 32 + ((tid >> 6) & 1) * 16);
+    } else {
+      const uint2 a = *(const uint2*)(base + k_code_at<D>((tid >> 6) * 16 + (lane & 15), lane >> 4));
+      const uint2 c = *(const uint2*)(base + 34 * D + ((tid >> 7) * 64 + lane) * 16 + ((tid >> 6) & 1) * 8);
+      const uint2 e = *(const uint2*)(base + 66 * D + ((lane >> 4) * 2 + (tid >> 7)) * 16 + ((tid >> 6) & 1) * 8);
+      k = make_uint4(a.x, a.y, 0, 0);
+      v = make_uint4(c.x, c.y, 0, 0);
+      vs = make_uint4(e.x, e.y, 0, 0);
+    }
+  }
+  // Into sk[token][chunk of 8 channels], sv[channel][chunk of 8 tokens, in the
+  // order that a lane's weights have: runs of four 0 2 | 1 3 of each 16].
+  // Tokens from `left` on get V = 0, whatever their bytes are.
+  __device__ __forceinline__ void store(half8* sk, half8* sv, int tid, int left) {
+    const int lane = tid & 63, r = lane & 15, kq = lane >> 4;
+    {
+      const int tok = (tid >> 6) * 16 + r;
+      const half2v s = scale_pair(ks, 0, 0);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const int chunk = kq * (D / 32) + j;
+        sk[tok * (D / 8) + (chunk ^ (tok & (D / 8 - 1)))] = dequant(word(k, j), s, s, s, s);
+      }
+    }
+    const int sg = tid >> 7, x = (tid >> 6) & 1;
+    if (left < kPage) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {  // words: 4 tokens each, runs alternate
+        const int live = min(max(left - (32 * sg + 16 * (i & 1) + 4 * kq), 0), 4);
+        const uint32_t msk = live == 4 ? ~0u : (1u << (8 * live)) - 1u;
+        if (i == 0) vs.x &= msk;
+        if (i == 1) vs.y &= msk;
+        if (i == 2) vs.z &= msk;
+        if (i == 3) vs.w &= msk;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint32_t w0 = word(vs, D == 128 ? (j >> 1) * 2 : 0), w1 = word(vs, D == 128 ? (j >> 1) * 2 + 1 : 1);
+      const int ch = D == 128 ? 64 * x + 16 * j + r : 32 * x + 16 * j + r;
+      const half8 f = dequant(word(v, j), scale_pair(w0, 0, 1), scale_pair(w0, 2, 3), scale_pair(w1, 0, 1), scale_pair(w1, 2, 3));
+      typedef half_t half4 __attribute__((ext_vector_type(4)));
+      half4* row = (half4*)(sv + ch * 8);
+      const int c0 = 4 * sg + (kq & 1);
+      row[(c0 ^ (ch & 7)) * 2 + (kq >> 1)] = half4{f[0], f[1], f[2], f[3]};
+      row[((c0 + 2) ^ (ch & 7)) * 2 + (kq >> 1)] = half4{f[4], f[5], f[6], f[7]};
+    }
+  }
+};
+
+constexpr int kTileRows = 128;
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2)
+void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
+  constexpr int QS = D / 16;  // k-steps of a score
+  constexpr int CT = D / 32;  // channel tiles of the output
+  __shared__ half8 sk[2][kPage * (D / 8)], sv[2][D * 8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hi = lane >> 5;
+  // kv heads innermost: with 8 of them each has an XCD (workgroup id mod 8) and
+  // its L2 to itself; long row tiles first
+  const int g = blockIdx.x % a.n_kv_heads, b = blockIdx.y;
+  const int unit = blockIdx.x / a.n_kv_heads;
+  const int split = unit % w.n_splits;
+  const Seq s = seq_of(a, b);
+  const int group = a.n_q_heads / a.n_kv_heads;
+  const int n_rows = s.n * group;
+  const int keys = min(s.len, s.cap);
+  const int tiles = (keys + kPage - 1) / kPage;
+  const int per = tiles_per_split(tiles, w.n_splits);
+  const int first = split * per, end = min(first + per, tiles);
+  if (w.n_splits > 1 && first >= tiles) return;
+  const int n_tiles = (n_rows + kTileRows - 1) / kTileRows;
+
+  for (int back = unit / w.n_splits; back < n_tiles; back += w.row_tiles) {
+    const int rt = n_tiles - 1 - back;
+    const int r0 = rt * kTileRows + wave * 32;             // the wave's first row
+    const int r = r0 + col;
+    const bool live = r < n_rows;
+    const int i = live ? r / group : 0, h = live ? r - i * group : 0;
+    const int lim = live ? min(max(s.len - s.n + i + 1, 0), keys) : 0;
+    const int r_last = min(r0 + 31, n_rows - 1), t_last = min(rt * kTileRows + kTileRows, n_rows) - 1;
+    const int lim_min = r0 + 31 < n_rows ? min(max(s.len - s.n + r0 / group + 1, 0), keys) : 0;
+    const int lim_max = r0 < n_rows ? min(max(s.len - s.n + r_last / group + 1, 0), keys) : 0;
+    const int lim_all = min(max(s.len - s.n + t_last / group + 1, 0), keys);
+    const int last = min(end, (lim_all + kPage - 1) / kPage);
+
+    half8 q[QS];
+    float sc = fabsf(a.scale) * 1.4426950408889634f;
+    {
+      // the scale's sign goes into q, so that the largest product is the largest score
+      const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+      if (a.scale == 0.f) sc = 1.f;
+      const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + 8 * hi;
+      if constexpr (__is_same(T, half_t)) {
+#pragma unroll
+        for (int j = 0; j < QS; ++j) {
+          q[j] = live ? *(const half8*)(qp + 16 * j) : half8{};
+          q[j] *= (half_t)sign;
+        }
+      } else {
+        float mx = 0.f;
+#pragma unroll
+        for (int j = 0; j < QS; ++j) {
+          float x[8] = {};
+          if (live) load8(qp + 16 * j, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+        }
+        float other, mine;
+        perm32_swap(mx, mine, other);
+        mx = fmaxf(mine, other);
+        const int ex = mx > 0.f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
+#pragma unroll
+        for (int j = 0; j < QS; ++j) {
+          float x[8] = {};
+          if (live) load8(qp + 16 * j, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[j][e] = (half_t)(sign * ldexpf(x[e], -ex));
+        }
+        sc = ldexpf(sc, ex);
+      }
+    }
+    float m = -INFINITY, l = 0.f;
+    float16v acc[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[c][e] = 0.f;
+
+    TileRegs<D> regs;
+    int page = -1, page_next = -1;  // of the tile in regs, of the one after
+    if (first < last) {
+      page = page_of(a, b, first * kPage);
+      if (page >= 0) regs.load(head_of<D>(a, page, g), tid);
+      if (first + 1 < last) page_next = page_of(a, b, (first + 1) * kPage);
+    }
+    __syncthreads();  // the buffers' readers of the tile of rows before
+    bool have = page >= 0, have_next = false;
+    if (have) regs.store(sk[0], sv[0], tid, keys - first * kPage);
+    if (page_next >= 0) regs.load(head_of<D>(a, page_next, g), tid);
+    page = page_next;
+    page_next = first + 2 < last ? page_of(a, b, (first + 2) * kPage) : -1;
+    __syncthreads();
+
+    int cur = 0;
+    for (int tile = first; tile < last; ++tile, cur ^= 1) {
+      have_next = page >= 0;
+      if (have_next) regs.store(sk[cur ^ 1], sv[cur ^ 1], tid, keys - (tile + 1) * kPage);
+      if (page_next >= 0) regs.load(head_of<D>(a, page_next, g), tid);
+      page = page_next;
+      page_next = tile + 3 < last ? page_of(a, b, (tile + 3) * kPage) : -1;
+      if (have && tile * kPage < lim_max) {
+        const half8 *bk = sk[cur], *bv = sv[cur];
+        float16v S[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
+#pragma unroll
+          for (int j = 0; j < QS; ++j) {
+            const int tok = 32 * t + col;
+            S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bk[tok * (D / 8) + ((2 * j + hi) ^ (tok & (D / 8 - 1)))], q[j], S[t], 0, 0, 0);
+          }
+        }
+        if ((tile + 1) * kPage > lim_min) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              S[t][e] = tile * kPage + 32 * t + 8 * (e >> 2) + 4 * hi + (e & 3) < lim ? S[t][e] : -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, S[t][e]);
+        float other, mine;
+        perm32_swap(mx, mine, other);
+        mx = fmaxf(mine, other) * sc;
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
+          const float to = fmaxf(m, mx);
+          const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+          m = to;
+          l *= alpha;
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[c][e] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        half8 P[4];
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][e], sc, -base));
+            sum += p;
+            P[2 * t + (e >> 3)][e & 7] = (half_t)p;
+          }
+        l += sum;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            const int ch = 32 * c + col;
+            acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bv[ch * 8 + ((2 * st + hi) ^ (ch & 7))], P[st], acc[c], 0, 0, 0);
+          }
+      }
+      have = have_next;
+      __syncthreads();
+    }
+
+    float other, mine;
+    perm32_swap(l, mine, other);
+    l = mine + other;
+    if (live) {
+      const int64_t row = (int64_t)(s.row0 + i) * a.n_q_heads + g * group + h;
+      if (w.n_splits == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            vec4 o;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = (T)(acc[c][e + k] * inv);
+            *(vec4*)((T*)a.out + row * D + 32 * c + 2 * e + 4 * hi) = o;
+          }
+      } else {
+        const int64_t part = row * w.n_splits + split;
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *(float4v*)(w.acc + part * D + 32 * c + 2 * e + 4 * hi) = float4v{acc[c][e], acc[c][e + 1], acc[c][e + 2], acc[c][e + 3]};
+        if (hi == 0) {
+          w.m[part] = m;
+          w.l[part] = l;
+        }
+      }
+    }
+  }
+}
+
 // Joins the splits of a row: a wave a row, each lane D / 64 channels.
 template <class T, int D>
 __global__ __launch_bounds__(256)
@@ -704,20 +970,22 @@ int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens
 // CUs four times over (a split takes 4 tiles at least), and at most 32 tiles
 // (2,048 tokens) a split, so that a batch of uneven lengths ends together.
 struct AttnPlan {
-  int nq, row_tiles, n_splits;
+  int nq;         // 16-row groups of a workgroup: 1 or 2 (rows), 8 (tile)
+  int row_tiles, n_splits;
 };
 AttnPlan plan_of(const shard_kv4_args* a) {
   AttnPlan p;
   const int group = a->n_q_heads / a->n_kv_heads;
   const int64_t n = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
   const int64_t rows = (a->cu_seqlens ? n : 1) * group;
-  p.nq = rows <= 16 ? 1 : 2;
+  p.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
   p.row_tiles = (int)((rows + 16 * p.nq - 1) / (16 * p.nq));
   const int64_t cap = (int64_t)a->table_width * kPage;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t tiles = (len + kPage - 1) / kPage;
   const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
-  int64_t sp = (1024 + wg - 1) / wg;
+  const int64_t fill = p.nq == 8 ? 512 : 1024;
+  int64_t sp = (fill + wg - 1) / wg;
   const int64_t even = (tiles + 31) / 32;
   if (rows <= 32 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
@@ -817,7 +1085,7 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   AttnWork w{};
   w.n_splits = p.n_splits;
   w.row_tiles = p.row_tiles;
-  if ((int64_t)w.n_splits * w.row_tiles > INT32_MAX) return SHARD_ERR_SHAPE;
+  if ((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads > INT32_MAX) return SHARD_ERR_SHAPE;
   if (p.n_splits > 1) {
     const size_t need = shard_kv4_attn_workspace(a);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) {
@@ -832,7 +1100,8 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   }
   const hipStream_t s = (hipStream_t)stream;
   if (p.nq == 1) launch_rows<1>(a, w, s);
-  else launch_rows<2>(a, w, s);
+  else if (p.nq == 2) launch_rows<2>(a, w, s);
+  else KV4_DISPATCH(k_kv4_attn_tile, dim3((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch), s, *a, w);
   SHARD_LAUNCH_CHECK("shard_kv4_attn");
   if (p.n_splits > 1) {
     const int64_t per_seq = (a->cu_seqlens ? (a->max_new > 0 ? a->max_new : a->n_tokens) : 1) * (int64_t)a->n_q_heads;
