@@ -907,35 +907,84 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   }
 }
 
-// Joins the splits of a row: a wave a row, each lane D / 64 channels.
-template <class T, int D>
+// Joins the splits of a row.  WAVES waves take a row's splits in turn, several
+// splits a load (16 bytes a lane); every wave forms all weights itself (128
+// splits at most: two a lane).
+constexpr int kMaxSplits = 128;
+
+template <class T, int D, int WAVES>
+__device__ __forceinline__ void merge_row(const AttnWork& w, T* out, int64_t row, int n, int wave, int lane, float4v* sh) {
+  constexpr int LPS = D / 4;       // lanes of a split's row
+  constexpr int SPL = 64 / LPS;    // splits a load
+  const float* pm = w.m + row * w.n_splits;
+  const float* pl = w.l + row * w.n_splits;
+  const float m0 = lane < n ? pm[lane] : -INFINITY, m1 = lane + 64 < n ? pm[lane + 64] : -INFINITY;
+  const float l0 = lane < n ? pl[lane] : 0.f, l1 = lane + 64 < n ? pl[lane + 64] : 0.f;
+  const float* pa = w.acc + row * w.n_splits * D + (lane % LPS) * 4;
+  constexpr int U = 4;             // loads in flight
+  float4v v[U];
+  const int s0 = wave * SPL + lane / LPS;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = s0 + u * SPL * WAVES;
+    v[u] = i < n ? *(const float4v*)(pa + (int64_t)i * D) : float4v{0.f, 0.f, 0.f, 0.f};
+  }
+  const float M = wave64_reduce(fmaxf(m0, m1), OpMax());
+  const float base = M == -INFINITY ? 0.f : M;
+  const float f0 = exp2f(m0 - base), f1 = exp2f(m1 - base);
+  const float l = wave64_reduce(f0 * l0 + f1 * l1, OpAdd());
+  float4v x{0.f, 0.f, 0.f, 0.f};
+  for (int at = 0; at < n; at += SPL * WAVES * U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = at + s0 + u * SPL * WAVES;
+      const float f = i < 64 ? __shfl(f0, i & 63) : __shfl(f1, i & 63);
+      if (i < n) x += f * v[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = at + s0 + (u + U) * SPL * WAVES;
+      v[u] = i < n ? *(const float4v*)(pa + (int64_t)i * D) : float4v{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (LPS == 16) x[e] += xor_lane<16>(x[e]);
+    x[e] += xor_lane<32>(x[e]);
+  }
+  if constexpr (WAVES > 1) {
+    if (lane < LPS) sh[wave * LPS + lane] = x;
+    __syncthreads();
+    if (wave) return;
+    if (lane < LPS)
+#pragma unroll
+      for (int k = 1; k < WAVES; ++k) x += sh[k * LPS + lane];
+  }
+  if (lane < LPS) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    vec4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)(x[e] * inv);
+    *(vec4*)(out + row * D + lane * 4) = o;
+  }
+}
+
+// A row a workgroup (few rows or many splits: latency counts) or a row a wave.
+template <class T, int D, int WAVES>
 __global__ __launch_bounds__(256)
 void k_kv4_merge(const shard_kv4_args a, const AttnWork w) {
+  __shared__ float4v sh[WAVES > 1 ? WAVES * D / 4 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.y;
-  const Seq s = seq_of(a, b);
+  const Seq s = seq_of(a, blockIdx.y);
   const int tiles = (min(s.len, s.cap) + kPage - 1) / kPage;
-  const int n = (tiles + tiles_per_split(tiles, w.n_splits) - 1) / tiles_per_split(tiles, w.n_splits);
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < (int64_t)s.n * a.n_q_heads; r += (int64_t)gridDim.x * 4) {
-    const int64_t row = (int64_t)s.row0 * a.n_q_heads + r;
-    const float* pm = w.m + row * w.n_splits;
-    const float* pl = w.l + row * w.n_splits;
-    const float* pa = w.acc + row * w.n_splits * D;
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 64) M = fmaxf(M, pm[i]);
-    M = wave64_reduce(M, OpMax());
-    const float base = M == -INFINITY ? 0.f : M;
-    float x[D / 64] = {}, lt = 0.f;
-    for (int i = 0; i < n; ++i) {
-      const float f = exp2f(pm[i] - base);
-      lt += f * pl[i];
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) x[j] += f * pa[(int64_t)i * D + lane * (D / 64) + j];
-    }
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    T* o = (T*)a.out + row * D + lane * (D / 64);
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) o[j] = (T)(x[j] * inv);
+  const int per = tiles_per_split(tiles, w.n_splits);
+  const int n = (tiles + per - 1) / per;
+  constexpr int ROWS = 4 / WAVES;
+  const int64_t rows = (int64_t)s.n * a.n_q_heads, row0 = (int64_t)s.row0 * a.n_q_heads;
+  for (int64_t r = (int64_t)blockIdx.x * ROWS + (WAVES > 1 ? 0 : wave); r < rows; r += (int64_t)gridDim.x * ROWS) {
+    merge_row<T, D, WAVES>(w, (T*)a.out, row0 + r, n, WAVES > 1 ? wave : 0, lane, sh);
+    if constexpr (WAVES > 1) __syncthreads();
   }
 }
 
@@ -989,7 +1038,7 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   const int64_t even = (tiles + 31) / 32;
   if (rows <= 32 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
-  if (sp > 128) sp = 128;
+  if (sp > kMaxSplits) sp = kMaxSplits;
   p.n_splits = sp < 1 ? 1 : (int)sp;
   return p;
 }
@@ -1017,17 +1066,16 @@ using namespace shard;
     }                                                                                                           \
   } while (0)
 
-template <int NQ>
-static void launch_rows(const shard_kv4_args* a, const AttnWork& w, hipStream_t s) {
-  const dim3 grid((unsigned)(w.n_splits * w.row_tiles), a->n_kv_heads, a->batch);
-  if (a->dtype == SHARD_FP16) {
-    if (a->head_dim == 128) hipLaunchKernelGGL((k_kv4_attn_rows<half_t, 128, NQ>), grid, dim3(256), 0, s, *a, w);
-    else hipLaunchKernelGGL((k_kv4_attn_rows<half_t, 64, NQ>), grid, dim3(256), 0, s, *a, w);
-  } else {
-    if (a->head_dim == 128) hipLaunchKernelGGL((k_kv4_attn_rows<bf16_t, 128, NQ>), grid, dim3(256), 0, s, *a, w);
-    else hipLaunchKernelGGL((k_kv4_attn_rows<bf16_t, 64, NQ>), grid, dim3(256), 0, s, *a, w);
-  }
-}
+#define KV4_DISPATCH_N(KERNEL, N, grid, s, ...)                                                                 \
+  do {                                                                                                          \
+    if (a->dtype == SHARD_FP16) {                                                                               \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<half_t, 128, N>), grid, dim3(256), 0, s, __VA_ARGS__); \
+      else hipLaunchKernelGGL((KERNEL<half_t, 64, N>), grid, dim3(256), 0, s, __VA_ARGS__);                     \
+    } else {                                                                                                    \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16_t, 128, N>), grid, dim3(256), 0, s, __VA_ARGS__); \
+      else hipLaunchKernelGGL((KERNEL<bf16_t, 64, N>), grid, dim3(256), 0, s, __VA_ARGS__);                     \
+    }                                                                                                           \
+  } while (0)
 
 extern "C" {
 
@@ -1099,15 +1147,21 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
     w.l = w.m + rows * p.n_splits;
   }
   const hipStream_t s = (hipStream_t)stream;
-  if (p.nq == 1) launch_rows<1>(a, w, s);
-  else if (p.nq == 2) launch_rows<2>(a, w, s);
+  const dim3 rows_grid((unsigned)(w.n_splits * w.row_tiles), a->n_kv_heads, a->batch);
+  if (p.nq == 1) KV4_DISPATCH_N(k_kv4_attn_rows, 1, rows_grid, s, *a, w);
+  else if (p.nq == 2) KV4_DISPATCH_N(k_kv4_attn_rows, 2, rows_grid, s, *a, w);
   else KV4_DISPATCH(k_kv4_attn_tile, dim3((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch), s, *a, w);
   SHARD_LAUNCH_CHECK("shard_kv4_attn");
   if (p.n_splits > 1) {
     const int64_t per_seq = (a->cu_seqlens ? (a->max_new > 0 ? a->max_new : a->n_tokens) : 1) * (int64_t)a->n_q_heads;
-    const int64_t blocks = (per_seq + 3) / 4;
-    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), a->batch);
-    KV4_DISPATCH(k_kv4_merge, grid, s, *a, w);
+    if (p.n_splits > 8) {
+      const dim3 grid((unsigned)(per_seq < 4096 ? per_seq : 4096), a->batch);
+      KV4_DISPATCH_N(k_kv4_merge, 4, grid, s, *a, w);
+    } else {
+      const int64_t blocks = (per_seq + 3) / 4;
+      const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), a->batch);
+      KV4_DISPATCH_N(k_kv4_merge, 1, grid, s, *a, w);
+    }
     SHARD_LAUNCH_CHECK("shard_kv4_attn merge");
   }
   return SHARD_OK;

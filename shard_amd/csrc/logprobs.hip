@@ -9,10 +9,11 @@
 // The difference x - M is taken first, so that its rounding is relative to
 // itself and a row of equal logits far from 0 loses nothing.
 //
-// Top k: the k-th largest of the threads' best elements bounds the row's k-th
-// largest from below, so only the threads whose best reaches it (k of 256,
-// mostly) look through their elements once more and put those that reach it
-// into a list in LDS; an element's rank there is the number of larger ones.
+// Top k: the k-th largest of a wave's 64 best elements, one a thread, bounds
+// the row's k-th largest from below.  Only the threads whose best reaches the
+// largest such bound look through their elements once more and put those that
+// reach it into a list in LDS; an element's rank there is the number of larger
+// ones.
 // Elements are compared as (value, lower index first) in 64 bits, so no two
 // are equal.  Where more than the list holds reach the bound (many equal
 // logits), the list's own k-th largest is the next bound.
@@ -67,6 +68,10 @@ struct Row {
     mis = (int)(((uintptr_t)row & 15) / sizeof(T));
     count = (n + mis + VEC - 1) / VEC;
   }
+  // Granules lo .. hi - 1 lie wholly within the row.
+  __device__ __forceinline__ int64_t lo() const { return mis ? 1 : 0; }
+  __device__ __forceinline__ int64_t hi() const { return (n + mis) / VEC; }
+  __device__ __forceinline__ vec raw(int64_t j) const { return *(const vec*)(p + (j * VEC - mis)); }
   // Elements outside the row are -inf.  Returns the index of x[0].
   __device__ __forceinline__ int64_t load(int64_t j, float (&x)[VEC]) const {
     const int64_t e0 = j * VEC - mis;
@@ -81,6 +86,16 @@ struct Row {
     return e0;
   }
 };
+
+// The largest b such that at least k lanes hold v >= b (0 if none does).
+__device__ __forceinline__ uint32_t kth_largest(uint32_t v, int k) {
+  uint32_t b = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = b | 1u << bit;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= t)) >= k) b = t;
+  }
+  return b;
+}
 
 struct Stats {
   float M, l, t;
@@ -106,9 +121,9 @@ template <class T>
 __global__ __launch_bounds__(256)
 void k_logprobs(const LogprobArgs a) {
   constexpr int VEC = Row<T>::VEC;
-  __shared__ u64 best[256];
   __shared__ u64 list[kList];
   __shared__ float sh_M[4], sh_l[4], sh_t[4];
+  __shared__ uint32_t sh_b[4];
   __shared__ u64 bound;
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -120,9 +135,9 @@ void k_logprobs(const LogprobArgs a) {
   Stats s{kLowest, 0.f, 0.f};
   float bv = -INFINITY;
   int64_t bi = -1;
-  for (int64_t j = g0 + tid; j < g1; j += 256) {
-    float x[VEC];
-    const int64_t e0 = r.load(j, x);
+  float x[VEC];  // the granule at hand, its first index
+  int64_t e0 = 0;
+  const auto eat = [&] {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < VEC; ++i) m = fmaxf(m, x[i]);
@@ -142,14 +157,42 @@ void k_logprobs(const LogprobArgs a) {
       s.l += e;
       s.t += e * fmaxf(d, -1e4f);
     }
+  };
+  const auto eat_raw = [&](const typename Row<T>::vec& v, int64_t j) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = (float)v[i];
+    e0 = j * VEC - r.mis;
+    eat();
+  };
+  int64_t j = g0 + tid;
+  if (j < g1 && j < r.lo()) {
+    e0 = r.load(j, x);
+    eat();
+    j += 256;
+  }
+  const int64_t gf = g1 < r.hi() ? g1 : r.hi();
+  for (; j + 3 * 256 < gf; j += 4 * 256) {  // four granules in flight
+    typename Row<T>::vec v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = r.raw(j + u * 256);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) eat_raw(v[u], j + u * 256);
+  }
+  for (; j < gf; j += 256) eat_raw(r.raw(j), j);
+  if (j < g1) {
+    e0 = r.load(j, x);
+    eat();
   }
 
   // the row's (part's) sums
   float M = wave64_reduce(s.M, OpMax());
   if (lane == 0) sh_M[wave] = M;
-  const u64 mine = bi >= 0 ? key_of(bv, bi) : 0;
-  best[tid] = mine;
-  if (tid == 0) bound = 1;
+  const uint32_t mine = bi >= 0 ? f2ord(bv + 0.f) : 0;
+  if (a.top) {
+    const uint32_t b = kth_largest(mine, a.top);
+    if (lane == 0) sh_b[wave] = b;
+  }
+  if (tid == 0) found = 0;
   __syncthreads();
   M = fmaxf(fmaxf(sh_M[0], sh_M[1]), fmaxf(sh_M[2], sh_M[3]));
   move_to(s, M);
@@ -157,11 +200,6 @@ void k_logprobs(const LogprobArgs a) {
   if (lane == 0) {
     sh_l[wave] = l;
     sh_t[wave] = t;
-  }
-  if (a.top && mine) {
-    int rank = 0;
-    for (int i = 0; i < 256; ++i) rank += best[i] > mine;
-    if (rank == a.top - 1) bound = mine;
   }
   __syncthreads();
   const Stats all{M, (sh_l[0] + sh_l[1]) + (sh_l[2] + sh_l[3]), (sh_t[0] + sh_t[1]) + (sh_t[2] + sh_t[3])};
@@ -176,37 +214,42 @@ void k_logprobs(const LogprobArgs a) {
   if (a.top == 0) return;
 
   int n;
+  u64 need = (u64)max(max(sh_b[0], sh_b[1]), max(sh_b[2], sh_b[3])) << 32;
+  need = need ? need : 1;
   for (;;) {
-    if (tid == 0) found = 0;
-    __syncthreads();
-    const u64 need = bound;
-    if (mine >= need) {
-      for (int64_t j = g0 + tid; j < g1; j += 256) {
-        float x[VEC];
-        const int64_t e0 = r.load(j, x);
+    const auto collect = [&](const float(&x)[VEC], int64_t e0) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          if (e0 + i < 0 || e0 + i >= a.vocab) continue;
-          const u64 key = key_of(x[i], e0 + i);
-          if (key >= need) {
-            const int at = atomicAdd(&found, 1);
-            if (at < kList) list[at] = key;
-          }
+      for (int i = 0; i < VEC; ++i) {
+        const u64 key = e0 + i >= 0 && e0 + i < a.vocab ? key_of(x[i], e0 + i) : 0;
+        if (key >= need) {
+          const int at = atomicAdd(&found, 1);
+          if (at < kList) list[at] = key;
         }
       }
+    };
+    if (mine >= (uint32_t)(need >> 32) && mine) {
+      for (int64_t j = g0 + tid; j + 256 < g1; j += 256) {
+        float y[VEC];
+        const int64_t e = r.load(j, y);
+        collect(y, e);
+      }
+      collect(x, e0);  // the thread's last granule is still at hand
     }
     __syncthreads();
     n = found;
     if (n <= kList) break;
-    // more than fit: kList of them are in the list; its k-th largest is at
-    // least the present bound's successor, as kList > top
+    // more than fit: kList of them are in the list, and its k-th largest lies
+    // above the present bound, as kList > top
+    __syncthreads();
     for (int u = tid; u < kList; u += 256) {
       const u64 key = list[u];
       int rank = 0;
       for (int i = 0; i < kList; ++i) rank += list[i] > key;
       if (rank == a.top - 1) bound = key;
     }
+    if (tid == 0) found = 0;
     __syncthreads();
+    need = bound;
   }
   // ranks of the list's elements; what a row does not have is 0
   const float ln = logf(all.l);
@@ -228,67 +271,68 @@ void k_logprobs(const LogprobArgs a) {
   }
 }
 
-// Joins the parts of a row.  A part's keys are in descending order, so an
-// element's rank is found by one binary search in every other part's; elements
-// below some part's k-th cannot be among the k largest.
+// Joins the parts of a row.  A part's keys are in descending order; the largest
+// of the parts' k-th bounds the row's k-th from below, and what reaches it is
+// ranked by counting.
 template <class T>
 __global__ __launch_bounds__(256)
 void k_logprobs_join(const LogprobArgs a) {
-  extern __shared__ u64 keys[];  // parts * top
-  __shared__ float sh[3];
+  extern __shared__ u64 list[];  // parts * top
+  __shared__ float sh[2];
   __shared__ u64 bound;
-  const int tid = threadIdx.x;
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const int k = a.top, n = a.parts * k;
-  for (int u = tid; u < n; u += 256) keys[u] = a.ws_keys[row * n + u];
-  if (tid < 64) {
+  const u64* keys = a.ws_keys + row * n;
+  u64 b = 0;
+  for (int p = tid; k && p < a.parts; p += 256) b = keys[p * k + k - 1];   // parts <= 64: one a thread
+  const int64_t tok = a.tokens ? a.tokens[row] : -1;
+  const float logit = tok >= 0 && tok < a.vocab ? (float)((const T*)a.logits)[row * a.stride + tok] : 0.f;
+  if (tid == 0) found = 0;
+  if (wave == 0) {
+    const uint32_t top32 = (uint32_t)(b >> 32);
+    // the largest b: by its value, then by its index
+    uint32_t hi = top32;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+    uint32_t lo = top32 == hi ? (uint32_t)b : 0;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) lo = max(lo, (uint32_t)__shfl_xor((int)lo, o));
     float4 f = make_float4(kLowest, 0.f, 0.f, 0.f);
-    if (tid < a.parts) f = a.ws_stats[row * a.parts + tid];
+    if (lane < a.parts) f = a.ws_stats[row * a.parts + lane];
     Stats s{f.x, f.y, f.z};
     const float M = wave64_reduce(s.M, OpMax());
     move_to(s, M);
     const Stats all{M, wave64_reduce(s.l, OpAdd()), wave64_reduce(s.t, OpAdd())};
-    if (tid == 0) {
-      const int64_t tok = a.tokens ? a.tokens[row] : -1;
-      const T* p = (const T*)a.logits + row * a.stride;
-      write_row(a, row, all, tok >= 0 && tok < a.vocab ? (float)p[tok] : 0.f, tok);
+    if (lane == 0) {
+      write_row(a, row, all, logit, tok);
       sh[0] = all.M;
       sh[1] = all.l;
-      bound = 0;
+      bound = (u64)hi << 32 | lo;
     }
   }
   if (k == 0) return;
   __syncthreads();
-  if (tid < a.parts) atomicMax(&bound, keys[tid * k + k - 1]);
-  __syncthreads();
-  const u64 need = bound;
-  const float M = sh[0], ln = logf(sh[1]);
-  // places that no key takes: the k-th and later of a row with fewer
-  int have = 0;
-  if (need == 0) {
-    for (int u = 0; u < n; ++u) have += keys[u] != 0;
-    for (int i = have + tid; i < k; i += 256) {
-      a.top_ids[row * k + i] = -1;
-      a.top_logprobs[row * k + i] = NAN;
-    }
-  }
+  const u64 need = bound ? bound : 1;
   for (int u = tid; u < n; u += 256) {
     const u64 key = keys[u];
-    if (key == 0 || key < need) continue;
-    int rank = 0;
-    for (int p = 0; p < a.parts && rank < k; ++p) {
-      int lo = 0, hi = k;  // elements of part p above key
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (keys[p * k + mid] > key) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
+    if (key >= need) list[atomicAdd(&found, 1)] = key;
+  }
+  __syncthreads();
+  const int have = found;
+  const float M = sh[0], ln = logf(sh[1]);
+  for (int u = tid; u < have + k; u += 256) {
+    u64 key = 0;
+    int rank = u;  // u >= have: the places behind them
+    if (u < have) {
+      key = list[u];
+      rank = 0;
+      for (int i = 0; i < have; ++i) rank += list[i] > key;
     }
-    if (rank < k) {
-      a.top_ids[row * k + rank] = index_of(key);
-      a.top_logprobs[row * k + rank] = value_of(key) - M - ln;
-    }
+    if (rank >= k) continue;
+    a.top_ids[row * k + rank] = key ? index_of(key) : -1;
+    a.top_logprobs[row * k + rank] = key ? value_of(key) - M - ln : NAN;
   }
 }
 
