@@ -9,11 +9,11 @@
 // The difference x - M is taken first, so that its rounding is relative to
 // itself and a row of equal logits far from 0 loses nothing.
 //
-// Top k: the k-th largest of a wave's 64 best elements, one a thread, bounds
-// the row's k-th largest from below.  Only the threads whose best reaches the
-// largest such bound look through their elements once more and put those that
-// reach it into a list in LDS; an element's rank there is the number of larger
-// ones.
+// Top k: every thread also notes the largest logit of each eighth of its
+// elements (a slot).  The k-th largest of the 256 threads' largest bounds the
+// row's k-th largest from below, so only the slots that reach it (about k of
+// 2,048) are read once more; their elements that reach it go into a list in
+// LDS, where an element's rank is the number of larger ones.
 // Elements are compared as (value, lower index first) in 64 bits, so no two
 // are equal.  Where more than the list holds reach the bound (many equal
 // logits), the list's own k-th largest is the next bound.
@@ -87,12 +87,16 @@ struct Row {
   }
 };
 
-// The largest b such that at least k lanes hold v >= b (0 if none does).
-__device__ __forceinline__ uint32_t kth_largest(uint32_t v, int k) {
+// The largest b, its low 16 bits clear, such that at least k of the lanes' 4
+// values are >= b (0 if none is).
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[4], int k) {
   uint32_t b = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= 16; --bit) {
     const uint32_t t = b | 1u << bit;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= t)) >= k) b = t;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= t));
+    if (n >= k) b = t;
   }
   return b;
 }
@@ -117,39 +121,36 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, con
     a.logprob[row] = token < 0 ? 0.f : token < a.vocab ? token_logit - s.M - ln : NAN;
 }
 
+constexpr int kSlots = 8;
+
 template <class T>
 __global__ __launch_bounds__(256)
 void k_logprobs(const LogprobArgs a) {
   constexpr int VEC = Row<T>::VEC;
   __shared__ u64 list[kList];
+  __shared__ uint32_t slot[kSlots][256], most[256];  // largest logits, ordered
+  __shared__ uint16_t todo[kSlots * 256];
   __shared__ float sh_M[4], sh_l[4], sh_t[4];
-  __shared__ uint32_t sh_b[4];
   __shared__ u64 bound;
-  __shared__ int found;
+  __shared__ int found, n_todo;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const int part = blockIdx.y;
   const Row<T> r((const T*)a.logits + row * a.stride, a.vocab);
   const int64_t g0 = part * a.granules, g1 = g0 + a.granules < r.count ? g0 + a.granules : r.count;
+  // the thread's i-th granule is g0 + 256 i + tid, slot q its granules from q * size on
+  const int64_t own = (g1 - g0 + 255) / 256, size = own > kSlots ? (own + kSlots - 1) / kSlots : 1;
 
   Stats s{kLowest, 0.f, 0.f};
-  float bv = -INFINITY;
-  int64_t bi = -1;
-  float x[VEC];  // the granule at hand, its first index
-  int64_t e0 = 0;
-  const auto eat = [&] {
+  float best = -INFINITY;
+  // M follows the maximum only where that is 8 ahead (terms of at most e^8): few
+  // granules rescale.
+  const auto eat = [&](const float(&x)[VEC]) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < VEC; ++i) m = fmaxf(m, x[i]);
-    if (m > bv || bi < 0) {
-#pragma unroll
-      for (int i = VEC - 1; i >= 0; --i)
-        if (x[i] == m && e0 + i >= 0 && e0 + i < a.vocab) {
-          bi = e0 + i;
-          bv = m;
-        }
-      if (m > s.M) move_to(s, m);
-    }
+    best = fmaxf(best, m);
+    if (m > s.M + 8.f) move_to(s, m);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float d = (x[i] - s.M) * kLog2e;
@@ -158,41 +159,47 @@ void k_logprobs(const LogprobArgs a) {
       s.t += e * fmaxf(d, -1e4f);
     }
   };
-  const auto eat_raw = [&](const typename Row<T>::vec& v, int64_t j) {
+  uint32_t all_best = 0;
+  for (int q = 0; q < kSlots; ++q) {
+    best = -INFINITY;
+    bool any = false;
+    const int64_t i1 = (q + 1) * size < own ? (q + 1) * size : own;
+    for (int64_t i = q * size; i < i1; ) {
+      const int64_t j = g0 + 256 * i;   // of the first thread
+      if (i + 4 <= i1 && j >= r.lo() && j + 4 * 256 <= (g1 < r.hi() ? g1 : r.hi())) {
+        typename Row<T>::vec v[4];      // four granules in flight
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = (float)v[i];
-    e0 = j * VEC - r.mis;
-    eat();
-  };
-  int64_t j = g0 + tid;
-  if (j < g1 && j < r.lo()) {
-    e0 = r.load(j, x);
-    eat();
-    j += 256;
-  }
-  const int64_t gf = g1 < r.hi() ? g1 : r.hi();
-  for (; j + 3 * 256 < gf; j += 4 * 256) {  // four granules in flight
-    typename Row<T>::vec v[4];
+        for (int u = 0; u < 4; ++u) v[u] = r.raw(j + tid + u * 256);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = r.raw(j + u * 256);
+        for (int u = 0; u < 4; ++u) {
+          float x[VEC];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) eat_raw(v[u], j + u * 256);
-  }
-  for (; j < gf; j += 256) eat_raw(r.raw(j), j);
-  if (j < g1) {
-    e0 = r.load(j, x);
-    eat();
+          for (int k = 0; k < VEC; ++k) x[k] = (float)v[u][k];
+          eat(x);
+        }
+        any = true;
+        i += 4;
+      } else {
+        if (j + tid < g1) {
+          float x[VEC];
+          r.load(j + tid, x);
+          eat(x);
+          any = true;
+        }
+        ++i;
+      }
+    }
+    // a slot without a granule (or of NaN alone) has nothing; -inf is something
+    const uint32_t o = any ? f2ord(best + 0.f) : 0;
+    slot[q][tid] = o;
+    all_best = max(all_best, o);
   }
 
   // the row's (part's) sums
   float M = wave64_reduce(s.M, OpMax());
   if (lane == 0) sh_M[wave] = M;
-  const uint32_t mine = bi >= 0 ? f2ord(bv + 0.f) : 0;
-  if (a.top) {
-    const uint32_t b = kth_largest(mine, a.top);
-    if (lane == 0) sh_b[wave] = b;
-  }
-  if (tid == 0) found = 0;
+  most[tid] = all_best;
+  if (tid == 0) found = n_todo = 0;
   __syncthreads();
   M = fmaxf(fmaxf(sh_M[0], sh_M[1]), fmaxf(sh_M[2], sh_M[3]));
   move_to(s, M);
@@ -200,6 +207,14 @@ void k_logprobs(const LogprobArgs a) {
   if (lane == 0) {
     sh_l[wave] = l;
     sh_t[wave] = t;
+  }
+  u64 need = 1;
+  if (a.top) {
+    const uint32_t v[4] = {most[lane], most[lane + 64], most[lane + 128], most[lane + 192]};
+    const uint32_t b = kth_largest(v, a.top);
+    if (b) need = (u64)b << 32;
+    for (int q = 0; q < kSlots; ++q)
+      if (slot[q][tid] && slot[q][tid] >= b) todo[atomicAdd(&n_todo, 1)] = (uint16_t)(q * 256 + tid);
   }
   __syncthreads();
   const Stats all{M, (sh_l[0] + sh_l[1]) + (sh_l[2] + sh_l[3]), (sh_t[0] + sh_t[1]) + (sh_t[2] + sh_t[3])};
@@ -214,26 +229,22 @@ void k_logprobs(const LogprobArgs a) {
   if (a.top == 0) return;
 
   int n;
-  u64 need = (u64)max(max(sh_b[0], sh_b[1]), max(sh_b[2], sh_b[3])) << 32;
-  need = need ? need : 1;
   for (;;) {
-    const auto collect = [&](const float(&x)[VEC], int64_t e0) {
+    const uint32_t per = (uint32_t)size, items = n_todo * per;  // at most the part's granules and 2,048 more
+    for (uint32_t it = tid; it < items; it += 256) {
+      const int w = todo[it / per];
+      const int64_t i = (w >> 8) * size + it % per, j = g0 + 256 * i + (w & 255);
+      if (i >= own || j >= g1) continue;
+      float x[VEC];
+      const int64_t e0 = r.load(j, x);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const u64 key = e0 + i >= 0 && e0 + i < a.vocab ? key_of(x[i], e0 + i) : 0;
+      for (int k = 0; k < VEC; ++k) {
+        const u64 key = e0 + k >= 0 && e0 + k < a.vocab ? key_of(x[k], e0 + k) : 0;
         if (key >= need) {
           const int at = atomicAdd(&found, 1);
           if (at < kList) list[at] = key;
         }
       }
-    };
-    if (mine >= (uint32_t)(need >> 32) && mine) {
-      for (int64_t j = g0 + tid; j + 256 < g1; j += 256) {
-        float y[VEC];
-        const int64_t e = r.load(j, y);
-        collect(y, e);
-      }
-      collect(x, e0);  // the thread's last granule is still at hand
     }
     __syncthreads();
     n = found;
