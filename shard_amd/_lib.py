@@ -6,6 +6,7 @@ to load, every kernel entry point raises ``ShardHipUnavailable``.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SHARD_HIP_LIB") or os.path.join(_HERE, "libshard_hip.so")
@@ -50,7 +51,8 @@ class DecodeArgs(ctypes.Structure):
 
 
 class KV4Args(ctypes.Structure):
-    """Mirror of shard_kv4_args (include/shard_hip.h)."""
+    """Mirror of shard_kv4_args (include/shard_hip.h); KV4_PACK packs the same
+    fields, in this order, in one call."""
     _fields_ = [
         ("batch", c_int32), ("n_tokens", c_int32), ("n_q_heads", c_int32), ("n_kv_heads", c_int32),
         ("head_dim", c_int32), ("dtype", c_int32), ("n_pages", c_int32), ("table_width", c_int32),
@@ -63,6 +65,9 @@ class KV4Args(ctypes.Structure):
         ("phases", c_void_p), ("n_phases", c_int32), ("scale", c_float),
         ("q_out", c_void_p), ("k_out", c_void_p), ("v_out", c_void_p), ("out", c_void_p),
     ]
+
+
+KV4_PACK = struct.Struct("@10i Qq Qq QQ Qqq Qqq Qqq Qif QQQQ")
 
 
 # (name, restype, argtypes) of every exported symbol
@@ -119,10 +124,10 @@ SIGNATURES = [
     ("shard_rope_stream_append_dev", c_int32, [c_void_p] * 5 + [c_int64] + [c_int32] * 4 + [c_void_p] * 3 + [c_int32] + [c_void_p] * 10 + [c_void_p, c_int32] + [c_void_p]),
     ("shard_kv4_args_size", c_size_t, []),
     ("shard_kv4_page_bytes", c_int64, [c_int32, c_int32]),
-    ("shard_kv4_append", c_int32, [ctypes.POINTER(KV4Args), c_void_p]),
-    ("shard_kv4_read", c_int32, [ctypes.POINTER(KV4Args), c_void_p]),
-    ("shard_kv4_attn_workspace", c_size_t, [ctypes.POINTER(KV4Args)]),
-    ("shard_kv4_attn", c_int32, [ctypes.POINTER(KV4Args), c_void_p, c_size_t, c_void_p]),
+    ("shard_kv4_append", c_int32, [c_void_p, c_void_p]),
+    ("shard_kv4_read", c_int32, [c_void_p, c_void_p]),
+    ("shard_kv4_attn_workspace", c_size_t, [c_void_p]),
+    ("shard_kv4_attn", c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
     ("shard_token_logprobs_workspace", c_size_t, [c_int64, c_int64, c_int32]),
     ("shard_token_logprobs", c_int32, [c_void_p, c_int32] + [c_int64] * 3 + [c_void_p, c_int32] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     ("shard_stream_dequant_qjl", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
@@ -153,7 +158,7 @@ def load():
         fn.argtypes = args
     if lib.shard_decode_args_size() != ctypes.sizeof(DecodeArgs):
         raise ShardHipUnavailable("shard_decode_args layout mismatch between header and binding")
-    if lib.shard_kv4_args_size() != ctypes.sizeof(KV4Args):
+    if not lib.shard_kv4_args_size() == ctypes.sizeof(KV4Args) == KV4_PACK.size:
         raise ShardHipUnavailable("shard_kv4_args layout mismatch between header and binding")
     _lib = lib
     return lib

@@ -366,6 +366,8 @@ void k_kv4_read(const shard_kv4_args a) {
 // Scores are taken transposed, S^T = K Q^T (16 tokens x 16 rows an MFMA), so
 // that a lane's score registers hold four tokens of ONE row, and after the
 // softmax they are the right operand of O^T = V^T P^T as they stand.
+// The maximum that a row's weights refer to moves only where a weight would
+// exceed 2^8 (far inside fp16's range): most pages rescale no sums.
 // P is rounded to fp16 (2^-11 of each weight; the sums are fp32); the cache's
 // values are exact.  bf16 queries are scaled by a power of two a row (their
 // largest below 2) and are then exact in fp16 down to 2^-17 of that largest
@@ -392,13 +394,15 @@ template <int D>
 struct PageRegs {
   uint4 k[D / 32], v[D / 32], vs[D / 32];
   uint32_t ks;
-  __device__ __forceinline__ void load(const uint8_t* base, int lane) {
+  __device__ __forceinline__ void load_k(const uint8_t* base, int lane) {
     const uint4* pk = (const uint4*)base + lane;
-    const uint4* pv = (const uint4*)(base + 34 * D) + lane;
-    const uint4* ps = (const uint4*)(base + 66 * D + (lane >> 4) * (D / 2));
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) k[j] = pk[64 * j];
     ks = *(const uint32_t*)(base + 32 * D + ((D == 128 ? lane : (lane >> 5) * 16 + (lane & 15)) * 4));
+  }
+  __device__ __forceinline__ void load_v(const uint8_t* base, int lane) {
+    const uint4* pv = (const uint4*)(base + 34 * D) + lane;
+    const uint4* ps = (const uint4*)(base + 66 * D + (lane >> 4) * (D / 2));
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) v[j] = pv[64 * j];
 #pragma unroll
@@ -435,16 +439,19 @@ __device__ __forceinline__ float across_quarters_sum(float v) {
   return a + b;
 }
 
-// Few rows: a workgroup of 4 waves takes 16 NQ rows and a split of the pages;
-// every wave walks its own pages (registers only) and the four are joined in
-// LDS at the end.
+// Few rows: a workgroup of 4 waves takes 16 NQ rows and a split of the
+// pages; every wave walks its own pages (registers only) and the waves are
+// joined in LDS at the end.  The next page's K is loaded into the registers
+// that the scores have just freed, its V into those of the output's product, so
+// that each is on its way during the other half of the work.
 template <class T, int D, int NQ>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, (D == 128 ? 4 : 5) - NQ)
 void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
+  constexpr int WAVES = 4;
   constexpr int ST = D / 32;  // k-steps of a score, 32-channel blocks
   constexpr int NT = D / 16;  // channel tiles of the output
-  __shared__ float sh_acc[4][16 * NQ][D + 4];
-  __shared__ float sh_m[4][16 * NQ], sh_l[4][16 * NQ];
+  __shared__ float sh_acc[WAVES][16 * NQ][D + 4];
+  __shared__ float sh_m[WAVES][16 * NQ], sh_l[WAVES][16 * NQ];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
   const int g = blockIdx.y, b = blockIdx.z;
@@ -458,7 +465,9 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   const int first = split * per, last = min(first + per, tiles);
   // a split past the sequence's end has no part that the merge reads
   if (w.n_splits > 1 && first >= tiles) return;
-  const float scale2 = a.scale * 1.4426950408889634f;
+  // the scale's sign goes into q, so that the largest product is the largest score
+  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+  const half_t sign = a.scale < 0.f ? (half_t)-1.f : a.scale == 0.f ? (half_t)0.f : (half_t)1.f;
 
   for (int rt = blockIdx.x / w.n_splits; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
     half8 q[NQ][ST];
@@ -485,7 +494,7 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
       const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
       if constexpr (__is_same(T, half_t)) {
 #pragma unroll
-        for (int j = 0; j < ST; ++j) q[t][j] = live ? *(const half8*)(qp + 8 * j) : half8{};
+        for (int j = 0; j < ST; ++j) q[t][j] = live ? *(const half8*)(qp + 8 * j) * sign : half8{};
       } else {
         float x[ST][8], mx = 0.f;
 #pragma unroll
@@ -502,18 +511,27 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
 #pragma unroll
         for (int j = 0; j < ST; ++j)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q[t][j][e] = (half_t)ldexpf(x[j][e], -ex);
+          for (int e = 0; e < 8; ++e) q[t][j][e] = (half_t)ldexpf(x[j][e], -ex) * sign;
         sc[t] = ldexpf(scale2, ex);
       }
     }
 
-    for (int tile = first + wave; tile < last; tile += 4) {
-      if (tile * kPage >= lim_max) break;
-      const int page = page_of(a, b, tile * kPage);
-      if (page < 0) continue;         // keys of no page: not seen
-      PageRegs<D> pg;
-      pg.load(head_of<D>(a, page, g), lane);
-      const int left = lim_max - tile * kPage;
+    const int stop = min(last, (lim_max + kPage - 1) / kPage);
+    if (first + wave < stop) {
+    PageRegs<D> pg;
+    // pages of the wave's tile, of its next one and (on its way) the one after:
+    // the last tile's again where there is none, page 0 where there is no page
+    const auto page_near = [&](int tile) { return page_of(a, b, min(tile, stop - 1) * kPage); };
+    int page = page_near(first + wave), ahead = page_near(first + wave + WAVES);
+    pg.load_k(head_of<D>(a, max(page, 0), g), lane);
+    pg.load_v(head_of<D>(a, max(page, 0), g), lane);
+    for (int tile = first + wave; tile < stop; tile += WAVES) {
+      const int lim_page = page < 0 ? 0 : lim_max;   // keys of no page are not seen
+      const bool none = page < 0;
+      const uint8_t* next = head_of<D>(a, max(ahead, 0), g);
+      page = ahead;
+      ahead = page_near(tile + 2 * WAVES);
+      const int left = lim_page - tile * kPage;
       if (left < kPage) {
         // tokens behind the last key: whatever their bytes are, their V is finite
 #pragma unroll
@@ -545,36 +563,44 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
           for (int t = 0; t < NQ; ++t) S[t][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[t][j], S[t][sub], 0, 0, 0);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);  // K's registers are free from here on
+      pg.load_k(next, lane);
       half8 P[NQ][2];
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
-        const bool masked = (tile + 1) * kPage > lim_min;  // or a row of the tile has no tokens
+        if (none || (tile + 1) * kPage > lim_min) {
+          const int seen = none ? 0 : lim[t];
+#pragma unroll
+          for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              S[t][sub][i] = tile * kPage + 16 * sub + 4 * kq + i < seen ? S[t][sub][i] : -INFINITY;
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v = S[t][sub][i] * sc[t];
-            if (masked) v = tile * kPage + 16 * sub + 4 * kq + i < lim[t] ? v : -INFINITY;
-            S[t][sub][i] = v;
-            mx = fmaxf(mx, v);
-          }
-        mx = fmaxf(m[t], across_quarters_max(mx));
-        const float base = mx == -INFINITY ? 0.f : mx;
-        const float alpha = exp2f(m[t] - base);
-        m[t] = mx;
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, S[t][sub][i]);
+        mx = across_quarters_max(mx) * sc[t];
+        if (__builtin_amdgcn_ballot_w64(mx > m[t] + 8.f)) {
+          const float to = fmaxf(m[t], mx);
+          const float alpha = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.f : to));
+          m[t] = to;
+          l[t] *= alpha;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[t][n] *= alpha;
+        }
+        const float base = m[t] == -INFINITY ? 0.f : m[t];
         float sum = 0.f;
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float p = exp2f(S[t][sub][i] - base);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][sub][i], sc[t], -base));
             sum += p;
             P[t][sub >> 1][(sub & 1) * 4 + i] = (half_t)p;
           }
-        l[t] = l[t] * alpha + sum;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[t][n] *= alpha;
+        l[t] += sum;
       }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2)
@@ -591,9 +617,12 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
             for (int t = 0; t < NQ; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, P[t][s2], acc[t][n], 0, 0, 0);
           }
         }
+      __builtin_amdgcn_sched_barrier(0);
+      pg.load_v(next, lane);
+    }
     }
 
-    // join the four waves
+    // join the waves
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
@@ -606,16 +635,18 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
       for (int n = 0; n < NT; ++n) *(float4v*)&sh_acc[wave][16 * t + col][16 * n + 4 * kq] = acc[t][n];
     }
     __syncthreads();
-    for (int u = tid; u < 16 * NQ * (D / 8); u += 256) {
+    for (int u = tid; u < 16 * NQ * (D / 8); u += 64 * WAVES) {
       const int rr = u / (D / 8), ch = (u % (D / 8)) * 8;
       const int r = rt * 16 * NQ + rr;
       if (r >= n_rows) continue;
       const int i = r / group, h = g * group + r % group;
-      const float M = fmaxf(fmaxf(sh_m[0][rr], sh_m[1][rr]), fmaxf(sh_m[2][rr], sh_m[3][rr]));
+      float M = sh_m[0][rr];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) M = fmaxf(M, sh_m[v][rr]);
       const float base = M == -INFINITY ? 0.f : M;
       float x[8] = {}, lt = 0.f;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
+      for (int v = 0; v < WAVES; ++v) {
         const float f = exp2f(sh_m[v][rr] - base);
         lt += f * sh_l[v][rr];
 #pragma unroll
@@ -647,8 +678,6 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
 // and the one after it is on its way from memory), and read from there as
 // 32x32x16 operands.  Rows of 16-byte chunks, chunk ^ row: 8 lanes that read or
 // write one chunk of 8 rows use every bank once.
-// The maximum a row's weights refer to moves only where a score exceeds it by
-// 2^8 (weights stay below fp16's range by far): most pages rescale nothing.
 template <int D>
 struct TileRegs {  // a thread's part of a page
   uint4 k, v, vs;
@@ -1015,9 +1044,13 @@ int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens
   return n <= 1 ? 1 : (int)(((int64_t)n + 30) / 32 + 1);
 }
 
-// Row tiles and splits of an attention call.  Enough workgroups to fill 256
-// CUs four times over (a split takes 4 tiles at least), and at most 32 tiles
-// (2,048 tokens) a split, so that a batch of uneven lengths ends together.
+// Row tiles and splits of an attention call.  Workgroups for two a CU (a split
+// takes 4 tiles at least), and at most 64 tiles (4,096 tokens) a split of few
+// rows, so that a batch of uneven lengths ends together.  Measured (graph
+// replays, us; head_dim 128, 32 on 8 heads): 1 x 32K with 256 / 512 / 768
+// workgroups 15.5 / 15.3 / 17.0, 8 sequences of 2K to 8K 20.9 / 17.3 / 18.5;
+// 16 x 16K with 32 / 64 / 128 tiles at most 64.8 / 60.2 / 60.0, 64 sequences
+// of 128 to 8,192 tokens (head_dim 64) 27.3 / 26.9 / 36.3.
 struct AttnPlan {
   int nq;         // 16-row groups of a workgroup: 1 or 2 (rows), 8 (tile)
   int row_tiles, n_splits;
@@ -1033,9 +1066,8 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t tiles = (len + kPage - 1) / kPage;
   const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
-  const int64_t fill = p.nq == 8 ? 512 : 1024;
-  int64_t sp = (fill + wg - 1) / wg;
-  const int64_t even = (tiles + 31) / 32;
+  int64_t sp = (512 + wg - 1) / wg;
+  const int64_t even = (tiles + 63) / 64;
   if (rows <= 32 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;

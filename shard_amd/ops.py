@@ -948,12 +948,6 @@ KV4_PAGE = 64  # SHARD_KV4_PAGE: tokens of a page
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the call runs on {dev}")
-
-
 def kv4_cache(n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
     """Empty pages, (n_pages, n_kv_heads, 68 * head_dim) uint8: 64 tokens a page,
     4.25 bits an element.  head_dim 64 or 128."""
@@ -963,55 +957,76 @@ def kv4_cache(n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> to
     return torch.zeros(n_pages, n_kv_heads, 68 * head_dim, dtype=torch.uint8, device=device)
 
 
-def _kv4_args(cache, block_table, seq_lens, n_tokens, cu_seqlens, max_new, max_len=None) -> _lib.KV4Args:
-    """The batch's part of a call's argument block, checked."""
-    _require_gpu(cache, block_table, seq_lens, cu_seqlens)
-    dev = cache.device
-    _same_device(dev, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens)
+def _kv4_refuse(cache, block_table, seq_lens, n_tokens, cu_seqlens, **operands):
+    """Say what is wrong with a call whose quick checks failed."""
+    _require_gpu(cache, block_table, seq_lens, cu_seqlens, *operands.values())
+    for name, t in dict(block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens, **operands).items():
+        if t is not None and t.device != cache.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
     if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[2] not in (68 * 64, 68 * 128):
         raise TypeError("cache: expected the (pages, kv heads, 68 * head_dim) uint8 of kv4_cache")
-    n_pages, G, width = cache.shape
-    if cache.stride(2) != 1 or (G > 1 and cache.stride(1) != width):
-        raise ValueError("cache: the bytes of a page must be contiguous")
-    page_stride = cache.stride(0) if n_pages > 1 else G * width
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 and block_table.shape[1] > 1:
-        raise TypeError("block_table: expected (batch, pages a sequence) int32 with contiguous rows")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise TypeError("block_table: expected (batch, pages a sequence) int32")
     B, W = block_table.shape
     if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,) or not seq_lens.is_contiguous():
         raise TypeError(f"seq_lens: expected ({B},) contiguous int32")
-    if cu_seqlens is None:
-        if n_tokens != B:
-            raise ValueError(f"{n_tokens} tokens for {B} sequences: more than one each needs cu_seqlens")
-    elif cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (B + 1,) or not cu_seqlens.is_contiguous():
+    if cu_seqlens is not None and (cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (B + 1,)
+                                   or not cu_seqlens.is_contiguous()):
         raise TypeError(f"cu_seqlens: expected ({B + 1},) contiguous int32")
-    if page_stride < G * width or W == 0 or n_pages == 0 or G == 0:
-        raise ValueError("cache and block_table must hold pages, and pages must not overlap")
-    a = _lib.KV4Args()
-    a.batch, a.n_tokens, a.n_kv_heads, a.head_dim = B, n_tokens, G, width // 68
-    a.n_pages, a.table_width = n_pages, W
-    a.max_new, a.max_len = max_new or 0, max_len or 0
-    a.cache, a.page_stride = cache.data_ptr(), page_stride
-    a.block_table, a.table_stride = block_table.data_ptr(), block_table.stride(0) if B > 1 else W
-    a.seq_lens = seq_lens.data_ptr()
-    a.cu_seqlens = None if cu_seqlens is None else cu_seqlens.data_ptr()
-    return a
+    if cu_seqlens is None and n_tokens != B:
+        raise ValueError(f"{n_tokens} tokens for {B} sequences: more than one each needs cu_seqlens")
+    raise ValueError("the cache and the block table must hold pages, a page's bytes and a table's rows be "
+                     "contiguous and pages not overlap")
 
 
-def _kv4_rows(t, name, a, heads=None):
+def _kv4_batch(cache, block_table, seq_lens, n_tokens, cu_seqlens, max_new, max_len, *operands):
+    """The batch's part of an argument block, checked: (device, kv heads,
+    head_dim, fields of shard_kv4_args from n_pages to cu_seqlens)."""
+    dev = cache.get_device()
+    ok = dev >= 0 and block_table.get_device() == dev and seq_lens.get_device() == dev
+    for t in operands:
+        ok = ok and (t is None or t.get_device() == dev)
+    if cu_seqlens is not None:
+        ok = (ok and cu_seqlens.get_device() == dev and cu_seqlens.dtype is torch.int32
+              and cu_seqlens.shape == (block_table.shape[0] + 1,) and cu_seqlens.is_contiguous())
+    shape, table = cache.shape, block_table.shape
+    if (not ok or len(shape) != 3 or len(table) != 2 or shape[2] not in (68 * 64, 68 * 128)
+            or cache.dtype is not torch.uint8 or block_table.dtype is not torch.int32
+            or seq_lens.dtype is not torch.int32 or seq_lens.shape != table[:1] or not seq_lens.is_contiguous()
+            or (cu_seqlens is None and n_tokens != table[0])):
+        return None
+    n_pages, G, width = shape
+    B, W = table
+    s0, s1, s2 = cache.stride()
+    t0, t1 = block_table.stride()
+    if s2 != 1 or (s1 != width and G > 1) or (t1 != 1 and W > 1):
+        return None
+    if n_pages == 1:
+        s0 = G * width
+    if B == 1:
+        t0 = W
+    if not n_pages or not G or not W or s0 < G * width or t0 < W:
+        return None
+    return dev, G, width // 68, (n_pages, W, max_new or 0, max_len or 0, cache.data_ptr(), s0, block_table.data_ptr(), t0,
+                                 seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr())
+
+
+def _kv4_rows(t, name, n_tokens, heads, D):
     """A (tokens, heads, head_dim) operand as the kernels take it: rows of a
     head contiguous, strides multiples of 8 and 16-byte aligned (copied where
-    it is not), with its strides."""
-    if t.dim() != 3 or t.shape[0] != a.n_tokens or t.shape[2] != a.head_dim or heads not in (None, t.shape[1]):
-        raise ValueError(f"{name}: expected ({a.n_tokens}, {heads or 'heads'}, {a.head_dim}), got {tuple(t.shape)}")
+    it is not), with its address and strides."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != n_tokens or shape[2] != D or shape[1] != (heads or shape[1]):
+        raise ValueError(f"{name}: expected ({n_tokens}, {heads or 'heads'}, {D}), got {tuple(shape)}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s0 | s1) & 7 or t.data_ptr() & 15:
+    p = t.data_ptr()
+    if s2 != 1 or (s0 | s1) & 7 or p & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:  # contiguous at an odd place of its storage
             t = t.clone()
-        s0, s1, s2 = t.stride()
-        if (s0 | s1) & 7:      # strides of dimensions of size 1
-            s0, s1 = t.shape[1] * a.head_dim, a.head_dim
-    return t, s0, s1
+        s0, s1 = shape[1] * D, D
+        p = t.data_ptr()
+    return t, p, s0, s1
 
 
 def _half_type(t, name):
@@ -1021,13 +1036,18 @@ def _half_type(t, name):
     return code
 
 
-def _kv4_launch(fn, name, a, t, *more):
-    """fn on t's device and its current stream."""
-    if torch.cuda.current_device() == t.get_device():
-        _lib.check(name, fn(ctypes.byref(a), *more, _stream(t)))
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _launch_on(dev, name, fn, *args):
+    """fn(*args, stream) with dev the current device, on its current stream."""
+    if _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
     else:
-        with torch.cuda.device(t.device):
-            _lib.check(name, fn(ctypes.byref(a), *more, _stream(t)))
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(name, rc)
 
 
 def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=None, max_new=None):
@@ -1044,30 +1064,30 @@ def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=No
     are left out; rows behind the last sequence's are not read, and their
     rotated q not written.  Two sequences of one call must not append to the
     same page."""
-    _require_gpu(k, v, phases, q)
-    lib = _lib.load()
-    a = _kv4_args(cache, block_table, seq_lens, k.shape[0], cu_seqlens, max_new)
-    _same_device(cache.device, k=k, v=v, phases=phases, q=q)
-    a.dtype = _half_type(k, "k")
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    lib, T = _lib.load(), k.shape[0]
+    batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, 0, k, v, phases, q)
+    if batch is None:
+        _kv4_refuse(cache, block_table, seq_lens, T, cu_seqlens, k=k, v=v, phases=phases, q=q)
+    dev, G, D, fields = batch
+    code = _half_type(k, "k")
+    if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
         raise TypeError("q, k and v must have one type")
-    if (phases.dtype != torch.float32 or phases.dim() != 3 or tuple(phases.shape[1:]) != (a.head_dim // 2, 2)
+    if (phases.dtype is not torch.float32 or phases.dim() != 3 or phases.shape[1:] != (D // 2, 2)
             or not phases.is_contiguous() or phases.data_ptr() & 15):
-        raise TypeError(f"phases: expected (positions, {a.head_dim // 2}, 2) contiguous float32, 16-byte aligned")
-    if phases.shape[0] < KV4_PAGE * a.table_width:
-        raise ValueError(f"phases cover {phases.shape[0]} positions, the block table {KV4_PAGE * a.table_width}")
-    k, a.k_stride, a.k_head_stride = _kv4_rows(k, "k", a, a.n_kv_heads)
-    v, a.v_stride, a.v_head_stride = _kv4_rows(v, "v", a, a.n_kv_heads)
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.phases, a.n_phases = phases.data_ptr(), phases.shape[0]
-    q_out = None
+        raise TypeError(f"phases: expected (positions, {D // 2}, 2) contiguous float32, 16-byte aligned")
+    if phases.shape[0] < KV4_PAGE * fields[1]:
+        raise ValueError(f"phases cover {phases.shape[0]} positions, the block table {KV4_PAGE * fields[1]}")
+    k, *k_at = _kv4_rows(k, "k", T, G, D)
+    v, *v_at = _kv4_rows(v, "v", T, G, D)
+    H, q_at, q_out = 0, (0, 0, 0), None
     if q is not None:
-        q, a.q_stride, a.q_head_stride = _kv4_rows(q, "q", a)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        a.n_q_heads = q.shape[1]
-        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
-    if a.n_tokens:
-        _kv4_launch(lib.shard_kv4_append, "shard_kv4_append", a, cache)
+        q, *q_at = _kv4_rows(q, "q", T, None, D)
+        H = q.shape[1]
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if T:
+        args = _lib.KV4_PACK.pack(block_table.shape[0], T, H, G, D, code, *fields, *q_at, *k_at, *v_at,
+                                  phases.data_ptr(), phases.shape[0], 0.0, 0 if q is None else q_out.data_ptr(), 0, 0, 0)
+        _launch_on(dev, "shard_kv4_append", lib.shard_kv4_append, args)
     return q_out
 
 
@@ -1077,16 +1097,19 @@ def kv4_read(cache, block_table, seq_lens, n_tokens, dtype=torch.float16, cu_seq
     cu_seqlens reads whole sequences).  Exact in fp16; bf16 is exact too.  Rows
     of tokens that the table or the cache does not hold are zeros; rows behind
     the last sequence's are not written."""
-    lib = _lib.load()
-    a = _kv4_args(cache, block_table, seq_lens, int(n_tokens), cu_seqlens, max_new)
-    if dtype not in (torch.float16, torch.bfloat16):
+    lib, T = _lib.load(), int(n_tokens)
+    batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, 0)
+    if batch is None:
+        _kv4_refuse(cache, block_table, seq_lens, T, cu_seqlens)
+    dev, G, D, fields = batch
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError(f"dtype: expected float16 or bfloat16, got {dtype}")
-    a.dtype = _DTYPES[dtype]
-    k = torch.empty(a.n_tokens, a.n_kv_heads, a.head_dim, dtype=dtype, device=cache.device)
+    k = torch.empty(T, G, D, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
-    a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
-    if a.n_tokens:
-        _kv4_launch(lib.shard_kv4_read, "shard_kv4_read", a, cache)
+    if T:
+        args = _lib.KV4_PACK.pack(block_table.shape[0], T, 0, G, D, _DTYPES[dtype], *fields, *(0,) * 9,
+                                  0, 0, 0.0, 0, k.data_ptr(), v.data_ptr(), 0)
+        _launch_on(dev, "shard_kv4_read", lib.shard_kv4_read, args)
     return k, v
 
 
@@ -1101,27 +1124,26 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
     rows behind the last sequence's are not written.  max_new and max_len, the
     most new tokens and tokens of a sequence, size the launch where the caller
     knows them (a captured graph must be given what its replays reach)."""
-    _require_gpu(q)
-    lib = _lib.load()
-    a = _kv4_args(cache, block_table, seq_lens, q.shape[0], cu_seqlens, max_new, max_len)
-    _same_device(cache.device, q=q, out=out)
-    a.dtype = _half_type(q, "q")
-    q, a.q_stride, a.q_head_stride = _kv4_rows(q, "q", a)
-    a.n_q_heads = H = q.shape[1]
-    if H == 0 or H % a.n_kv_heads:
-        raise ValueError(f"{H} query heads do not divide among {a.n_kv_heads} kv heads")
-    a.q = q.data_ptr()
-    a.scale = a.head_dim ** -0.5 if scale is None else float(scale)
+    lib, T = _lib.load(), q.shape[0]
+    batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, max_len, q, out)
+    if batch is None:
+        _kv4_refuse(cache, block_table, seq_lens, T, cu_seqlens, q=q, out=out)
+    dev, G, D, fields = batch
+    code = _half_type(q, "q")
+    q, *q_at = _kv4_rows(q, "q", T, None, D)
+    H = q.shape[1]
+    if H == 0 or H % G:
+        raise ValueError(f"{H} query heads do not divide among {G} kv heads")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
         raise TypeError(f"out: expected {tuple(q.shape)} contiguous {q.dtype}, 16-byte aligned")
-    a.out = out.data_ptr()
-    if a.n_tokens == 0:
-        return out
-    need = lib.shard_kv4_attn_workspace(ctypes.byref(a))
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _kv4_launch(lib.shard_kv4_attn, "shard_kv4_attn", a, cache, None if ws is None else ws.data_ptr(), need)
+    if T:
+        args = _lib.KV4_PACK.pack(block_table.shape[0], T, H, G, D, code, *fields, *q_at, *(0,) * 6, 0, 0,
+                                  D ** -0.5 if scale is None else scale, 0, 0, 0, out.data_ptr())
+        need = lib.shard_kv4_attn_workspace(args)
+        ws = cache.new_empty(need) if need else None
+        _launch_on(dev, "shard_kv4_attn", lib.shard_kv4_attn, args, ws.data_ptr() if need else None, need)
     return out
 
 
@@ -1140,33 +1162,38 @@ def token_logprobs(logits, tokens=None, top=0):
     most probable tokens, equal ones by index (top up to 64).  A row without a
     logit above -inf, or with +inf or NaN, has NaN log probabilities; NaN
     logits are never among the top (id -1 where a row has too few others)."""
-    _require_gpu(logits, tokens)
-    lib = _lib.load()
-    if logits.dtype not in _DTYPES:
+    lib, dev = _lib.load(), logits.get_device()
+    if dev < 0 or (tokens is not None and tokens.get_device() != dev):
+        _require_gpu(logits, tokens)
+        raise ValueError(f"tokens are on {tokens.device}, the logits on {logits.device}")
+    code = _DTYPES.get(logits.dtype)
+    if code is None:
         raise TypeError(f"logits: expected float16, bfloat16 or float32, got {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[-1] == 0:
+    shape = logits.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("logits: expected (..., vocabulary)")
-    lead, V = logits.shape[:-1], logits.shape[-1]
+    lead, V = shape[:-1], shape[-1]
     if not 0 <= top <= min(TOP_LOGPROBS_MAX, V):
         raise ValueError(f"top: 0 .. {min(TOP_LOGPROBS_MAX, V)}, got {top}")
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.stride(1) != 1 and V > 1 or x.stride(0) < 0:
-        x = x.contiguous()
-    n, dev = x.shape[0], x.device
     if tokens is not None:
-        if tokens.dtype != torch.int64 or tokens.shape != lead:
+        if tokens.dtype is not torch.int64 or tokens.shape != lead:
             raise TypeError(f"tokens: expected {tuple(lead)} int64, got {tuple(tokens.shape)} {tokens.dtype}")
-        _same_device(dev, tokens=tokens)
         tokens = tokens.contiguous()
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
-    top_lp = torch.empty(*lead, top, dtype=torch.float32, device=dev)
-    top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+    x = logits if len(shape) == 2 else logits.reshape(-1, V)
+    stride = x.stride(0)
+    if x.stride(1) != 1 and V > 1:
+        x = x.contiguous()
+        stride = V
+    n = x.shape[0]
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    entropy = torch.empty(lead, **f32)
+    logprob = None if tokens is None else torch.empty_like(entropy)
+    top_lp = torch.empty(*lead, top, **f32)
+    top_ids = torch.empty_like(top_lp, dtype=torch.int64)
     if n:
         need = lib.shard_token_logprobs_workspace(n, V, top)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        with torch.cuda.device(dev):
-            _lib.check("shard_token_logprobs", lib.shard_token_logprobs(
-                x.data_ptr(), _DTYPES[x.dtype], n, V, x.stride(0), _p(tokens), top, _p(logprob), _p(entropy),
-                _p(top_lp), _p(top_ids), _p(ws), need, _stream(x)))
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        _launch_on(dev, "shard_token_logprobs", lib.shard_token_logprobs, x.data_ptr(), code, n, V, stride,
+                   None if tokens is None else tokens.data_ptr(), top, None if tokens is None else logprob.data_ptr(),
+                   entropy.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(), ws.data_ptr() if need else None, need)
     return logprob, entropy, top_lp, top_ids
