@@ -672,68 +672,91 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   }
 }
 
-// Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and walks a
-// split of the pages.  A page is dequantized once for all of them into LDS
-// (fp16, two buffers: the next page is written while this one is multiplied,
-// and the one after it is on its way from memory), and read from there as
-// 32x32x16 operands.  Rows of 16-byte chunks, chunk ^ row: 8 lanes that read or
-// write one chunk of 8 rows use every bank once.
+// Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and walks a split
+// of the pages.  A page is dequantized once for all of them into LDS (fp16, two
+// buffers) and read from there as 32x32x16 operands.  Rows are 16 bytes longer
+// than their data: 8 lanes that read or write one 16-byte chunk of 8 rows use
+// every bank once, and every read is an immediate offset from one address.
+//
+// A wave alternates two phases with a barrier after each: vector (the softmax of
+// page n; V of page n + 1 and K of page n + 2 into LDS, from registers that were
+// loaded a page earlier) and matrix (the output's product with V of page n, the
+// scores of page n + 1).  The second workgroup of a CU runs one while the first
+// runs the other.
+//
+// Measured: a whole prompt of 8,192 tokens, 32 heads on 8, 560 us, 0.98 PFLOP/s
+// of its causal half; an 8192^3 fp16 product of the library reaches 1.17 on the
+// same card.  The clock falls to 1.85 GHz under it; at that clock the matrix pipe
+// is busy half the time.  Not faster: 256 rows in two groups of waves a phase
+// apart (568), 64 rows a wave (1,073: registers), scores of the next page
+// between the maxima and the weights of this one (570).
+// Byte offsets are formed once: the loop adds a page's address and a buffer's.
+template <int W>
+struct Words {
+  uint32_t w[W];
+};
 template <int D>
-struct TileRegs {  // a thread's part of a page
-  uint4 k, v, vs;
-  uint32_t ks;
-  __device__ __forceinline__ void load(const uint8_t* base, int tid) {
-    const int lane = tid & 63;
-    ks = base[k_scale_at<D>((tid >> 6) * 16 + (lane & 15), D == 128 ? lane >> 4 : lane >> 5)];
-    if constexpr (D == 128) {
-      k = *((const uint4*)base + tid);
-      v = *((const uint4*)(base + 34 * D) + tid);
-      vs = *(const uint4*)(base + 66 * D + ((lane >> 4) * 2 + (tid >> 7)) * 32 + ((tid >> 6) & 1) * 16);
-    } else {
-      const uint2 a = *(const uint2*)(base + k_code_at<D>((tid >> 6) * 16 + (lane & 15), lane >> 4));
-      const uint2 c = *(const uint2*)(base + 34 * D + ((tid >> 7) * 64 + lane) * 16 + ((tid >> 6) & 1) * 8);
-      const uint2 e = *(const uint2*)(base + 66 * D + ((lane >> 4) * 2 + (tid >> 7)) * 16 + ((tid >> 6) & 1) * 8);
-      k = make_uint4(a.x, a.y, 0, 0);
-      v = make_uint4(c.x, c.y, 0, 0);
-      vs = make_uint4(e.x, e.y, 0, 0);
-    }
+struct KRegs {  // a thread's part of a page's K: a quarter of a token
+  static constexpr int W = D / 32;
+  static constexpr int kRow = 2 * D + 16, kBuffer = kPage * kRow;
+  Words<W> k;
+  uint32_t s;
+  uint32_t from, s_from, to;
+  __device__ __forceinline__ KRegs(int tid) {
+    const int kq = (tid & 63) >> 4, slot = (tid >> 6) * 16 + (tid & 15);
+    from = k_code_at<D>(slot, kq);
+    s_from = k_scale_at<D>(slot, D == 128 ? kq : kq >> 1);
+    to = slot * kRow + kq * W * 16;
   }
-  // Into sk[token][chunk of 8 channels], sv[channel][chunk of 8 tokens, in the
-  // order that a lane's weights have: runs of four 0 2 | 1 3 of each 16].
-  // Tokens from `left` on get V = 0, whatever their bytes are.
-  __device__ __forceinline__ void store(half8* sk, half8* sv, int tid, int left) {
-    const int lane = tid & 63, r = lane & 15, kq = lane >> 4;
-    {
-      const int tok = (tid >> 6) * 16 + r;
-      const half2v s = scale_pair(ks, 0, 0);
+  __device__ __forceinline__ void load(const uint8_t* base) {
+    s = base[s_from];
+    __builtin_memcpy(&k, __builtin_assume_aligned(base + from, 4 * W), 4 * W);
+  }
+  // rows [token][channel]
+  __device__ __forceinline__ void store(char* buffer) const {
+    const half2v sc = scale_pair(s, 0, 0);
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const int chunk = kq * (D / 32) + j;
-        sk[tok * (D / 8) + (chunk ^ (tok & (D / 8 - 1)))] = dequant(word(k, j), s, s, s, s);
-      }
-    }
-    const int sg = tid >> 7, x = (tid >> 6) & 1;
+    for (int j = 0; j < W; ++j) *(half8*)(buffer + to + 16 * j) = dequant(k.w[j], sc, sc, sc, sc);
+  }
+};
+
+template <int D>
+struct VRegs {  // a thread's part of a page's V: W channels 16 apart of 8 tokens
+  static constexpr int W = D / 32;
+  static constexpr int B = D / 64;  // blocks of 32 channels among them
+  static constexpr int kRow = 2 * kPage + 16, kBuffer = D * kRow;
+  Words<W> v;
+  Words<2 * B> s;
+  uint32_t from, s_from, to;
+  int t0;                           // first of its tokens
+  __device__ __forceinline__ VRegs(int tid) {
+    const int lane = tid & 63, kq = lane >> 4, sg = tid >> 7, x = (tid >> 6) & 1;
+    from = 34 * D + (D == 128 ? ((sg * 2 + x) * 64 + lane) * 16 : (sg * 64 + lane) * 16 + x * 8);
+    s_from = 66 * D + ((kq * 2 + sg) * (D / 32) + x * B) * 8;
+    to = (x * (D / 2) + (lane & 15)) * kRow + (4 * sg + kq) * 16;
+    t0 = 32 * sg + 4 * kq;
+  }
+  __device__ __forceinline__ void load(const uint8_t* base) {
+    __builtin_memcpy(&v, __builtin_assume_aligned(base + from, 4 * W), 4 * W);
+    __builtin_memcpy(&s, __builtin_assume_aligned(base + s_from, 8 * B), 8 * B);
+  }
+  // rows [channel][word: 8 tokens in the order of its codes].  Tokens from
+  // `left` on get V = 0, whatever their bytes are.
+  __device__ __forceinline__ void store(char* buffer, int left) {
     if (left < kPage) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {  // words: 4 tokens each, runs alternate
-        const int live = min(max(left - (32 * sg + 16 * (i & 1) + 4 * kq), 0), 4);
-        const uint32_t msk = live == 4 ? ~0u : (1u << (8 * live)) - 1u;
-        if (i == 0) vs.x &= msk;
-        if (i == 1) vs.y &= msk;
-        if (i == 2) vs.z &= msk;
-        if (i == 3) vs.w &= msk;
+      for (int run = 0; run < 2; ++run) {
+        const int n = min(max(left - (t0 + 16 * run), 0), 4);
+        const uint32_t m = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+#pragma unroll
+        for (int k = 0; k < B; ++k) s.w[2 * k + run] &= m;
       }
     }
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const uint32_t w0 = word(vs, D == 128 ? (j >> 1) * 2 : 0), w1 = word(vs, D == 128 ? (j >> 1) * 2 + 1 : 1);
-      const int ch = D == 128 ? 64 * x + 16 * j + r : 32 * x + 16 * j + r;
-      const half8 f = dequant(word(v, j), scale_pair(w0, 0, 1), scale_pair(w0, 2, 3), scale_pair(w1, 0, 1), scale_pair(w1, 2, 3));
-      typedef half_t half4 __attribute__((ext_vector_type(4)));
-      half4* row = (half4*)(sv + ch * 8);
-      const int c0 = 4 * sg + (kq & 1);
-      row[(c0 ^ (ch & 7)) * 2 + (kq >> 1)] = half4{f[0], f[1], f[2], f[3]};
-      row[((c0 + 2) ^ (ch & 7)) * 2 + (kq >> 1)] = half4{f[4], f[5], f[6], f[7]};
+    for (int j = 0; j < W; ++j) {
+      const uint32_t w0 = s.w[(j >> 1) * 2], w1 = s.w[(j >> 1) * 2 + 1];
+      *(half8*)(buffer + to + 16 * j * kRow) =
+          dequant(v.w[j], scale_pair(w0, 0, 1), scale_pair(w0, 2, 3), scale_pair(w1, 0, 1), scale_pair(w1, 2, 3));
     }
   }
 };
@@ -743,9 +766,11 @@ constexpr int kTileRows = 128;
 template <class T, int D>
 __global__ __launch_bounds__(256, 2)
 void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
-  constexpr int QS = D / 16;  // k-steps of a score
-  constexpr int CT = D / 32;  // channel tiles of the output
-  __shared__ half8 sk[2][kPage * (D / 8)], sv[2][D * 8];
+  constexpr int QS = D / 16;        // k-steps of a score
+  constexpr int CT = D / 32;        // channel tiles of the output
+  typedef KRegs<D> K;
+  typedef VRegs<D> V;
+  __shared__ __align__(16) char sk[2 * K::kBuffer], sv[2 * V::kBuffer];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hi = lane >> 5;
   // kv heads innermost: with 8 of them each has an XCD (workgroup id mod 8) and
@@ -762,104 +787,101 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   const int first = split * per, end = min(first + per, tiles);
   if (w.n_splits > 1 && first >= tiles) return;
   const int n_tiles = (n_rows + kTileRows - 1) / kTileRows;
+  const auto limit = [&](int row) { return min(max(s.len - s.n + row / group + 1, 0), keys); };
 
   for (int back = unit / w.n_splits; back < n_tiles; back += w.row_tiles) {
     const int rt = n_tiles - 1 - back;
-    const int r0 = rt * kTileRows + wave * 32;             // the wave's first row
+    const int r0 = rt * kTileRows + wave * 32;                  // the wave's first row
+    const int last = min(end, (limit(min(rt * kTileRows + kTileRows, n_rows) - 1) + kPage - 1) / kPage);
+    // keys that every row of the wave sees: pages below need no mask
+    const int lim_min = r0 + 32 <= n_rows ? limit(r0) : 0;
     const int r = r0 + col;
     const bool live = r < n_rows;
-    const int i = live ? r / group : 0, h = live ? r - i * group : 0;
-    const int lim = live ? min(max(s.len - s.n + i + 1, 0), keys) : 0;
-    const int r_last = min(r0 + 31, n_rows - 1), t_last = min(rt * kTileRows + kTileRows, n_rows) - 1;
-    const int lim_min = r0 + 31 < n_rows ? min(max(s.len - s.n + r0 / group + 1, 0), keys) : 0;
-    const int lim_max = r0 < n_rows ? min(max(s.len - s.n + r_last / group + 1, 0), keys) : 0;
-    const int lim_all = min(max(s.len - s.n + t_last / group + 1, 0), keys);
-    const int last = min(end, (lim_all + kPage - 1) / kPage);
-
+    const int i = live ? r / group : 0, h = g * group + (live ? r - i * group : 0);
+    const int lim = live ? limit(r) : 0;
     half8 q[QS];
-    float sc = fabsf(a.scale) * 1.4426950408889634f;
-    {
-      // the scale's sign goes into q, so that the largest product is the largest score
-      const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-      if (a.scale == 0.f) sc = 1.f;
-      const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + 8 * hi;
-      if constexpr (__is_same(T, half_t)) {
+    // the scale's sign goes into q, so that the largest product is the largest score
+    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+    float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)h * a.q_head_stride + 8 * hi;
+    if constexpr (__is_same(T, half_t)) {
 #pragma unroll
-        for (int j = 0; j < QS; ++j) {
-          q[j] = live ? *(const half8*)(qp + 16 * j) : half8{};
-          q[j] *= (half_t)sign;
-        }
-      } else {
-        float mx = 0.f;
+      for (int j = 0; j < QS; ++j) q[j] = live ? *(const half8*)(qp + 16 * j) * (half_t)sign : half8{};
+    } else {
+      float mx = 0.f;
 #pragma unroll
-        for (int j = 0; j < QS; ++j) {
-          float x[8] = {};
-          if (live) load8(qp + 16 * j, x);
+      for (int j = 0; j < QS; ++j) {
+        float x[8] = {};
+        if (live) load8(qp + 16 * j, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-        }
-        float other, mine;
-        perm32_swap(mx, mine, other);
-        mx = fmaxf(mine, other);
-        const int ex = mx > 0.f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
-#pragma unroll
-        for (int j = 0; j < QS; ++j) {
-          float x[8] = {};
-          if (live) load8(qp + 16 * j, x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) q[j][e] = (half_t)(sign * ldexpf(x[e], -ex));
-        }
-        sc = ldexpf(sc, ex);
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
       }
+      float other, mine;
+      perm32_swap(mx, mine, other);
+      mx = fmaxf(mine, other);
+      const int ex = mx > 0.f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
+#pragma unroll
+      for (int j = 0; j < QS; ++j) {
+        float x[8] = {};
+        if (live) load8(qp + 16 * j, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[j][e] = (half_t)(sign * ldexpf(x[e], -ex));
+      }
+      sc = ldexpf(sc, ex);
     }
     float m = -INFINITY, l = 0.f;
-    float16v acc[CT];
+    float16v acc[CT], S[2];
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+    for (int k = 0; k < CT; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[c][e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc[k][e] = 0.f;
 
-    TileRegs<D> regs;
-    int page = -1, page_next = -1;  // of the tile in regs, of the one after
+    const auto scores = [&](uint32_t buffer) {
+      const char* from = sk + buffer + col * K::kRow + 16 * hi;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < QS; ++j)
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8*)(from + 32 * t * K::kRow + 32 * j), q[j], S[t], 0, 0, 0);
+      }
+    };
+
+    __syncthreads();  // the buffers' readers of the row tile before
     if (first < last) {
-      page = page_of(a, b, first * kPage);
-      if (page >= 0) regs.load(head_of<D>(a, page, g), tid);
-      if (first + 1 < last) page_next = page_of(a, b, (first + 1) * kPage);
-    }
-    __syncthreads();  // the buffers' readers of the tile of rows before
-    bool have = page >= 0, have_next = false;
-    if (have) regs.store(sk[0], sv[0], tid, keys - first * kPage);
-    if (page_next >= 0) regs.load(head_of<D>(a, page_next, g), tid);
-    page = page_next;
-    page_next = first + 2 < last ? page_of(a, b, (first + 2) * kPage) : -1;
-    __syncthreads();
-
-    int cur = 0;
-    for (int tile = first; tile < last; ++tile, cur ^= 1) {
-      have_next = page >= 0;
-      if (have_next) regs.store(sk[cur ^ 1], sv[cur ^ 1], tid, keys - (tile + 1) * kPage);
-      if (page_next >= 0) regs.load(head_of<D>(a, page_next, g), tid);
-      page = page_next;
-      page_next = tile + 3 < last ? page_of(a, b, (tile + 3) * kPage) : -1;
-      if (have && tile * kPage < lim_max) {
-        const half8 *bk = sk[cur], *bv = sv[cur];
-        float16v S[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
-#pragma unroll
-          for (int j = 0; j < QS; ++j) {
-            const int tok = 32 * t + col;
-            S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bk[tok * (D / 8) + ((2 * j + hi) ^ (tok & (D / 8 - 1)))], q[j], S[t], 0, 0, 0);
-          }
-        }
-        if ((tile + 1) * kPage > lim_min) {
+      // pages of tiles n .. n + 3; past the last tile it again, page 0 where there is none
+      const auto page_near = [&](int tile) { return page_of(a, b, min(tile, last - 1) * kPage); };
+      const auto at = [&](int page) { return head_of<D>(a, max(page, 0), g); };
+      const auto left = [&](int page, int tile) { return page < 0 ? 0 : keys - tile * kPage; };
+      int p0 = page_near(first), p1 = page_near(first + 1), p2 = page_near(first + 2), p3 = page_near(first + 3);
+      K kr(tid);
+      V vr(tid);
+      kr.load(at(p0));
+      vr.load(at(p0));
+      kr.store(sk);
+      kr.load(at(p1));
+      vr.store(sv, left(p0, first));
+      vr.load(at(p1));
+      kr.store(sk + K::kBuffer);
+      kr.load(at(p2));
+      __syncthreads();
+      scores(0);
+      __syncthreads();
+      uint32_t k0 = 0, k1 = K::kBuffer, v0 = 0, v1 = V::kBuffer;  // buffers of pages n, n + 1
+      for (int tile = first; tile < last; ++tile) {
+        // vector phase
+        vr.store(sv + v1, left(p1, tile + 1));
+        vr.load(at(p2));
+        kr.store(sk + k0);
+        kr.load(at(p3));
+        if (p0 < 0 || (tile + 1) * kPage > lim_min) {
+          const int seen = p0 < 0 ? 0 : lim;          // keys of no page are not seen
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              S[t][e] = tile * kPage + 32 * t + 8 * (e >> 2) + 4 * hi + (e & 3) < lim ? S[t][e] : -INFINITY;
+              S[t][e] = tile * kPage + 32 * t + 8 * (e >> 2) + 4 * hi + (e & 3) < seen ? S[t][e] : -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -875,9 +897,9 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
           m = to;
           l *= alpha;
 #pragma unroll
-          for (int c = 0; c < CT; ++c)
+          for (int k = 0; k < CT; ++k)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[c][e] *= alpha;
+            for (int e = 0; e < 16; ++e) acc[k][e] *= alpha;
         }
         const float base = m == -INFINITY ? 0.f : m;
         half8 P[4];
@@ -888,45 +910,69 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
           for (int e = 0; e < 16; ++e) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][e], sc, -base));
             sum += p;
-            P[2 * t + (e >> 3)][e & 7] = (half_t)p;
+            P[2 * t + ((e >> 2) & 1)][(e & 3) + 4 * (e >> 3)] = (half_t)p;  // runs of tokens 0 2 | 1 3, as V's words
           }
         l += sum;
+        p0 = p1;
+        p1 = p2;
+        p2 = p3;
+        p3 = page_near(tile + 4);
+        __builtin_amdgcn_sched_barrier(0);            // nothing of a phase moves into the other
+        __syncthreads();
+        // matrix phase; the scores past the last tile are those of it again, unused
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+        const char* from = sv + v0 + col * V::kRow + 16 * hi;
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            const int ch = 32 * c + col;
-            acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bv[ch * 8 + ((2 * st + hi) ^ (ch & 7))], P[st], acc[c], 0, 0, 0);
-          }
+          for (int k = 0; k < CT; ++k)
+            acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8*)(from + 32 * k * V::kRow + 32 * st), P[st], acc[k], 0, 0, 0);
+        scores(k1);
+        // operands six reads ahead of their products
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int k = 0; k < 4 * CT + 2 * QS; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (k < 4 * CT + 2 * QS - 6) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t kt = k0, vt = v0;
+        k0 = k1;
+        k1 = kt;
+        v0 = v1;
+        v1 = vt;
       }
-      have = have_next;
-      __syncthreads();
     }
 
     float other, mine;
     perm32_swap(l, mine, other);
     l = mine + other;
     if (live) {
-      const int64_t row = (int64_t)(s.row0 + i) * a.n_q_heads + g * group + h;
+      const int64_t row = (int64_t)(s.row0 + i) * a.n_q_heads + h;
       if (w.n_splits == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees no key: zeros
         typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int k = 0; k < CT; ++k)
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             vec4 o;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = (T)(acc[c][e + k] * inv);
-            *(vec4*)((T*)a.out + row * D + 32 * c + 2 * e + 4 * hi) = o;
+            for (int x = 0; x < 4; ++x) o[x] = (T)(acc[k][e + x] * inv);
+            *(vec4*)((T*)a.out + row * D + 32 * k + 2 * e + 4 * hi) = o;
           }
       } else {
         const int64_t part = row * w.n_splits + split;
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int k = 0; k < CT; ++k)
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
-            *(float4v*)(w.acc + part * D + 32 * c + 2 * e + 4 * hi) = float4v{acc[c][e], acc[c][e + 1], acc[c][e + 2], acc[c][e + 3]};
+            *(float4v*)(w.acc + part * D + 32 * k + 2 * e + 4 * hi) =
+                float4v{acc[k][e], acc[k][e + 1], acc[k][e + 2], acc[k][e + 3]};
         if (hi == 0) {
           w.m[part] = m;
           w.l[part] = l;
@@ -1050,7 +1096,9 @@ int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens
 // replays, us; head_dim 128, 32 on 8 heads): 1 x 32K with 256 / 512 / 768
 // workgroups 15.5 / 15.3 / 17.0, 8 sequences of 2K to 8K 20.9 / 17.3 / 18.5;
 // 16 x 16K with 32 / 64 / 128 tiles at most 64.8 / 60.2 / 60.0, 64 sequences
-// of 128 to 8,192 tokens (head_dim 64) 27.3 / 26.9 / 36.3.
+// of 128 to 8,192 tokens (head_dim 64) 27.3 / 26.9 / 36.3.  Rows by rows or by
+// tiles: 2 x 8,000 with 12 / 32 new tokens (48 / 128 rows) 20.3 / 27.1 by rows,
+// 26.6 / 33.7 by tiles; 16 x 4,000 with 16 (64 rows) 40.8 / 52.1.
 struct AttnPlan {
   int nq;         // 16-row groups of a workgroup: 1 or 2 (rows), 8 (tile)
   int row_tiles, n_splits;
@@ -1060,7 +1108,7 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   const int group = a->n_q_heads / a->n_kv_heads;
   const int64_t n = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
   const int64_t rows = (a->cu_seqlens ? n : 1) * group;
-  p.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
+  p.nq = rows <= 16 ? 1 : rows <= 128 ? 2 : 8;
   p.row_tiles = (int)((rows + 16 * p.nq - 1) / (16 * p.nq));
   const int64_t cap = (int64_t)a->table_width * kPage;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
@@ -1068,7 +1116,7 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
   int64_t sp = (512 + wg - 1) / wg;
   const int64_t even = (tiles + 63) / 64;
-  if (rows <= 32 && even > sp) sp = even;
+  if (p.nq != 8 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;
   p.n_splits = sp < 1 ? 1 : (int)sp;
@@ -1098,15 +1146,15 @@ using namespace shard;
     }                                                                                                           \
   } while (0)
 
-#define KV4_DISPATCH_N(KERNEL, N, grid, s, ...)                                                                 \
-  do {                                                                                                          \
-    if (a->dtype == SHARD_FP16) {                                                                               \
-      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<half_t, 128, N>), grid, dim3(256), 0, s, __VA_ARGS__); \
-      else hipLaunchKernelGGL((KERNEL<half_t, 64, N>), grid, dim3(256), 0, s, __VA_ARGS__);                     \
-    } else {                                                                                                    \
-      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16_t, 128, N>), grid, dim3(256), 0, s, __VA_ARGS__); \
-      else hipLaunchKernelGGL((KERNEL<bf16_t, 64, N>), grid, dim3(256), 0, s, __VA_ARGS__);                     \
-    }                                                                                                           \
+#define KV4_DISPATCH_N(KERNEL, N, grid, s, ...)                                                              \
+  do {                                                                                                                \
+    if (a->dtype == SHARD_FP16) {                                                                                     \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<half_t, 128, N>), grid, dim3(256), 0, s, __VA_ARGS__);   \
+      else hipLaunchKernelGGL((KERNEL<half_t, 64, N>), grid, dim3(256), 0, s, __VA_ARGS__);                       \
+    } else {                                                                                                          \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16_t, 128, N>), grid, dim3(256), 0, s, __VA_ARGS__);   \
+      else hipLaunchKernelGGL((KERNEL<bf16_t, 64, N>), grid, dim3(256), 0, s, __VA_ARGS__);                       \
+    }                                                                                                                 \
   } while (0)
 
 extern "C" {
@@ -1182,7 +1230,10 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   const dim3 rows_grid((unsigned)(w.n_splits * w.row_tiles), a->n_kv_heads, a->batch);
   if (p.nq == 1) KV4_DISPATCH_N(k_kv4_attn_rows, 1, rows_grid, s, *a, w);
   else if (p.nq == 2) KV4_DISPATCH_N(k_kv4_attn_rows, 2, rows_grid, s, *a, w);
-  else KV4_DISPATCH(k_kv4_attn_tile, dim3((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch), s, *a, w);
+  else {
+    const dim3 grid((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch);
+    KV4_DISPATCH(k_kv4_attn_tile, grid, s, *a, w);
+  }
   SHARD_LAUNCH_CHECK("shard_kv4_attn");
   if (p.n_splits > 1) {
     const int64_t per_seq = (a->cu_seqlens ? (a->max_new > 0 ? a->max_new : a->n_tokens) : 1) * (int64_t)a->n_q_heads;
