@@ -110,9 +110,11 @@ def fused_attention_compressed_full(q_rope, layer, pos_q, inv_freq, attn_mask=No
 def enable_llama_fused_attention(model=None):
     """Patch LlamaAttention.forward process-wide so decode steps (q_len == 1) on a
     compressed shard Cache layer go through the fused HIP kernel; everything else
-    calls the original forward (attention.py:345-414).  Returns False when the
+    calls the original forward (attention.py:345-414).  A step of a PagedCache
+    runs through its own pages, whatever its lengths.  Returns False when the
     transformers Llama module is unavailable."""
     from .cache import Cache
+    from .paged import PagedCache, paged_forward
     try:
         from transformers.models.llama.modeling_llama import LlamaAttention, apply_rotary_pos_emb
     except ImportError:
@@ -123,6 +125,8 @@ def enable_llama_fused_attention(model=None):
 
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None,
                 past_key_values=None, cache_position=None, **kwargs):
+        if isinstance(past_key_values, PagedCache):
+            return paged_forward(self, hidden_states, past_key_values)
         is_shard = isinstance(past_key_values, Cache)
         layer = past_key_values.layers[self.layer_idx] if is_shard else None
         gc = getattr(layer, "_gpu_compressed", None) if layer is not None else None

@@ -24,6 +24,7 @@ weighs the stream both empty and full.
 """
 import torch
 
+from . import ops
 from .attention import _workspaces, fused_supported
 
 
@@ -32,9 +33,15 @@ class DecodeGraph:
     the workspaces), the second one captured and replayed, every later one
     replayed.  `next_ids` (B, 1) int64 on the device are the tokens of the
     first step; each step returns the (B,) greedy tokens it produced, which
-    are also the next step's input unless `step(ids)` supplies other ones."""
+    are also the next step's input unless `step(ids)` supplies other ones.
 
-    def __init__(self, model, cache, next_ids, max_steps):
+    With `top_logprobs` = n (0 .. 64) every step also computes, in the same
+    graph, the log probabilities of its tokens (`logprob`, (B,)), the entropy
+    of its distributions (`entropy`, (B,)) and their n most probable tokens
+    (`top_ids`, `top_logprobs`, (B, n)): fp32 and int64 tensors that hold the
+    last step's values until the next step."""
+
+    def __init__(self, model, cache, next_ids, max_steps, top_logprobs=None):
         from .cache import Cache
         if not isinstance(cache, Cache):
             raise TypeError("DecodeGraph needs a shard Cache")
@@ -52,6 +59,8 @@ class DecodeGraph:
             raise ValueError("next_ids must be (B, 1) on the GPU")
         if max_steps < 1:
             raise ValueError("max_steps must be positive")
+        if top_logprobs is not None and not 0 <= top_logprobs <= min(ops.TOP_LOGPROBS_MAX, model.config.vocab_size):
+            raise ValueError(f"top_logprobs: 0 .. {min(ops.TOP_LOGPROBS_MAX, model.config.vocab_size)}")
         B = next_ids.shape[0]
         n_q = model.config.num_attention_heads
         layers = cache.layers
@@ -84,6 +93,8 @@ class DecodeGraph:
         self.graph = None
         self.next = None
         self.logits = None
+        self._top = top_logprobs
+        self.logprob = self.entropy = self.top_logprobs = self.top_ids = None
         self._pinned = None
         cache._graph = self
 
@@ -92,6 +103,8 @@ class DecodeGraph:
                          past_key_values=self.cache, use_cache=True)
         logits = out.logits[:, -1]
         nxt = logits.argmax(-1)
+        if self._top is not None:
+            self.logprob, self.entropy, self.top_logprobs, self.top_ids = ops.token_logprobs(logits, nxt, top=self._top)
         self.ids.copy_(nxt.view(-1, 1))
         self.rows.add_(1)
         self.pos.add_(1)
