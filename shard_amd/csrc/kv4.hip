@@ -166,10 +166,10 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 constexpr int kHeadsQ = 4;
 
 template <class T, int D>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, 4)
 void k_kv4_append(const shard_kv4_args a) {
   constexpr int PB = D / 64;  // pairs of 32-channel blocks: (pb, pb + PB)
-  __shared__ uint8_t codes[32][D + 4];
+  __shared__ __align__(4) uint8_t codes[32][D + 4];
   const int tid = threadIdx.x, b = blockIdx.z;
   const Seq s = seq_of(a, b);
   if (s.n == 0) return;
@@ -220,16 +220,42 @@ void k_kv4_append(const shard_kv4_args a) {
     const int page = page_of(a, b, t0);
     if (page < 0) continue;
     uint8_t* base = head_of<D>(a, page, g);
-    const int slot = (t0 & 63) + tok;
+    const int slot0 = t0 & 63, slot = slot0 + tok;
+    const auto is_new = [&](int t) { return (unsigned)(t0 + t - start) < (unsigned)s.n && t0 + t < a.n_phases; };
+    // all that the group reads, before anything waits: k, v, and the words of V
+    // codes that earlier tokens share
+    constexpr int VU = D / 64;                        // 8-channel pieces of V a thread, words a thread
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    vec8 kx{}, ky{}, vx[VU];
+    uint32_t old[VU], keep[VU];
     if (there) {
       const T* k = (const T*)a.k + (int64_t)(s.row0 + i) * a.k_stride + (int64_t)g * a.k_head_stride + ch;
-      float x[8], y[8], r[2][8];
-      load8(k, x);
-      load8(k + D / 2, y);
+      kx = *(const vec8*)k;
+      ky = *(const vec8*)(k + D / 2);
+    }
+#pragma unroll
+    for (int n = 0; n < VU; ++n) {
+      const int u = tid + 256 * n, vt = u / (D / 8), vc = (u % (D / 8)) * 8;
+      if (is_new(vt))
+        vx[n] = *(const vec8*)((const T*)a.v + (int64_t)(s.row0 + t0 + vt - start) * a.v_stride + (int64_t)g * a.v_head_stride + vc);
+    }
+#pragma unroll
+    for (int n = 0; n < VU; ++n) {
+      const int u = tid + 256 * n, kq = u / D, vc = u % D;
+      keep[n] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!is_new(16 * (e >> 2) + 4 * kq + (e & 3))) keep[n] |= 15u << (4 * e);
+      old[n] = 0;
+      if (keep[n] != 0 && keep[n] != ~0u) old[n] = *(const uint32_t*)(base + v_word_at<D>(slot0 >> 5, kq, vc));
+    }
+    if (there) {
+      float r[2][8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const double dl = (double)x[j] * c[j] - (double)y[j] * sn[j];
-        const double dh = (double)y[j] * c[j] + (double)x[j] * sn[j];
+        const double x = (double)(float)kx[j], y = (double)(float)ky[j];
+        const double dl = x * c[j] - y * sn[j];
+        const double dh = y * c[j] + x * sn[j];
         r[0][j] = dl == dl ? to_odd(dl) : 0.f;
         r[1][j] = dh == dh ? to_odd(dh) : 0.f;
       }
@@ -249,38 +275,36 @@ void k_kv4_append(const shard_kv4_args a) {
       }
     }
     // V: codes into LDS by token, words of 8 tokens out
-    for (int u = tid; u < 32 * (D / 8); u += 256) {  // quads of lanes share a block of 32 channels
-      const int vt = u / (D / 8), vc = (u % (D / 8)) * 8;
-      const int vi = t0 + vt - start;
-      if (vi >= 0 && vi < s.n && t0 + vt < a.n_phases) {
-        const T* v = (const T*)a.v + (int64_t)(s.row0 + vi) * a.v_stride + (int64_t)g * a.v_head_stride + vc;
+#pragma unroll
+    for (int n = 0; n < VU; ++n) {  // quads of lanes share a block of 32 channels
+      const int u = tid + 256 * n, vt = u / (D / 8), vc = (u % (D / 8)) * 8;
+      if (is_new(vt)) {
         float x[8], m = 0.f;
-        load8(v, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          x[j] = (float)vx[n][j];
           x[j] = x[j] == x[j] ? x[j] : 0.f;
           m = fmaxf(m, fabsf(x[j]));
         }
         const unsigned sb = scale_byte(quad_max(m));
         const float sc = e5m2(sb);
+        uint32_t w[2] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) codes[vt][vc + j] = (uint8_t)code4(x[j], sc);
-        if ((vc & 31) == 0) base[v_scale_at<D>((t0 & 63) + vt, vc / 32)] = (uint8_t)sb;
+        for (int j = 0; j < 8; ++j) w[j >> 2] |= code4(x[j], sc) << (8 * (j & 3));
+        *(uint32_t*)&codes[vt][vc] = w[0];
+        *(uint32_t*)&codes[vt][vc + 4] = w[1];
+        if ((vc & 31) == 0) base[v_scale_at<D>(slot0 + vt, vc / 32)] = (uint8_t)sb;
       }
     }
     __syncthreads();
-    for (int u = tid; u < 4 * D; u += 256) {
-      const int kq = u / D, vc = u % D;
-      uint32_t w = 0, keep = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int vt = 16 * (e >> 2) + 4 * kq + (e & 3), vi = t0 + vt - start;
-        if (vi >= 0 && vi < s.n && t0 + vt < a.n_phases) w |= (uint32_t)codes[vt][vc] << (4 * e);
-        else keep |= 15u << (4 * e);
-      }
-      uint32_t* at = (uint32_t*)(base + v_word_at<D>((t0 & 63) >> 5, kq, vc));
-      if (keep == 0) *at = w;
-      else if (keep != ~0u) *at = (*at & keep) | w;
+    for (int n = 0; n < VU; ++n) {
+      const int u = tid + 256 * n, kq = u / D, vc = u % D;
+      if (keep[n] == ~0u) continue;
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w |= (codes[16 * (e >> 2) + 4 * kq + (e & 3)][vc] & 15u) << (4 * e);  // whatever lies in the others
+      *(uint32_t*)(base + v_word_at<D>(slot0 >> 5, kq, vc)) = (old[n] & keep[n]) | (w & ~keep[n]);
     }
     __syncthreads();
   }
@@ -312,49 +336,50 @@ void k_kv4_read(const shard_kv4_args a) {
     const int t0 = grp * 32;
     const int page = t0 >= 0 && t0 < s.cap ? page_of(a, b, t0) : -1;
     const uint8_t* base = page >= 0 ? head_of<D>(a, page, g) : nullptr;
-    for (int u = tid; u < 32 * (D / 8); u += 256) {
-      const int t = u / (D / 8), ch = (u % (D / 8)) * 8, i = t0 + t - start;
-      if (i < 0 || i >= s.n) continue;
-      float x[8] = {};
-      if (base) {
-        const int slot = (t0 & 63) + t;
-        const uint32_t w = *(const uint32_t*)(base + k_code_at<D>(slot, ch / (D / 4)) + (ch % (D / 4)) / 2);
-        const float sc = e5m2(base[k_scale_at<D>(slot, ch / 32)]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const half2v p = fp4_pair(w, j);
-          x[2 * j] = (float)p[0] * sc;
-          x[2 * j + 1] = (float)p[1] * sc;
-        }
-      }
-      store8((T*)a.k_out + ((int64_t)(s.row0 + i) * a.n_kv_heads + g) * D + ch, x);
-    }
-    __syncthreads();
+    constexpr int U = D / 64;  // 8-channel pieces a thread, of K and of V; words of V codes
+    uint32_t kw[U] = {}, vw[U] = {};
+    uint8_t ksc[U] = {}, vsc[U] = {};
     if (base) {
-      for (int u = tid; u < 4 * D; u += 256) {
-        const int kq = u / D, vc = u % D;
-        const uint32_t w = *(const uint32_t*)(base + v_word_at<D>((t0 & 63) >> 5, kq, vc));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const half2v p = fp4_pair(w, j);
-          const int vt = 16 * (j >> 1) + 4 * kq + 2 * (j & 1);
-          rows[vt][vc] = p[0];
-          rows[vt + 1][vc] = p[1];
-        }
+      for (int n = 0; n < U; ++n) {
+        const int u = tid + 256 * n, slot = (t0 & 63) + u / (D / 8), ch = (u % (D / 8)) * 8;
+        kw[n] = *(const uint32_t*)(base + k_code_at<D>(slot, ch / (D / 4)) + (ch % (D / 4)) / 2);
+        ksc[n] = base[k_scale_at<D>(slot, ch / 32)];
+        vsc[n] = base[v_scale_at<D>(slot, ch / 32)];
+        vw[n] = *(const uint32_t*)(base + v_word_at<D>((t0 & 63) >> 5, u / D, u % D));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+      const int u = tid + 256 * n, kq = u / D, vc = u % D;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const half2v p = fp4_pair(vw[n], j);
+        const int vt = 16 * (j >> 1) + 4 * kq + 2 * (j & 1);
+        rows[vt][vc] = p[0];
+        rows[vt + 1][vc] = p[1];
       }
     }
     __syncthreads();
-    for (int u = tid; u < 32 * (D / 8); u += 256) {
-      const int t = u / (D / 8), ch = (u % (D / 8)) * 8, i = t0 + t - start;
-      if (i < 0 || i >= s.n) continue;
-      float x[8] = {};
-      if (base) {
-        const float sc = e5m2(base[v_scale_at<D>((t0 & 63) + t, ch / 32)]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)rows[t][ch + j] * sc;
+    for (int n = 0; n < U; ++n) {
+      const int u = tid + 256 * n, t = u / (D / 8), ch = (u % (D / 8)) * 8, i = t0 + t - start;
+      if (i < 0 || i >= s.n) continue;
+      const float ks = base ? e5m2(ksc[n]) : 0.f, vs = base ? e5m2(vsc[n]) : 0.f;
+      float x[8], y[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const half2v p = fp4_pair(kw[n], j);
+        x[2 * j] = (float)p[0] * ks;
+        x[2 * j + 1] = (float)p[1] * ks;
       }
-      store8((T*)a.v_out + ((int64_t)(s.row0 + i) * a.n_kv_heads + g) * D + ch, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = (float)rows[t][ch + j] * vs;
+      const int64_t at = ((int64_t)(s.row0 + i) * a.n_kv_heads + g) * D + ch;
+      store8((T*)a.k_out + at, x);
+      store8((T*)a.v_out + at, y);
     }
+    __syncthreads();
   }
 }
 
@@ -1127,6 +1152,7 @@ int check_attn(const shard_kv4_args* a) {
   const int rc = check_batch(a);
   if (rc) return rc;
   if (a->n_q_heads <= 0 || a->n_q_heads % a->n_kv_heads) return SHARD_ERR_SHAPE;
+  if ((int64_t)a->n_tokens * a->n_q_heads > INT32_MAX) return SHARD_ERR_SHAPE;  // rows are counted in 32 bits
   return SHARD_OK;
 }
 
