@@ -510,7 +510,8 @@ int shard_eigh_top(double* a, int32_t n, int32_t top, double* evals, double* eve
  * 0 .. n_pages - 1 are left out: not stored, not attended to, read as zeros.
  * Rows behind the last sequence's are neither read nor written.
  *
- * head_dim 64 or 128, any number of query heads per kv head; dtype of q, k, v
+ * head_dim 64 or 128, any number of query heads per kv head, up to 1,024 kv
+ * heads, 65,535 sequences and INT32_MAX rows times query heads; dtype of q, k, v
  * and the outputs.  Strides are in elements, multiples of 8; rows of a head
  * are contiguous; pointers 16-byte aligned; page_stride (bytes) a multiple of
  * 16; q_out, k_out, v_out and out are contiguous (n_tokens, heads, head_dim).

@@ -405,6 +405,8 @@ void k_kv4_read(const shard_kv4_args a) {
 // (below it they lose bits, 2^-26 of the largest at most); the power goes back
 // in through the softmax scale.
 // --------------------------------------------------------------------------
+constexpr float kLeast = 1.17549435e-38f;  // a factor of scores is never 0: -inf stays what it is
+
 struct AttnWork {
   float* m;      // [row][split], rows (token, query head)
   float* l;
@@ -505,7 +507,7 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   // a split past the sequence's end has no part that the merge reads
   if (w.n_splits > 1 && first >= tiles) return;
   // the scale's sign goes into q, so that the largest product is the largest score
-  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+  const float scale2 = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * 1.4426950408889634f, kLeast);
   const half_t sign = a.scale < 0.f ? (half_t)-1.f : a.scale == 0.f ? (half_t)0.f : (half_t)1.f;
 
   for (int rt = blockIdx.x / w.n_splits; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
@@ -551,7 +553,7 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
         for (int j = 0; j < ST; ++j)
 #pragma unroll
           for (int e = 0; e < 8; ++e) q[t][j][e] = (half_t)ldexpf(x[j][e], -ex) * sign;
-        sc[t] = ldexpf(scale2, ex);
+        sc[t] = fmaxf(ldexpf(scale2, ex), kLeast);
       }
     }
 
@@ -841,7 +843,7 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
     half8 q[QS];
     // the scale's sign goes into q, so that the largest product is the largest score
     const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-    float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    float sc = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * 1.4426950408889634f, kLeast);
     const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)h * a.q_head_stride + 8 * hi;
     if constexpr (__is_same(T, half_t)) {
 #pragma unroll
@@ -866,7 +868,7 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[j][e] = (half_t)(sign * ldexpf(x[e], -ex));
       }
-      sc = ldexpf(sc, ex);
+      sc = fmaxf(ldexpf(sc, ex), kLeast);
     }
     float m = -INFINITY, l = 0.f;
     float16v acc[CT], S[2];
@@ -1125,7 +1127,7 @@ bool rows_ok(const void* p, int64_t stride, int64_t head_stride) {
 }
 
 int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens can touch
-  const int n = a->max_new > 0 ? a->max_new : a->n_tokens;
+  const int n = !a->cu_seqlens ? 1 : a->max_new > 0 ? a->max_new : a->n_tokens;
   return n <= 1 ? 1 : (int)(((int64_t)n + 30) / 32 + 1);
 }
 

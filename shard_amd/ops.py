@@ -1123,7 +1123,8 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
     the given contiguous one or a new one: rows that see no token are zeros,
     rows behind the last sequence's are not written.  max_new and max_len, the
     most new tokens and tokens of a sequence, size the launch where the caller
-    knows them (a captured graph must be given what its replays reach)."""
+    knows them; other lengths give the same result, only slower (a captured
+    graph does best with what its replays reach)."""
     lib, T = _lib.load(), q.shape[0]
     batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, max_len, q, out)
     if batch is None:

@@ -95,9 +95,10 @@ class PagedCache(HFCache):
         return seq
 
     def drop(self, seq):
-        """Give a sequence's pages back."""
+        """Give a sequence's pages back.  An open step is closed."""
         self._free += reversed(self._pages.pop(seq))
         del self._lens[seq]
+        self._step = None
 
     def length(self, seq) -> int:
         return self._lens[seq]
@@ -134,8 +135,18 @@ class PagedCache(HFCache):
         B = len(seqs)
         table, lens, cu_dev = meta[:B * width].view(B, width), meta[B * width:B * width + B], meta[B * width + B:]
         self._step = dict(table=table, lens=lens, cu=None if max(new) == min(new) == 1 else cu_dev, rows=cu[-1],
-                          max_new=max(new), max_len=max(total))
+                          max_new=max(new), max_len=max(total), undo=list(zip(seqs, new, want)))
         return torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)])[None].to(dev)
+
+    def cancel(self):
+        """Undo the open step: its tokens were not stored in every layer."""
+        step, self._step = self._step, None
+        if step is None:
+            raise ValueError("no step is open")
+        for seq, n, pages in step["undo"]:
+            self._lens[seq] -= n
+            for _ in range(pages):
+                self._free.append(self._pages[seq].pop())
 
     def attend(self, layer_idx, q, k, v, scale=None):
         """One layer of the open step: q (T, H, D), k and v (T, G, D) before RoPE,
@@ -157,12 +168,16 @@ class PagedCache(HFCache):
         tokens = [torch.as_tensor(t).reshape(-1) for t in tokens]
         if min(len(t) for t in tokens) == 0:
             raise ValueError("every sequence of a step of the model needs a token")
-        pos = self.begin(seqs, [len(t) for t in tokens])
         ids = torch.cat([t.to(dev) for t in tokens])[None]
         keep = 0
         if last_only:
             keep = torch.tensor([len(t) for t in tokens]).cumsum(0).to(dev) - 1
-        return model(input_ids=ids, position_ids=pos, past_key_values=self, use_cache=True, logits_to_keep=keep).logits[0]
+        pos = self.begin(seqs, [len(t) for t in tokens])
+        try:
+            return model(input_ids=ids, position_ids=pos, past_key_values=self, use_cache=True, logits_to_keep=keep).logits[0]
+        except BaseException:
+            self.cancel()
+            raise
 
 
 def paged_forward(attention, hidden_states, cache):

@@ -139,6 +139,22 @@ def test_append_in_steps_gives_the_same_bytes(cuda, D):
     assert torch.equal(caches[0], caches[1]) and torch.equal(caches[0], caches[2])
 
 
+@pytest.mark.parametrize("kw", [dict(max_new=1), dict(max_new=1000), dict()], ids=str)
+def test_launch_hints_change_nothing(cuda, kw):
+    """Whatever max_new says, all tokens are stored and read; block tables that are part of wider ones."""
+    b = Batch([300, 64, 31], [290, 1, 30], 4, 2, 64, seed=14)
+    want_q = b.append(q=b.d_q)
+    want, (k, v) = b.d_cache.clone(), b.read()
+    b.d_cache = b.cache.to(cuda)
+    wide = torch.full((3, 40), 1 << 30, dtype=torch.int32, device=cuda)
+    wide[:, 7:7 + b.table.shape[1]] = b.d_table
+    b.d_table = wide[:, 7:7 + b.table.shape[1]]
+    assert not b.d_table.is_contiguous()
+    assert torch.equal(b.append(q=b.d_q, **kw), want_q) and torch.equal(b.d_cache, want)
+    k2, v2 = b.read(**kw)
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
 def test_append_strided_operands(cuda):
     """q, k and v as slices of one fused projection's rows, and rows at odd places."""
     b = Batch([70, 40], [50, 3], 4, 2, 128, seed=6)
@@ -261,6 +277,16 @@ def test_attention_scale_and_large_scores(cuda):
     _check_attention(b, b.attn(scale=0.0), scale=0.0)
     _check_attention(b, b.attn(scale=2.0), scale=2.0)
     _check_attention(b, b.attn(scale=-0.1), scale=-0.1)
+
+
+@pytest.mark.parametrize("new", [3, 40])
+def test_attention_scores_that_vanish(cuda, new):
+    """bf16 queries of the smallest numbers and a scale that takes them below fp32's: all keys weigh the same."""
+    b = Batch([100], [new], 8, 2, 64, "bf16", seed=15).fill()
+    b.q *= 1e-39
+    out = b.attn(scale=1e-20)
+    assert bool(torch.isfinite(out).all())
+    _check_attention(b, out, scale=1e-20)
 
 
 def test_attention_specials(cuda):

@@ -136,6 +136,34 @@ def test_refusals(cuda):
         cache.attend(0, x, x, x)
     with pytest.raises(RuntimeError):
         cache.update(x[None], x[None], 0)
+    cache.cancel()
+    assert cache.free_pages() == 3 and cache.length(a) == cache.length(b) == 0
+    with pytest.raises(ValueError):
+        cache.cancel()
+    with pytest.raises(ValueError):
+        cache.attend(0, x, x, x)
+
+
+def test_a_failed_step_changes_nothing(cuda):
+    """A model whose second layer fails: the step is undone, the next one is as if it had not been."""
+    from shard_amd import PagedCache, enable_llama_fused_attention
+    model = _model(cuda)
+    enable_llama_fused_attention(model)
+    ids = torch.arange(80) % VOCAB
+    caches = [PagedCache.from_model(model, n_pages=4, max_len=128) for _ in range(2)]
+    seqs = [c.add() for c in caches]
+    for c, s in zip(caches, seqs):
+        c.run(model, [s], [ids[:50]])
+
+    def fail(*args):
+        raise ArithmeticError
+    hook = model.model.layers[1].register_forward_pre_hook(fail)
+    with pytest.raises(ArithmeticError):
+        caches[0].run(model, [seqs[0]], [ids[60:]])
+    hook.remove()
+    assert caches[0].length(seqs[0]) == 50 and caches[0].free_pages() == 3
+    got, want = (c.run(model, [s], [ids[50:]]) for c, s in zip(caches, seqs))
+    assert torch.equal(got, want)
 
 
 def test_decode_graph_reports_log_probabilities(cuda):
