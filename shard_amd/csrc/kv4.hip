@@ -511,50 +511,27 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   const half_t sign = a.scale < 0.f ? (half_t)-1.f : a.scale == 0.f ? (half_t)0.f : (half_t)1.f;
 
   for (int rt = blockIdx.x / w.n_splits; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
-    half8 q[NQ][ST];
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    vec8 raw[NQ][ST];
     float sc[NQ], m[NQ], l[NQ];
     int lim[NQ];                      // keys that the lane's row sees
     float4v acc[NQ][NT];
-    int lim_min = keys, lim_max = 0;  // of the tile's rows (uniform)
-    {
-      const int r0 = rt * 16 * NQ, r1 = min(r0 + 16 * NQ, n_rows) - 1;
-      lim_min = min(max(s.len - s.n + r0 / group + 1, 0), keys);
-      lim_max = min(max(s.len - s.n + r1 / group + 1, 0), keys);
-    }
+    const int r0 = rt * 16 * NQ, r1 = min(r0 + 16 * NQ, n_rows) - 1;
+    // of the tile's rows (uniform)
+    const int lim_min = min(max(s.len - s.n + r0 / group + 1, 0), keys);
+    const int lim_max = min(max(s.len - s.n + r1 / group + 1, 0), keys);
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-      const int r = (rt * NQ + t) * 16 + col;
-      const bool live = r < n_rows;
-      const int i = live ? r / group : 0, h = live ? r - i * group : 0;
-      lim[t] = live ? min(max(s.len - s.n + i + 1, 0), keys) : 0;
+      const int r = min(r0 + 16 * t + col, r1);   // columns behind the last row repeat it, unused
+      const int i = r / group, h = r - i * group;
+      lim[t] = min(max(s.len - s.n + i + 1, 0), keys);
+      const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
+#pragma unroll
+      for (int j = 0; j < ST; ++j) raw[t][j] = *(const vec8*)(qp + 8 * j);
       m[t] = -INFINITY;
       l[t] = 0.f;
-      sc[t] = scale2;
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[t][n] = float4v{0.f, 0.f, 0.f, 0.f};
-      const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
-      if constexpr (__is_same(T, half_t)) {
-#pragma unroll
-        for (int j = 0; j < ST; ++j) q[t][j] = live ? *(const half8*)(qp + 8 * j) * sign : half8{};
-      } else {
-        float x[ST][8], mx = 0.f;
-#pragma unroll
-        for (int j = 0; j < ST; ++j) {
-          if (live) load8(qp + 8 * j, x[j]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (!live) x[j][e] = 0.f;
-            mx = fmaxf(mx, fabsf(x[j][e]));
-          }
-        }
-        mx = across_quarters_max(mx);
-        const int ex = mx > 0.f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
-#pragma unroll
-        for (int j = 0; j < ST; ++j)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) q[t][j][e] = (half_t)ldexpf(x[j][e], -ex) * sign;
-        sc[t] = fmaxf(ldexpf(scale2, ex), kLeast);
-      }
     }
 
     const int stop = min(last, (lim_max + kPage - 1) / kPage);
@@ -566,6 +543,29 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
     int page = page_near(first + wave), ahead = page_near(first + wave + WAVES);
     pg.load_k(head_of<D>(a, max(page, 0), g), lane);
     pg.load_v(head_of<D>(a, max(page, 0), g), lane);
+    __builtin_amdgcn_sched_barrier(0);  // q is not waited for before the first page is on its way
+    half8 q[NQ][ST];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      if constexpr (__is_same(T, half_t)) {
+        sc[t] = scale2;
+#pragma unroll
+        for (int j = 0; j < ST; ++j) q[t][j] = raw[t][j] * sign;
+      } else {
+        float mx = 0.f;
+#pragma unroll
+        for (int j = 0; j < ST; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf((float)raw[t][j][e]));
+        mx = across_quarters_max(mx);
+        const int ex = mx > 0.f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
+#pragma unroll
+        for (int j = 0; j < ST; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[t][j][e] = (half_t)ldexpf((float)raw[t][j][e], -ex) * sign;
+        sc[t] = fmaxf(ldexpf(scale2, ex), kLeast);
+      }
+    }
     for (int tile = first + wave; tile < stop; tile += WAVES) {
       const int lim_page = page < 0 ? 0 : lim_max;   // keys of no page are not seen
       const bool none = page < 0;
