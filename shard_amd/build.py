@@ -4,17 +4,20 @@
 
 Each ``csrc/*.hip`` is compiled to an object with its own flags (the integer
 chains in quant.hip with -ffp-contract=off so no multiply-add is fused), then
-all objects are linked into ``shard_amd/libshard_hip.so``.
+all objects are linked into ``shard_amd/libshard_hip.so``.  ``csrc/dispatch.cpp``,
+host code against torch's headers, becomes ``shard_amd/_dispatch.so``.
 """
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libshard_hip.so")
+DISPATCH = os.path.join(HERE, "_dispatch.so")
 ARCH = os.environ.get("SHARD_OFFLOAD_ARCH", "gfx950")
 
 COMMON = [
@@ -44,12 +47,27 @@ def sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
+def dispatch_command(out: str):
+    import torch
+    root = os.path.dirname(torch.__file__)
+    return [shutil.which("g++") or "c++", "-O2", "-fPIC", "-shared", "-std=c++17",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-isystem", os.path.join(root, "include"),
+            "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "dispatch.cpp"), "-o", out,
+            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+
+
 def build(verbose: bool = False, jobs: int = 4) -> str:
     """Compile every csrc/*.hip for gfx950 and link libshard_hip.so. Returns its path."""
     cc = hipcc()
     objdir = tempfile.mkdtemp(prefix="shard_build_")
     try:
         procs, objs = [], []
+        cmd = dispatch_command(DISPATCH + ".tmp")
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        dispatch = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         for src in sources():
             obj = os.path.join(objdir, src.replace(".hip", ".o"))
             cmd = [cc, *COMMON, *PER_FILE.get(src, []), "-c", os.path.join(CSRC, src), "-o", obj]
@@ -67,6 +85,8 @@ def build(verbose: bool = False, jobs: int = 4) -> str:
         if out.returncode != 0:
             raise RuntimeError("link failed:\n" + out.stdout)
         os.replace(tmp, LIB)
+        _drain([("dispatch.cpp", dispatch)])
+        os.replace(DISPATCH + ".tmp", DISPATCH)
     finally:
         shutil.rmtree(objdir, ignore_errors=True)
     return LIB

@@ -945,6 +945,25 @@ def kv_rebuild(fmt, batch: int, stream_n: int = 0):
 # ---------------------------------------------------------------------------
 KV4_PAGE = 64  # SHARD_KV4_PAGE: tokens of a page
 
+# The compiled way of the calls below (csrc/dispatch.cpp): takes operands that need
+# neither a copy nor an explanation, returns None for all others.  None until the
+# first call, False where it was not built.
+_direct = None
+
+
+def _bind_direct():
+    global _direct
+    if _direct is None:
+        _lib.load()
+        try:
+            from . import _dispatch
+            _dispatch.bind(_lib.LIB_PATH)
+            _direct = _dispatch if _raw_stream is not None else False
+        except ImportError:
+            _direct = False
+    return _direct
+
+
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
@@ -1064,6 +1083,12 @@ def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=No
     are left out; rows behind the last sequence's are not read, and their
     rotated q not written.  Two sequences of one call must not append to the
     same page."""
+    direct = _direct or _bind_direct()
+    if direct and k.is_cuda:
+        dev = _current_device()
+        done = direct.kv4_append(k, v, cache, block_table, seq_lens, phases, q, cu_seqlens, max_new, dev, _raw_stream(dev))
+        if done is not None:
+            return None if q is None else done
     lib, T = _lib.load(), k.shape[0]
     batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, 0, k, v, phases, q)
     if batch is None:
@@ -1097,6 +1122,13 @@ def kv4_read(cache, block_table, seq_lens, n_tokens, dtype=torch.float16, cu_seq
     cu_seqlens reads whole sequences).  Exact in fp16; bf16 is exact too.  Rows
     of tokens that the table or the cache does not hold are zeros; rows behind
     the last sequence's are not written."""
+    direct = _direct or _bind_direct()
+    if direct and cache.is_cuda and (dtype is torch.float16 or dtype is torch.bfloat16):
+        dev = _current_device()
+        done = direct.kv4_read(cache, block_table, seq_lens, n_tokens, dtype is torch.bfloat16, cu_seqlens, max_new, dev,
+                               _raw_stream(dev))
+        if done is not None:
+            return done
     lib, T = _lib.load(), int(n_tokens)
     batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, 0)
     if batch is None:
@@ -1125,6 +1157,12 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
     most new tokens and tokens of a sequence, size the launch where the caller
     knows them; other lengths give the same result, only slower (a captured
     graph does best with what its replays reach)."""
+    direct = _direct or _bind_direct()
+    if direct and out is None and q.is_cuda:
+        dev = _current_device()
+        done = direct.kv4_attn(q, cache, block_table, seq_lens, cu_seqlens, scale, max_new, max_len, dev, _raw_stream(dev))
+        if done is not None:
+            return done
     lib, T = _lib.load(), q.shape[0]
     batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, max_len, q, out)
     if batch is None:
@@ -1163,6 +1201,12 @@ def token_logprobs(logits, tokens=None, top=0):
     most probable tokens, equal ones by index (top up to 64).  A row without a
     logit above -inf, or with +inf or NaN, has NaN log probabilities; NaN
     logits are never among the top (id -1 where a row has too few others)."""
+    direct = _direct or _bind_direct()
+    if direct and logits.is_cuda:
+        dev = _current_device()
+        done = direct.token_logprobs(logits, tokens, top, dev, _raw_stream(dev))
+        if done is not None:
+            return done
     lib, dev = _lib.load(), logits.get_device()
     if dev < 0 or (tokens is not None and tokens.get_device() != dev):
         _require_gpu(logits, tokens)

@@ -464,3 +464,28 @@ def test_refusals(cuda):
     assert b.attn(q=empty, cu_seqlens=none).shape == (0, 4, 128)
     assert b.append(k=b.d_k[:0], v=b.d_v[:0], q=empty, cu_seqlens=none).shape == (0, 4, 128)
     assert b.read(0, cu_seqlens=none)[0].shape == (0, 2, 128)
+
+
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+def test_compiled_and_plain_dispatch_agree(cuda, type, monkeypatch):
+    """The compiled way and the one through Python give the same bits, and the
+    compiled one takes plain calls."""
+    from shard_amd import ops
+    results = []
+    for direct in (ops._bind_direct(), False):
+        monkeypatch.setattr(ops, "_direct", direct)
+        b = Batch([300, 64, 90], [20, 1, 90], 8, 2, 128, type, seed=16).fill()
+        if direct:
+            assert direct.kv4_attn(b.d_q, b.d_cache, b.d_table, b.d_lens, b.d_cu, None, 90, 300, 0, 0) is not None
+        q = b.append(q=b.d_q)
+        assert b.append() is None
+        res = [q, b.d_cache, *b.read(dtype=b.type), *b.read(), b.attn(), b.attn(scale=0.3, max_new=90), b.attn(max_len=300)]
+        x = torch.randn(3, 5000, generator=torch.Generator().manual_seed(1)).to(b.type).to(cuda)
+        t = torch.tensor([1, 4999, 0], device=cuda)
+        for y in (x, x[:, 3:], x[::2]):
+            res += ops.token_logprobs(y, t[:y.shape[0]].clamp(max=4900), top=4)
+            res += ops.token_logprobs(y, top=0)[1:]
+        results.append(res)
+    assert len(results[0]) == len(results[1])
+    for x, y in zip(*results):
+        assert x.dtype == y.dtype and x.shape == y.shape and x.device == y.device and torch.equal(x, y)

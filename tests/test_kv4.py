@@ -139,3 +139,24 @@ def test_logprobs_refusals():
     assert str(need).encode() in lib.shard_last_error()
     assert lib.shard_token_logprobs_workspace(4096, 128256, 5) == 0    # a workgroup a row
     assert lib.shard_token_logprobs_workspace(4, 128256, 65) == 0
+
+
+def test_compiled_dispatch_is_built_and_leaves_odd_calls():
+    """_dispatch.so loads, binds the library, and returns None (the way through
+    ops.py) for operands it does not take."""
+    import torch
+    from shard_amd import _lib, ops
+    _lib.load()
+    d = ops._bind_direct()
+    assert d, "shard_amd/_dispatch.so is not built"
+    c = ops.kv4_cache(2, 2, 64, device="cpu")
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    k = torch.zeros(1, 2, 64, dtype=torch.float16)
+    assert d.kv4_attn(k, c, t, n, None, None, None, None, 0, 0) is None
+    assert d.kv4_append(k, k, c, t, n, torch.zeros(128, 32, 2), None, None, None, 0, 0) is None
+    assert d.kv4_read(c, t, n, 1, False, None, None, 0, 0) is None
+    assert d.token_logprobs(torch.zeros(2, 5), None, 1, 0, 0) is None
+    for bad in ((), (None,) * 10, ("q", c, t, n, None, None, None, None, 0, 0), (k, c, t, n, None, None, 1 << 70, None, 0, 0)):
+        assert d.kv4_attn(*bad) is None
+    with pytest.raises(ImportError):
+        d.bind("/nowhere/lib.so")
