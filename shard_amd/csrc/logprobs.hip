@@ -160,6 +160,7 @@ void k_logprobs(const LogprobArgs a) {
     }
   };
   uint32_t all_best = 0;
+  float only[VEC];   // the granule of a thread that has one alone
   for (int q = 0; q < kSlots; ++q) {
     best = -INFINITY;
     bool any = false;
@@ -181,9 +182,8 @@ void k_logprobs(const LogprobArgs a) {
         i += 4;
       } else {
         if (j + tid < g1) {
-          float x[VEC];
-          r.load(j + tid, x);
-          eat(x);
+          r.load(j + tid, only);
+          eat(only);
           any = true;
         }
         ++i;
@@ -213,8 +213,9 @@ void k_logprobs(const LogprobArgs a) {
     const uint32_t v[4] = {most[lane], most[lane + 64], most[lane + 128], most[lane + 192]};
     const uint32_t b = kth_largest(v, a.top);
     if (b) need = (u64)b << 32;
-    for (int q = 0; q < kSlots; ++q)
-      if (slot[q][tid] && slot[q][tid] >= b) todo[atomicAdd(&n_todo, 1)] = (uint16_t)(q * 256 + tid);
+    if (own > 1)
+      for (int q = 0; q < kSlots; ++q)
+        if (slot[q][tid] && slot[q][tid] >= b) todo[atomicAdd(&n_todo, 1)] = (uint16_t)(q * 256 + tid);
   }
   __syncthreads();
   const Stats all{M, (sh_l[0] + sh_l[1]) + (sh_l[2] + sh_l[3]), (sh_t[0] + sh_t[1]) + (sh_t[2] + sh_t[3])};
@@ -230,13 +231,7 @@ void k_logprobs(const LogprobArgs a) {
 
   int n;
   for (;;) {
-    const uint32_t per = (uint32_t)size, items = n_todo * per;  // at most the part's granules and 2,048 more
-    for (uint32_t it = tid; it < items; it += 256) {
-      const int w = todo[it / per];
-      const int64_t i = (w >> 8) * size + it % per, j = g0 + 256 * i + (w & 255);
-      if (i >= own || j >= g1) continue;
-      float x[VEC];
-      const int64_t e0 = r.load(j, x);
+    const auto collect = [&](const float(&x)[VEC], int64_t e0) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const u64 key = e0 + k >= 0 && e0 + k < a.vocab ? key_of(x[k], e0 + k) : 0;
@@ -244,6 +239,19 @@ void k_logprobs(const LogprobArgs a) {
           const int at = atomicAdd(&found, 1);
           if (at < kList) list[at] = key;
         }
+      }
+    };
+    if (own == 1) {
+      if (all_best && all_best >= (uint32_t)(need >> 32)) collect(only, (g0 + tid) * VEC - r.mis);
+    } else {
+      const uint32_t per = (uint32_t)size, items = n_todo * per;  // at most the part's granules and 2,048 more
+      for (uint32_t it = tid; it < items; it += 256) {
+        const int w = todo[it / per];
+        const int64_t i = (w >> 8) * size + it % per, j = g0 + 256 * i + (w & 255);
+        if (i >= own || j >= g1) continue;
+        float x[VEC];
+        const int64_t e0 = r.load(j, x);
+        collect(x, e0);
       }
     }
     __syncthreads();
