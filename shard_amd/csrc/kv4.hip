@@ -411,15 +411,33 @@ struct AttnWork {
   float* m;      // [row][split], rows (token, query head)
   float* l;
   float* acc;    // [row][split][D]
-  int n_splits;
-  int row_tiles; // workgroups along a sequence's rows
+  int n_splits, split_shift;    // a power of two
+  int group, group_shift;       // query heads of a kv head; -1: no power of two
+  int row_tiles;                // workgroups along a sequence's rows
 };
 
 // Tiles (pages) a split of a sequence of `tiles` takes: at least kMinTiles, one
 // for each wave of the workgroup.
 constexpr int kMinTiles = 4;
-__device__ __forceinline__ int tiles_per_split(int tiles, int n_splits) {
-  return max(kMinTiles, (tiles + n_splits - 1) / n_splits);
+__device__ __forceinline__ int tiles_per_split(const AttnWork& w, int tiles) {
+  return max(kMinTiles, (tiles + w.n_splits - 1) >> w.split_shift);
+}
+
+// Token of a sequence's row, and its head within the group.  (An integer division
+// costs a launch's first instructions about 150 cycles each.)
+__device__ __forceinline__ int token_of(const AttnWork& w, int r) {
+  return w.group_shift >= 0 ? r >> w.group_shift : r / w.group;
+}
+
+// A split past a sequence's end: the merge reads that it has nothing.  Rows tid,
+// tid + 256, ... of every 256 row_tiles.
+__device__ __forceinline__ void nothing(const shard_kv4_args& a, const AttnWork& w, const Seq& s, int g, int split, int at) {
+  for (int r = at * 256 + (int)threadIdx.x; r < s.n * w.group; r += w.row_tiles * 256) {
+    const int i = token_of(w, r), h = g * w.group + r - i * w.group;
+    const int64_t part = ((int64_t)(s.row0 + i) * a.n_q_heads + h) * w.n_splits + split;
+    w.m[part] = -INFINITY;
+    w.l[part] = 0.f;
+  }
 }
 
 // A page's operands for one wave.
@@ -496,21 +514,20 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
   const int g = blockIdx.y, b = blockIdx.z;
-  const int split = blockIdx.x % w.n_splits;
+  const int split = blockIdx.x & (w.n_splits - 1), rt0 = blockIdx.x >> w.split_shift;
   const Seq s = seq_of(a, b);
-  const int group = a.n_q_heads / a.n_kv_heads;
+  const int group = w.group;
   const int n_rows = s.n * group;
   const int keys = min(s.len, s.cap);
   const int tiles = (keys + kPage - 1) / kPage;
-  const int per = tiles_per_split(tiles, w.n_splits);
+  const int per = tiles_per_split(w, tiles);
   const int first = split * per, last = min(first + per, tiles);
-  // a split past the sequence's end has no part that the merge reads
-  if (w.n_splits > 1 && first >= tiles) return;
+  if (w.n_splits > 1 && first >= tiles) return nothing(a, w, s, g, split, rt0);
   // the scale's sign goes into q, so that the largest product is the largest score
   const float scale2 = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * 1.4426950408889634f, kLeast);
   const half_t sign = a.scale < 0.f ? (half_t)-1.f : a.scale == 0.f ? (half_t)0.f : (half_t)1.f;
 
-  for (int rt = blockIdx.x / w.n_splits; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
+  for (int rt = rt0; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
     typedef T vec8 __attribute__((ext_vector_type(8)));
     vec8 raw[NQ][ST];
     float sc[NQ], m[NQ], l[NQ];
@@ -518,12 +535,12 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
     float4v acc[NQ][NT];
     const int r0 = rt * 16 * NQ, r1 = min(r0 + 16 * NQ, n_rows) - 1;
     // of the tile's rows (uniform)
-    const int lim_min = min(max(s.len - s.n + r0 / group + 1, 0), keys);
-    const int lim_max = min(max(s.len - s.n + r1 / group + 1, 0), keys);
+    const int lim_min = min(max(s.len - s.n + token_of(w, r0) + 1, 0), keys);
+    const int lim_max = min(max(s.len - s.n + token_of(w, r1) + 1, 0), keys);
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       const int r = min(r0 + 16 * t + col, r1);   // columns behind the last row repeat it, unused
-      const int i = r / group, h = r - i * group;
+      const int i = token_of(w, r), h = r - i * group;
       lim[t] = min(max(s.len - s.n + i + 1, 0), keys);
       const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
 #pragma unroll
@@ -680,7 +697,7 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
       const int rr = u / (D / 8), ch = (u % (D / 8)) * 8;
       const int r = rt * 16 * NQ + rr;
       if (r >= n_rows) continue;
-      const int i = r / group, h = g * group + r % group;
+      const int i = token_of(w, r), h = g * group + r - i * group;
       float M = sh_m[0][rr];
 #pragma unroll
       for (int v = 1; v < WAVES; ++v) M = fmaxf(M, sh_m[v][rr]);
@@ -818,19 +835,19 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   // its L2 to itself; long row tiles first
   const int g = blockIdx.x % a.n_kv_heads, b = blockIdx.y;
   const int unit = blockIdx.x / a.n_kv_heads;
-  const int split = unit % w.n_splits;
+  const int split = unit & (w.n_splits - 1), at = unit >> w.split_shift;
   const Seq s = seq_of(a, b);
-  const int group = a.n_q_heads / a.n_kv_heads;
+  const int group = w.group;
   const int n_rows = s.n * group;
   const int keys = min(s.len, s.cap);
   const int tiles = (keys + kPage - 1) / kPage;
-  const int per = tiles_per_split(tiles, w.n_splits);
+  const int per = tiles_per_split(w, tiles);
   const int first = split * per, end = min(first + per, tiles);
-  if (w.n_splits > 1 && first >= tiles) return;
+  if (w.n_splits > 1 && first >= tiles) return nothing(a, w, s, g, split, at);
   const int n_tiles = (n_rows + kTileRows - 1) / kTileRows;
-  const auto limit = [&](int row) { return min(max(s.len - s.n + row / group + 1, 0), keys); };
+  const auto limit = [&](int row) { return min(max(s.len - s.n + token_of(w, row) + 1, 0), keys); };
 
-  for (int back = unit / w.n_splits; back < n_tiles; back += w.row_tiles) {
+  for (int back = at; back < n_tiles; back += w.row_tiles) {
     const int rt = n_tiles - 1 - back;
     const int r0 = rt * kTileRows + wave * 32;                  // the wave's first row
     const int last = min(end, (limit(min(rt * kTileRows + kTileRows, n_rows) - 1) + kPage - 1) / kPage);
@@ -838,7 +855,7 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
     const int lim_min = r0 + 32 <= n_rows ? limit(r0) : 0;
     const int r = r0 + col;
     const bool live = r < n_rows;
-    const int i = live ? r / group : 0, h = g * group + (live ? r - i * group : 0);
+    const int i = live ? token_of(w, r) : 0, h = g * group + (live ? r - i * group : 0);
     const int lim = live ? limit(r) : 0;
     half8 q[QS];
     // the scale's sign goes into q, so that the largest product is the largest score
@@ -893,19 +910,19 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
     if (first < last) {
       // pages of tiles n .. n + 3; past the last tile it again, page 0 where there is none
       const auto page_near = [&](int tile) { return page_of(a, b, min(tile, last - 1) * kPage); };
-      const auto at = [&](int page) { return head_of<D>(a, max(page, 0), g); };
+      const auto page_at = [&](int page) { return head_of<D>(a, max(page, 0), g); };
       const auto left = [&](int page, int tile) { return page < 0 ? 0 : keys - tile * kPage; };
       int p0 = page_near(first), p1 = page_near(first + 1), p2 = page_near(first + 2), p3 = page_near(first + 3);
       K kr(tid);
       V vr(tid);
-      kr.load(at(p0));
-      vr.load(at(p0));
+      kr.load(page_at(p0));
+      vr.load(page_at(p0));
       kr.store(sk);
-      kr.load(at(p1));
+      kr.load(page_at(p1));
       vr.store(sv, left(p0, first));
-      vr.load(at(p1));
+      vr.load(page_at(p1));
       kr.store(sk + K::kBuffer);
-      kr.load(at(p2));
+      kr.load(page_at(p2));
       __syncthreads();
       scores(0);
       __syncthreads();
@@ -913,9 +930,9 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
       for (int tile = first; tile < last; ++tile) {
         // vector phase
         vr.store(sv + v1, left(p1, tile + 1));
-        vr.load(at(p2));
+        vr.load(page_at(p2));
         kr.store(sk + k0);
-        kr.load(at(p3));
+        kr.load(page_at(p3));
         if (p0 < 0 || (tile + 1) * kPage > lim_min) {
           const int seen = p0 < 0 ? 0 : lim;          // keys of no page are not seen
 #pragma unroll
@@ -1023,20 +1040,23 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   }
 }
 
-// Joins the splits of a row; 3.5 to 5 us, latency, up to 64 splits.  WAVES waves take a row's splits in turn, several
-// splits a load (16 bytes a lane); every wave forms all weights itself (128
-// splits at most: two a lane).
+// Joins the splits of a row; 3.3 to 4.7 us, latency, up to 64 splits.  WAVES waves
+// take a row's splits in turn, several a load (16 bytes a lane); every wave forms
+// all weights itself (128 splits at most: two a lane).  Nothing here waits for
+// lengths: splits without keys have a maximum of -inf, their sums are whatever
+// was there and not used.
 constexpr int kMaxSplits = 128;
 
 template <class T, int D, int WAVES>
-__device__ __forceinline__ void merge_row(const AttnWork& w, T* out, int64_t row, int n, int wave, int lane, float4v* sh) {
+__device__ __forceinline__ void merge_row(const AttnWork& w, T* out, int64_t row, int wave, int lane, float4v* sh) {
   constexpr int LPS = D / 4;       // lanes of a split's row
   constexpr int SPL = 64 / LPS;    // splits a load
-  const float* pm = w.m + row * w.n_splits;
-  const float* pl = w.l + row * w.n_splits;
+  const int n = w.n_splits;
+  const float* pm = w.m + row * n;
+  const float* pl = w.l + row * n;
   const float m0 = lane < n ? pm[lane] : -INFINITY, m1 = lane + 64 < n ? pm[lane + 64] : -INFINITY;
   const float l0 = lane < n ? pl[lane] : 0.f, l1 = lane + 64 < n ? pl[lane + 64] : 0.f;
-  const float* pa = w.acc + row * w.n_splits * D + (lane % LPS) * 4;
+  const float* pa = w.acc + row * n * D + (lane % LPS) * 4;
   constexpr int U = 4;             // loads in flight
   float4v v[U];
   const int s0 = wave * SPL + lane / LPS;
@@ -1045,6 +1065,7 @@ __device__ __forceinline__ void merge_row(const AttnWork& w, T* out, int64_t row
     const int i = s0 + u * SPL * WAVES;
     v[u] = i < n ? *(const float4v*)(pa + (int64_t)i * D) : float4v{0.f, 0.f, 0.f, 0.f};
   }
+  // a row of NaN has NaN in its sums, not in its maxima
   const float M = wave64_reduce(fmaxf(m0, m1), OpMax());
   const float base = M == -INFINITY ? 0.f : M;
   const float f0 = exp2f(m0 - base), f1 = exp2f(m1 - base);
@@ -1055,7 +1076,7 @@ __device__ __forceinline__ void merge_row(const AttnWork& w, T* out, int64_t row
     for (int u = 0; u < U; ++u) {
       const int i = at + s0 + u * SPL * WAVES;
       const float f = i < 64 ? __shfl(f0, i & 63) : __shfl(f1, i & 63);
-      if (i < n) x += f * v[u];
+      if (i < n && f != 0.f) x += f * v[u];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1092,16 +1113,14 @@ __global__ __launch_bounds__(256)
 void k_kv4_merge(const shard_kv4_args a, const AttnWork w) {
   __shared__ float4v sh[WAVES > 1 ? WAVES * D / 4 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Seq s = seq_of(a, blockIdx.y);
-  const int tiles = (min(s.len, s.cap) + kPage - 1) / kPage;
-  const int per = tiles_per_split(tiles, w.n_splits);
-  const int n = (tiles + per - 1) / per;
-  constexpr int ROWS = 4 / WAVES;
-  const int64_t rows = (int64_t)s.n * a.n_q_heads, row0 = (int64_t)s.row0 * a.n_q_heads;
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + (WAVES > 1 ? 0 : wave); r < rows; r += (int64_t)gridDim.x * ROWS) {
-    merge_row<T, D, WAVES>(w, (T*)a.out, row0 + r, n, WAVES > 1 ? wave : 0, lane, sh);
-    if constexpr (WAVES > 1) __syncthreads();
+  const int64_t r = WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  int t0 = 0, t1 = a.n_tokens;   // rows of sequences
+  if (a.cu_seqlens) {
+    t0 = max(a.cu_seqlens[0], 0);
+    t1 = min(a.cu_seqlens[a.batch], a.n_tokens);
   }
+  if (r >= (int64_t)t0 * a.n_q_heads && r < (int64_t)t1 * a.n_q_heads)
+    merge_row<T, D, WAVES>(w, (T*)a.out, r, WAVES > 1 ? wave : 0, lane, sh);
 }
 
 // --------------------------------------------------------------------------
@@ -1142,7 +1161,7 @@ int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens
 // 26.6 / 33.7 by tiles; 16 x 4,000 with 16 (64 rows) 40.8 / 52.1.
 struct AttnPlan {
   int nq;         // 16-row groups of a workgroup: 1 or 2 (rows), 8 (tile)
-  int row_tiles, n_splits;
+  int row_tiles, n_splits, split_shift;
 };
 AttnPlan plan_of(const shard_kv4_args* a) {
   AttnPlan p;
@@ -1160,7 +1179,10 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   if (p.nq != 8 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;
-  p.n_splits = sp < 1 ? 1 : (int)sp;
+  // the nearest power of two
+  p.split_shift = 0;
+  while ((int64_t)2 << p.split_shift <= kMaxSplits && (int64_t)2 << (2 * p.split_shift) < sp * sp) ++p.split_shift;
+  p.n_splits = 1 << p.split_shift;
   return p;
 }
 
@@ -1254,6 +1276,9 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   const int64_t rows = (int64_t)a->n_tokens * a->n_q_heads;
   AttnWork w{};
   w.n_splits = p.n_splits;
+  w.split_shift = p.split_shift;
+  w.group = a->n_q_heads / a->n_kv_heads;
+  w.group_shift = w.group & (w.group - 1) ? -1 : __builtin_ctz(w.group);
   w.row_tiles = p.row_tiles;
   if ((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads > INT32_MAX) return SHARD_ERR_SHAPE;
   if (p.n_splits > 1) {
@@ -1278,15 +1303,9 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   }
   SHARD_LAUNCH_CHECK("shard_kv4_attn");
   if (p.n_splits > 1) {
-    const int64_t per_seq = (a->cu_seqlens ? (a->max_new > 0 ? a->max_new : a->n_tokens) : 1) * (int64_t)a->n_q_heads;
-    if (p.n_splits > 8) {
-      const dim3 grid((unsigned)(per_seq < 4096 ? per_seq : 4096), a->batch);
-      KV4_DISPATCH_N(k_kv4_merge, 4, grid, s, *a, w);
-    } else {
-      const int64_t blocks = (per_seq + 3) / 4;
-      const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), a->batch);
-      KV4_DISPATCH_N(k_kv4_merge, 1, grid, s, *a, w);
-    }
+    // up to 8 splits of a row are one load's; more, and few rows, spread over waves
+    if (p.n_splits > 8) KV4_DISPATCH_N(k_kv4_merge, 4, dim3((unsigned)rows), s, *a, w);
+    else KV4_DISPATCH_N(k_kv4_merge, 1, dim3((unsigned)((rows + 3) / 4)), s, *a, w);
     SHARD_LAUNCH_CHECK("shard_kv4_attn merge");
   }
   return SHARD_OK;
