@@ -585,7 +585,7 @@ int shard_kv4_attn(const shard_kv4_args* args, void* workspace, size_t workspace
  *     ones by index; NaN logits are not among them (-1 and NaN where a row has
  *     fewer others).
  * Sums in 32 bits.  A row without a logit above -inf, or with +inf or NaN,
- * has NaN results.  top <= 64 and <= vocab.  Workspace:
+ * has NaN results.  Fewer than 2^24 rows; top <= 64 and <= vocab.  Workspace:
  * shard_token_logprobs_workspace bytes, 16-byte aligned (0: none needed);
  * nothing in it needs clearing. */
 size_t shard_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top);

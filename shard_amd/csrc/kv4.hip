@@ -32,6 +32,8 @@
 // the table or the phases and page numbers outside the cache are left out.
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "common.h"
 
 namespace shard {
@@ -1145,9 +1147,11 @@ bool rows_ok(const void* p, int64_t stride, int64_t head_stride) {
   return p && (uintptr_t)p % 16 == 0 && stride >= 0 && head_stride >= 0 && stride % 8 == 0 && head_stride % 8 == 0;
 }
 
-int groups_of(const shard_kv4_args* a) {  // 32-token groups that max_new tokens can touch
-  const int n = !a->cu_seqlens ? 1 : a->max_new > 0 ? a->max_new : a->n_tokens;
-  return n <= 1 ? 1 : (int)(((int64_t)n + 30) / 32 + 1);
+// 32-token groups that max_new tokens can touch; the kernels stride where a launch
+// (2^32 - 1 threads) holds no more.
+int groups_of(const shard_kv4_args* a) {
+  const int n = !a->cu_seqlens ? 1 : a->max_new > 0 ? std::min(a->max_new, a->n_tokens) : a->n_tokens;
+  return n <= 1 ? 1 : std::min((n - 1) / 32 + 2, 1 << 20);
 }
 
 // Row tiles and splits of an attention call.  Workgroups for two a CU (a split
@@ -1179,6 +1183,7 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   if (p.nq != 8 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;
+  if ((int64_t)a->n_tokens * a->n_q_heads >= 1 << 24) sp = 1;  // more rows than a launch of the join takes
   // the nearest power of two
   p.split_shift = 0;
   while ((int64_t)2 << p.split_shift <= kMaxSplits && (int64_t)2 << (2 * p.split_shift) < sp * sp) ++p.split_shift;

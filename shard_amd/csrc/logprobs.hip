@@ -364,8 +364,9 @@ int parts_of(int64_t rows, int64_t vocab) {
   return p < 1 ? 1 : (int)p;
 }
 
+// A launch has at most 2^32 - 1 threads, a row 256.
 bool sizes_ok(int64_t rows, int64_t vocab, int32_t top) {
-  return rows > 0 && rows <= INT32_MAX && vocab > 0 && vocab <= INT32_MAX && top >= 0 && top <= kMaxTop && top <= vocab;
+  return rows > 0 && rows < 1 << 24 && vocab > 0 && vocab <= INT32_MAX && top >= 0 && top <= kMaxTop && top <= vocab;
 }
 
 }  // namespace

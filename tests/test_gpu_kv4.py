@@ -155,6 +155,20 @@ def test_launch_hints_change_nothing(cuda, kw):
     assert torch.equal(k, k2) and torch.equal(v, v2)
 
 
+def test_largest_launch_hints(cuda):
+    """Hints far beyond what the call holds are only hints."""
+    b = Batch([300, 64, 31], [290, 1, 30], 4, 2, 64, seed=15)
+    want_q, want_out = b.append(q=b.d_q), b.attn()
+    want, (k, v) = b.d_cache.clone(), b.read()
+    b.d_cache = b.cache.to(cuda)
+    hint = 2 ** 31 - 1
+    assert torch.equal(b.append(q=b.d_q, max_new=hint), want_q) and torch.equal(b.d_cache, want)
+    k2, v2 = b.read(max_new=hint)
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+    # the bits: old tokens are whatever random bytes say, NaN among them
+    assert torch.equal(b.attn(max_new=hint, max_len=hint).view(torch.int16), want_out.view(torch.int16))
+
+
 def test_append_strided_operands(cuda):
     """q, k and v as slices of one fused projection's rows, and rows at odd places."""
     b = Batch([70, 40], [50, 3], 4, 2, 128, seed=6)

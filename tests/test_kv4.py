@@ -160,3 +160,15 @@ def test_compiled_dispatch_is_built_and_leaves_odd_calls():
         assert d.kv4_attn(*bad) is None
     with pytest.raises(ImportError):
         d.bind("/nowhere/lib.so")
+
+
+def test_rows_beyond_a_launch():
+    """A launch has at most 2^32 - 1 threads: rows of logits are refused there, attention does without splits."""
+    from shard_amd import _lib
+    lib = _lib.load()
+    rows = lambda n: lib.shard_token_logprobs(P, 0, n, 100, 100, None, 0, None, P, None, None, P, 1 << 40, None)
+    assert rows(1 << 24) == -2 and rows(1 << 31) == -2
+    wide = dict(n_q_heads=1024, n_kv_heads=1024, page_stride=1024 * 68 * 128, table_width=1 << 16, table_stride=1 << 16)
+    fits, over = (1 << 14) - 1, 1 << 14   # tokens of 1,024 heads: below 2^24 rows, and 2^24
+    assert lib.shard_kv4_attn_workspace(_args(**wide, batch=fits, n_tokens=fits)) == fits * 1024 * 128 * 130 * 4
+    assert lib.shard_kv4_attn_workspace(_args(**wide, batch=over, n_tokens=over)) == 0
