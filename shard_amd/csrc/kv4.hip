@@ -492,23 +492,34 @@ __device__ __forceinline__ float across_quarters_sum(float v) {
   return a + b;
 }
 
-// Few rows: a workgroup of 4 waves takes 16 NQ rows and a split of the
+// Few rows: a workgroup of 4 waves takes ROWS (4 to 32) rows and a split of the
 // pages; every wave walks its own pages (registers only) and the waves are
 // joined in LDS at the end.  The next page's K is loaded into the registers
 // that the scores have just freed, its V into those of the output's product, so
 // that each is on its way during the other half of the work.
-// A page of a head costs a wave about 360 vector instructions (256 of them expand
-// and scale the 16,384 codes) and 32 matrix ones, 0.7 us; four waves a SIMD hide
-// the memory behind it.  Measured (32 query heads on 8 of 128, fp16, one token):
-// 16 sequences of 16,384 tokens 54 us, 5.3 TB/s of 285 MB; one of 32,768 11 us,
-// 3.4 TB/s, of 2,048 5.5 us: launch and the chain table -> page -> join.
+// Up to 4 (8) rows stand in the 16 columns of a tile 4 (2) times: a column weighs
+// the tokens of its own quarter (half) of every page, a softmax of its own that
+// the end joins, and a lane forms 4 (8) exponentials a page, not 16.  The longer
+// join is worth it from two pages a wave on: graph replays, us, with / without,
+// 4 rows: 64 sequences of 128 to 8,192 tokens (head_dim 64) 24.7 / 26.5, 8 of 2K
+// to 8K 16.9 / 17.4, one of 32K 14.7 / 14.9, one of 2,048 (a page a wave) 8.3 /
+// 8.15; 8 rows: the 64 sequences 26.7 / 27.1, the 8 17.5 / 17.6.
+// A page of a head costs a wave about 380 vector instructions at head_dim 128
+// (256 of them expand and scale the 16,384 codes) and 32 matrix ones; three waves
+// a SIMD hide the memory behind it.  Measured (32 query heads on 8 of 128, fp16,
+// one token): 16 sequences of 16,384 tokens 53 us, 5.4 TB/s of 285 MB; one of
+// 32,768 11 us, 3.3 TB/s, of 2,048 5.2 us: launch and the chain table -> page ->
+// join.
 // Not faster: 8 or 16 waves a workgroup without splits (one sequence of 2,048
 // 13.4 us against 8.2 with the merge), work cut on the device by the sequences'
-// lengths (64 sequences of 128 to 8,192 tokens 27.7 us against 26.9).
-template <class T, int D, int NQ>
-__global__ __launch_bounds__(256, (D == 128 ? 4 : 5) - NQ)
+// lengths (the 64 sequences 27.7 us against 26.9 then).
+template <class T, int D, int ROWS>
+__global__ __launch_bounds__(256, (D == 128 ? 4 : 5) - (ROWS > 16 ? 2 : 1))
 void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   constexpr int WAVES = 4;
+  constexpr int NQ = ROWS > 16 ? ROWS / 16 : 1;     // tiles of 16 columns
+  constexpr int F = ROWS < 16 ? 16 / ROWS : 1;      // columns of a row
+  constexpr int NS = 4 / F;                         // quarters of a page whose tokens a lane weighs
   constexpr int ST = D / 32;  // k-steps of a score, 32-channel blocks
   constexpr int NT = D / 16;  // channel tiles of the output
   __shared__ float sh_acc[WAVES][16 * NQ][D + 4];
@@ -529,19 +540,20 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   const float scale2 = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * 1.4426950408889634f, kLeast);
   const half_t sign = a.scale < 0.f ? (half_t)-1.f : a.scale == 0.f ? (half_t)0.f : (half_t)1.f;
 
-  for (int rt = rt0; rt * 16 * NQ < n_rows; rt += w.row_tiles) {
+  const int fold = F == 1 ? 0 : col / ROWS;         // the lane's share: quarters fold * NS + 0 .. NS - 1
+  for (int rt = rt0; rt * ROWS < n_rows; rt += w.row_tiles) {
     typedef T vec8 __attribute__((ext_vector_type(8)));
     vec8 raw[NQ][ST];
     float sc[NQ], m[NQ], l[NQ];
     int lim[NQ];                      // keys that the lane's row sees
     float4v acc[NQ][NT];
-    const int r0 = rt * 16 * NQ, r1 = min(r0 + 16 * NQ, n_rows) - 1;
+    const int r0 = rt * ROWS, r1 = min(r0 + ROWS, n_rows) - 1;
     // of the tile's rows (uniform)
     const int lim_min = min(max(s.len - s.n + token_of(w, r0) + 1, 0), keys);
     const int lim_max = min(max(s.len - s.n + token_of(w, r1) + 1, 0), keys);
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-      const int r = min(r0 + 16 * t + col, r1);   // columns behind the last row repeat it, unused
+      const int r = min(r0 + 16 * t + (F == 1 ? col : col % ROWS), r1);   // columns behind the last row repeat it, unused
       const int i = token_of(w, r), h = r - i * group;
       lim[t] = min(max(s.len - s.n + i + 1, 0), keys);
       const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
@@ -628,19 +640,31 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
       half8 P[NQ][2];
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
+        float4v X[NS];                                // the lane's own scores
+        if constexpr (F == 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float lo = fold & 1 ? S[t][1][i] : S[t][0][i], hi = fold & 1 ? S[t][3][i] : S[t][2][i];
+            X[0][i] = fold & 2 ? hi : lo;
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) X[u][i] = F == 2 && fold ? S[t][(u + NS) & 3][i] : S[t][u][i];
+        }
         if (none || (tile + 1) * kPage > lim_min) {
-          const int seen = none ? 0 : lim[t];
+          const int seen = (none ? 0 : lim[t]) - tile * kPage - 16 * NS * fold - 4 * kq;
 #pragma unroll
-          for (int sub = 0; sub < 4; ++sub)
+          for (int u = 0; u < NS; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              S[t][sub][i] = tile * kPage + 16 * sub + 4 * kq + i < seen ? S[t][sub][i] : -INFINITY;
+            for (int i = 0; i < 4; ++i) X[u][i] = 16 * u + i < seen ? X[u][i] : -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int sub = 0; sub < 4; ++sub)
+        for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, S[t][sub][i]);
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, X[u][i]);
         mx = across_quarters_max(mx) * sc[t];
         if (__builtin_amdgcn_ballot_w64(mx > m[t] + 8.f)) {
           const float to = fmaxf(m[t], mx);
@@ -652,14 +676,27 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
         }
         const float base = m[t] == -INFINITY ? 0.f : m[t];
         float sum = 0.f;
+        uint32_t pairs[NS][2];
 #pragma unroll
-        for (int sub = 0; sub < 4; ++sub)
+        for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][sub][i], sc[t], -base));
+          for (int i = 0; i < 4; i += 2) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(X[u][i], sc[t], -base));
+            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(X[u][i + 1], sc[t], -base));
             sum += p;
-            P[t][sub >> 1][(sub & 1) * 4 + i] = (half_t)p;
+            sum += p2;
+            pairs[u][i / 2] = __builtin_bit_cast(uint32_t, half2v{(half_t)p, (half_t)p2});
           }
+        // the other quarters' tokens are not the column's: weights of 0
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          uint4 words;
+          words.x = F == 1 || fold == 2 * s2 / NS ? pairs[2 * s2 % NS][0] : 0u;
+          words.y = F == 1 || fold == 2 * s2 / NS ? pairs[2 * s2 % NS][1] : 0u;
+          words.z = F == 1 || fold == (2 * s2 + 1) / NS ? pairs[(2 * s2 + 1) % NS][0] : 0u;
+          words.w = F == 1 || fold == (2 * s2 + 1) / NS ? pairs[(2 * s2 + 1) % NS][1] : 0u;
+          P[t][s2] = __builtin_bit_cast(half8, words);
+        }
         l[t] += sum;
       }
 #pragma unroll
@@ -695,38 +732,62 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
       for (int n = 0; n < NT; ++n) *(float4v*)&sh_acc[wave][16 * t + col][16 * n + 4 * kq] = acc[t][n];
     }
     __syncthreads();
-    for (int u = tid; u < 16 * NQ * (D / 8); u += 64 * WAVES) {
-      const int rr = u / (D / 8), ch = (u % (D / 8)) * 8;
-      const int r = rt * 16 * NQ + rr;
-      if (r >= n_rows) continue;
+    const auto write = [&](int r, int ch, auto x, float M, float lt) {  // some channels of a row
+      constexpr int N = sizeof(x) / sizeof(float);
       const int i = token_of(w, r), h = g * group + r - i * group;
-      float M = sh_m[0][rr];
-#pragma unroll
-      for (int v = 1; v < WAVES; ++v) M = fmaxf(M, sh_m[v][rr]);
-      const float base = M == -INFINITY ? 0.f : M;
-      float x[8] = {}, lt = 0.f;
-#pragma unroll
-      for (int v = 0; v < WAVES; ++v) {
-        const float f = exp2f(sh_m[v][rr] - base);
-        lt += f * sh_l[v][rr];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += f * sh_acc[v][rr][ch + j];
-      }
       const int64_t row = (int64_t)(s.row0 + i) * a.n_q_heads + h;
       if (w.n_splits == 1) {
         const float inv = lt == 0.f ? 0.f : 1.f / lt;   // a row that sees no key: zeros
+        typedef T vec __attribute__((ext_vector_type(N)));
+        vec o;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= inv;
-        store8((T*)a.out + row * D + ch, x);
+        for (int j = 0; j < N; ++j) o[j] = (T)(x[j] * inv);
+        *(vec*)((T*)a.out + row * D + ch) = o;
       } else {
         const int64_t part = row * w.n_splits + split;
-        float4v* o = (float4v*)(w.acc + part * D + ch);
-        o[0] = float4v{x[0], x[1], x[2], x[3]};
-        o[1] = float4v{x[4], x[5], x[6], x[7]};
+        *(decltype(x)*)(w.acc + part * D + ch) = x;
         if (ch == 0) {
           w.m[part] = M;
           w.l[part] = lt;
         }
+      }
+    };
+    if constexpr (F == 1) {
+      typedef float float8v __attribute__((ext_vector_type(8)));
+      for (int u = tid; u < ROWS * (D / 8); u += 64 * WAVES) {
+        const int rr = u / (D / 8), ch = (u % (D / 8)) * 8;
+        if (rt * ROWS + rr >= n_rows) continue;
+        float M = sh_m[0][rr];
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) M = fmaxf(M, sh_m[v][rr]);
+        const float base = M == -INFINITY ? 0.f : M;
+        float8v x{};
+        float lt = 0.f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+          const float k = __builtin_amdgcn_exp2f(sh_m[v][rr] - base);
+          lt += k * sh_l[v][rr];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] += k * sh_acc[v][rr][ch + j];
+        }
+        write(rt * ROWS + rr, ch, x, M, lt);
+      }
+    } else {
+      // a row a wave, its weights in the lanes of 16
+      typedef float pair __attribute__((ext_vector_type(D / 64)));
+      const int p = lane % (WAVES * F), ch = lane * (D / 64);
+      for (int rr = wave; rr < ROWS && rt * ROWS + rr < n_rows; rr += WAVES) {
+        pair y[WAVES * F];
+#pragma unroll
+        for (int u = 0; u < WAVES * F; ++u) y[u] = *(const pair*)&sh_acc[u / F][rr + ROWS * (u % F)][ch];
+        const float mp = sh_m[p / F][rr + ROWS * (p % F)], lp = sh_l[p / F][rr + ROWS * (p % F)];
+        const float M = row16_reduce(mp, OpMax());
+        const float k = __builtin_amdgcn_exp2f(mp - (M == -INFINITY ? 0.f : M));
+        const float lt = row16_reduce((lane & 15) < WAVES * F ? k * lp : 0.f, OpAdd());
+        pair x{};
+#pragma unroll
+        for (int u = 0; u < WAVES * F; ++u) x += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k), u)) * y[u];
+        write(rt * ROWS + rr, ch, x, M, lt);
       }
     }
   }
@@ -1164,7 +1225,7 @@ int groups_of(const shard_kv4_args* a) {
 // tiles: 2 x 8,000 with 12 / 32 new tokens (48 / 128 rows) 20.3 / 27.1 by rows,
 // 26.6 / 33.7 by tiles; 16 x 4,000 with 16 (64 rows) 40.8 / 52.1.
 struct AttnPlan {
-  int nq;         // 16-row groups of a workgroup: 1 or 2 (rows), 8 (tile)
+  int rows;       // of a workgroup: 4, 8, 16 or 32 (rows kernel), 128 (tile kernel)
   int row_tiles, n_splits, split_shift;
 };
 AttnPlan plan_of(const shard_kv4_args* a) {
@@ -1172,15 +1233,15 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   const int group = a->n_q_heads / a->n_kv_heads;
   const int64_t n = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
   const int64_t rows = (a->cu_seqlens ? n : 1) * group;
-  p.nq = rows <= 16 ? 1 : rows <= 128 ? 2 : 8;
-  p.row_tiles = (int)((rows + 16 * p.nq - 1) / (16 * p.nq));
+  p.rows = rows <= 16 ? 16 : rows <= 128 ? 32 : 128;
+  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
   const int64_t cap = (int64_t)a->table_width * kPage;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t tiles = (len + kPage - 1) / kPage;
   const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
   int64_t sp = (512 + wg - 1) / wg;
   const int64_t even = (tiles + 63) / 64;
-  if (p.nq != 8 && even > sp) sp = even;
+  if (p.rows != 128 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;
   if ((int64_t)a->n_tokens * a->n_q_heads >= 1 << 24) sp = 1;  // more rows than a launch of the join takes
@@ -1188,6 +1249,8 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   p.split_shift = 0;
   while ((int64_t)2 << p.split_shift <= kMaxSplits && (int64_t)2 << (2 * p.split_shift) < sp * sp) ++p.split_shift;
   p.n_splits = 1 << p.split_shift;
+  // few rows fold where a wave has more than a page (k_kv4_attn_rows)
+  if (rows <= 8 && tiles > kMinTiles * p.n_splits) p.rows = rows <= 4 ? 4 : 8;
   return p;
 }
 
@@ -1300,8 +1363,10 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   }
   const hipStream_t s = (hipStream_t)stream;
   const dim3 rows_grid((unsigned)(w.n_splits * w.row_tiles), a->n_kv_heads, a->batch);
-  if (p.nq == 1) KV4_DISPATCH_N(k_kv4_attn_rows, 1, rows_grid, s, *a, w);
-  else if (p.nq == 2) KV4_DISPATCH_N(k_kv4_attn_rows, 2, rows_grid, s, *a, w);
+  if (p.rows == 4) KV4_DISPATCH_N(k_kv4_attn_rows, 4, rows_grid, s, *a, w);
+  else if (p.rows == 8) KV4_DISPATCH_N(k_kv4_attn_rows, 8, rows_grid, s, *a, w);
+  else if (p.rows == 16) KV4_DISPATCH_N(k_kv4_attn_rows, 16, rows_grid, s, *a, w);
+  else if (p.rows == 32) KV4_DISPATCH_N(k_kv4_attn_rows, 32, rows_grid, s, *a, w);
   else {
     const dim3 grid((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch);
     KV4_DISPATCH(k_kv4_attn_tile, grid, s, *a, w);

@@ -285,6 +285,25 @@ def test_attention(cuda, total, new, H, G, D, type):
         _check_attention(b, b.attn(**kw))
 
 
+FOLDED = [  # total, new, H, G, D: few rows a kv head and more than four pages a split
+    ([400, 321], [1, 1], 256, 256, 64), ([417, 330], [2, 1], 512, 256, 64), ([500, 1], [1, 1], 1024, 256, 64),
+    ([385, 200], [1, 1], 2048, 256, 64), ([400, 390], [2, 0], 768, 256, 64), ([338, 337], [3, 3], 256, 256, 64),
+    ([2300], [1], 256, 64, 64), ([2300], [3], 128, 64, 64), ([700, 10, 64, 65, 330, 450, 129, 1], [1] * 8, 256, 64, 128),
+    ([350, 10, 64, 65, 330, 450, 129, 1], [1] * 8, 448, 64, 128),
+]
+
+
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+@pytest.mark.parametrize("total,new,H,G,D", FOLDED, ids=str)
+def test_attention_few_rows_many_pages(cuda, total, new, H, G, D, type):
+    """A column of the scores' tiles for every quarter of a page; hints below what the call holds too."""
+    b = Batch(total, new, H, G, D, type, seed=len(total) + H, wide=2).fill()
+    for kw in (dict(max_new=max(new)), dict(max_new=max(new), max_len=max(total)), dict(max_new=1)):
+        if set(new) == {1}:
+            kw["cu_seqlens"] = None
+        _check_attention(b, b.attn(**kw))
+
+
 def test_attention_scale_and_large_scores(cuda):
     """Scores of hundreds: one key takes all; and a scale of 0: the mean."""
     b = Batch([200], [3], 8, 2, 128, seed=3).fill()
