@@ -805,11 +805,11 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
 // scores of page n + 1).  The second workgroup of a CU runs one while the first
 // runs the other.
 //
-// Measured: a whole prompt of 8,192 tokens, 32 heads on 8, 560 us, 0.98 PFLOP/s
+// Measured: a whole prompt of 8,192 tokens, 32 heads on 8, 570 us, 0.96 PFLOP/s
 // of its causal half; an 8192^3 fp16 product of the library reaches 1.17 on the
 // same card.  The clock falls to 1.85 GHz under it; at that clock the matrix pipe
 // is busy half the time.  Not faster: 256 rows in two groups of waves a phase
-// apart (568), 64 rows a wave (1,073: registers), scores of the next page
+// apart (568 us against 560 then), 64 rows a wave (1,073: registers), scores of the next page
 // between the maxima and the weights of this one (570).
 // Byte offsets are formed once: the loop adds a page's address and a buffer's.
 template <int W>
@@ -1103,7 +1103,7 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   }
 }
 
-// Joins the splits of a row; 3.3 to 4.7 us, latency, up to 64 splits.  WAVES waves
+// Joins the splits of a row; 2.9 to 4.8 us, latency, up to 64 splits.  WAVES waves
 // take a row's splits in turn, several a load (16 bytes a lane); every wave forms
 // all weights itself (128 splits at most: two a lane).  Nothing here waits for
 // lengths: splits without keys have a maximum of -inf, their sums are whatever
