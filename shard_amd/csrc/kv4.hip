@@ -809,8 +809,8 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
 // of its causal half; an 8192^3 fp16 product of the library reaches 1.17 on the
 // same card.  The clock falls to 1.85 GHz under it; at that clock the matrix pipe
 // is busy half the time.  Not faster: 256 rows in two groups of waves a phase
-// apart (568 us against 560 then), 64 rows a wave (1,073: registers), scores of the next page
-// between the maxima and the weights of this one (570).
+// apart (568 us against 560 then), 64 rows a wave (1,073: registers), scores of
+// the next page between the maxima and the weights of this one (570).
 // Byte offsets are formed once: the loop adds a page's address and a buffer's.
 template <int W>
 struct Words {
