@@ -49,7 +49,7 @@ struct Seq {
   int cap;          // tokens its block table can hold
 };
 
-__device__ __forceinline__ Seq seq_of(const shard_kv4_args& a, int b) {
+__device__ __forceinline__ Seq seq_of(const shard_kv4_args& a, int b, int len) {
   Seq s;
   int c0 = b, c1 = b + 1;
   if (a.cu_seqlens) {
@@ -60,10 +60,11 @@ __device__ __forceinline__ Seq seq_of(const shard_kv4_args& a, int b) {
   c1 = min(max(c1, c0), a.n_tokens);
   s.row0 = c0;
   s.n = c1 - c0;
-  s.len = max(a.seq_lens[b], 0);
+  s.len = max(len, 0);
   s.cap = a.table_width * kPage;
   return s;
 }
+__device__ __forceinline__ Seq seq_of(const shard_kv4_args& a, int b) { return seq_of(a, b, a.seq_lens[b]); }
 
 // The page that holds token t of sequence b (t < cap), -1 if the table names none.
 __device__ __forceinline__ int page_of(const shard_kv4_args& a, int b, int t) {
@@ -416,6 +417,7 @@ struct AttnWork {
   int n_splits, split_shift;    // a power of two
   int group, group_shift;       // query heads of a kv head; -1: no power of two
   int row_tiles;                // workgroups along a sequence's rows
+  float sorted;                 // 16 / longest length where longer sequences go first, or 0
 };
 
 // Tiles (pages) a split of a sequence of `tiles` takes: at least kMinTiles, one
@@ -429,6 +431,20 @@ __device__ __forceinline__ int tiles_per_split(const AttnWork& w, int tiles) {
 // costs a launch's first instructions about 150 cycles each.)
 __device__ __forceinline__ int token_of(const AttnWork& w, int r) {
   return w.group_shift >= 0 ? r >> w.group_shift : r / w.group;
+}
+
+// The z-th sequence by length, longest first, of z's 64 (lengths in 16 classes,
+// equal ones in their order), and its length.
+__device__ __forceinline__ int by_length(const shard_kv4_args& a, const AttnWork& w, int z, int lane, int& len) {
+  const int z0 = z & ~63, mine = z0 + lane < a.batch ? a.seq_lens[z0 + lane] : 0;
+  const int of = z0 + lane < a.batch ? (int)fminf((float)max(mine, 0) * w.sorted, 15.f) : -1;
+  int k = z & 63, c = 15;
+  uint64_t in = __builtin_amdgcn_ballot_w64(of == c);
+  for (int n; c > 0 && k >= (n = __builtin_popcountll(in)); in = __builtin_amdgcn_ballot_w64(of == --c)) k -= n;
+  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+  const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(of == c && before == k));
+  len = __builtin_amdgcn_readlane(mine, at);
+  return z0 + at;
 }
 
 // A split past a sequence's end: the merge reads that it has nothing.  Rows tid,
@@ -526,9 +542,12 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   __shared__ float sh_m[WAVES][16 * NQ], sh_l[WAVES][16 * NQ];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
-  const int g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y;
   const int split = blockIdx.x & (w.n_splits - 1), rt0 = blockIdx.x >> w.split_shift;
-  const Seq s = seq_of(a, b);
+  int b = blockIdx.z, len;
+  if (w.sorted != 0.f) b = by_length(a, w, b, lane, len);
+  else len = a.seq_lens[b];
+  const Seq s = seq_of(a, b, len);
   const int group = w.group;
   const int n_rows = s.n * group;
   const int keys = min(s.len, s.cap);
@@ -1220,13 +1239,18 @@ int groups_of(const shard_kv4_args* a) {
 // rows, so that a batch of uneven lengths ends together.  Measured (graph
 // replays, us; head_dim 128, 32 on 8 heads): 1 x 32K with 256 / 512 / 768
 // workgroups 15.5 / 15.3 / 17.0, 8 sequences of 2K to 8K 20.9 / 17.3 / 18.5;
-// 16 x 16K with 32 / 64 / 128 tiles at most 64.8 / 60.2 / 60.0, 64 sequences
-// of 128 to 8,192 tokens (head_dim 64) 27.3 / 26.9 / 36.3.  Rows by rows or by
-// tiles: 2 x 8,000 with 12 / 32 new tokens (48 / 128 rows) 20.3 / 27.1 by rows,
+// 16 x 16K with 32 / 64 / 128 tiles at most 64.8 / 60.2 / 60.0.  Rows by rows or
+// by tiles: 2 x 8,000 with 12 / 32 new tokens (48 / 128 rows) 20.3 / 27.1 by rows,
 // 26.6 / 33.7 by tiles; 16 x 4,000 with 16 (64 rows) 40.8 / 52.1.
+// With several workgroups a CU those of longer sequences start first, and 32
+// tiles are a split's most where that makes 2,048 workgroups or fewer.  Without /
+// with both: 64 sequences of 128 to 8,192 tokens at head_dim 64 24.9 / 23.9
+// (either alone: 24.0 and 25.2), at 128 39.8 / 37.9, 256 of 62 to 4,000 74.5 /
+// 67.3, 100 of 250 to 16,000 60.7 / 56.5; equal lengths, 128 of 3,000, 83.6 / 84.4.
 struct AttnPlan {
   int rows;       // of a workgroup: 4, 8, 16 or 32 (rows kernel), 128 (tile kernel)
   int row_tiles, n_splits, split_shift;
+  float sorted;
 };
 AttnPlan plan_of(const shard_kv4_args* a) {
   AttnPlan p;
@@ -1240,7 +1264,8 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   const int64_t tiles = (len + kPage - 1) / kPage;
   const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
   int64_t sp = (512 + wg - 1) / wg;
-  const int64_t even = (tiles + 63) / 64;
+  int64_t even = (tiles + 63) / 64;
+  if (wg >= 512 && even > 1 && 2 * even * wg <= 2048) even *= 2;  // room to even out
   if (p.rows != 128 && even > sp) sp = even;
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;
@@ -1249,6 +1274,8 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   p.split_shift = 0;
   while ((int64_t)2 << p.split_shift <= kMaxSplits && (int64_t)2 << (2 * p.split_shift) < sp * sp) ++p.split_shift;
   p.n_splits = 1 << p.split_shift;
+  // several workgroups a CU: the longest first
+  p.sorted = a->batch > 1 && wg * p.n_splits >= 1024 ? 16.f / len : 0.f;
   // few rows fold where a wave has more than a page (k_kv4_attn_rows)
   if (rows <= 8 && tiles > kMinTiles * p.n_splits) p.rows = rows <= 4 ? 4 : 8;
   return p;
@@ -1345,6 +1372,7 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   AttnWork w{};
   w.n_splits = p.n_splits;
   w.split_shift = p.split_shift;
+  w.sorted = p.sorted;
   w.group = a->n_q_heads / a->n_kv_heads;
   w.group_shift = w.group & (w.group - 1) ? -1 : __builtin_ctz(w.group);
   w.row_tiles = p.row_tiles;

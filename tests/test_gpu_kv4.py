@@ -304,6 +304,23 @@ def test_attention_few_rows_many_pages(cuda, total, new, H, G, D, type):
         _check_attention(b, b.attn(**kw))
 
 
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,most,G,H,D", [(70, 1, 16, 64, 64), (130, 3, 8, 16, 64), (65, 9, 16, 32, 128), (64, 1, 32, 32, 64)], ids=str)
+def test_attention_of_many_uneven_sequences(cuda, B, most, G, H, D, type):
+    """Workgroups that take sequences by length: more than 64 of them, empty ones, equal lengths, hints too short."""
+    g = torch.Generator().manual_seed(B)
+    total = [int(n) for n in torch.randint(0, 200, (B,), generator=g)]
+    total[3:9] = [0, 1, 64, 64, 64, 350]
+    if most == 1:
+        total = [max(n, 1) for n in total]
+    new = [min(n, 1 + i % most) for i, n in enumerate(total)]
+    b = Batch(total, new, H, G, D, type, seed=B, wide=1).fill()
+    for kw in (dict(max_new=most, max_len=max(total)), dict(max_new=most), dict(max_new=1, max_len=30)):
+        if most == 1:
+            kw["cu_seqlens"] = None
+        _check_attention(b, b.attn(**kw))
+
+
 def test_attention_scale_and_large_scores(cuda):
     """Scores of hundreds: one key takes all; and a scale of 0: the mean."""
     b = Batch([200], [3], 8, 2, 128, seed=3).fill()
