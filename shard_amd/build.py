@@ -55,7 +55,7 @@ def dispatch_command(out: str):
             "-isystem", os.path.join(root, "include"),
             "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
             "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "dispatch.cpp"), "-o", out,
-            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10"]
 
 
 def build(verbose: bool = False, jobs: int = 4) -> str:
