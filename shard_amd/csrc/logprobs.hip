@@ -161,7 +161,8 @@ void k_logprobs(const LogprobArgs a) {
   };
   uint32_t all_best = 0;
   float only[VEC];   // the granule of a thread that has one alone
-  for (int q = 0; q < kSlots; ++q) {
+  const int slots = own > 1 ? kSlots : 1;
+  for (int q = 0; q < slots; ++q) {
     best = -INFINITY;
     bool any = false;
     const int64_t i1 = (q + 1) * size < own ? (q + 1) * size : own;
