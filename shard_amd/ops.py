@@ -1200,7 +1200,8 @@ def token_logprobs(logits, tokens=None, top=0):
     below V; None without tokens), of the rows' distributions, and of their
     most probable tokens, equal ones by index (top up to 64).  A row without a
     logit above -inf, or with +inf or NaN, has NaN log probabilities; NaN
-    logits are never among the top (id -1 where a row has too few others)."""
+    logits are never among the top (id -1 where a row has too few others).
+    For answers, not for training: no gradient flows back."""
     direct = _direct or _bind_direct()
     if direct and logits.is_cuda:
         dev = _current_device()
