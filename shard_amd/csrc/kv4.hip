@@ -400,14 +400,17 @@ void k_kv4_read(const shard_kv4_args a) {
 // Scores are taken transposed, S^T = K Q^T (16 tokens x 16 rows an MFMA), so
 // that a lane's score registers hold four tokens of ONE row, and after the
 // softmax they are the right operand of O^T = V^T P^T as they stand.
-// The maximum that a row's weights refer to moves only where a weight would
-// exceed 2^8 (far inside fp16's range): most pages rescale no sums.
-// P is rounded to fp16 (2^-11 of each weight; the sums are fp32); the cache's
-// values are exact.  bf16 queries are scaled by a power of two a row (their
+// A row's weights are 2^(score - m), m at most kLead below the largest score so
+// far and moved only where a weight would exceed 2^kMost: most pages rescale no
+// sums, and the largest weight lies between 2^kLead and 2^kMost, fp16's upper end.
+// P is rounded to fp16: 2^-11 of each weight down to 2^-(14 + kLead) of a row's
+// largest, 2^-(25 + kLead) of that largest below, so that what many keys far
+// below one key add up to is kept; the sums are fp32.  The cache's values are exact.  bf16 queries are scaled by a power of two a row (their
 // largest below 2) and are then exact in fp16 down to 2^-17 of that largest
 // (below it they lose bits, 2^-26 of the largest at most); the power goes back
 // in through the softmax scale.
 // --------------------------------------------------------------------------
+constexpr float kLead = 11.f, kMost = 15.f;
 constexpr float kLeast = 1.17549435e-38f;  // a factor of scores is never 0: -inf stays what it is
 
 struct AttnWork {
@@ -685,8 +688,8 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, X[u][i]);
         mx = across_quarters_max(mx) * sc[t];
-        if (__builtin_amdgcn_ballot_w64(mx > m[t] + 8.f)) {
-          const float to = fmaxf(m[t], mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m[t] + kMost)) {
+          const float to = fmaxf(m[t], mx - kLead);
           const float alpha = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.f : to));
           m[t] = to;
           l[t] *= alpha;
@@ -1031,8 +1034,8 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
         float other, mine;
         perm32_swap(mx, mine, other);
         mx = fmaxf(mine, other) * sc;
-        if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
-          const float to = fmaxf(m, mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + kMost)) {
+          const float to = fmaxf(m, mx - kLead);
           const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
           m = to;
           l *= alpha;

@@ -539,3 +539,49 @@ def test_compiled_and_plain_dispatch_agree(cuda, type, monkeypatch):
     assert len(results[0]) == len(results[1])
     for x, y in zip(*results):
         assert x.dtype == y.dtype and x.shape == y.shape and x.device == y.device and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+@pytest.mark.parametrize("n,new,H,G,D", [(8192, 1, 64, 64, 64), (8192, 1, 512, 64, 64), (8192, 3, 8, 1, 128), (8192, 4096, 32, 8, 64),
+                                         (4096, 2048, 32, 8, 128)], ids=str)
+@pytest.mark.parametrize("gap", [17.4, 22.7, 24.9, 27.0])
+def test_attention_many_keys_far_below_one(cuda, n, new, H, G, D, type, gap):
+    """One key has almost all of the weight and a value of zero (as models' first tokens have): the output is what
+    thousands of keys, 2^-gap of its weight and less, add up to."""
+    from shard_amd import ops
+    g = torch.Generator().manual_seed(n + new)
+    k, v = torch.zeros(n, D), torch.ones(n, D) * 0.5
+    k[0, 0] = 6.0
+    k[1:, 1] = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6])[torch.randint(0, 8, (n - 1,), generator=g)]
+    v[1:, ::3] = torch.tensor([0.5, 1, 1.5, 2, 3])[torch.randint(0, 5, v[1:, ::3].shape, generator=g)]
+    k[1:, 2], v[:, 31::32] = 6.0, 6.0                              # scale 1: every value is held as it is
+    v[0] = 0
+    q = torch.zeros(new, D)
+    q[:, 0], q[:, 1] = 1, -1 / 64                                  # the other keys within 2^-(gap / 64) of each other
+    dtype = TYPES[type]
+    pages = n // 64
+    cache = ops.kv4_cache(pages, G, D)
+    table = torch.randperm(pages, generator=g).int()[None].to(cuda)
+    lens, cu = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in ([n], [0, n]))
+    still = torch.zeros(n, D // 2, 2, device=cuda)
+    still[..., 0] = 1                                              # no rotation
+    held = [x.to(cuda, dtype)[:, None].expand(n, G, D) for x in (k, v)]
+    ops.kv4_append(*held, cache, table, lens, still, cu_seqlens=cu)
+    assert all(torch.equal(a, b) for a, b in zip(ops.kv4_read(cache, table, lens, n, dtype=dtype, cu_seqlens=cu), held))
+    scale = float(np.float32(gap * np.log(2) / 6))
+    out = ops.kv4_attn(q.to(cuda, dtype)[:, None].expand(new, H, D), cache, table, lens, scale=scale, max_new=new, max_len=n,
+                       cu_seqlens=torch.tensor([0, new], dtype=torch.int32, device=cuda))
+    assert bool((out == out[:, :1]).all())                         # every head has the same
+    rows = torch.arange(max(0, new - 64), new)
+    s = q[rows].double() @ k.double().T * scale
+    s = s.masked_fill(torch.arange(n) > (n - new + rows)[:, None], -np.inf)
+    w = torch.softmax(s, -1)
+    want = w @ v.double()
+    # scores: the largest is gap ln 2 < 19, each off by (D + 4) 2^-24 of it.  Weights: fp16, 2^-11 each; below
+    # 2^-25 of the largest 2^-36 of the largest, which is all but 1 of their sum.  Their sums as in _check_attention.
+    rel = 2 * (D + 4) * 2.0 ** -24 * 19 + 2.0 ** -11 + (n + 200) * 2.0 ** -24
+    err = 2 * rel * want + n * 2.0 ** -36 * float(v.max())
+    off = (out[rows.to(cuda), 0].double().cpu() - want).abs()
+    tol = err + torch.finfo(dtype).eps / 2 * (want + err) + 2.0 ** -25
+    print(f"largest error {off.max():.2e}, {(off / tol).max():.2f} of the bound", flush=True)
+    assert bool((off <= tol).all())
