@@ -9,6 +9,8 @@
 // The difference x - M is taken first, so that its rounding is relative to
 // itself and a row of equal logits far from 0 loses nothing.
 //
+// M is the thread's true maximum, the row's after the joins.
+//
 // Top k: every thread also notes the largest logit of each eighth of its
 // elements (a slot).  The k-th largest of the 256 threads' largest bounds the
 // row's k-th largest from below, so only the slots that reach it (about k of
@@ -112,7 +114,7 @@ struct Stats {
 // the sums at another maximum (no smaller than s.M)
 __device__ __forceinline__ void move_to(Stats& s, float M) {
   const float d = fmaxf((s.M - M) * kLog2e, -1e4f);
-  const float f = exp2f(d);
+  const float f = __builtin_amdgcn_exp2f(d);
   s.t = f * (s.t + d * s.l);
   s.l *= f;
   s.M = M;
@@ -148,14 +150,17 @@ void k_logprobs(const LogprobArgs a) {
 
   Stats s{kLowest, 0.f, 0.f};
   float best = -INFINITY;
-  // M follows the maximum only where that is 8 ahead (terms of at most e^8): few
-  // granules rescale.
+  // M is the largest so far, so that no term is above 1: an M further down would
+  // make the sums of a row that one logit outweighs large and cancel them in the
+  // end, 2^-24 of 8 nats instead of 2^-24.  2,048 rows of 128,256 bf16 logits 114.1
+  // us in a graph, 113.2 with M moved only where the maximum is 8 ahead, 120.4 with
+  // one maximum for four granules.
   const auto eat = [&](const float(&x)[VEC]) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < VEC; ++i) m = fmaxf(m, x[i]);
     best = fmaxf(best, m);
-    if (m > s.M + 8.f) move_to(s, m);
+    if (m > s.M) move_to(s, m);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float d = (x[i] - s.M) * kLog2e;

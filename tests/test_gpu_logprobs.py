@@ -196,3 +196,28 @@ def test_refusals(cuda):
         ops.token_logprobs(x[:, :0], t)
     assert ops.token_logprobs(x[:0], t[:0], top=2)[2].shape == (0, 2)
     assert np.isfinite(ops.token_logprobs(x, t)[0].cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("type", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,at", [(1, 20000), (1200, 8192), (1200, 39999), (3000, 3073)])
+def test_one_logit_above_a_thread_s_first(cuda, rows, at, type):
+    """A token nearly certain, found by a thread after a lesser one: errors of a few 2^-24, signs as they must be."""
+    from shard_amd import ops
+    V, u = 40000, 2.0 ** -24
+    x = torch.full((rows, V), -90.0, dtype=TYPES[type], device=cuda)
+    x[:, at % 2048 if type != "fp32" else at % 1024] = 0            # in the same thread's first granule where a workgroup has a row
+    tok = torch.full((rows,), at, device=cuda)
+    for i in range(8, 129):
+        d = i / 16
+        x[:, at] = d
+        lp, entropy, top_lp, ids = (t.cpu() for t in ops.token_logprobs(x, tok, top=1))
+        tail = math.exp(-d)
+        want, want_e = -math.log1p(tail), math.log1p(tail) + d * tail / (1 + tail)
+        assert bool((ids == at).all()) and torch.equal(lp, top_lp[:, 0])
+        assert bool((lp <= 0).all()) and bool((entropy >= 0).all())
+        # the sum 1 + tail rounds once (2^-24); the tail's exponent is off by 2 roundings of it and exp2 by 2 units of
+        # its result; ln by 2 units, the last differences a rounding of the result each
+        tail_off = tail * (2 * d + 8)
+        assert float((lp.double() - want).abs().max()) <= u * (1 + tail_off + 6 * -want), d
+        # E[d] = d tail / (1 + tail): its own three roundings and the sum's
+        assert float((entropy.double() - want_e).abs().max()) <= u * (1 + tail_off + 6 * want_e + d * tail * (2 * d + 12)), d
