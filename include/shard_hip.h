@@ -543,7 +543,7 @@ typedef struct shard_kv4_args {
   int64_t v_stride, v_head_stride;
   const float* phases;              /* (n_phases, head_dim / 2, 2) cos, sin */
   int32_t n_phases;
-  float scale;                      /* of the scores */
+  float scale;                      /* of the scores: a number, of at most 2e38 */
   void* q_out;
   void* k_out;
   void* v_out;

@@ -30,6 +30,7 @@
 // block_table[b][t / 64], slot t % 64.  Everything read from device memory is
 // checked where it is used: rows and lengths are clamped, positions outside
 // the table or the phases and page numbers outside the cache are left out.
+#include <math.h>
 #include <stdio.h>
 
 #include <algorithm>
@@ -410,6 +411,7 @@ void k_kv4_read(const shard_kv4_args a) {
 // (below it they lose bits, 2^-26 of the largest at most); the power goes back
 // in through the softmax scale.
 // --------------------------------------------------------------------------
+constexpr float kMostScale = 2e38f;
 constexpr float kLead = 11.f, kMost = 15.f;
 constexpr float kLeast = 1.17549435e-38f;  // a factor of scores is never 0: -inf stays what it is
 
@@ -1369,6 +1371,7 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   const int rc = check_attn(a);
   if (rc) return rc;
   if (!rows_ok(a->q, a->q_stride, a->q_head_stride) || !a->out || (uintptr_t)a->out % 16) return SHARD_ERR_ARG;
+  if (!(fabsf(a->scale) <= kMostScale)) return SHARD_ERR_ARG;  // NaN, or infinite times log2(e)
   if (a->n_tokens == 0) return SHARD_OK;
   const AttnPlan p = plan_of(a);
   const int64_t rows = (int64_t)a->n_tokens * a->n_q_heads;

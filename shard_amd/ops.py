@@ -1177,9 +1177,13 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or out.data_ptr() & 15:
         raise TypeError(f"out: expected {tuple(q.shape)} contiguous {q.dtype}, 16-byte aligned")
+    if scale is None:
+        scale = D ** -0.5
+    elif not abs(scale) <= 2e38:
+        raise ValueError(f"scale: expected a finite number of at most 2e38, got {scale}")
     if T:
         args = _lib.KV4_PACK.pack(block_table.shape[0], T, H, G, D, code, *fields, *q_at, *(0,) * 6, 0, 0,
-                                  D ** -0.5 if scale is None else scale, 0, 0, 0, out.data_ptr())
+                                  scale, 0, 0, 0, out.data_ptr())
         need = lib.shard_kv4_attn_workspace(args)
         ws = cache.new_empty(need) if need else None
         _launch_on(dev, "shard_kv4_attn", lib.shard_kv4_attn, args, ws.data_ptr() if need else None, need)

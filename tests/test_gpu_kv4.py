@@ -585,3 +585,13 @@ def test_attention_many_keys_far_below_one(cuda, n, new, H, G, D, type, gap):
     tol = err + torch.finfo(dtype).eps / 2 * (want + err) + 2.0 ** -25
     print(f"largest error {off.max():.2e}, {(off / tol).max():.2f} of the bound", flush=True)
     assert bool((off <= tol).all())
+
+
+def test_scale_is_a_number(cuda):
+    b = Batch([70], [3], 4, 2, 64).fill()
+    for bad in (float("nan"), float("inf"), -float("inf"), 1e300):
+        with pytest.raises(ValueError):
+            b.attn(scale=bad)
+        with pytest.raises(ValueError):
+            b.attn(scale=bad, out=torch.empty_like(b.d_q))
+    _check_attention(b, b.attn(scale=1), scale=1)

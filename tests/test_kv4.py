@@ -172,3 +172,13 @@ def test_rows_beyond_a_launch():
     fits, over = (1 << 14) - 1, 1 << 14   # tokens of 1,024 heads: below 2^24 rows, and 2^24
     assert lib.shard_kv4_attn_workspace(_args(**wide, batch=fits, n_tokens=fits)) == fits * 1024 * 128 * 130 * 4
     assert lib.shard_kv4_attn_workspace(_args(**wide, batch=over, n_tokens=over)) == 0
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38, -3e38])
+def test_scale_is_a_number(scale):
+    """No answer for a scale that leaves no scores; refused before the workspace is looked at, with tokens or without."""
+    from shard_amd import _lib
+    lib = _lib.load()
+    assert lib.shard_kv4_attn(_args(scale=scale), None, 0, None) == -1
+    assert lib.shard_kv4_attn(_args(scale=scale, n_tokens=0, cu_seqlens=P), None, 0, None) == -1
+    assert lib.shard_kv4_attn(_args(scale=2e38, n_tokens=0, cu_seqlens=P), None, 0, None) == 0
