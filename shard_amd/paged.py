@@ -112,8 +112,8 @@ class PagedCache(HFCache):
     # -- a step ------------------------------------------------------------
     def begin(self, seqs, new):
         """Open a step in which sequence seqs[i] gets new[i] tokens (0 allowed),
-        packed in this order.  Pages are taken here: RuntimeError, with nothing
-        changed, where too few are free.  Returns the tokens' positions, (1, T)."""
+        packed in this order.  Pages are taken here: RuntimeError where too few are
+        free; a call that fails, for whatever reason, changes nothing.  Returns the tokens' positions, (1, T)."""
         seqs, new = list(seqs), [int(n) for n in new]
         if len(seqs) != len(new) or not seqs or len(set(seqs)) != len(seqs) or min(new) < 0 or max(new) == 0:
             raise ValueError("a step needs distinct sequences and at least one new token")
@@ -123,20 +123,27 @@ class PagedCache(HFCache):
         want = [(t + KV4_PAGE - 1) // KV4_PAGE - len(self._pages[s]) for s, t in zip(seqs, total)]
         if sum(want) > len(self._free):
             raise RuntimeError(f"the step needs {sum(want)} more pages, {len(self._free)} are free")
-        for s, n, t in zip(seqs, want, total):
-            self._pages[s] += [self._free.pop() for _ in range(n)]
-            self._lens[s] = t
-        dev, width = self.pool.device, max(len(self._pages[s]) for s in seqs)
-        rows = [self._pages[s] + [0] * (width - len(self._pages[s])) for s in seqs]
+        took = self._free[len(self._free) - sum(want):][::-1]
+        pages, at = [], 0
+        for s, n in zip(seqs, want):
+            pages.append(self._pages[s] + took[at:at + n])
+            at += n
+        dev, width = self.pool.device, max(len(p) for p in pages)
+        rows = [p + [0] * (width - len(p)) for p in pages]
         cu = [0]
         for n in new:
             cu.append(cu[-1] + n)
         meta = torch.tensor([x for r in rows for x in r] + total + cu, dtype=torch.int32).to(dev)  # one copy
         B = len(seqs)
         table, lens, cu_dev = meta[:B * width].view(B, width), meta[B * width:B * width + B], meta[B * width + B:]
+        pos = torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)])[None].to(dev)
+        # nothing has changed so far; nothing below fails
+        del self._free[len(self._free) - sum(want):]
+        for s, p, t in zip(seqs, pages, total):
+            self._pages[s], self._lens[s] = p, t
         self._step = dict(table=table, lens=lens, cu=None if max(new) == min(new) == 1 else cu_dev, rows=cu[-1],
                           max_new=max(new), max_len=max(total), undo=list(zip(seqs, new, want)))
-        return torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)])[None].to(dev)
+        return pos
 
     def cancel(self):
         """Undo the open step: its tokens were not stored in every layer."""

@@ -1,0 +1,54 @@
+"""PagedCache's bookkeeping on the CPU: the operators are stood in for, sequences, pages and steps are the class's own."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def paged(monkeypatch):
+    """A cache of two layers on the CPU; its operators return q as it is."""
+    from shard_amd import PagedCache, ops
+    monkeypatch.setattr(ops, "rope_phases", lambda start, n, inv: torch.zeros(n, inv.numel(), 2))
+    monkeypatch.setattr(ops, "kv4_append", lambda k, v, *args, q=None, **kw: q)
+    monkeypatch.setattr(ops, "kv4_attn", lambda q, *args, **kw: q)
+    return PagedCache(8, 300, head_dim=64, num_layers=2, n_kv_heads=2, device="cpu")
+
+
+def _attend(cache, layer, rows):
+    x = torch.zeros(rows, 2, 64)
+    return cache.attend(layer, x, x, x)
+
+
+def _state(cache):
+    return {s: (cache.length(s), list(cache._pages[s])) for s in cache._pages}, list(cache._free)
+
+
+def test_pages_and_positions(paged):
+    a, b = paged.add(), paged.add()
+    assert paged.begin([a, b], [70, 3]).tolist() == [[*range(70), *range(3)]]
+    st = paged._step
+    assert st["table"].tolist() == [[0, 1], [2, 0]] and st["lens"].tolist() == [70, 3] and st["cu"].tolist() == [0, 70, 73]
+    for layer in range(2):
+        _attend(paged, layer, 73)
+    assert paged.begin([b, a], [62, 1]).tolist() == [[*range(3, 65), 70]]
+    assert paged._step["table"].tolist() == [[2, 3], [0, 1]] and paged.free_pages() == 4
+    paged.cancel()
+    assert _state(paged) == ({a: (70, [0, 1]), b: (3, [2])}, [7, 6, 5, 4, 3])
+
+
+@pytest.mark.parametrize("what", ["tensor", "arange", "cat"])
+def test_a_begin_that_fails_changes_nothing(paged, monkeypatch, what):
+    """Out of memory at any of begin()'s tensors: lengths, pages and the step as they were."""
+    a, b = paged.add(), paged.add()
+    paged.begin([a], [70])
+    for layer in range(2):
+        _attend(paged, layer, 70)
+    before, step = _state(paged), paged._step
+
+    def fail(*args, **kw):
+        raise MemoryError
+    with monkeypatch.context() as m:
+        m.setattr(torch, what, fail)
+        with pytest.raises(MemoryError):
+            paged.begin([a, b], [100, 5])
+    assert _state(paged) == before and paged._step is step
+    assert paged.begin([a, b], [1, 5]).tolist() == [[70, *range(5)]]
