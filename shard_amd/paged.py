@@ -15,7 +15,9 @@ of q and k, 4-bit rounding, writing) and ops.kv4_attn.
     cache.drop(a)
 
 The tokens of a step are packed in rows, one sequence after the other; there is
-no padding and no attention mask.
+no padding and no attention mask.  A step is open from begin() until every layer
+has stored its tokens (run() does both); one that will not come to that is undone
+by cancel(), as no other can begin over tokens that are not there.
 """
 import torch
 from transformers.cache_utils import Cache as HFCache, CacheLayerMixin
@@ -110,10 +112,17 @@ class PagedCache(HFCache):
         return self.pool.numel() + self.phases.numel() * 4
 
     # -- a step ------------------------------------------------------------
+    def _open(self):
+        """The step that some layer has not stored yet, or None."""
+        return self._step if self._step is not None and self._step["left"] else None
+
     def begin(self, seqs, new):
         """Open a step in which sequence seqs[i] gets new[i] tokens (0 allowed),
         packed in this order.  Pages are taken here: RuntimeError where too few are
-        free; a call that fails, for whatever reason, changes nothing.  Returns the tokens' positions, (1, T)."""
+        free; ValueError while another step is open; a call that fails, for
+        whatever reason, changes nothing.  Returns the tokens' positions, (1, T)."""
+        if self._open():
+            raise ValueError("a step is open: run its layers or cancel() it")
         seqs, new = list(seqs), [int(n) for n in new]
         if len(seqs) != len(new) or not seqs or len(set(seqs)) != len(seqs) or min(new) < 0 or max(new) == 0:
             raise ValueError("a step needs distinct sequences and at least one new token")
@@ -142,14 +151,18 @@ class PagedCache(HFCache):
         for s, p, t in zip(seqs, pages, total):
             self._pages[s], self._lens[s] = p, t
         self._step = dict(table=table, lens=lens, cu=None if max(new) == min(new) == 1 else cu_dev, rows=cu[-1],
-                          max_new=max(new), max_len=max(total), undo=list(zip(seqs, new, want)))
+                          max_new=max(new), max_len=max(total), undo=list(zip(seqs, new, want)),
+                          left=set(range(len(self.layers))))
         return pos
 
     def cancel(self):
         """Undo the open step: its tokens were not stored in every layer."""
-        step, self._step = self._step, None
-        if step is None:
+        if not self._open():
             raise ValueError("no step is open")
+        self._undo()
+
+    def _undo(self):
+        step, self._step = self._step, None
         for seq, n, pages in step["undo"]:
             self._lens[seq] -= n
             for _ in range(pages):
@@ -157,14 +170,17 @@ class PagedCache(HFCache):
 
     def attend(self, layer_idx, q, k, v, scale=None):
         """One layer of the open step: q (T, H, D), k and v (T, G, D) before RoPE,
-        stored and attended to.  Returns (T, H, D)."""
-        st = self._step
+        stored and attended to.  The step is closed with its last layer.  Returns
+        (T, H, D)."""
+        st = self._open()
         if st is None or k.shape[0] != st["rows"]:
             raise ValueError(f"{k.shape[0]} rows for a step of {None if st is None else st['rows']}: open it with begin()")
         pages = self.pool[layer_idx]
         q = ops.kv4_append(k, v, pages, st["table"], st["lens"], self.phases, q=q, cu_seqlens=st["cu"], max_new=st["max_new"])
-        return ops.kv4_attn(q, pages, st["table"], st["lens"], cu_seqlens=st["cu"], scale=scale, max_new=st["max_new"],
-                            max_len=st["max_len"])
+        out = ops.kv4_attn(q, pages, st["table"], st["lens"], cu_seqlens=st["cu"], scale=scale, max_new=st["max_new"],
+                           max_len=st["max_len"])
+        st["left"].discard(layer_idx % len(self.layers))
+        return out
 
     @torch.no_grad()
     def run(self, model, seqs, tokens, last_only=True):
@@ -180,11 +196,15 @@ class PagedCache(HFCache):
         if last_only:
             keep = torch.tensor([len(t) for t in tokens]).cumsum(0).to(dev) - 1
         pos = self.begin(seqs, [len(t) for t in tokens])
+        step = self._step
         try:
-            return model(input_ids=ids, position_ids=pos, past_key_values=self, use_cache=True, logits_to_keep=keep).logits[0]
+            logits = model(input_ids=ids, position_ids=pos, past_key_values=self, use_cache=True, logits_to_keep=keep).logits[0]
         except BaseException:
-            self.cancel()
+            if self._step is step:
+                self._undo()
             raise
+        step["left"].clear()
+        return logits
 
 
 def paged_forward(attention, hidden_states, cache):

@@ -52,3 +52,65 @@ def test_a_begin_that_fails_changes_nothing(paged, monkeypatch, what):
             paged.begin([a, b], [100, 5])
     assert _state(paged) == before and paged._step is step
     assert paged.begin([a, b], [1, 5]).tolist() == [[70, *range(5)]]
+
+
+def test_a_step_is_open_until_every_layer_has_stored_it(paged):
+    a = paged.add()
+    paged.begin([a], [5])
+    with pytest.raises(ValueError):                      # nothing stored yet
+        paged.begin([a], [1])
+    _attend(paged, 0, 5)
+    _attend(paged, 0, 5)                                 # a layer again, in the same step
+    with pytest.raises(ValueError):                      # nor in the second layer
+        paged.begin([a], [1])
+    assert paged.length(a) == 5
+    _attend(paged, -1, 5)
+    before = _state(paged)
+    with pytest.raises(ValueError):                      # stored: no step to undo, none to store over
+        paged.cancel()
+    with pytest.raises(ValueError):
+        _attend(paged, 0, 5)
+    assert _state(paged) == before
+    assert paged.begin([a], [1]).tolist() == [[5]]
+    _attend(paged, 0, 1)
+    paged.cancel()
+    assert _state(paged) == before
+    assert paged.begin([a], [2]).tolist() == [[5, 6]]
+
+
+class _Model:
+    """Attends in `layers`, then fails where asked to."""
+
+    def __init__(self, layers, fails=False):
+        self.layers, self.fails = layers, fails
+
+    def __call__(self, input_ids, past_key_values, **kw):
+        for layer in self.layers:
+            _attend(past_key_values, layer, input_ids.numel())
+        if self.fails:
+            raise ArithmeticError
+        return type("Output", (), dict(logits=torch.zeros(1, 1, 7)))
+
+
+def test_run_closes_its_step(paged):
+    a, ids = paged.add(), torch.arange(70)
+    paged.run(_Model([0, 1]), [a], [ids])
+    before = _state(paged)
+    with pytest.raises(ValueError):
+        paged.cancel()
+    for layers in ([], [0], [0, 1]):                     # before, between and after the layers
+        with pytest.raises(ArithmeticError):
+            paged.run(_Model(layers, fails=True), [a], [ids])
+        assert _state(paged) == before
+        with pytest.raises(ValueError):
+            paged.cancel()
+    paged.run(_Model([0]), [a], [ids])                   # a model without the cache's last layer
+    paged.run(_Model([0, 1]), [a], [ids])
+    assert paged.length(a) == 210 and paged.free_pages() == 8 - 4
+    paged.begin([a], [3])
+    step = _state(paged)
+    with pytest.raises(ValueError):                      # somebody else's step stays open
+        paged.run(_Model([0, 1]), [a], [ids])
+    assert _state(paged) == step
+    paged.cancel()
+    assert paged.length(a) == 210
