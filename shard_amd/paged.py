@@ -97,10 +97,15 @@ class PagedCache(HFCache):
         return seq
 
     def drop(self, seq):
-        """Give a sequence's pages back.  An open step is closed."""
+        """Give a sequence's pages back.  A step that is open for it is undone, for
+        all its sequences; one of other sequences stays open."""
+        if seq not in self._pages:
+            raise KeyError(seq)
+        step = self._open()
+        if step is not None and any(s == seq for s, _, _ in step["undo"]):
+            self._undo()
         self._free += reversed(self._pages.pop(seq))
         del self._lens[seq]
-        self._step = None
 
     def length(self, seq) -> int:
         return self._lens[seq]

@@ -114,3 +114,25 @@ def test_run_closes_its_step(paged):
     assert _state(paged) == step
     paged.cancel()
     assert paged.length(a) == 210
+
+
+def test_a_sequence_dropped_from_an_open_step(paged):
+    """The other sequences of the step hold what they held before it: nothing of it was stored in every layer."""
+    a, b, c = paged.add(), paged.add(), paged.add()
+    paged.run(_Model([0, 1]), [a, b], [torch.arange(60), torch.arange(10)])
+    paged.begin([a, b], [100, 3])
+    _attend(paged, 0, 103)
+    paged.drop(a)
+    assert paged.length(b) == 10 and len(paged._pages[b]) == 1 and paged.free_pages() == 7
+    with pytest.raises(ValueError):
+        paged.cancel()
+    with pytest.raises(ValueError):
+        _attend(paged, 1, 103)
+    assert paged.begin([b], [2]).tolist() == [[10, 11]]
+    paged.drop(c)                                        # not of this step: it stays open
+    with pytest.raises(KeyError):
+        paged.drop(c)
+    for layer in range(2):
+        _attend(paged, layer, 2)
+    paged.drop(b)                                        # its step is closed
+    assert _state(paged)[0] == {} and sorted(paged._free) == list(range(8))
