@@ -551,6 +551,24 @@ typedef struct shard_kv4_args {
 } shard_kv4_args;
 
 size_t shard_kv4_args_size(void);
+/* Of the block that the library was built with: callers built apart from it
+ * compare with their own SHARD_KV4_ARGS_LAYOUT.  Its size and its fields'
+ * offsets, each times an odd number of its own: differs where a field has been
+ * added, taken out, moved or changed in size. */
+uint64_t shard_kv4_args_layout(void);
+#define SHARD_KV4_AT(i, field) ((uint64_t)(2 * (i) + 1) * offsetof(shard_kv4_args, field))
+#define SHARD_KV4_ARGS_LAYOUT                                                                              \
+  (((uint64_t)sizeof(shard_kv4_args) << 32) + SHARD_KV4_AT(0, batch) + SHARD_KV4_AT(1, n_tokens) +         \
+   SHARD_KV4_AT(2, n_q_heads) + SHARD_KV4_AT(3, n_kv_heads) + SHARD_KV4_AT(4, head_dim) +                  \
+   SHARD_KV4_AT(5, dtype) + SHARD_KV4_AT(6, n_pages) + SHARD_KV4_AT(7, table_width) +                      \
+   SHARD_KV4_AT(8, max_new) + SHARD_KV4_AT(9, max_len) + SHARD_KV4_AT(10, cache) +                         \
+   SHARD_KV4_AT(11, page_stride) + SHARD_KV4_AT(12, block_table) + SHARD_KV4_AT(13, table_stride) +        \
+   SHARD_KV4_AT(14, seq_lens) + SHARD_KV4_AT(15, cu_seqlens) + SHARD_KV4_AT(16, q) +                       \
+   SHARD_KV4_AT(17, q_stride) + SHARD_KV4_AT(18, q_head_stride) + SHARD_KV4_AT(19, k) +                    \
+   SHARD_KV4_AT(20, k_stride) + SHARD_KV4_AT(21, k_head_stride) + SHARD_KV4_AT(22, v) +                    \
+   SHARD_KV4_AT(23, v_stride) + SHARD_KV4_AT(24, v_head_stride) + SHARD_KV4_AT(25, phases) +               \
+   SHARD_KV4_AT(26, n_phases) + SHARD_KV4_AT(27, scale) + SHARD_KV4_AT(28, q_out) +                        \
+   SHARD_KV4_AT(29, k_out) + SHARD_KV4_AT(30, v_out) + SHARD_KV4_AT(31, out))
 /* Bytes of a page (0: unsupported). */
 int64_t shard_kv4_page_bytes(int32_t n_kv_heads, int32_t head_dim);
 

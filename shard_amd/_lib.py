@@ -67,6 +67,9 @@ class KV4Args(ctypes.Structure):
     ]
 
 
+# SHARD_KV4_ARGS_LAYOUT of the header
+KV4_LAYOUT = (ctypes.sizeof(KV4Args) << 32) + sum((2 * i + 1) * getattr(KV4Args, name).offset
+                                                  for i, (name, _) in enumerate(KV4Args._fields_))
 KV4_PACK = struct.Struct("@10i Qq Qq QQ Qqq Qqq Qqq Qif QQQQ")
 
 
@@ -123,6 +126,7 @@ SIGNATURES = [
     ("shard_rope_stream_append", c_int32, [c_void_p] * 5 + [c_int64] + [c_int32] * 4 + [c_void_p] * 3 + [c_int32] + [c_void_p] * 10 + [c_void_p]),
     ("shard_rope_stream_append_dev", c_int32, [c_void_p] * 5 + [c_int64] + [c_int32] * 4 + [c_void_p] * 3 + [c_int32] + [c_void_p] * 10 + [c_void_p, c_int32] + [c_void_p]),
     ("shard_kv4_args_size", c_size_t, []),
+    ("shard_kv4_args_layout", ctypes.c_uint64, []),
     ("shard_kv4_page_bytes", c_int64, [c_int32, c_int32]),
     ("shard_kv4_append", c_int32, [c_void_p, c_void_p]),
     ("shard_kv4_read", c_int32, [c_void_p, c_void_p]),
@@ -158,7 +162,7 @@ def load():
         fn.argtypes = args
     if lib.shard_decode_args_size() != ctypes.sizeof(DecodeArgs):
         raise ShardHipUnavailable("shard_decode_args layout mismatch between header and binding")
-    if not lib.shard_kv4_args_size() == ctypes.sizeof(KV4Args) == KV4_PACK.size:
+    if lib.shard_kv4_args_layout() != KV4_LAYOUT or KV4_PACK.size != ctypes.sizeof(KV4Args):
         raise ShardHipUnavailable("shard_kv4_args layout mismatch between header and binding")
     _lib = lib
     return lib

@@ -224,20 +224,28 @@ PyObject* logprobs(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(path): the library's entry points; it is loaded already
+// bind(path): the library's entry points; it is loaded already.  ImportError, and
+// what was bound before stays, where it has not all of them or was built with
+// another argument block than this file.
 PyObject* bind(PyObject*, PyObject* path) {
   const char* p = PyUnicode_AsUTF8(path);
   if (!p) return nullptr;
   void* lib = dlopen(p, RTLD_NOW);
   if (!lib) return PyErr_Format(PyExc_ImportError, "%s", dlerror());
-  const auto get = [&](const char* name, auto& f) {
-    f = (std::decay_t<decltype(f)>)dlsym(lib, name);
-    return f != nullptr;
-  };
-  if (!get("shard_kv4_append", p_append) || !get("shard_kv4_read", p_read) || !get("shard_kv4_attn_workspace", p_attn_workspace) ||
-      !get("shard_kv4_attn", p_attn) || !get("shard_token_logprobs_workspace", p_logprobs_workspace) ||
-      !get("shard_token_logprobs", p_logprobs))
-    return PyErr_Format(PyExc_ImportError, "%s misses an entry point", p);
+  const auto layout = (decltype(&shard_kv4_args_layout))dlsym(lib, "shard_kv4_args_layout");
+  if (!layout || layout() != SHARD_KV4_ARGS_LAYOUT)
+    return PyErr_Format(PyExc_ImportError, "%s was built with another shard_kv4_args", p);
+  const char* const names[] = {"shard_kv4_append", "shard_kv4_read", "shard_kv4_attn_workspace", "shard_kv4_attn",
+                               "shard_token_logprobs_workspace", "shard_token_logprobs"};
+  void* f[6];
+  for (int i = 0; i < 6; ++i)
+    if (!(f[i] = dlsym(lib, names[i]))) return PyErr_Format(PyExc_ImportError, "%s misses %s", p, names[i]);
+  p_append = (decltype(p_append))f[0];
+  p_read = (decltype(p_read))f[1];
+  p_attn_workspace = (decltype(p_attn_workspace))f[2];
+  p_attn = (decltype(p_attn))f[3];
+  p_logprobs_workspace = (decltype(p_logprobs_workspace))f[4];
+  p_logprobs = (decltype(p_logprobs))f[5];
   Py_RETURN_NONE;
 }
 

@@ -1324,6 +1324,7 @@ using namespace shard;
 extern "C" {
 
 size_t shard_kv4_args_size(void) { return sizeof(shard_kv4_args); }
+uint64_t shard_kv4_args_layout(void) { return SHARD_KV4_ARGS_LAYOUT; }
 
 int64_t shard_kv4_page_bytes(int32_t n_kv_heads, int32_t head_dim) {
   if (n_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;

@@ -182,3 +182,56 @@ def test_scale_is_a_number(scale):
     assert lib.shard_kv4_attn(_args(scale=scale), None, 0, None) == -1
     assert lib.shard_kv4_attn(_args(scale=scale, n_tokens=0, cu_seqlens=P), None, 0, None) == -1
     assert lib.shard_kv4_attn(_args(scale=2e38, n_tokens=0, cu_seqlens=P), None, 0, None) == 0
+
+
+STUB = r"""
+#include "shard_hip.h"
+extern "C" {
+LAYOUT
+int shard_kv4_append(const shard_kv4_args*, void*) { return 0; }
+int shard_kv4_read(const shard_kv4_args*, void*) { return 0; }
+size_t shard_kv4_attn_workspace(const shard_kv4_args*) { return 0; }
+ATTN
+size_t shard_token_logprobs_workspace(int64_t, int64_t, int32_t) { return 0; }
+int shard_token_logprobs(const void*, int32_t, int64_t, int64_t, int64_t, const int64_t*, int32_t, float*, float*, float*, int64_t*,
+                         void*, size_t, void*) { return 0; }
+}
+"""
+LAYOUT = "uint64_t shard_kv4_args_layout(void) { return SHARD_KV4_ARGS_LAYOUT%s; }"
+ATTN = "int shard_kv4_attn(const shard_kv4_args*, void*, size_t, void*) { return 0; }"
+
+
+@pytest.mark.parametrize("layout,attn,fits", [(LAYOUT % "", ATTN, True), (LAYOUT % " + 8", ATTN, False), ("", ATTN, False),
+                                              (LAYOUT % "", "", False)], ids=["fits", "other", "none", "misses"])
+def test_compiled_dispatch_binds_no_other_argument_block(tmp_path, layout, attn, fits):
+    """A library from before a change of shard_kv4_args, or from after it, is not called with this one's."""
+    import os
+    import subprocess
+    from conftest import ROOT
+    from shard_amd import _lib, ops
+    src, so = tmp_path / "stub.cpp", str(tmp_path / "stub.so")
+    src.write_text(STUB.replace("LAYOUT\n", layout + "\n", 1).replace("ATTN\n", attn + "\n", 1))
+    subprocess.run(["g++", "-shared", "-fPIC", "-I", os.path.join(ROOT, "include"), str(src), "-o", so], check=True)
+    _lib.load()
+    d = ops._bind_direct()
+    assert d
+    if fits:
+        d.bind(so)
+    else:
+        with pytest.raises(ImportError):
+            d.bind(so)
+    d.bind(_lib.LIB_PATH)
+
+
+def test_argument_block_layout():
+    """The binding's block is the header's, and no two equally large fields could change places unseen."""
+    from shard_amd import _lib
+    assert _lib.load().shard_kv4_args_layout() == _lib.KV4_LAYOUT
+    fields = _lib.KV4Args._fields_
+    for i in range(len(fields)):
+        for j in range(i):
+            moved = list(fields)
+            moved[i], moved[j] = moved[j], moved[i]
+            other = type("Other", (ctypes.Structure,), {"_fields_": moved})
+            total = (ctypes.sizeof(other) << 32) + sum((2 * n + 1) * getattr(other, f).offset for n, (f, _) in enumerate(fields))
+            assert total != _lib.KV4_LAYOUT, (fields[i], fields[j])
