@@ -39,6 +39,21 @@ c10::DataPtr scratch(size_t bytes) {  // of the current device and stream, given
   return bytes ? c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes) : c10::DataPtr();
 }
 
+// Other Python threads run while this one allocates and launches (a launch waits
+// where the stream's queue is full, an allocation where it reaches the driver).
+// No Python object is made or looked at within; operands stay alive, the caller
+// holds them.
+class Unlocked {
+ public:
+  Unlocked() : state(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state); }
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+
+ private:
+  PyThreadState* state;
+};
+
 // A tensor argument on the current device; `none`: may be None (then null).
 bool tensor(PyObject* o, int64_t device, const at::Tensor** t, bool none = false) {
   *t = nullptr;
@@ -130,14 +145,21 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
     Py_RETURN_NONE;
   a.phases = (const float*)phases->data_ptr();
   a.n_phases = (int32_t)phases->size(0);
-  at::Tensor out;
   if (q) {
     if (!rows(*q, a.n_tokens, 0, D, &a.q, &a.q_stride, &a.q_head_stride) || q->size(1) <= 0 || q->size(1) > INT32_MAX) Py_RETURN_NONE;
     a.n_q_heads = (int32_t)q->size(1);
-    out = make(q->sizes(), *q, q->scalar_type());
-    a.q_out = out.data_ptr();
   }
-  if (p_append(&a, (void*)stream)) Py_RETURN_NONE;
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    if (q) {
+      out = make(q->sizes(), *q, q->scalar_type());
+      a.q_out = out.data_ptr();
+    }
+    rc = p_append(&a, (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
   if (!q) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -157,10 +179,17 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
   a.dtype = bf16 ? SHARD_BF16 : SHARD_FP16;
   const int64_t size[3] = {a.n_tokens, a.n_kv_heads, a.head_dim};
   const auto type = bf16 ? at::kBFloat16 : at::kHalf;
-  at::Tensor k = make(size, *cache, type), v = make(size, *cache, type);
-  a.k_out = k.data_ptr();
-  a.v_out = v.data_ptr();
-  if (p_read(&a, (void*)stream)) Py_RETURN_NONE;
+  at::Tensor k, v;
+  int rc;
+  {
+    const Unlocked unlocked;
+    k = make(size, *cache, type);
+    v = make(size, *cache, type);
+    a.k_out = k.data_ptr();
+    a.v_out = v.data_ptr();
+    rc = p_read(&a, (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
   return Py_BuildValue("NN", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
   END_HANDLE_TH_ERRORS
 }
@@ -184,11 +213,17 @@ PyObject* attn(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (o[5] == Py_None) a.scale = (float)std::pow((double)a.head_dim, -0.5);
   else if (PyFloat_CheckExact(o[5])) a.scale = (float)PyFloat_AS_DOUBLE(o[5]);
   else Py_RETURN_NONE;
-  at::Tensor out = make(q->sizes(), *q, q->scalar_type());
-  a.out = out.data_ptr();
-  const size_t need = p_attn_workspace(&a);
-  const c10::DataPtr ws = scratch(need);
-  if (p_attn(&a, ws.get(), need, (void*)stream)) Py_RETURN_NONE;
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = make(q->sizes(), *q, q->scalar_type());
+    a.out = out.data_ptr();
+    const size_t need = p_attn_workspace(&a);
+    const c10::DataPtr ws = scratch(need);
+    rc = p_attn(&a, ws.get(), need, (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -208,14 +243,21 @@ PyObject* logprobs(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const int64_t R = x->size(0), V = x->size(1);
   if (tok && (tok->scalar_type() != at::kLong || tok->dim() != 1 || tok->size(0) != R || !tok->is_contiguous())) Py_RETURN_NONE;
   const int64_t one[1] = {R}, two[2] = {R, top};
-  at::Tensor entropy = make(one, *x, at::kFloat), top_lp = make(two, *x, at::kFloat), top_ids = make(two, *x, at::kLong), lp;
-  if (tok) lp = make(one, *x, at::kFloat);
-  const size_t need = p_logprobs_workspace(R, V, (int32_t)top);
-  const c10::DataPtr ws = scratch(need);
-  if (p_logprobs(x->data_ptr(), code, R, V, x->stride(0), tok ? (const int64_t*)tok->data_ptr() : nullptr, (int32_t)top,
-                 tok ? (float*)lp.data_ptr() : nullptr, (float*)entropy.data_ptr(), (float*)top_lp.data_ptr(),
-                 (int64_t*)top_ids.data_ptr(), ws.get(), need, (void*)stream))
-    Py_RETURN_NONE;
+  at::Tensor entropy, top_lp, top_ids, lp;
+  int rc;
+  {
+    const Unlocked unlocked;
+    entropy = make(one, *x, at::kFloat);
+    top_lp = make(two, *x, at::kFloat);
+    top_ids = make(two, *x, at::kLong);
+    if (tok) lp = make(one, *x, at::kFloat);
+    const size_t need = p_logprobs_workspace(R, V, (int32_t)top);
+    const c10::DataPtr ws = scratch(need);
+    rc = p_logprobs(x->data_ptr(), code, R, V, x->stride(0), tok ? (const int64_t*)tok->data_ptr() : nullptr, (int32_t)top,
+                    tok ? (float*)lp.data_ptr() : nullptr, (float*)entropy.data_ptr(), (float*)top_lp.data_ptr(),
+                    (int64_t*)top_ids.data_ptr(), ws.get(), need, (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
   PyObject* first = Py_None;
   if (tok) first = THPVariable_Wrap(std::move(lp));
   else Py_INCREF(Py_None);

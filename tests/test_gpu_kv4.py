@@ -595,3 +595,98 @@ def test_scale_is_a_number(cuda):
         with pytest.raises(ValueError):
             b.attn(scale=bad, out=torch.empty_like(b.d_q))
     _check_attention(b, b.attn(scale=1), scale=1)
+
+
+SLOW = r"""
+#include <unistd.h>
+#include "shard_hip.h"
+extern "C" {
+volatile int entered, go;
+static int wait_for_go() {
+  entered = 1;
+  for (int i = 0; i < 3000 && !go; ++i) usleep(1000);
+  return go ? 0 : -1;
+}
+uint64_t shard_kv4_args_layout(void) { return SHARD_KV4_ARGS_LAYOUT; }
+int shard_kv4_append(const shard_kv4_args*, void*) { return wait_for_go(); }
+int shard_kv4_read(const shard_kv4_args*, void*) { return wait_for_go(); }
+size_t shard_kv4_attn_workspace(const shard_kv4_args*) { return 4096; }
+int shard_kv4_attn(const shard_kv4_args*, void*, size_t, void*) { return wait_for_go(); }
+size_t shard_token_logprobs_workspace(int64_t, int64_t, int32_t) { return 0; }
+int shard_token_logprobs(const void*, int32_t, int64_t, int64_t, int64_t, const int64_t*, int32_t, float*, float*, float*, int64_t*,
+                         void*, size_t, void*) { return wait_for_go(); }
+}
+"""
+
+
+def test_other_threads_run_during_a_compiled_call(cuda, tmp_path):
+    """A call that waits in the library (a full queue, say) leaves Python to the other threads.  The library is stood in
+    for by one that launches nothing and waits, 3 s at most, for what only another thread can tell it."""
+    import ctypes
+    import os
+    import subprocess
+    import threading
+    import time
+    from conftest import ROOT
+    from shard_amd import _lib, ops
+    src, so = tmp_path / "slow.cpp", str(tmp_path / "slow.so")
+    src.write_text(SLOW)
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-I", os.path.join(ROOT, "include"), str(src), "-o", so], check=True)
+    lib = ctypes.CDLL(so)
+    entered, go = (ctypes.c_int.in_dll(lib, name) for name in ("entered", "go"))
+    b = Batch([70], [3], 4, 2, 64)
+    d, st = ops._bind_direct(), torch.cuda.current_stream().cuda_stream
+    x = torch.zeros(2, 50, device=cuda)
+    args = b.d_cache, b.d_table, b.d_lens
+    calls = [lambda: d.kv4_append(b.d_k, b.d_v, *args, b.d_phases, b.d_q, b.d_cu, None, 0, st),
+             lambda: d.kv4_read(*args, 3, False, b.d_cu, None, 0, st),
+             lambda: d.kv4_attn(b.d_q, *args, b.d_cu, None, None, None, 0, st),
+             lambda: d.token_logprobs(x, None, 2, 0, st)]
+    assert all(call() is not None for call in calls)    # with the library itself
+    d.bind(so)
+    try:
+        for call in calls:
+            entered.value = go.value = 0
+            done = []
+            t = threading.Thread(target=lambda: done.append(call()))
+            t.start()
+            while not entered.value and t.is_alive():
+                time.sleep(0.001)
+            go.value = 1
+            t.join()
+            assert done[0] is not None, "the call waited in vain"
+    finally:
+        d.bind(_lib.LIB_PATH)
+
+
+def test_two_threads_at_once(cuda):
+    """Each on its own stream and its own batch: the results of one after the other."""
+    import threading
+    from shard_amd import ops
+    batches = [Batch([400, 77], [9, 2], 8, 2, 128, "fp16", seed=20).fill(), Batch([1000], [1], 8, 2, 64, "bf16", seed=21).fill()]
+    x = [torch.randn(3, 9000, generator=torch.Generator().manual_seed(i)).cuda() for i in range(2)]
+
+    def work(i, n):
+        b, out = batches[i], []
+        for _ in range(n):
+            q = b.append(q=b.d_q)
+            out.append([q, b.attn(q=q), *b.read(dtype=b.type), *ops.token_logprobs(x[i], top=3)[1:]])
+        return out
+    for b in batches:
+        b.append()
+    want = [work(i, 1)[0] for i in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got[i] = work(i, 50)
+        s.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert all(torch.equal(a, b) for row in got[i] for a, b in zip(row, want[i]))
