@@ -59,43 +59,67 @@ def dispatch_command(out: str):
 
 
 def build(verbose: bool = False, jobs: int = 4) -> str:
-    """Compile every csrc/*.hip for gfx950 and link libshard_hip.so. Returns its path."""
+    """Compile every csrc/*.hip for gfx950 and link libshard_hip.so. Returns its path.
+
+    _dispatch.so, which only makes eager calls cheaper, may fail to build (no
+    g++, no headers): a warning says so, and the one of an earlier build, which
+    may not fit the new library, is removed.  Where the library does not build,
+    both files stay as they were."""
     cc = hipcc()
     objdir = tempfile.mkdtemp(prefix="shard_build_")
+    procs, dispatch = [], None
     try:
-        procs, objs = [], []
-        cmd = dispatch_command(DISPATCH + ".tmp")
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        dispatch = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        new_lib, new_dispatch = os.path.join(objdir, "lib.so"), os.path.join(objdir, "dispatch.so")
+        try:
+            dispatch = _start(dispatch_command(new_dispatch), verbose)
+        except Exception as exc:  # no compiler, no torch to build against
+            no_dispatch = repr(exc)
+        objs = []
         for src in sources():
             obj = os.path.join(objdir, src.replace(".hip", ".o"))
-            cmd = [cc, *COMMON, *PER_FILE.get(src, []), "-c", os.path.join(CSRC, src), "-o", obj]
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE,
-                                                stderr=subprocess.STDOUT, text=True)))
+            procs.append((src, _start([cc, *COMMON, *PER_FILE.get(src, []), "-c", os.path.join(CSRC, src), "-o", obj], verbose)))
             objs.append(obj)
             if len(procs) >= jobs:
                 _drain(procs)
         _drain(procs)
-        tmp = LIB + ".tmp"
-        cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
-        out = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-        if out.returncode != 0:
-            raise RuntimeError("link failed:\n" + out.stdout)
-        os.replace(tmp, LIB)
-        _drain([("dispatch.cpp", dispatch)])
-        os.replace(DISPATCH + ".tmp", DISPATCH)
+        procs.append(("the library", _start([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", new_lib], verbose)))
+        _drain(procs)
+        if dispatch is not None:
+            out, _ = dispatch.communicate()
+            no_dispatch = out if dispatch.returncode else None
+        if os.path.exists(DISPATCH):  # never an old one beside a new library
+            os.remove(DISPATCH)
+        _put(new_lib, LIB)
+        if no_dispatch is None:
+            _put(new_dispatch, DISPATCH)
+        else:
+            sys.stderr.write(f"warning: _dispatch.so not built, eager calls go through Python:\n{no_dispatch}\n")
     finally:
+        for p in [p for _, p in procs] + [dispatch]:  # what a failure left running
+            if p is not None and p.poll() is None:
+                p.kill()
+                p.wait()
         shutil.rmtree(objdir, ignore_errors=True)
     return LIB
 
 
+def _start(cmd, verbose):
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def _put(src, dst):
+    """In one step, as a process may have the old file open."""
+    shutil.copy(src, dst + ".tmp")
+    os.replace(dst + ".tmp", dst)
+
+
 def _drain(procs):
     while procs:
-        src, p = procs.pop(0)
+        src, p = procs[0]
         out, _ = p.communicate()
+        procs.pop(0)
         if p.returncode != 0:
             raise RuntimeError(f"hipcc failed on {src}:\n{out}")
         warn = [ln for ln in out.splitlines() if "warning" in ln and "packed-fp32-ops" not in ln]
