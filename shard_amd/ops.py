@@ -93,8 +93,8 @@ def rope_phases(start: int, n: int, inv_freq: torch.Tensor) -> torch.Tensor:
     inv_freq = _contig(inv_freq, torch.float32, "inv_freq")
     hd2 = inv_freq.numel()
     out = torch.empty(n, hd2, 2, dtype=torch.float32, device=inv_freq.device)
-    _lib.check("shard_rope_phases", lib.shard_rope_phases(start, n, hd2, _p(inv_freq), _p(out),
-                                                          _stream(inv_freq)))
+    # inv_freq's device need not be the current one (a PagedCache on another)
+    _launch_on(inv_freq.get_device(), "shard_rope_phases", lib.shard_rope_phases, start, n, hd2, _p(inv_freq), _p(out))
     return out
 
 

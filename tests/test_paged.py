@@ -136,3 +136,34 @@ def test_a_sequence_dropped_from_an_open_step(paged):
         _attend(paged, layer, 2)
     paged.drop(b)                                        # its step is closed
     assert _state(paged)[0] == {} and sorted(paged._free) == list(range(8))
+
+
+@pytest.mark.parametrize("current,other", [(0, False), (1, True)])
+def test_phases_are_made_on_their_own_device(monkeypatch, current, other):
+    """A PagedCache on a device that is not the current one: the table's launch makes it the current one."""
+    from types import SimpleNamespace
+    from shard_amd import _lib, ops
+    seen, made = [], []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            made.append(self.dev)
+
+        def __exit__(self, *args):
+            made.pop()
+    freq = torch.ones(32)
+    monkeypatch.setattr(ops, "_require_gpu", lambda *args: None)
+    monkeypatch.setattr(ops, "_contig", lambda t, *args: SimpleNamespace(
+        numel=t.numel, device=t.device, data_ptr=t.data_ptr, get_device=lambda: 0, is_cuda=True))
+    monkeypatch.setattr(ops, "_current_device", lambda: current)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 70 + dev)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev: SimpleNamespace(cuda_stream=70 + dev))
+    stub = SimpleNamespace(shard_rope_phases=lambda *args: seen.append((list(made), args[-1])) or 0)
+    monkeypatch.setattr(_lib, "load", lambda: stub)
+    assert ops.rope_phases(0, 64, freq).shape == (64, 32, 2)
+    stream = getattr(seen[0][1], "value", seen[0][1])
+    assert len(seen) == 1 and seen[0][0] == ([0] if other else []) and stream == 70
