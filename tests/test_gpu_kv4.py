@@ -690,3 +690,39 @@ def test_two_threads_at_once(cuda):
         t.join()
     for i in range(2):
         assert all(torch.equal(a, b) for row in got[i] for a, b in zip(row, want[i]))
+
+
+def _splits(b, **hints):
+    """Splits that a call of the batch takes, from its workspace."""
+    import ctypes
+    from shard_amd import _lib
+    a = _lib.KV4Args(batch=len(b.total), n_tokens=b.q.shape[0], n_q_heads=b.H, n_kv_heads=b.G, head_dim=b.D, n_pages=b.n_pages,
+                     table_width=b.table.shape[1], cache=4096, page_stride=b.G * 68 * b.D, block_table=4096,
+                     table_stride=b.table.shape[1], seq_lens=4096, cu_seqlens=4096, **hints)
+    size = _lib.load().shard_kv4_attn_workspace(ctypes.byref(a))
+    return size // (b.q.shape[0] * b.H * (b.D + 2) * 4)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("total,new,wide,splits,type", [
+    ([8192], [1], 0, 32, "fp16"), ([16384], [1], 0, 64, "bf16"), ([32768], [1], 0, 128, "fp16"), ([24001], [2], 3, 128, "bf16"),
+    ([300], [1], 507, 128, "fp16"), ([20000, 31000], [1, 3], 0, 128, "fp16")], ids=str)
+def test_attention_joins_many_splits(cuda, total, new, wide, splits, type, D):
+    """Up to 128 splits of a row, empty ones at the end; the heads' heaviest keys lie in splits of their own, at both
+    sides of every 32: a split left out, or weighed as another, is off by most of the output."""
+    H = 8
+    b = Batch(total, new, H, 1, D, type, seed=splits + D, wide=wide, spare=1).fill()
+    assert _splits(b) == splits
+    K, _ = plain.held(b.cache.numpy())
+    for r, s, pos in b.where():
+        n = pos + 1
+        per = max(4, -(-((total[s] + 63) // 64) // splits))               # pages of a split
+        last = (n - 1) // (per * 64)
+        for h, at in enumerate((0, 31, 32, 63, 64, 95, 96, last)):
+            page = b.table[s, min(at, last) * per:][:per]
+            keys = K[page[page < b.n_pages].long(), :, 0].reshape(-1, D)[:n - min(at, last) * per * 64]
+            key = keys[(keys * keys).sum(-1).argmax()]
+            # a score of 14, the others' a few either side of 0: a large part of the weight
+            b.q[r, h] = torch.from_numpy(key * (14 / (key @ key) * D ** 0.5)).to(b.type)
+    _check_attention(b, b.attn())
+    _check_attention(b, b.attn(max_new=max(new), max_len=max(total)))
