@@ -167,3 +167,53 @@ def test_phases_are_made_on_their_own_device(monkeypatch, current, other):
     assert ops.rope_phases(0, 64, freq).shape == (64, 32, 2)
     stream = getattr(seen[0][1], "value", seen[0][1])
     assert len(seen) == 1 and seen[0][0] == ([0] if other else []) and stream == 70
+
+
+ROPES = {
+    "default": dict(), "linear": dict(factor=4.0), "llama3": dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                                                                   original_max_position_embeddings=512),
+    "yarn": dict(factor=4.0, original_max_position_embeddings=512),
+    "dynamic": dict(factor=2.0), "longrope": dict(short_factor=[1.0] * 32, long_factor=[2.0] * 32, factor=4.0,
+                                                   original_max_position_embeddings=512),
+}
+
+
+def rope_model(kind, dtype=torch.float32):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    cfg = LlamaConfig(vocab_size=32, hidden_size=128, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2,
+                      num_key_value_heads=1, max_position_embeddings=2048,
+                      rope_parameters=dict(rope_type=kind, rope_theta=500000.0, **ROPES[kind]))
+    torch.manual_seed(0)
+    return LlamaForCausalLM(cfg).to(dtype).eval()
+
+
+def check_phases(cache, model):
+    """The cache's table against the model's own cosines and sines, both fp32."""
+    n = cache.phases.shape[0]
+    x = torch.zeros(1, 1, 1, device=cache.phases.device)
+    cos, sin = (t[0, :, :32].double().cpu() for t in model.model.rotary_emb(x, torch.arange(n, device=x.device)[None]))
+    size = float(cos.abs().max())
+    got = cache.phases.double().cpu()
+    # the angle is one fp32 product on both sides; cosine and sine are off by 2 units each, their factor by one rounding
+    assert float((got[..., 0] - cos).abs().max()) <= 6 * 2.0 ** -24 * size
+    assert float((got[..., 1] - sin).abs().max()) <= 6 * 2.0 ** -24 * size
+
+
+@pytest.mark.parametrize("kind", ROPES)
+def test_rope_kinds(monkeypatch, kind):
+    """A model's frequencies and their factor; kinds whose frequencies follow the length are refused."""
+    from shard_amd import PagedCache, ops
+
+    def phases(start, n, inv):
+        angle = torch.arange(start, start + n, dtype=torch.float32)[:, None] * inv
+        return torch.stack([angle.cos(), angle.sin()], -1)
+    monkeypatch.setattr(ops, "rope_phases", phases)
+    model = rope_model(kind)
+    if kind in ("dynamic", "longrope"):
+        with pytest.raises(ValueError, match=kind):
+            PagedCache.from_model(model, n_pages=2, max_len=100)
+        return
+    cache = PagedCache.from_model(model, n_pages=2, max_len=1000)
+    assert cache.phases.shape == (1024, 32, 2)
+    check_phases(cache, model)
+    assert (kind == "yarn") == (float(cache.phases.abs().max()) > 1.01)
