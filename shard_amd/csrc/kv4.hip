@@ -415,6 +415,24 @@ constexpr float kMostScale = 2e38f;
 constexpr float kLead = 11.f, kMost = 15.f;
 constexpr float kLeast = 1.17549435e-38f;  // a factor of scores is never 0: -inf stays what it is
 
+// The reference that scores up to mx move a row's to; rounded by itself, as the
+// differences below are.
+__device__ __forceinline__ float reference(float m, float mx) {
+#pragma clang fp contract(off)
+  return fmaxf(m, mx - kLead);
+}
+// A weight's exponent, x sc - ref, rounded twice: the product as in the largest,
+// so that none is above it.  Weights take it in one step, fma(x, sc, -ref), which
+// is closer but leaves what the largest itself was rounded by: nothing that
+// matters up to a reference of kFar, and beyond it as much as fp16 cannot hold.
+constexpr float kFar = 4194304.f;   // 2^22: below it that is 2^-3 at most
+__device__ __forceinline__ float far_exponent(float x, float sc, float ref) {
+#pragma clang fp contract(off)
+  const float s = x * sc;
+  const float d = s - ref;
+  return d > kMost ? kMost : d;      // NaN stays
+}
+
 struct AttnWork {
   float* m;      // [row][split], rows (token, query head)
   float* l;
@@ -691,7 +709,7 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, X[u][i]);
         mx = across_quarters_max(mx) * sc[t];
         if (__builtin_amdgcn_ballot_w64(mx > m[t] + kMost)) {
-          const float to = fmaxf(m[t], mx - kLead);
+          const float to = reference(m[t], mx);
           const float alpha = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.f : to));
           m[t] = to;
           l[t] *= alpha;
@@ -699,14 +717,24 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
           for (int n = 0; n < NT; ++n) acc[t][n] *= alpha;
         }
         const float base = m[t] == -INFINITY ? 0.f : m[t];
+        float by = sc[t], from = -base;
+        if (__builtin_amdgcn_ballot_w64(fabsf(base) > kFar)) {
+          const bool far = fabsf(base) > kFar;
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) X[u][i] = far ? far_exponent(X[u][i], sc[t], base) : X[u][i];
+          by = far ? 1.f : by;
+          from = far ? 0.f : from;
+        }
         float sum = 0.f;
         uint32_t pairs[NS][2];
 #pragma unroll
         for (int u = 0; u < NS; ++u)
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(X[u][i], sc[t], -base));
-            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(X[u][i + 1], sc[t], -base));
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(X[u][i], by, from));
+            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(X[u][i + 1], by, from));
             sum += p;
             sum += p2;
             pairs[u][i / 2] = __builtin_bit_cast(uint32_t, half2v{(half_t)p, (half_t)p2});
@@ -1037,7 +1065,7 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
         perm32_swap(mx, mine, other);
         mx = fmaxf(mine, other) * sc;
         if (__builtin_amdgcn_ballot_w64(mx > m + kMost)) {
-          const float to = fmaxf(m, mx - kLead);
+          const float to = reference(m, mx);
           const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
           m = to;
           l *= alpha;
@@ -1047,13 +1075,23 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
             for (int e = 0; e < 16; ++e) acc[k][e] *= alpha;
         }
         const float base = m == -INFINITY ? 0.f : m;
+        float by = sc, from_m = -base;
+        if (__builtin_amdgcn_ballot_w64(fabsf(base) > kFar)) {
+          const bool far = fabsf(base) > kFar;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) S[t][e] = far ? far_exponent(S[t][e], sc, base) : S[t][e];
+          by = far ? 1.f : by;
+          from_m = far ? 0.f : from_m;
+        }
         half8 P[4];
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][e], sc, -base));
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][e], by, from_m));
             sum += p;
             P[2 * t + ((e >> 2) & 1)][(e & 3) + 4 * (e >> 3)] = (half_t)p;  // runs of tokens 0 2 | 1 3, as V's words
           }

@@ -726,3 +726,38 @@ def test_attention_joins_many_splits(cuda, total, new, wide, splits, type, D):
             b.q[r, h] = torch.from_numpy(key * (14 / (key @ key) * D ** 0.5)).to(b.type)
     _check_attention(b, b.attn())
     _check_attention(b, b.attn(max_new=max(new), max_len=max(total)))
+
+
+@pytest.mark.parametrize("type,size", [("fp16", 40.0), ("fp16", 3e3), ("fp16", 3e4), ("bf16", 3e4), ("bf16", 1e25)], ids=str)
+@pytest.mark.parametrize("total,new,H,G,D", [([300, 90], [1, 1], 8, 2, 128), ([300], [20], 4, 1, 64), ([400, 200], [180, 200], 8, 4, 64),
+                                             ([2300], [3], 128, 64, 64), ([300], [200], 4, 1, 128)], ids=str)
+def test_attention_huge_scores(cuda, total, new, H, G, D, type, size):
+    """Scores up to 1e9 and (bf16 queries) 1e30, far from each other: every row's weight is on its one best key, whatever
+    fp32 leaves of the differences."""
+    b = Batch(total, new, H, G, D, type, seed=17, wide=1)
+    b.new = b.total                                                # every token is appended
+    T = sum(total)
+    cu = torch.tensor([sum(total[:i]) for i in range(len(total) + 1)], dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(3)
+    k = (torch.sign(torch.randn(T, G, D, generator=g)) * min(size, 3e4)).to(b.type)
+    v = torch.randn(T, G, D, generator=g).to(b.type)
+    still = torch.zeros(b.table.shape[1] * 64, D // 2, 2, device=cuda)
+    still[..., 0] = 1                                              # no rotation
+    from shard_amd import ops
+    ops.kv4_append(k.to(cuda), v.to(cuda), b.d_cache, b.d_table, b.d_lens, still, cu_seqlens=cu)
+    want = torch.empty(b.q.shape, dtype=torch.float64)
+    K, V = plain.held(b.d_cache.cpu().numpy())
+    best = torch.randint(0, 1 << 30, (b.q.shape[0], H), generator=g)
+    for r, s, pos in b.where():
+        for h in range(H):
+            t = int(best[r, h]) % (pos + 1)                        # its query: the key's own signs
+            at = int(b.table[s, t // 64]), t % 64, h // (H // G)
+            b.q[r, h] = torch.from_numpy(np.sign(K[at]) * size).to(b.type)
+            want[r, h] = torch.from_numpy(V[at])
+    # keys of random signs: the best key's score is D |q k| scale, any other's at least 8 |q k| scale less (4 signs apart;
+    # 20 and more in fact), so that its weight is below e^-100 and the output the best key's value, times its weight in
+    # fp16 over its weight in fp32 (2^-11), the division and one rounding to the type
+    assert size * min(size, 3e4) * 8 * D ** -0.5 > 100
+    out = b.attn().cpu()
+    assert bool(out.isfinite().all())
+    assert bool(((out.double() - want).abs() <= (2.0 ** -11 + torch.finfo(b.type).eps / 2 + 2.0 ** -21) * want.abs()).all())
