@@ -1026,7 +1026,8 @@ def _kv4_batch(cache, block_table, seq_lens, n_tokens, cu_seqlens, max_new, max_
         t0 = W
     if not n_pages or not G or not W or s0 < G * width or t0 < W:
         return None
-    return dev, G, width // 68, (n_pages, W, max_new or 0, max_len or 0, cache.data_ptr(), s0, block_table.data_ptr(), t0,
+    max_new, max_len = (min(max(n or 0, 0), 0x7FFFFFFF) for n in (max_new, max_len))  # hints: any number will do
+    return dev, G, width // 68, (n_pages, W, max_new, max_len, cache.data_ptr(), s0, block_table.data_ptr(), t0,
                                  seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr())
 
 

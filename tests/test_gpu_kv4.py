@@ -761,3 +761,14 @@ def test_attention_huge_scores(cuda, total, new, H, G, D, type, size):
     out = b.attn().cpu()
     assert bool(out.isfinite().all())
     assert bool(((out.double() - want).abs() <= (2.0 ** -11 + torch.finfo(b.type).eps / 2 + 2.0 ** -21) * want.abs()).all())
+
+
+@pytest.mark.parametrize("hint", [1 << 31, 1 << 40, 1 << 70, -1, -(1 << 40)])
+def test_hints_of_any_size(cuda, hint):
+    """Below zero is unknown, beyond 32 bits the largest: neither is an error, by either way through the calls."""
+    b = Batch([130, 40], [30, 1], 4, 2, 64, seed=18).fill()
+    want_q = b.append(q=b.d_q)
+    want, read = b.attn(), b.read()
+    assert torch.equal(b.append(q=b.d_q, max_new=hint), want_q)
+    assert all(torch.equal(x, y) for x, y in zip(b.read(max_new=hint), read))
+    assert torch.equal(b.attn(max_new=hint, max_len=hint), want)
