@@ -517,7 +517,9 @@ int shard_eigh_top(double* a, int32_t n, int32_t top, double* evals, double* eve
  * 16; q_out, k_out, v_out and out are contiguous (n_tokens, heads, head_dim).
  * max_new and max_len (0: unknown) are the largest numbers of new tokens and
  * of tokens of a sequence: they size launches, the results do not depend on
- * them beyond the order of fp32 sums. */
+ * them beyond the order of fp32 sums.  Attention takes one kernel for the whole
+ * call, by max_new: sequences of one or a few new tokens are up to 8 times faster
+ * in a call of their own than beside a prompt. */
 #define SHARD_KV4_PAGE 64
 #define SHARD_FP16 0
 #define SHARD_BF16 1
@@ -575,7 +577,8 @@ int64_t shard_kv4_page_bytes(int32_t n_kv_heads, int32_t head_dim);
 /* New tokens into the cache: k rotated at its position by phases (x_i c -
  * x_{i + D/2} s, x_{i + D/2} c + x_i s, in 64 bits) and v, rounded to 4 bits;
  * with q, its rows rotated into q_out as well, rounded once.  One launch.
- * A page that two sequences of the call append to is a race. */
+ * A page that two sequences of the call append to, or one of them in two places
+ * of its table, is a race. */
 int shard_kv4_append(const shard_kv4_args* args, void* stream);
 
 /* K and V that the cache holds for the rows' tokens, exact in both types. */
@@ -584,7 +587,10 @@ int shard_kv4_read(const shard_kv4_args* args, void* stream);
 /* Causal attention of the rows' tokens over their sequences: out =
  * sum_t softmax_t(scale q . k_t) v_t over tokens t up to the row's own; rows
  * that see none are zeros.  Scores, softmax statistics and sums in 32 bits,
- * the weights of V in fp16.  Workspace: shard_kv4_attn_workspace(args) bytes,
+ * the weights of V in fp16 (2^-11 of each, or 2^-36 of a row's largest), bf16
+ * queries to 2^-26 of their row's largest.  Tokens within seq_lens that have a
+ * page are taken as stored: those that an append left out because its phases end
+ * before them must not be.  Workspace: shard_kv4_attn_workspace(args) bytes,
  * 16-byte aligned (0: none needed); nothing in it needs clearing. */
 size_t shard_kv4_attn_workspace(const shard_kv4_args* args);
 int shard_kv4_attn(const shard_kv4_args* args, void* workspace, size_t workspace_bytes, void* stream);

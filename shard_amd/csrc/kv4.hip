@@ -169,7 +169,10 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // Measured (32 query heads on 8, head_dim 128, fp16): four prompts of 8,192
 // tokens 179 us, 4.0 TB/s of the 724 MB it reads and writes (a large copy: 4.75),
 // the vector pipe half busy with K's 64-bit rotation and the roundings; one token
-// 6 us, a chain of five dependent memory accesses.
+// 6 us.  That is not its chain of memory accesses (arguments, length, table, page,
+// store): the read has the same and takes 3.2.  Most likely it is the serial work of
+// few lanes: 8 threads rotate, round and code 16 elements of K each, and 8 of a
+// query workgroup take 4 heads one after the other.
 // --------------------------------------------------------------------------
 constexpr int kHeadsQ = 4;
 
@@ -1290,6 +1293,11 @@ int groups_of(const shard_kv4_args* a) {
 // with both: 64 sequences of 128 to 8,192 tokens at head_dim 64 24.9 / 23.9
 // (either alone: 24.0 and 25.2), at 128 39.8 / 37.9, 256 of 62 to 4,000 74.5 /
 // 67.3, 100 of 250 to 16,000 60.7 / 56.5; equal lengths, 128 of 3,000, 83.6 / 84.4.
+// One choice for the call, by its longest sequence of new tokens: a prompt beside
+// single tokens puts those into tiles of 128 rows, without splits of their own.  A
+// prompt of 2,048 beside 32 single tokens at 8K to 32K 1,414 us (the two in calls
+// of their own 181), a chunk of 512 at 8K beside them 1,391 (203), 40 new tokens
+// 932 (144).
 struct AttnPlan {
   int rows;       // of a workgroup: 4, 8, 16 or 32 (rows kernel), 128 (tile kernel)
   int row_tiles, n_splits, split_shift;

@@ -20,8 +20,8 @@
 // are equal.  Where more than the list holds reach the bound (many equal
 // logits), the list's own k-th largest is the next bound.
 //
-// Measured: 2,048 rows of 128,256 bf16 logits with 20 alternatives 109 us, 4.8
-// TB/s, a large copy's rate, the vector pipe 82% busy; one fp16 row with 5, in 63
+// Measured: 2,048 rows of 128,256 bf16 logits with 20 alternatives 110 us, 4.8
+// TB/s, a large copy's rate, the vector pipe 87% busy; one fp16 row with 5, in 63
 // parts, 5 us and 4 for the join, each a chain of latencies: load, sums, bound,
 // list.
 #include <stdio.h>

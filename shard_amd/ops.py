@@ -1083,7 +1083,7 @@ def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=No
     device: tokens at positions outside the table or in pages outside the cache
     are left out; rows behind the last sequence's are not read, and their
     rotated q not written.  Two sequences of one call must not append to the
-    same page."""
+    same page, nor one to a page that its table names twice."""
     direct = _direct or _bind_direct()
     if direct and k.is_cuda:
         dev = _current_device()
@@ -1157,7 +1157,9 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
     rows behind the last sequence's are not written.  max_new and max_len, the
     most new tokens and tokens of a sequence, size the launch where the caller
     knows them; other lengths give the same result, only slower (a captured
-    graph does best with what its replays reach)."""
+    graph does best with what its replays reach).  The call is made for its
+    longest sequence of new tokens: where a prompt stands beside sequences of one
+    or a few new tokens, a call for each kind is up to 8 times faster."""
     direct = _direct or _bind_direct()
     if direct and out is None and q.is_cuda:
         dev = _current_device()
