@@ -126,7 +126,7 @@ def enable_llama_fused_attention(model=None):
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None,
                 past_key_values=None, cache_position=None, **kwargs):
         if isinstance(past_key_values, PagedCache):
-            return paged_forward(self, hidden_states, past_key_values)
+            return paged_forward(self, hidden_states, past_key_values, attention_mask)
         is_shard = isinstance(past_key_values, Cache)
         layer = past_key_values.layers[self.layer_idx] if is_shard else None
         gc = getattr(layer, "_gpu_compressed", None) if layer is not None else None

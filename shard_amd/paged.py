@@ -202,6 +202,7 @@ class PagedCache(HFCache):
             keep = torch.tensor([len(t) for t in tokens]).cumsum(0).to(dev) - 1
         pos = self.begin(seqs, [len(t) for t in tokens])
         step = self._step
+        step["unmasked"] = True
         try:
             logits = model(input_ids=ids, position_ids=pos, past_key_values=self, use_cache=True, logits_to_keep=keep).logits[0]
         except BaseException:
@@ -212,8 +213,24 @@ class PagedCache(HFCache):
         return logits
 
 
-def paged_forward(attention, hidden_states, cache):
-    """LlamaAttention.forward on an open step of a PagedCache."""
+def _hides(mask) -> bool:
+    """Whether an attention mask as transformers hands it to a layer keeps a token from one at or before its own place."""
+    if mask.dim() == 2:
+        return not bool(mask.bool().all())
+    seen = mask if mask.dtype == torch.bool else mask == 0
+    n, keys = mask.shape[-2:]
+    return not bool((seen | torch.ones(n, keys, dtype=torch.bool, device=mask.device).triu(1 + keys - n)).all())
+
+
+def paged_forward(attention, hidden_states, cache, attention_mask=None):
+    """LlamaAttention.forward on an open step of a PagedCache.  A mask that hides
+    tokens (a padded batch) is refused: there is none in a step, whose pages
+    would keep the padding.  It is looked at once a step, and not in run()'s."""
+    step = cache._open()
+    if isinstance(attention_mask, torch.Tensor) and step is not None and not step.get("unmasked"):
+        if _hides(attention_mask):
+            raise ValueError("a PagedCache takes no padding and no attention mask: pack the sequences' tokens in one row (run() does)")
+        step["unmasked"] = True
     shape = hidden_states.shape[:-1]
     x = hidden_states.reshape(-1, hidden_states.shape[-1])
     q, k, v = (proj(x).unflatten(-1, (-1, attention.head_dim)) for proj in (attention.q_proj, attention.k_proj, attention.v_proj))

@@ -68,3 +68,28 @@ def test_layers_of_uneven_steps(cuda, shape, dtype):
     cache.run(model, [b, a], logits.argmax(-1, keepdim=True).flip(0))
     cache.run(model, [a, c, b], [ids(1), ids(150), ids(3)])
     assert seen == [92, 92, 2, 2, 154, 154]
+
+
+@pytest.mark.parametrize("how", ["sdpa", "eager"])
+def test_padded_batches_are_refused(cuda, how):
+    """A batch of rows of one length runs through the model as it is; one with padding does not, and its step is undone."""
+    from shard_amd import PagedCache, enable_llama_fused_attention
+    model = _model(cuda)
+    model.set_attn_implementation(how)
+    enable_llama_fused_attention(model)
+    ids = torch.randint(0, VOCAB, (2, 20), generator=torch.Generator().manual_seed(1)).to(cuda)
+    cache = PagedCache.from_model(model, n_pages=4, max_len=64)
+    a, b, c, d = (cache.add() for _ in range(4))
+    mask = torch.ones(2, 20, dtype=torch.int64, device=cuda)
+    mask[0, :5] = 0
+    with torch.no_grad():
+        pos = cache.begin([a, b], [20, 20])
+        with pytest.raises(ValueError, match="mask"):
+            model(input_ids=ids, attention_mask=mask, position_ids=pos.view(2, 20), past_key_values=cache, use_cache=True)
+        cache.cancel()
+        assert cache.length(a) == 0 and cache.free_pages() == 4
+        pos = cache.begin([a, b], [20, 20])
+        got = model(input_ids=ids, attention_mask=torch.ones_like(mask), position_ids=pos.view(2, 20), past_key_values=cache,
+                    use_cache=True).logits
+    want = cache.run(model, [c, d], list(ids), last_only=False)
+    assert torch.equal(got.view(40, -1), want)

@@ -217,3 +217,32 @@ def test_rope_kinds(monkeypatch, kind):
     assert cache.phases.shape == (1024, 32, 2)
     check_phases(cache, model)
     assert (kind == "yarn") == (float(cache.phases.abs().max()) > 1.01)
+
+
+def _masks(B, n, hidden):
+    """What transformers hands to a layer for a batch whose first row begins with `hidden` pad tokens."""
+    keep = torch.ones(B, n, dtype=torch.bool)
+    keep[0, :hidden] = False
+    both = torch.ones(n, n, dtype=torch.bool).tril() & keep[:, None, None]
+    low = torch.finfo(torch.float16).min
+    return [both, torch.zeros(both.shape, dtype=torch.float16).masked_fill(~both, low), keep, keep.long()]
+
+
+@pytest.mark.parametrize("form", range(4), ids=["bool", "additive", "rows", "0 and 1"])
+def test_a_padded_batch_is_refused(paged, form):
+    """Before anything is stored; a mask that is only causal is none."""
+    from types import SimpleNamespace
+    from shard_amd.paged import paged_forward
+    layer = SimpleNamespace(head_dim=64, layer_idx=0, scaling=0.125, o_proj=lambda x: x, **{
+        name: (lambda x: x) for name in ("q_proj", "k_proj", "v_proj")})
+    a, b = paged.add(), paged.add()
+    x = torch.randn(2, 6, 128)
+    paged.begin([a, b], [6, 6])
+    with pytest.raises(ValueError, match="mask"):
+        paged_forward(layer, x, paged, _masks(2, 6, 2)[form])
+    assert paged._open()["left"] == {0, 1}
+    out, weights = paged_forward(layer, x, paged, _masks(2, 6, 0)[form])
+    assert torch.equal(out, x) and weights is None and paged._open()["left"] == {1}
+    paged.cancel()
+    paged.begin([a], [6])
+    assert torch.equal(paged_forward(layer, x[:1], paged)[0], x[:1])
