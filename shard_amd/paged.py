@@ -55,6 +55,11 @@ class PagedLayer(CacheLayerMixin):
     def lazy_initialization(self, *args, **kwargs):
         pass
 
+    def _rows(self, *args, **kwargs):
+        raise RuntimeError("a PagedCache has sequences, not rows of a batch: add(), drop() and run() by their numbers")
+
+    reset = reorder_cache = crop = batch_repeat_interleave = batch_select_indices = _rows
+
 
 class PagedCache(HFCache):
     def __init__(self, n_pages, max_len, head_dim=128, num_layers=32, n_kv_heads=8, device="cuda", rope_inv_freq=None,

@@ -246,3 +246,12 @@ def test_a_padded_batch_is_refused(paged, form):
     paged.cancel()
     paged.begin([a], [6])
     assert torch.equal(paged_forward(layer, x[:1], paged)[0], x[:1])
+
+
+def test_calls_of_batched_caches_are_refused(paged):
+    """transformers' own reorder_cache would do nothing, for a length of 0, and say nothing."""
+    idx = torch.tensor([0])
+    for call in (lambda: paged.reorder_cache(idx), paged.reset, lambda: paged.crop(1), lambda: paged.batch_repeat_interleave(2),
+                 lambda: paged.batch_select_indices(idx)):
+        with pytest.raises(RuntimeError, match="sequences"):
+            call()
