@@ -409,12 +409,15 @@ void k_kv4_read(const shard_kv4_args a) {
 // sums, and the largest weight lies between 2^kLead and 2^kMost, fp16's upper end.
 // P is rounded to fp16: 2^-11 of each weight down to 2^-(14 + kLead) of a row's
 // largest, 2^-(25 + kLead) of that largest below, so that what many keys far
-// below one key add up to is kept; the sums are fp32.  The cache's values are exact.  bf16 queries are scaled by a power of two a row (their
-// largest below 2) and are then exact in fp16 down to 2^-17 of that largest
+// below one key add up to is kept; the sums are fp32.  A longer lead moves m more
+// often: a prompt of 8,192 tokens 570 us with m moved at 8 above it and no lead,
+// 574 with leads of 7 and 11, 575 with 13; a chunk of 512 over 16K 163, 163.5, 165.7.
+// The cache's values are exact.  bf16 queries are scaled by a power of two a row
+// (their largest below 2) and are then exact in fp16 down to 2^-17 of that largest
 // (below it they lose bits, 2^-26 of the largest at most); the power goes back
 // in through the softmax scale.
 // --------------------------------------------------------------------------
-constexpr float kMostScale = 2e38f;
+constexpr float kMostScale = 2e38f;  // times log2(e) it is finite
 constexpr float kLead = 11.f, kMost = 15.f;
 constexpr float kLeast = 1.17549435e-38f;  // a factor of scores is never 0: -inf stays what it is
 
