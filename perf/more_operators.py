@@ -513,7 +513,8 @@ def run(st):
                                  max_new=st["max_new"], max_len=st["max_len"])
     if kind == "verify":
         rows, counts, tokens = ops.verify_drafts(st["logits"], st["tokens"], st["parents"], st["uniforms"], cu_seqlens=st["cu"],
-                                                 draft_probs=st["probs"], temperature=st["temperature"], max_new=st["max_new"])
+                                                 draft_probs=st["probs"], temperature=st["temperature"], max_new=st["max_new"],
+                                                 max_depth=st["levels"])
         return {"rows": rows, "counts": counts, "next": tokens}
     mask, positions = ops.draft_tree(st["parents"], st["lens"], cu_seqlens=st["cu"], max_new=st["max_new"])
     flat = st["cache"].flatten(0, 1)
