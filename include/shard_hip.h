@@ -596,6 +596,96 @@ size_t shard_kv4_attn_workspace(const shard_kv4_args* args);
 int shard_kv4_attn(const shard_kv4_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Drafted tokens: a step whose rows are a tree (speculative decoding)
+ * ------------------------------------------------------------------------ */
+
+/* A sequence's rows: row 0 follows its tokens before the step, every other row
+ * names the row of its parent, parents[row] (counted within the sequence, an
+ * earlier row; anything else: no parent, the row follows the tokens before the
+ * step as well).  All rows take a place in the cache, in their order; a row's
+ * position is that of its parent + 1.
+ *
+ * The step's plan, one launch: mask (n_tokens, words), bit j % 64 of word j / 64
+ * set where the row sees row j of its sequence (its ancestors and itself);
+ * positions (n_tokens).  Rows from 64 * words on of a sequence see no row and
+ * have position -1; rows behind the last sequence's are not written.  words up
+ * to SHARD_TREE_ROWS / 64. */
+#define SHARD_TREE_ROWS 1024
+int shard_draft_tree(const int32_t* parents, const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t batch,
+                     int32_t n_tokens, int32_t words, uint64_t* mask, int32_t* positions, void* stream);
+
+/* shard_kv4_append with rows rotated at positions[row] (n_tokens, device; null:
+ * their own places); rows whose position is negative or past the phases are
+ * left out. */
+int shard_kv4_append_at(const shard_kv4_args* args, const int32_t* positions, void* stream);
+
+/* shard_kv4_attn where a row sees the tokens before its sequence's rows and those
+ * rows whose bits mask (n_tokens, words; as shard_draft_tree's, any bits will do)
+ * has for it.  Workspace as shard_kv4_attn's. */
+int shard_kv4_tree_attn(const shard_kv4_args* args, const uint64_t* mask, int32_t words, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* After a step: the token of row rows[b * rows_stride + j] of sequence b moves to
+ * the place of its row j, for j < min(counts[b], width, its rows), K and V as they
+ * are stored, in n_layers caches of one layout, layer_stride bytes apart (args'
+ * cache is the first).  seq_lens and cu_seqlens are the step's.  An entry below j,
+ * not below the sequence's rows, or of a token without a place moves nothing.
+ * Rows and counts live in device memory. */
+int shard_kv4_keep(const shard_kv4_args* args, int32_t n_layers, int64_t layer_stride, const int32_t* rows,
+                   int64_t rows_stride, int32_t width, const int32_t* counts, void* stream);
+
+/* Verification of a step's drafted tokens against the target model's logits
+ * (n_tokens, vocab; row stride in elements; dtype SHARD_FP16, SHARD_BF16 or
+ * SHARD_FP32, aligned to its elements), one walk a sequence from its row 0 on.
+ * With s = p = softmax(logits / temperature) of the row it is at, the row's
+ * children are tried in their order, child c with token x = tokens[c]:
+ *   draft_probs null  accepted where uniforms[c][0] sum(s) < s[x]; else s[x] = 0
+ *   q = draft_probs[c] (n_tokens, vocab; fp32), the distribution that x was drawn
+ *     from  accepted where uniforms[c][0] q[x] sum(s) < s[x]; else
+ *     s = max(s / sum(s) - q, 0), unless that leaves nothing
+ * The walk goes on at an accepted child; it ends where none is, or max_depth
+ * children have been.  path[b] (batch, width) are the rows it went through from
+ * row 0 on, -1 behind them, counts[b] their number; next[b] is the first token at
+ * which the running sum of s exceeds uniforms[row][1] sum(s), row the last one.
+ * Weights and sums in 64 bits.  A temperature (temperatures[b], or temperature where
+ * that is null) of 0 or below: p is 1 at the largest logit, the first of equal ones,
+ * and no random number counts.  Numbers are in [0, 1).
+ *
+ * A sequence's rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (null: row b alone),
+ * parents as in shard_draft_tree; width, up to SHARD_TREE_ROWS, bounds the rows
+ * of a sequence that are looked at.  A child whose token is not of the vocabulary
+ * is passed over.  A row of NaN, +inf (temperature above 0) or without a logit
+ * above -inf has no answer: the walk ends there, next -1.  A sequence without rows:
+ * count 0, next -1.  A child tried after a rejected one with draft_probs takes a
+ * pass over the row by its sequence's workgroups each (one row of 128,256: 30 us).
+ *
+ * Workspace: shard_verify_drafts_workspace(args) bytes, 16-byte aligned; nothing in
+ * it needs clearing. */
+typedef struct shard_verify_args {
+  int32_t batch, n_tokens;
+  int64_t vocab;
+  const void* logits;
+  int64_t row_stride;
+  int32_t dtype, width;
+  const int64_t* tokens;            /* (n_tokens); a sequence's first one is not read */
+  const int32_t* parents;           /* (n_tokens) */
+  const float* uniforms;            /* (n_tokens, 2) */
+  const int32_t* cu_seqlens;        /* (batch + 1) or null */
+  const float* draft_probs;         /* or null */
+  int64_t probs_stride;
+  const float* temperatures;        /* (batch) or null */
+  float temperature;
+  int32_t max_depth;
+  int32_t* path;
+  int32_t* counts;
+  int64_t* next;
+} shard_verify_args;
+
+size_t shard_verify_args_size(void);
+size_t shard_verify_drafts_workspace(const shard_verify_args* args);
+int shard_verify_drafts(const shard_verify_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Log probabilities of a model's answers
  * ------------------------------------------------------------------------ */
 

@@ -67,6 +67,16 @@ class KV4Args(ctypes.Structure):
     ]
 
 
+class VerifyArgs(ctypes.Structure):
+    """Mirror of shard_verify_args (include/shard_hip.h)."""
+    _fields_ = [
+        ("batch", c_int32), ("n_tokens", c_int32), ("vocab", c_int64), ("logits", c_void_p), ("row_stride", c_int64),
+        ("dtype", c_int32), ("width", c_int32), ("tokens", c_void_p), ("parents", c_void_p), ("uniforms", c_void_p),
+        ("cu_seqlens", c_void_p), ("draft_probs", c_void_p), ("probs_stride", c_int64), ("temperatures", c_void_p),
+        ("temperature", c_float), ("max_depth", c_int32), ("path", c_void_p), ("counts", c_void_p), ("next", c_void_p),
+    ]
+
+
 # SHARD_KV4_ARGS_LAYOUT of the header
 KV4_LAYOUT = (ctypes.sizeof(KV4Args) << 32) + sum((2 * i + 1) * getattr(KV4Args, name).offset
                                                   for i, (name, _) in enumerate(KV4Args._fields_))
@@ -132,6 +142,13 @@ SIGNATURES = [
     ("shard_kv4_read", c_int32, [c_void_p, c_void_p]),
     ("shard_kv4_attn_workspace", c_size_t, [c_void_p]),
     ("shard_kv4_attn", c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("shard_kv4_append_at", c_int32, [c_void_p, c_void_p, c_void_p]),
+    ("shard_kv4_tree_attn", c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
+    ("shard_kv4_keep", c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
+    ("shard_draft_tree", c_int32, [c_void_p] * 3 + [c_int32] * 3 + [c_void_p] * 3),
+    ("shard_verify_args_size", c_size_t, []),
+    ("shard_verify_drafts_workspace", c_size_t, [c_void_p]),
+    ("shard_verify_drafts", c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
     ("shard_token_logprobs_workspace", c_size_t, [c_int64, c_int64, c_int32]),
     ("shard_token_logprobs", c_int32, [c_void_p, c_int32] + [c_int64] * 3 + [c_void_p, c_int32] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     ("shard_stream_dequant_qjl", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
@@ -164,6 +181,8 @@ def load():
         raise ShardHipUnavailable("shard_decode_args layout mismatch between header and binding")
     if lib.shard_kv4_args_layout() != KV4_LAYOUT or KV4_PACK.size != ctypes.sizeof(KV4Args):
         raise ShardHipUnavailable("shard_kv4_args layout mismatch between header and binding")
+    if lib.shard_verify_args_size() != ctypes.sizeof(VerifyArgs):
+        raise ShardHipUnavailable("shard_verify_args layout mismatch between header and binding")
     _lib = lib
     return lib
 

@@ -176,9 +176,11 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // --------------------------------------------------------------------------
 constexpr int kHeadsQ = 4;
 
-template <class T, int D>
+// AT: a row is rotated at positions[row] instead of its own place (drafted tokens
+// of a tree: siblings have places of their own and one position).
+template <class T, int D, bool AT>
 __global__ __launch_bounds__(256, 4)
-void k_kv4_append(const shard_kv4_args a) {
+void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions) {
   constexpr int PB = D / 64;  // pairs of 32-channel blocks: (pb, pb + PB)
   __shared__ __align__(4) uint8_t codes[32][D + 4];
   const int tid = threadIdx.x, b = blockIdx.z;
@@ -194,10 +196,17 @@ void k_kv4_append(const shard_kv4_args a) {
     const int t0 = grp * 32;
     const int pos = t0 + tok, i = pos - start;
     const bool mine = tok < 32 && i >= 0 && i < s.n;
-    const bool there = mine && pos >= 0 && pos < s.cap && pos < a.n_phases;
+    const int turn = AT ? (mine ? positions[s.row0 + i] : -1) : pos;
+    const bool there = mine && pos >= 0 && pos < s.cap && turn >= 0 && turn < a.n_phases;
+    uint32_t new_bits = 0;                          // AT: of the group's tokens
+    if constexpr (AT) {
+      const int bit = threadIdx.x & 31, row = t0 + bit - start;
+      const int at = row >= 0 && row < s.n ? positions[s.row0 + row] : -1;
+      new_bits = (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0 && at < a.n_phases && t0 + bit >= 0);
+    }
     float c[8], sn[8];
     if (there) {
-      const float4* ph = (const float4*)(a.phases + ((int64_t)pos * (D / 2) + ch) * 2);
+      const float4* ph = (const float4*)(a.phases + ((int64_t)turn * (D / 2) + ch) * 2);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float4 f = ph[j];
@@ -232,7 +241,9 @@ void k_kv4_append(const shard_kv4_args a) {
     if (page < 0) continue;
     uint8_t* base = head_of<D>(a, page, g);
     const int slot0 = t0 & 63, slot = slot0 + tok;
-    const auto is_new = [&](int t) { return (unsigned)(t0 + t - start) < (unsigned)s.n && t0 + t < a.n_phases; };
+    const auto is_new = [&](int t) {
+      return AT ? (bool)(new_bits >> t & 1) : (unsigned)(t0 + t - start) < (unsigned)s.n && t0 + t < a.n_phases;
+    };
     // all that the group reads, before anything waits: k, v, and the words of V
     // codes that earlier tokens share
     constexpr int VU = D / 64;                        // 8-channel pieces of V a thread, words a thread
@@ -447,6 +458,8 @@ struct AttnWork {
   int group, group_shift;       // query heads of a kv head; -1: no power of two
   int row_tiles;                // workgroups along a sequence's rows
   float sorted;                 // 16 / longest length where longer sequences go first, or 0
+  const uint64_t* mask;         // [row][words]: which rows of its sequence a row sees (trees)
+  int words;
 };
 
 // Tiles (pages) a split of a sequence of `tiles` takes: at least kMinTiles, one
@@ -485,6 +498,24 @@ __device__ __forceinline__ void nothing(const shard_kv4_args& a, const AttnWork&
     w.m[part] = -INFINITY;
     w.l[part] = 0.f;
   }
+}
+
+// Trees of drafted tokens: row i of a sequence sees the tokens before its rows and
+// those rows whose bits its mask has.  The page's 64 tokens as bits, from token
+// `from` of the sequence on; `first` is the place of row 0.  Words that the mask
+// does not have are 0.
+__device__ __forceinline__ uint64_t seen_bits(const AttnWork& w, int64_t row, int from, int first, int keys) {
+  const int o = from - first;                         // row of the page's first token
+  uint64_t bits = ~0ull;
+  if (o > -64) {
+    const uint64_t* m = w.mask + row * w.words;
+    const int at = o >> 6, sh = o & 63;               // floor: at is -1 where the page begins before the rows
+    const uint64_t lo = at < 0 ? ~0ull : at < w.words ? m[at] : 0ull;
+    const uint64_t hi = sh && at + 1 < w.words ? m[at + 1] : 0ull;
+    bits = sh ? lo >> sh | hi << (64 - sh) : lo;
+  }
+  const int left = keys - from;
+  return left >= 64 ? bits : left <= 0 ? 0ull : bits & ((1ull << left) - 1);
 }
 
 // A page's operands for one wave.
@@ -558,7 +589,7 @@ __device__ __forceinline__ float across_quarters_sum(float v) {
 // Not faster: 8 or 16 waves a workgroup without splits (one sequence of 2,048
 // 13.4 us against 8.2 with the merge), work cut on the device by the sequences'
 // lengths (the 64 sequences 27.7 us against 26.9 then).
-template <class T, int D, int ROWS>
+template <class T, int D, int ROWS, bool TREE>
 __global__ __launch_bounds__(256, (D == 128 ? 4 : 5) - (ROWS > 16 ? 2 : 1))
 void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   constexpr int WAVES = 4;
@@ -593,17 +624,17 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
     typedef T vec8 __attribute__((ext_vector_type(8)));
     vec8 raw[NQ][ST];
     float sc[NQ], m[NQ], l[NQ];
-    int lim[NQ];                      // keys that the lane's row sees
+    int lim[NQ];                      // keys that the lane's row sees; TREE: its row
     float4v acc[NQ][NT];
     const int r0 = rt * ROWS, r1 = min(r0 + ROWS, n_rows) - 1;
     // of the tile's rows (uniform)
-    const int lim_min = min(max(s.len - s.n + token_of(w, r0) + 1, 0), keys);
-    const int lim_max = min(max(s.len - s.n + token_of(w, r1) + 1, 0), keys);
+    const int lim_min = min(max(s.len - s.n + (TREE ? 0 : token_of(w, r0) + 1), 0), keys);
+    const int lim_max = TREE ? keys : min(max(s.len - s.n + token_of(w, r1) + 1, 0), keys);
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       const int r = min(r0 + 16 * t + (F == 1 ? col : col % ROWS), r1);   // columns behind the last row repeat it, unused
       const int i = token_of(w, r), h = r - i * group;
-      lim[t] = min(max(s.len - s.n + i + 1, 0), keys);
+      lim[t] = TREE ? s.row0 + i : min(max(s.len - s.n + i + 1, 0), keys);
       const T* qp = (const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(g * group + h) * a.q_head_stride + kq * (D / 4);
 #pragma unroll
       for (int j = 0; j < ST; ++j) raw[t][j] = *(const vec8*)(qp + 8 * j);
@@ -702,11 +733,19 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
             for (int i = 0; i < 4; ++i) X[u][i] = F == 2 && fold ? S[t][(u + NS) & 3][i] : S[t][u][i];
         }
         if (none || (tile + 1) * kPage > lim_min) {
-          const int seen = (none ? 0 : lim[t]) - tile * kPage - 16 * NS * fold - 4 * kq;
+          if constexpr (TREE) {
+            const uint64_t seen = none ? 0ull : seen_bits(w, lim[t], tile * kPage, s.len - s.n, keys) >> (16 * NS * fold + 4 * kq);
 #pragma unroll
-          for (int u = 0; u < NS; ++u)
+            for (int u = 0; u < NS; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) X[u][i] = 16 * u + i < seen ? X[u][i] : -INFINITY;
+              for (int i = 0; i < 4; ++i) X[u][i] = seen >> (16 * u + i) & 1 ? X[u][i] : -INFINITY;
+          } else {
+            const int seen = (none ? 0 : lim[t]) - tile * kPage - 16 * NS * fold - 4 * kq;
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) X[u][i] = 16 * u + i < seen ? X[u][i] : -INFINITY;
+          }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -942,7 +981,7 @@ struct VRegs {  // a thread's part of a page's V: W channels 16 apart of 8 token
 
 constexpr int kTileRows = 128;
 
-template <class T, int D>
+template <class T, int D, bool TREE>
 __global__ __launch_bounds__(256, 2)
 void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   constexpr int QS = D / 16;        // k-steps of a score
@@ -966,14 +1005,14 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
   const int first = split * per, end = min(first + per, tiles);
   if (w.n_splits > 1 && first >= tiles) return nothing(a, w, s, g, split, at);
   const int n_tiles = (n_rows + kTileRows - 1) / kTileRows;
-  const auto limit = [&](int row) { return min(max(s.len - s.n + token_of(w, row) + 1, 0), keys); };
+  const auto limit = [&](int row) { return TREE ? keys : min(max(s.len - s.n + token_of(w, row) + 1, 0), keys); };
 
   for (int back = at; back < n_tiles; back += w.row_tiles) {
     const int rt = n_tiles - 1 - back;
     const int r0 = rt * kTileRows + wave * 32;                  // the wave's first row
     const int last = min(end, (limit(min(rt * kTileRows + kTileRows, n_rows) - 1) + kPage - 1) / kPage);
     // keys that every row of the wave sees: pages below need no mask
-    const int lim_min = r0 + 32 <= n_rows ? limit(r0) : 0;
+    const int lim_min = r0 + 32 > n_rows ? 0 : TREE ? min(max(s.len - s.n, 0), keys) : limit(r0);
     const int r = r0 + col;
     const bool live = r < n_rows;
     const int i = live ? token_of(w, r) : 0, h = g * group + (live ? r - i * group : 0);
@@ -1055,12 +1094,20 @@ void k_kv4_attn_tile(const shard_kv4_args a, const AttnWork w) {
         kr.store(sk + k0);
         kr.load(page_at(p3));
         if (p0 < 0 || (tile + 1) * kPage > lim_min) {
-          const int seen = p0 < 0 ? 0 : lim;          // keys of no page are not seen
+          if constexpr (TREE) {
+            const uint64_t seen = p0 < 0 || !live ? 0ull : seen_bits(w, s.row0 + i, tile * kPage, s.len - s.n, keys) >> (4 * hi);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              S[t][e] = tile * kPage + 32 * t + 8 * (e >> 2) + 4 * hi + (e & 3) < seen ? S[t][e] : -INFINITY;
+              for (int e = 0; e < 16; ++e) S[t][e] = seen >> (32 * t + 8 * (e >> 2) + (e & 3)) & 1 ? S[t][e] : -INFINITY;
+          } else {
+            const int seen = p0 < 0 ? 0 : lim;        // keys of no page are not seen
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                S[t][e] = tile * kPage + 32 * t + 8 * (e >> 2) + 4 * hi + (e & 3) < seen ? S[t][e] : -INFINITY;
+          }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -1255,6 +1302,139 @@ void k_kv4_merge(const shard_kv4_args a, const AttnWork w) {
 }
 
 // --------------------------------------------------------------------------
+// A step's plan: which of its sequence's rows a drafted token sees, and where it
+// stands.  A row's ancestors have falling indices, so its words are written from
+// the last to the first as the walk up its parents passes them.
+// --------------------------------------------------------------------------
+struct TreeArgs {
+  const int32_t* parents;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  int batch, n_tokens, words;
+  uint64_t* mask;
+  int32_t* positions;
+};
+
+__global__ __launch_bounds__(256)
+void k_draft_tree(const TreeArgs t) {
+  __shared__ int32_t up[SHARD_TREE_ROWS];
+  const int b = blockIdx.x;
+  int c0 = b, c1 = b + 1;
+  if (t.cu_seqlens) {
+    c0 = t.cu_seqlens[b];
+    c1 = t.cu_seqlens[b + 1];
+  }
+  c0 = min(max(c0, 0), t.n_tokens);
+  c1 = min(max(c1, c0), t.n_tokens);
+  const int n = c1 - c0, most = min(n, 64 * t.words), first = max(t.seq_lens[b], 0) - n;
+  for (int i = threadIdx.x; i < most; i += 256) {
+    const int p = t.parents[c0 + i];
+    up[i] = p >= 0 && p < i ? p : -1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += 256) {
+    int at = i < most ? i : -1, depth = -1;
+    uint64_t* m = t.mask + (int64_t)(c0 + i) * t.words;
+    for (int word = t.words - 1; word >= 0; --word) {
+      uint64_t bits = 0;
+      for (; at >= 64 * word; at = up[at], ++depth) bits |= 1ull << (at & 63);
+      m[word] = bits;
+    }
+    t.positions[c0 + i] = depth < 0 ? -1 : first + depth;
+  }
+}
+
+// --------------------------------------------------------------------------
+// Keep: of a sequence's new tokens those on the accepted path, moved to the places
+// that follow the tokens before them, in every layer; codes and scales as they are.
+//
+// A wave moves a kv head's tokens, 4 aligned places at a time: one word of V codes
+// holds those of a channel (and 4 others), so it is read, merged and written once.
+// rows[j] >= j, so a place is read before or in the round that writes it, and what
+// a round writes of words that later ones read are the nibbles that were there.
+// --------------------------------------------------------------------------
+struct KeepArgs {
+  int64_t layer_stride;
+  const int32_t* rows;
+  int64_t rows_stride;
+  const int32_t* counts;
+  int width;
+};
+
+template <int D>
+__global__ __launch_bounds__(256)
+void k_kv4_keep(const shard_kv4_args a, const KeepArgs p) {
+  constexpr int W = D / 64;                           // words of V codes a lane
+  typedef uint32_t words __attribute__((ext_vector_type(W)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = blockIdx.x * 4 + wave, b = blockIdx.z;
+  if (g >= a.n_kv_heads) return;
+  const Seq s = seq_of(a, b);
+  const int start = s.len - s.n;                      // place of row 0
+  const int count = min(min(p.counts[b], p.width), s.n);
+  if (count <= 0) return;
+  const int32_t* rows = p.rows + b * p.rows_stride;
+  uint8_t* layer = a.cache + blockIdx.y * p.layer_stride + (int64_t)g * (68 * D);
+  const auto place = [&](int t) -> uint8_t* {         // of token t's page, null where it has none
+    if (t < 0 || t >= s.cap) return nullptr;
+    const int page = page_of(a, b, t);
+    return page < 0 ? nullptr : layer + (int64_t)page * a.page_stride;
+  };
+  const int c16 = lane & 15, n0 = (lane >> 4) * W;    // the lane's channels: 16 (n0 + i) + c16
+  const auto v_at = [&](int slot) { return v_word_at<D>(slot >> 5, slot >> 2 & 3, 16 * n0 + c16); };
+  const auto v_shift = [](int slot) { return 4 * ((slot >> 4 & 1) << 2 | (slot & 3)); };
+
+  for (int t0 = (start & ~3); t0 < start + count; t0 += 4) {
+    uint8_t* to = place(t0 < 0 ? -1 : t0);            // of all four
+    int src[4];
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = t0 + u - start;
+      int r = j >= 0 && j < count ? rows[j] : -1;
+      if (r <= j || r >= s.n) r = -1;                 // stays, or is none
+      src[u] = r < 0 ? -1 : start + r;
+      any |= src[u] >= 0;
+    }
+    if (!to || !any) continue;
+    const uint8_t* from[4];
+    words v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      from[u] = src[u] < 0 ? nullptr : place(src[u]);
+      v[u] = 0;
+      if (from[u]) v[u] = *(const words*)(from[u] + v_at(src[u] & 63));
+    }
+    words held = *(const words*)(to + v_at(t0 & 63));
+    // K codes and scales: 16 lanes a token, V scales among them
+    const int u = lane >> 4, l = lane & 15;
+    const int su = u == 0 ? src[0] : u == 1 ? src[1] : u == 2 ? src[2] : src[3];
+    const uint8_t* fu = u == 0 ? from[0] : u == 1 ? from[1] : u == 2 ? from[2] : from[3];
+    const int ss = su & 63, ts = (t0 & 63) + u;
+    uint32_t k = 0;
+    uint8_t sc = 0;
+    constexpr int KL = D / 8;                         // lanes of 4 bytes of K codes: 16 or 8
+    const int kq = l / (KL / 4), kw = l % (KL / 4) * 4;
+    const int blk = l % (D / 32);
+    if (fu) {
+      if (l < KL) k = *(const uint32_t*)(fu + k_code_at<D>(ss, kq) + kw);
+      if (l < D / 16) sc = fu[l < D / 32 ? k_scale_at<D>(ss, blk) : v_scale_at<D>(ss, blk)];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (from[i]) {
+        const int sh = v_shift((t0 & 63) + i);
+        held = (held & ~(15u << sh)) | ((v[i] >> v_shift(src[i] & 63) & 15u) << sh);
+      }
+    *(words*)(to + v_at(t0 & 63)) = held;
+    if (fu) {
+      if (l < KL) *(uint32_t*)(to + k_code_at<D>(ts, kq) + kw) = k;
+      if (l < D / 16) to[l < D / 32 ? k_scale_at<D>(ts, blk) : v_scale_at<D>(ts, blk)] = sc;
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
 // host side
 // --------------------------------------------------------------------------
 int check_batch(const shard_kv4_args* a) {
@@ -1370,6 +1550,17 @@ using namespace shard;
     }                                                                                                                 \
   } while (0)
 
+#define KV4_DISPATCH_NM(KERNEL, N, M, grid, s, ...)                                                              \
+  do {                                                                                                                \
+    if (a->dtype == SHARD_FP16) {                                                                                     \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<half_t, 128, N, M>), grid, dim3(256), 0, s, __VA_ARGS__);   \
+      else hipLaunchKernelGGL((KERNEL<half_t, 64, N, M>), grid, dim3(256), 0, s, __VA_ARGS__);                       \
+    } else {                                                                                                          \
+      if (a->head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16_t, 128, N, M>), grid, dim3(256), 0, s, __VA_ARGS__);   \
+      else hipLaunchKernelGGL((KERNEL<bf16_t, 64, N, M>), grid, dim3(256), 0, s, __VA_ARGS__);                       \
+    }                                                                                                                 \
+  } while (0)
+
 extern "C" {
 
 size_t shard_kv4_args_size(void) { return sizeof(shard_kv4_args); }
@@ -1380,7 +1571,7 @@ int64_t shard_kv4_page_bytes(int32_t n_kv_heads, int32_t head_dim) {
   return (int64_t)n_kv_heads * 68 * head_dim;
 }
 
-int shard_kv4_append(const shard_kv4_args* a, void* stream) {
+int shard_kv4_append_at(const shard_kv4_args* a, const int32_t* positions, void* stream) {
   const int rc = check_batch(a);
   if (rc) return rc;
   if (!a->phases || (uintptr_t)a->phases % 16 || a->n_phases <= 0) return SHARD_ERR_ARG;
@@ -1394,10 +1585,13 @@ int shard_kv4_append(const shard_kv4_args* a, void* stream) {
   }
   if (a->n_tokens == 0) return SHARD_OK;
   const dim3 grid(groups_of(a), a->n_kv_heads + q_groups, a->batch);
-  KV4_DISPATCH(k_kv4_append, grid, (hipStream_t)stream, *a);
+  if (positions) KV4_DISPATCH_N(k_kv4_append, true, grid, (hipStream_t)stream, *a, positions);
+  else KV4_DISPATCH_N(k_kv4_append, false, grid, (hipStream_t)stream, *a, positions);
   SHARD_LAUNCH_CHECK("shard_kv4_append");
   return SHARD_OK;
 }
+
+int shard_kv4_append(const shard_kv4_args* a, void* stream) { return shard_kv4_append_at(a, nullptr, stream); }
 
 int shard_kv4_read(const shard_kv4_args* a, void* stream) {
   const int rc = check_batch(a);
@@ -1417,7 +1611,8 @@ size_t shard_kv4_attn_workspace(const shard_kv4_args* a) {
   return (size_t)a->n_tokens * a->n_q_heads * p.n_splits * (a->head_dim + 2) * sizeof(float);
 }
 
-int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+static int launch_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t words, void* workspace, size_t workspace_bytes,
+                       void* stream) {
   const int rc = check_attn(a);
   if (rc) return rc;
   if (!rows_ok(a->q, a->q_stride, a->q_head_stride) || !a->out || (uintptr_t)a->out % 16) return SHARD_ERR_ARG;
@@ -1432,6 +1627,8 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   w.group = a->n_q_heads / a->n_kv_heads;
   w.group_shift = w.group & (w.group - 1) ? -1 : __builtin_ctz(w.group);
   w.row_tiles = p.row_tiles;
+  w.mask = mask;
+  w.words = words;
   if ((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads > INT32_MAX) return SHARD_ERR_SHAPE;
   if (p.n_splits > 1) {
     const size_t need = shard_kv4_attn_workspace(a);
@@ -1447,13 +1644,19 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
   }
   const hipStream_t s = (hipStream_t)stream;
   const dim3 rows_grid((unsigned)(w.n_splits * w.row_tiles), a->n_kv_heads, a->batch);
-  if (p.rows == 4) KV4_DISPATCH_N(k_kv4_attn_rows, 4, rows_grid, s, *a, w);
-  else if (p.rows == 8) KV4_DISPATCH_N(k_kv4_attn_rows, 8, rows_grid, s, *a, w);
-  else if (p.rows == 16) KV4_DISPATCH_N(k_kv4_attn_rows, 16, rows_grid, s, *a, w);
-  else if (p.rows == 32) KV4_DISPATCH_N(k_kv4_attn_rows, 32, rows_grid, s, *a, w);
-  else {
-    const dim3 grid((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch);
-    KV4_DISPATCH(k_kv4_attn_tile, grid, s, *a, w);
+  const dim3 tile_grid((unsigned)((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads), a->batch);
+  if (mask) {
+    if (p.rows == 4) KV4_DISPATCH_NM(k_kv4_attn_rows, 4, true, rows_grid, s, *a, w);
+    else if (p.rows == 8) KV4_DISPATCH_NM(k_kv4_attn_rows, 8, true, rows_grid, s, *a, w);
+    else if (p.rows == 16) KV4_DISPATCH_NM(k_kv4_attn_rows, 16, true, rows_grid, s, *a, w);
+    else if (p.rows == 32) KV4_DISPATCH_NM(k_kv4_attn_rows, 32, true, rows_grid, s, *a, w);
+    else KV4_DISPATCH_N(k_kv4_attn_tile, true, tile_grid, s, *a, w);
+  } else {
+    if (p.rows == 4) KV4_DISPATCH_NM(k_kv4_attn_rows, 4, false, rows_grid, s, *a, w);
+    else if (p.rows == 8) KV4_DISPATCH_NM(k_kv4_attn_rows, 8, false, rows_grid, s, *a, w);
+    else if (p.rows == 16) KV4_DISPATCH_NM(k_kv4_attn_rows, 16, false, rows_grid, s, *a, w);
+    else if (p.rows == 32) KV4_DISPATCH_NM(k_kv4_attn_rows, 32, false, rows_grid, s, *a, w);
+    else KV4_DISPATCH_N(k_kv4_attn_tile, false, tile_grid, s, *a, w);
   }
   SHARD_LAUNCH_CHECK("shard_kv4_attn");
   if (p.n_splits > 1) {
@@ -1462,6 +1665,49 @@ int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_by
     else KV4_DISPATCH_N(k_kv4_merge, 1, dim3((unsigned)((rows + 3) / 4)), s, *a, w);
     SHARD_LAUNCH_CHECK("shard_kv4_attn merge");
   }
+  return SHARD_OK;
+}
+
+int shard_kv4_attn(const shard_kv4_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  return launch_attn(a, nullptr, 0, workspace, workspace_bytes, stream);
+}
+
+int shard_kv4_tree_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t words, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  if (!mask || (uintptr_t)mask % 8 || words <= 0) return SHARD_ERR_ARG;
+  return launch_attn(a, mask, words, workspace, workspace_bytes, stream);
+}
+
+int shard_draft_tree(const int32_t* parents, const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t batch, int32_t n_tokens,
+                     int32_t words, uint64_t* mask, int32_t* positions, void* stream) {
+  if (!parents || !seq_lens || !mask || (uintptr_t)mask % 8 || !positions || batch <= 0 || n_tokens < 0 || words <= 0)
+    return SHARD_ERR_ARG;
+  if (!cu_seqlens && n_tokens != batch) return SHARD_ERR_ARG;
+  if (words > SHARD_TREE_ROWS / 64 || batch > 65535) return SHARD_ERR_SHAPE;
+  if (n_tokens == 0) return SHARD_OK;
+  const TreeArgs t{parents, seq_lens, cu_seqlens, batch, n_tokens, words, mask, positions};
+  hipLaunchKernelGGL(k_draft_tree, dim3(batch), dim3(256), 0, (hipStream_t)stream, t);
+  SHARD_LAUNCH_CHECK("shard_draft_tree");
+  return SHARD_OK;
+}
+
+int shard_kv4_keep(const shard_kv4_args* a, int32_t n_layers, int64_t layer_stride, const int32_t* rows, int64_t rows_stride,
+                   int32_t width, const int32_t* counts, void* stream) {
+  const int rc = check_batch(a);
+  if (rc) return rc;
+  if (n_layers <= 0 || !rows || !counts || width < 0 || rows_stride < width) return SHARD_ERR_ARG;
+  // layers side by side or page by page, never on each other
+  const int64_t page = (int64_t)a->n_kv_heads * 68 * a->head_dim;
+  if (n_layers > 1 && (layer_stride % 16 || !(layer_stride >= (a->n_pages - 1) * a->page_stride + page ||
+                                             (layer_stride >= page && (n_layers - 1) * layer_stride + page <= a->page_stride))))
+    return SHARD_ERR_ARG;
+  if (n_layers > 65535) return SHARD_ERR_SHAPE;
+  if (a->n_tokens == 0 || width == 0) return SHARD_OK;
+  const KeepArgs p{layer_stride, rows, rows_stride, counts, width};
+  const dim3 grid((a->n_kv_heads + 3) / 4, n_layers, a->batch);
+  if (a->head_dim == 128) hipLaunchKernelGGL(k_kv4_keep<128>, grid, dim3(256), 0, (hipStream_t)stream, *a, p);
+  else hipLaunchKernelGGL(k_kv4_keep<64>, grid, dim3(256), 0, (hipStream_t)stream, *a, p);
+  SHARD_LAUNCH_CHECK("shard_kv4_keep");
   return SHARD_OK;
 }
 

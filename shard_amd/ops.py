@@ -1070,7 +1070,17 @@ def _launch_on(dev, name, fn, *args):
         _lib.check(name, rc)
 
 
-def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=None, max_new=None):
+def _row_indexes(t, name, n, dev):
+    """An (n,) contiguous int32 operand's address."""
+    if t.get_device() != dev:
+        _require_gpu(t)
+        raise ValueError(f"{name} is on {t.device}, the call on cuda:{dev}")
+    if t.dtype is not torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise TypeError(f"{name}: expected ({n},) contiguous int32, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=None, max_new=None, positions=None):
     """Write new tokens into a paged 4-bit cache, k rotated at its position.
 
     k, v (T, G, D) fp16 or bf16, before RoPE; cache from kv4_cache; block_table
@@ -1083,9 +1093,13 @@ def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=No
     device: tokens at positions outside the table or in pages outside the cache
     are left out; rows behind the last sequence's are not read, and their
     rotated q not written.  Two sequences of one call must not append to the
-    same page, nor one to a page that its table names twice."""
+    same page, nor one to a page that its table names twice.
+
+    positions (T,) int32: where rows are rotated, where that is not their own
+    place (draft_tree's: drafted tokens that are siblings); a row whose position
+    is negative or not below P is left out."""
     direct = _direct or _bind_direct()
-    if direct and k.is_cuda:
+    if direct and positions is None and k.is_cuda:
         dev = _current_device()
         done = direct.kv4_append(k, v, cache, block_table, seq_lens, phases, q, cu_seqlens, max_new, dev, _raw_stream(dev))
         if done is not None:
@@ -1111,9 +1125,10 @@ def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=No
         H = q.shape[1]
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if T:
+        at = None if positions is None else _row_indexes(positions, "positions", T, dev)
         args = _lib.KV4_PACK.pack(block_table.shape[0], T, H, G, D, code, *fields, *q_at, *k_at, *v_at,
                                   phases.data_ptr(), phases.shape[0], 0.0, 0 if q is None else q_out.data_ptr(), 0, 0, 0)
-        _launch_on(dev, "shard_kv4_append", lib.shard_kv4_append, args)
+        _launch_on(dev, "shard_kv4_append", lib.shard_kv4_append_at, args, at)
     return q_out
 
 
@@ -1166,10 +1181,15 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
         done = direct.kv4_attn(q, cache, block_table, seq_lens, cu_seqlens, scale, max_new, max_len, dev, _raw_stream(dev))
         if done is not None:
             return done
+    return _kv4_attn(q, cache, block_table, seq_lens, None, cu_seqlens, scale, out, max_new, max_len)
+
+
+def _kv4_attn(q, cache, block_table, seq_lens, mask, cu_seqlens, scale, out, max_new, max_len):
     lib, T = _lib.load(), q.shape[0]
-    batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, max_len, q, out)
+    batch = _kv4_batch(cache, block_table, seq_lens, T, cu_seqlens, max_new, max_len, q, out, mask)
     if batch is None:
-        _kv4_refuse(cache, block_table, seq_lens, T, cu_seqlens, q=q, out=out)
+        more = {} if mask is None else {"mask": mask}
+        _kv4_refuse(cache, block_table, seq_lens, T, cu_seqlens, q=q, out=out, **more)
     dev, G, D, fields = batch
     code = _half_type(q, "q")
     q, *q_at = _kv4_rows(q, "q", T, None, D)
@@ -1189,8 +1209,187 @@ def kv4_attn(q, cache, block_table, seq_lens, cu_seqlens=None, scale=None, out=N
                                   scale, 0, 0, 0, out.data_ptr())
         need = lib.shard_kv4_attn_workspace(args)
         ws = cache.new_empty(need) if need else None
-        _launch_on(dev, "shard_kv4_attn", lib.shard_kv4_attn, args, ws.data_ptr() if need else None, need)
+        at = ws.data_ptr() if need else None
+        if mask is None:
+            _launch_on(dev, "shard_kv4_attn", lib.shard_kv4_attn, args, at, need)
+        else:
+            _launch_on(dev, "shard_kv4_tree_attn", lib.shard_kv4_tree_attn, args, mask.data_ptr(), mask.shape[1], at, need)
     return out
+
+
+# ---------------------------------------------------------------------------
+# drafted tokens: steps whose rows are trees
+# ---------------------------------------------------------------------------
+TREE_ROWS_MAX = 1024  # SHARD_TREE_ROWS: rows of a sequence's tree
+
+
+def _tree_width(max_new, T, name):
+    n = T if max_new is None else min(int(max_new), T)
+    if n < 0 or n > TREE_ROWS_MAX:
+        raise ValueError(f"{name}: trees of at most {TREE_ROWS_MAX} rows, got {n} (max_new, or all rows where it is None)")
+    return max(n, 1)
+
+
+def _cu(cu_seqlens, batch, rows, dev):
+    """The address of a batch's cu_seqlens, None where every sequence has one row."""
+    if cu_seqlens is None:
+        if rows != batch:
+            raise ValueError(f"{rows} rows for {batch} sequences: more than one each needs cu_seqlens")
+        return None
+    return _row_indexes(cu_seqlens, "cu_seqlens", batch + 1, dev)
+
+
+def draft_tree(parents, seq_lens, cu_seqlens=None, max_new=None):
+    """The plan of a step whose rows are trees of drafted tokens: (mask (T, W)
+    int64, positions (T,) int32), the same for every layer.
+
+    parents (T,) int32: for each row the row of its parent, counted within its
+    sequence and before it; anything else (-1): none, the row follows the
+    sequence's tokens before the step, as its first row does.  seq_lens and
+    cu_seqlens as in kv4_append, all rows among the lengths.  Bit j % 64 of word
+    j / 64 of a row's mask is set where it sees row j of its sequence: its
+    ancestors and itself.  Its position is its parent's + 1.  max_new, the most
+    rows of a sequence (all rows where None; at most TREE_ROWS_MAX), is a bound: W
+    holds as many, rows from 64 W on see no row and have position -1."""
+    lib, T = _lib.load(), parents.shape[0] if parents.dim() else 0
+    _require_gpu(parents, seq_lens, cu_seqlens)
+    dev, B = parents.get_device(), seq_lens.shape[0] if seq_lens.dim() else 0
+    _row_indexes(parents, "parents", T, dev)
+    _row_indexes(seq_lens, "seq_lens", B, dev)
+    cu = _cu(cu_seqlens, B, T, dev)
+    words = (_tree_width(max_new, T, "draft_tree") + 63) // 64
+    mask = torch.empty(T, words, dtype=torch.int64, device=parents.device)
+    positions = torch.empty_like(parents)
+    if T and B:
+        _launch_on(dev, "shard_draft_tree", lib.shard_draft_tree, parents.data_ptr(), seq_lens.data_ptr(), cu, B, T, words,
+                   mask.data_ptr(), positions.data_ptr())
+    return mask, positions
+
+
+def kv4_tree_attn(q, cache, block_table, seq_lens, mask, cu_seqlens=None, scale=None, out=None, max_new=None, max_len=None):
+    """kv4_attn for trees of drafted tokens: a row sees the tokens before its
+    sequence's rows and those rows whose bits its mask has.
+
+    mask (T, W) int64 of draft_tree, or any bits: rows that a mask has no bit for
+    are not seen, the row itself included.  Everything else as in kv4_attn; rows
+    that see nothing are zeros."""
+    if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != q.shape[0] or mask.shape[1] < 1 or not mask.is_contiguous():
+        raise TypeError(f"mask: expected ({q.shape[0]}, words) contiguous int64, got {tuple(mask.shape)} {mask.dtype}")
+    return _kv4_attn(q, cache, block_table, seq_lens, mask, cu_seqlens, scale, out, max_new, max_len)
+
+
+def kv4_keep(cache, block_table, seq_lens, rows, counts, cu_seqlens=None):
+    """After a step: of each sequence's rows those on its accepted path, moved to
+    the places that follow its tokens before the step, codes and scales as they
+    are.
+
+    cache from kv4_cache, or (layers, pages, G, bytes): all layers in one call;
+    block_table, seq_lens and cu_seqlens the step's (the lengths with all its
+    rows); rows (B, P) int32 and counts (B,) int32, verify_drafts' path and
+    counts: the token of row rows[b, j] moves to the place of row j, j <
+    counts[b].  A path's rows ascend; an entry below j, or not a row of the
+    sequence, moves nothing.  The lengths are the caller's: the sequence holds
+    seq_lens[b] less its rows, plus counts[b], tokens afterwards, and what lies
+    behind them is no longer used.  Two sequences of one call must not share a
+    page that holds rows of the step."""
+    layers = cache.unsqueeze(0) if cache.dim() == 3 else cache
+    if layers.dim() != 4 or layers.shape[0] < 1:
+        raise TypeError("cache: expected the (pages, kv heads, 68 * head_dim) uint8 of kv4_cache, or layers of them")
+    lib, one = _lib.load(), layers[0]
+    # the number of rows is not in any operand's shape: the last of cu_seqlens, on the device, bounds it
+    T = block_table.shape[0] if cu_seqlens is None else 0x7FFFFFFF
+    batch = _kv4_batch(one, block_table, seq_lens, T, cu_seqlens, 0, 0, rows, counts)
+    if batch is None:
+        _kv4_refuse(one, block_table, seq_lens, T, cu_seqlens, rows=rows, counts=counts)
+    dev, G, D, fields = batch
+    B = block_table.shape[0]
+    _row_indexes(counts, "counts", B, dev)
+    if rows.dtype is not torch.int32 or rows.dim() != 2 or rows.shape[0] != B or (rows.stride(1) != 1 and rows.shape[1] > 1):
+        raise TypeError(f"rows: expected ({B}, path) int32, got {tuple(rows.shape)} {rows.dtype}")
+    L, P = layers.shape[0], rows.shape[1]
+    stride = rows.stride(0) if B > 1 else P
+    if stride < P:
+        raise TypeError("rows: its rows overlap")
+    if B and P:
+        args = _lib.KV4_PACK.pack(B, T, 0, G, D, 0, *fields, *(0,) * 9, 0, 0, 0.0, 0, 0, 0, 0)
+        _launch_on(dev, "shard_kv4_keep", lib.shard_kv4_keep, args, L, layers.stride(0) if L > 1 else 0, rows.data_ptr(),
+                   stride, P, counts.data_ptr())
+
+
+def verify_drafts(logits, tokens, parents, uniforms, cu_seqlens=None, draft_probs=None, temperature=1.0, max_new=None,
+                  max_depth=None):
+    """Drafted tokens against the target model's logits, from given random
+    numbers: (path (B, P) int32, counts (B,) int32, next_tokens (B,) int64).
+
+    Rows as in draft_tree: logits (T, V) fp16, bf16 or fp32 of every row; tokens
+    (T,) int64, a sequence's first one the last token that was decided on (not
+    read); parents (T,) int32; uniforms (T, 2) fp32 in [0, 1): whether a row's
+    token is accepted, and what follows where the walk ends at the row.
+    cu_seqlens (B + 1,) int32, None: one row a sequence.  temperature: a number,
+    or (B,) fp32; 0: the largest logit, the first of equal ones.
+
+    A sequence's walk starts at its first row, with s = softmax(logits /
+    temperature).  A row's children are tried in their order.  Without
+    draft_probs, one of token x is accepted with probability s[x] / sum(s), and s[x]
+    becomes 0 where it is not.  draft_probs (T, V) fp32: row c is the distribution q
+    that token c was drawn from; it is accepted with probability s[x] / (q[x] sum(s)),
+    and s becomes max(s / sum(s) - q, 0) where it is not.  The walk goes on at an
+    accepted child and ends where there is none, or max_depth have been accepted:
+    the next token is drawn from s.  Accepted and next tokens are distributed as
+    the target's own, whatever was drafted.  Weights and sums are held in 64 bits.
+
+    path: the rows of the walk, its first one included, -1 behind the counts[b] of
+    them.  max_new bounds the rows of a sequence (P; all rows where None; at most
+    TREE_ROWS_MAX): those behind it are not looked at.  next_tokens is -1 where the
+    walk ends at a row of NaN, +inf (unless greedy) or no logit above -inf, or a
+    sequence has no rows.  Tokens outside the vocabulary are never accepted."""
+    lib = _lib.load()
+    temps = temperature if isinstance(temperature, torch.Tensor) else None
+    _require_gpu(logits, tokens, parents, uniforms, cu_seqlens, draft_probs, temps)
+    code = _DTYPES.get(logits.dtype)
+    if code is None or logits.dim() != 2 or logits.shape[1] == 0:
+        raise TypeError(f"logits: expected (rows, vocabulary) float16, bfloat16 or float32, got {tuple(logits.shape)} {logits.dtype}")
+    dev, (T, V) = logits.get_device(), logits.shape
+    for name, t in dict(tokens=tokens, uniforms=uniforms, draft_probs=draft_probs, temperature=temps).items():
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, the logits on {logits.device}")
+    if tokens.dtype is not torch.int64 or tuple(tokens.shape) != (T,):
+        raise TypeError(f"tokens: expected ({T},) int64, got {tuple(tokens.shape)} {tokens.dtype}")
+    if uniforms.dtype is not torch.float32 or tuple(uniforms.shape) != (T, 2):
+        raise TypeError(f"uniforms: expected ({T}, 2) float32, got {tuple(uniforms.shape)} {uniforms.dtype}")
+    up = _row_indexes(parents, "parents", T, dev)
+    B = T if cu_seqlens is None else cu_seqlens.numel() - 1
+    if B < 0 or (B == 0 and T):
+        raise ValueError("cu_seqlens: expected a sequence's rows at least")
+    cu = _cu(cu_seqlens, B, T, dev)
+    if draft_probs is not None and (draft_probs.dtype is not torch.float32 or draft_probs.shape != logits.shape):
+        raise TypeError(f"draft_probs: expected {tuple(logits.shape)} float32, got {tuple(draft_probs.shape)} {draft_probs.dtype}")
+    number = 0.0
+    if temps is None:
+        number = float(temperature)
+        if not 0.0 <= number <= 3.4e38:
+            raise ValueError(f"temperature: expected a number of at least 0, got {temperature}")
+    elif temps.dtype is not torch.float32 or tuple(temps.shape) != (B,):
+        raise TypeError(f"temperature: expected a number or ({B},) float32, got {tuple(temps.shape)} {temps.dtype}")
+    if max_depth is not None and max_depth < 0:
+        raise ValueError(f"max_depth: expected at least 0, got {max_depth}")
+    width = _tree_width(max_new, T, "verify_drafts")
+    plain = lambda t: t if t is None or (t.stride(1) == 1 and t.stride(0) >= 0) or t.numel() == 0 else t.contiguous()
+    logits, draft_probs = plain(logits), plain(draft_probs)
+    tokens, uniforms, temps = (t if t is None else t.contiguous() for t in (tokens, uniforms, temps))
+    i32 = dict(dtype=torch.int32, device=logits.device)
+    path, counts = torch.empty(B, width, **i32), torch.empty(B, **i32)
+    following = torch.empty(B, dtype=torch.int64, device=logits.device)
+    if B:
+        p = lambda t: None if t is None else t.data_ptr()
+        args = _lib.VerifyArgs(B, T, V, p(logits) or 16, logits.stride(0), code, width, p(tokens) or 16, up or 16, p(uniforms) or 16,
+                               cu, p(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), p(temps), number,
+                               min(0x7FFFFFFF if max_depth is None else int(max_depth), 0x7FFFFFFF), p(path), p(counts), p(following))
+        args = ctypes.byref(args)
+        need = lib.shard_verify_drafts_workspace(args)
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        _launch_on(dev, "shard_verify_drafts", lib.shard_verify_drafts, args, p(ws), need)
+    return path, counts, following
 
 
 # ---------------------------------------------------------------------------

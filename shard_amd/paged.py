@@ -14,10 +14,19 @@ of q and k, 4-bit rounding, writing) and ops.kv4_attn.
     logits = cache.run(model, [a, b], logits.argmax(-1, keepdim=True))
     cache.drop(a)
 
+Drafted tokens (speculative decoding) are a step whose rows are trees, each
+sequence's last token first and every drafted one after its parent:
+
+    new = cache.speculate(model, [a, b], [[last_a, x, y], [last_b, z]], parents=[[-1, 0, 0], [-1, 0]])
+
+runs the model on all of them, verifies them, keeps the accepted path and gives
+the tokens that each sequence has gained.
+
 The tokens of a step are packed in rows, one sequence after the other; there is
 no padding and no attention mask.  A step is open from begin() until every layer
 has stored its tokens (run() does both); one that will not come to that is undone
-by cancel(), as no other can begin over tokens that are not there.
+by cancel(), as no other can begin over tokens that are not there.  A step of
+trees is followed by accept() or cancel(), before any other.
 """
 import torch
 from transformers.cache_utils import Cache as HFCache, CacheLayerMixin
@@ -102,11 +111,12 @@ class PagedCache(HFCache):
         return seq
 
     def drop(self, seq):
-        """Give a sequence's pages back.  A step that is open for it is undone, for
-        all its sequences; one of other sequences stays open."""
+        """Give a sequence's pages back.  A step that is open for it, or of trees and
+        not accepted yet, is undone, for all its sequences; one of other sequences
+        stays as it is."""
         if seq not in self._pages:
             raise KeyError(seq)
-        step = self._open()
+        step = self._open() or self._drafted()
         if step is not None and any(s == seq for s, _, _ in step["undo"]):
             self._undo()
         self._free += reversed(self._pages.pop(seq))
@@ -126,16 +136,32 @@ class PagedCache(HFCache):
         """The step that some layer has not stored yet, or None."""
         return self._step if self._step is not None and self._step["left"] else None
 
-    def begin(self, seqs, new):
+    def _drafted(self):
+        """The step of trees that neither accept() nor cancel() has settled, or None."""
+        return self._step if self._step is not None and self._step["tree"] is not None else None
+
+    def begin(self, seqs, new, parents=None):
         """Open a step in which sequence seqs[i] gets new[i] tokens (0 allowed),
         packed in this order.  Pages are taken here: RuntimeError where too few are
         free; ValueError while another step is open; a call that fails, for
-        whatever reason, changes nothing.  Returns the tokens' positions, (1, T)."""
+        whatever reason, changes nothing.  Returns the tokens' positions, (1, T).
+
+        parents: the tokens are trees, parents[i][j] is the row of its parent of row
+        j of sequence seqs[i], -1 for row 0 alone.  Every row takes a place in the
+        cache until accept() or cancel()."""
         if self._open():
             raise ValueError("a step is open: run its layers or cancel() it")
+        if self._drafted():
+            raise ValueError("drafted tokens are in the cache: accept() or cancel() them")
         seqs, new = list(seqs), [int(n) for n in new]
         if len(seqs) != len(new) or not seqs or len(set(seqs)) != len(seqs) or min(new) < 0 or max(new) == 0:
             raise ValueError("a step needs distinct sequences and at least one new token")
+        trees = None if parents is None else [[int(p) for p in t] for t in parents]
+        if trees is not None:
+            if [len(t) for t in trees] != new or max(new) > ops.TREE_ROWS_MAX:
+                raise ValueError(f"parents: expected one for each row, at most {ops.TREE_ROWS_MAX} of a sequence")
+            if any(not (0 <= p < i if i else p == -1) for t in trees for i, p in enumerate(t)):
+                raise ValueError("parents: -1 for a sequence's first row, an earlier row for every other")
         total = [self._lens[s] + n for s, n in zip(seqs, new)]
         if max(total) > self.max_len:
             raise ValueError(f"a sequence would hold {max(total)} tokens, max_len is {self.max_len}")
@@ -152,24 +178,57 @@ class PagedCache(HFCache):
         cu = [0]
         for n in new:
             cu.append(cu[-1] + n)
-        meta = torch.tensor([x for r in rows for x in r] + total + cu, dtype=torch.int32).to(dev)  # one copy
+        up = [] if trees is None else [p for t in trees for p in t]
+        meta = torch.tensor([x for r in rows for x in r] + total + cu + up, dtype=torch.int32).to(dev)  # one copy
         B = len(seqs)
-        table, lens, cu_dev = meta[:B * width].view(B, width), meta[B * width:B * width + B], meta[B * width + B:]
-        pos = torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)])[None].to(dev)
+        table, lens, cu_dev, up = meta.split([B * width, B, B + 1, len(up)])
+        table, tree, depth = table.view(B, width), None, 0
+        if trees is None:
+            pos = torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)])[None].to(dev)
+        else:
+            mask, places = ops.draft_tree(up, lens, cu_seqlens=cu_dev, max_new=max(new))
+            levels = []
+            for t in trees:
+                at = []
+                for p in t:
+                    at.append(at[p] + 1 if at else 0)
+                levels += at
+            tree, depth, pos = (mask, places, up), max(levels), places[None].long()
         # nothing has changed so far; nothing below fails
         del self._free[len(self._free) - sum(want):]
         for s, p, t in zip(seqs, pages, total):
             self._pages[s], self._lens[s] = p, t
         self._step = dict(table=table, lens=lens, cu=None if max(new) == min(new) == 1 else cu_dev, rows=cu[-1],
                           max_new=max(new), max_len=max(total), undo=list(zip(seqs, new, want)),
-                          left=set(range(len(self.layers))))
+                          left=set(range(len(self.layers))), tree=tree, depth=depth)
         return pos
 
     def cancel(self):
-        """Undo the open step: its tokens were not stored in every layer."""
-        if not self._open():
+        """Undo the open step, whose tokens were not stored in every layer, or the
+        step of trees that has not been accepted."""
+        if not self._open() and not self._drafted():
             raise ValueError("no step is open")
         self._undo()
+
+    def accept(self, path, counts):
+        """Settle a step of trees: of each of its sequences, in the step's order, the
+        rows path[i, :counts[i]] stay (path (B, P) and counts (B,) int32 on the
+        device, of ops.verify_drafts), moved to where the sequence goes on; its other
+        rows leave the cache.  Returns the counts as a list."""
+        step = self._drafted()
+        if step is None or self._open():
+            raise ValueError("no drafted tokens to accept: a step of trees that every layer has stored comes first")
+        n = counts.tolist()
+        if len(n) != len(step["undo"]) or any(not 0 <= c <= min(new, path.shape[1]) for c, (_, new, _) in zip(n, step["undo"])):
+            raise ValueError("counts: expected one for each sequence of the step, at most its rows and the path's length")
+        ops.kv4_keep(self.pool, step["table"], step["lens"], path, counts, cu_seqlens=step["cu"])
+        step["tree"] = None
+        for c, (seq, new, _) in zip(n, step["undo"]):
+            self._lens[seq] -= new - c
+            keep = (self._lens[seq] + KV4_PAGE - 1) // KV4_PAGE
+            while len(self._pages[seq]) > keep:
+                self._free.append(self._pages[seq].pop())
+        return n
 
     def _undo(self):
         step, self._step = self._step, None
@@ -186,17 +245,25 @@ class PagedCache(HFCache):
         if st is None or k.shape[0] != st["rows"]:
             raise ValueError(f"{k.shape[0]} rows for a step of {None if st is None else st['rows']}: open it with begin()")
         pages = self.pool[layer_idx]
-        q = ops.kv4_append(k, v, pages, st["table"], st["lens"], self.phases, q=q, cu_seqlens=st["cu"], max_new=st["max_new"])
-        out = ops.kv4_attn(q, pages, st["table"], st["lens"], cu_seqlens=st["cu"], scale=scale, max_new=st["max_new"],
-                           max_len=st["max_len"])
+        if st["tree"] is None:
+            q = ops.kv4_append(k, v, pages, st["table"], st["lens"], self.phases, q=q, cu_seqlens=st["cu"], max_new=st["max_new"])
+            out = ops.kv4_attn(q, pages, st["table"], st["lens"], cu_seqlens=st["cu"], scale=scale, max_new=st["max_new"],
+                               max_len=st["max_len"])
+        else:
+            mask, positions, _ = st["tree"]
+            q = ops.kv4_append(k, v, pages, st["table"], st["lens"], self.phases, q=q, cu_seqlens=st["cu"], max_new=st["max_new"],
+                               positions=positions)
+            out = ops.kv4_tree_attn(q, pages, st["table"], st["lens"], mask, cu_seqlens=st["cu"], scale=scale, max_new=st["max_new"],
+                                    max_len=st["max_len"])
         st["left"].discard(layer_idx % len(self.layers))
         return out
 
     @torch.no_grad()
-    def run(self, model, seqs, tokens, last_only=True):
+    def run(self, model, seqs, tokens, last_only=True, parents=None):
         """A step of a patched Llama model: tokens[i], a 1-D sequence of token ids,
         go to sequence seqs[i].  Returns the logits of each sequence's last token
-        (len(seqs), vocab), or of every token (T, vocab), rows packed."""
+        (len(seqs), vocab), or of every token (T, vocab), rows packed.  parents: the
+        tokens are trees (begin()), to be settled by accept() or cancel()."""
         dev = self.pool.device
         tokens = [torch.as_tensor(t).reshape(-1) for t in tokens]
         if min(len(t) for t in tokens) == 0:
@@ -205,7 +272,7 @@ class PagedCache(HFCache):
         keep = 0
         if last_only:
             keep = torch.tensor([len(t) for t in tokens]).cumsum(0).to(dev) - 1
-        pos = self.begin(seqs, [len(t) for t in tokens])
+        pos = self.begin(seqs, [len(t) for t in tokens], parents)
         step = self._step
         step["unmasked"] = True
         try:
@@ -216,6 +283,33 @@ class PagedCache(HFCache):
             raise
         step["left"].clear()
         return logits
+
+    @torch.no_grad()
+    def speculate(self, model, seqs, tokens, parents, draft_probs=None, temperature=0.0, uniforms=None):
+        """A step of trees from the model's run to the accepted tokens: tokens[i] are
+        the last token of sequence seqs[i] and its drafted ones, parents[i] their
+        parents (begin()).  draft_probs, temperature and uniforms as in
+        ops.verify_drafts, rows packed; torch.rand where uniforms is None.  Returns
+        for each sequence the tokens that it has gained: the accepted ones and the
+        one that follows, which the cache does not hold yet (-1 where the model's
+        logits gave none)."""
+        logits = self.run(model, seqs, tokens, last_only=False, parents=parents)
+        step = self._step
+        try:
+            ids = torch.cat([torch.as_tensor(t).reshape(-1).to(logits.device) for t in tokens]).long()
+            if uniforms is None:
+                uniforms = torch.rand(len(ids), 2, device=logits.device)
+            path, counts, following = ops.verify_drafts(
+                logits, ids, step["tree"][2], uniforms, cu_seqlens=step["cu"], draft_probs=draft_probs, temperature=temperature,
+                max_new=step["max_new"], max_depth=step["depth"])
+            first = torch.tensor([0] + [new for _, new, _ in step["undo"]][:-1]).cumsum(0).to(ids.device)[:, None]
+            gained = torch.cat([ids[first + path.clamp(min=0)], following[:, None]], 1).tolist()
+            n = self.accept(path, counts)
+        except BaseException:
+            if self._step is step and self._drafted():
+                self._undo()
+            raise
+        return [row[1:c] + row[-1:] for row, c in zip(gained, n)]
 
 
 def _hides(mask) -> bool:
