@@ -621,7 +621,9 @@ int shard_kv4_append_at(const shard_kv4_args* args, const int32_t* positions, vo
 
 /* shard_kv4_attn where a row sees the tokens before its sequence's rows and those
  * rows whose bits mask (n_tokens, words; as shard_draft_tree's, any bits will do)
- * has for it.  Workspace as shard_kv4_attn's. */
+ * has for it.  Workspace: shard_kv4_tree_attn_workspace(args) bytes, 16-byte
+ * aligned (0: none needed); nothing in it needs clearing. */
+size_t shard_kv4_tree_attn_workspace(const shard_kv4_args* args);
 int shard_kv4_tree_attn(const shard_kv4_args* args, const uint64_t* mask, int32_t words, void* workspace,
                         size_t workspace_bytes, void* stream);
 
@@ -649,7 +651,7 @@ int shard_kv4_keep(const shard_kv4_args* args, int32_t n_layers, int64_t layer_s
  * which the running sum of s exceeds uniforms[row][1] sum(s), row the last one.
  * Weights and sums in 64 bits.  A temperature (temperatures[b], or temperature where
  * that is null) of 0 or below: p is 1 at the largest logit, the first of equal ones,
- * and no random number counts.  Numbers are in [0, 1).
+ * and no random number counts.  Numbers are in [0, 1) (others: any token, or -1).
  *
  * A sequence's rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (null: row b alone),
  * parents as in shard_draft_tree; width, up to SHARD_TREE_ROWS, bounds the rows

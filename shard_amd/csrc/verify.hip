@@ -16,13 +16,15 @@
 // weight is formed in 64 bits (2^-48 of it): 32 bits move each of 128,256 borders
 // by some 2^-25, which would change about one answer in a hundred.
 //
-// Rows are cut into parts of at most 64, a granule pair a thread or more.
-//   k_verify_stats   a part of a row a workgroup: its largest logit M and
+// Rows are cut into at most 64 parts.
+//   k_verify_stats   a part of a row a wave: its largest logit M and
 //                    sum exp2((x - M) log2(e) / t)
 //   k_verify_walk    a sequence a workgroup: the walk, then the part that the
 //                    answer lies in from the parts' sums, and in it the token
-// With draft_probs s is another function of every token after a rejection, so a
-// launch between the two sums its parts (k_verify_rest).
+// With draft_probs s is another function of every token after a rejection, so two
+// more launches sum its parts (k_verify_rest) and answer (k_verify_answer).  Many
+// rows, few of which are on a path, go a launch a level instead (k_verify_level,
+// k_verify_end), and only the rows on the paths are read.
 #include <math.h>
 #include <stdio.h>
 
@@ -37,9 +39,9 @@ constexpr int kThreads = 256;
 constexpr double kLog2e = 1.4426950408889634074;
 
 struct Part {
-  double sum;    // of exp2((x - most) rate); NaN where the row has no distribution
-  float most;
-  int32_t at;    // of the largest logit, the first of equal ones
+  double sum;    // of exp2((x - most) rate)
+  float most;    // the largest logit, NaN where one is
+  int32_t at;    // greedy: of the largest logit, the first of equal ones
 };
 struct State {   // of a sequence whose walk has ended
   double total;  // sum of the last row's weights
@@ -47,10 +49,16 @@ struct State {   // of a sequence whose walk has ended
   int32_t at, row, rejected;   // row -1: nothing to answer
 };
 
+struct Level {   // of a sequence's walk, a launch a level
+  int32_t row, count, done;    // done: the level at which it was seen to end, or 0
+};
+
 struct VerifyWork {
+  int levels;        // launches of a level each, 0: all rows at once
   int parts;
   int64_t granules;  // of a part
   Part* stats;       // [row][part]
+  Level* level;      // [2][sequence]; stats: [2][sequence][part]
   // with draft_probs
   State* state;      // [sequence]
   double* rest;      // [sequence][part]
@@ -58,41 +66,80 @@ struct VerifyWork {
   double* left;      // [row]: what their subtraction left, 0: nothing, so it was not made
 };
 
-// 2^y, y <= 0 or NaN, to 2^-50: Taylor's series of 2^r, |r| <= 1/2 (the first
-// term left out is 7e-18 of the sum).
+// 2^y to 2^-51, 0 below 2^-1074; y <= 1, a number or -inf.  y is split at the
+// nearest whole number, whose bits the addition of 1.5 2^52 leaves in the low word;
+// the polynomial is 2^r's interpolation at Chebyshev's points of [-1/2, 1/2],
+// 3.2e-16 off at most.
 __device__ __forceinline__ double exp2_of(double y) {
-  constexpr double ln2 = 0.69314718055994530942;
-  constexpr double c1 = ln2, c2 = c1 * ln2 / 2, c3 = c2 * ln2 / 3, c4 = c3 * ln2 / 4, c5 = c4 * ln2 / 5, c6 = c5 * ln2 / 6,
-                   c7 = c6 * ln2 / 7, c8 = c7 * ln2 / 8, c9 = c8 * ln2 / 9, c10 = c9 * ln2 / 10, c11 = c10 * ln2 / 11,
-                   c12 = c11 * ln2 / 12, c13 = c12 * ln2 / 13;
-  y = y < -1100.0 ? -1100.0 : y;
-  const double k = rint(y), r = y - k;
-  double p = c13;
-  p = fma(p, r, c12);
-  p = fma(p, r, c11);
-  p = fma(p, r, c10);
-  p = fma(p, r, c9);
-  p = fma(p, r, c8);
-  p = fma(p, r, c7);
-  p = fma(p, r, c6);
-  p = fma(p, r, c5);
-  p = fma(p, r, c4);
-  p = fma(p, r, c3);
-  p = fma(p, r, c2);
-  p = fma(p, r, c1);
+  constexpr double whole = 6755399441055744.0;
+  y = fmax(y, -1100.0);
+  const double t = y + whole;
+  const double r = y - (t - whole);
+  double p = 7.072585949269223e-09;
+  p = fma(p, r, 1.0208690299958306e-07);
+  p = fma(p, r, 1.321544258792169e-06);
+  p = fma(p, r, 1.5252657260200837e-05);
+  p = fma(p, r, 0.0001540353044173605);
+  p = fma(p, r, 0.0013333558230164974);
+  p = fma(p, r, 0.009618129107606888);
+  p = fma(p, r, 0.05550410866444772);
+  p = fma(p, r, 0.24022650695910097);
+  p = fma(p, r, 0.69314718055995);
   p = fma(p, r, 1.0);
-  return ldexp(p, (int)k);
+  return ldexp(p, __double2loint(t));
 }
-__device__ __forceinline__ float base_of(float most) { return most == -INFINITY ? 0.f : most; }
-__device__ __forceinline__ double weight(float x, float most, double rate) {
-  return exp2_of(((double)x - (double)base_of(most)) * rate);
-}
+// A row's (or part's) weights 2^((x - most) rate), x not NaN.  The difference comes
+// first: it is exact, or rounded relative to itself, however far from 0 the row lies.
+struct Scale {
+  double rate, from;
+  __device__ __forceinline__ Scale(float most, double rate) : rate(rate), from(most == -INFINITY ? 0.0 : (double)most) {}
+  __device__ __forceinline__ double operator()(float x) const { return exp2_of(((double)x - from) * rate); }
+};
 
+// Lanes' values without the LDS crossbar.
+template <int CTRL>
+__device__ __forceinline__ double dpp_mov(double v) {
+  const int lo = __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xF, 0xF, false);
+  const int hi = __builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xF, 0xF, false);
+  return __hiloint2double(hi, lo);
+}
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  v += dpp_mov<kDppXor1>(v);
+  v += dpp_mov<kDppXor2>(v);
+  v += dpp_mov<kDppHalfMirror>(v);
+  v += dpp_mov<kDppMirror>(v);
+  {
+    const auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+    v = __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+  }
+  const auto lo = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+  return __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+}
+// A lane's sum of the lanes up to it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {   // 0 where nothing comes in
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false);
+  return __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double wave_scan(double v) {
+  v += moved<0x111, 0xF>(v);   // within rows of 16: from 1, 2, 4, 8 lanes below
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);   // the last lane of rows 0 and 2 to rows 1 and 3
+  v += moved<0x143, 0xC>(v);   // lane 31 to the upper half
   return v;
 }
+__device__ __forceinline__ double lane_value(double v, int lane) {   // lane is the same in all
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // NaN stays
+struct OpMaxOf { __device__ float operator()(float a, float b) const { return max_of(a, b); } };
+// A row's largest logit says whether it has a distribution: a greedy one may be +inf.
+__device__ __forceinline__ bool has_answer(float most, double rate) { return most > -INFINITY && (most < INFINITY || rate == 0.0); }
 
 // log2(e) / temperature of a sequence; 0: greedy.
 __device__ __forceinline__ double rate_of(const shard_verify_args& a, int b) {
@@ -109,72 +156,74 @@ __device__ __forceinline__ int sequence_of(const shard_verify_args& a, int r, in
   return max(before - 1, 0);
 }
 
+// A part a wave: no barrier, nothing in LDS.  kTurn granules a turn, all on their way
+// before the first is looked at.
+constexpr int kTurn = 256;
+
 template <class T>
-__global__ __launch_bounds__(kThreads)
-void k_verify_stats(const shard_verify_args a, const VerifyWork w) {
-  constexpr int VEC = Row<T>::VEC;
-  __shared__ float sh_most[4];
-  __shared__ int sh_at[4];
-  __shared__ double sh_sum[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = blockIdx.x, part = blockIdx.y;
-  const double rate = rate_of(a, a.temperatures ? sequence_of(a, row, lane) : 0);
+__device__ __forceinline__ void part_of(const shard_verify_args& a, const VerifyWork& w, int row, int part, int sequence, Part* out) {
+  constexpr int VEC = Row<T>::VEC, PER = kTurn / 64;
+  const int lane = threadIdx.x & 63;
   const Row<T> r((const T*)a.logits + row * a.row_stride, a.vocab);
   const int64_t g0 = part * w.granules, g1 = min(g0 + w.granules, r.count);
   float most = -INFINITY;
   int at = INT32_MAX;
-  double sum = 0.0;
-  for (int64_t g = g0 + 2 * tid; g < g1; g += 2 * kThreads) {
-    float x[2][VEC];
-    int64_t e[2];
-    e[0] = r.load(g, x[0]);
-    e[1] = g + 1 < g1 ? r.load(g + 1, x[1]) : 0;
-    if (g + 1 >= g1)
+  double sum = 0.0, rate = -1.0;
+  for (int64_t g = g0; g < g1; g += kTurn) {
+    typename Row<T>::vec raw[PER];
+    if (g >= r.lo() && g + kTurn <= min(g1, r.hi())) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[1][k] = -INFINITY;
-    float m = most;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        if (x[u][k] > m) at = (int)(e[u] + k);
-        m = fmaxf(m, x[u][k]);
-      }
-    if (rate > 0.0) {
-      if (m > most) sum *= weight(most, m, rate);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) sum += weight(x[u][k], m, rate);
+      for (int u = 0; u < PER; ++u) raw[u] = r.raw(g + 64 * u + lane);
     } else {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < PER; ++u) {
+        float x[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sum = x[u][k] == x[u][k] ? sum : (double)NAN;
+        for (int k = 0; k < VEC; ++k) x[k] = -INFINITY;
+        if (g + 64 * u + lane < g1) r.load(g + 64 * u + lane, x);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) raw[u][k] = (T)x[k];   // as it was
+      }
+    }
+    if (rate < 0.0) rate = rate_of(a, !a.temperatures ? 0 : sequence < 0 ? sequence_of(a, row, lane) : sequence);
+    float m = most;
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) m = max_of(m, (float)raw[u][k]);
+    m = wave64_reduce(m, OpMaxOf());
+    // the logits are kept in their own type, half the registers, and widened again
+#pragma unroll
+    for (int u = 0; u < PER; ++u) asm volatile("" : "+v"(raw[u]));
+    if (rate > 0.0) {
+      const Scale scale(m, rate);
+      if (g > g0) sum *= scale(most);
+#pragma unroll
+      for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum += scale((float)raw[u][k]);
+    } else if (m > most) {
+      at = INT32_MAX;
+#pragma unroll
+      for (int u = PER - 1; u >= 0; --u)
+#pragma unroll
+        for (int k = VEC - 1; k >= 0; --k)
+          if ((float)raw[u][k] == m) at = (int)((g + 64 * u + lane) * VEC - r.mis + k);
     }
     most = m;
   }
-  const float M = wave64_reduce(most, OpMax());
-  if (lane == 0) sh_most[wave] = M;
-  __syncthreads();
-  const float all = fmaxf(fmaxf(sh_most[0], sh_most[1]), fmaxf(sh_most[2], sh_most[3]));
-  if (rate > 0.0 && sum != 0.0) sum *= weight(most, all, rate);
   sum = wave_sum(sum);
-  int first = most == all ? at : INT32_MAX;
+  if (rate == 0.0)
 #pragma unroll
-  for (int o = 32; o; o >>= 1) first = min(first, __shfl_xor(first, o));
-  if (lane == 0) {
-    sh_sum[wave] = sum;
-    sh_at[wave] = first;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    Part p;
-    p.sum = (sh_sum[0] + sh_sum[1]) + (sh_sum[2] + sh_sum[3]);
-    p.most = all;
-    p.at = min(min(sh_at[0], sh_at[1]), min(sh_at[2], sh_at[3]));
-    w.stats[(int64_t)row * w.parts + part] = p;
-  }
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+  if (lane == 0) *out = Part{sum, most, at};
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void k_verify_stats(const shard_verify_args a, const VerifyWork w) {
+  const int part = blockIdx.y * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (part < w.parts) part_of<T>(a, w, blockIdx.x, part, -1, w.stats + (int64_t)blockIdx.x * w.parts + part);
 }
 
 // A row's parts joined, in every lane of a wave; `mine` is the lane's part at the
@@ -184,111 +233,148 @@ struct Joined {
   float most;
   int at;
 };
-__device__ __forceinline__ Joined join(const VerifyWork& w, int64_t row, double rate, int lane) {
+__device__ __forceinline__ Joined join(const Part* row, int parts, double rate, int lane) {
   Part p{0.0, -INFINITY, INT32_MAX};
-  if (lane < w.parts) p = w.stats[row * w.parts + lane];
+  if (lane < parts) p = row[lane];
   Joined j;
-  j.most = wave64_reduce(p.most, OpMax());
-  int at = p.most == j.most ? p.at : INT32_MAX;
+  j.most = wave64_reduce(p.most, OpMaxOf());
+  int at = INT32_MAX;
+  if (rate == 0.0) {
+    at = p.most == j.most ? p.at : INT32_MAX;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+  }
   j.at = at;
-  j.mine = rate > 0.0 && p.sum != 0.0 ? p.sum * weight(p.most, j.most, rate) : p.sum;
+  j.mine = p.sum != 0.0 ? p.sum * Scale(j.most, rate)(p.most) : 0.0;
   j.sum = wave_sum(j.mine);
   return j;
 }
 
 // What a sequence's walk needs of its rows.
+constexpr int kWalk = 1024;                              // threads of a walk, a row each
+constexpr int kHeld = 2048;                              // parts of rows in LDS, where a sequence has no more
+static_assert(SHARD_TREE_ROWS <= kWalk, "a thread a row");
 struct Nodes {
   int32_t up[SHARD_TREE_ROWS], token[SHARD_TREE_ROWS];   // token -1: none of the vocabulary
-  float u[SHARD_TREE_ROWS], logit[SHARD_TREE_ROWS];      // of the token in its parent's row
-  int32_t rejected[SHARD_TREE_ROWS];                     // rows, in their order
-  double amount[SHARD_TREE_ROWS];                        // weights of their tokens; draft_probs: what they left
+  float u[SHARD_TREE_ROWS], after[SHARD_TREE_ROWS];      // random numbers
+  float logit[SHARD_TREE_ROWS];                          // of the token in its parent's row
+  float q[SHARD_TREE_ROWS];                              // of the token in what it was drawn from
 };
-
-// s of a token before any normalisation by sums that are not known yet: the weight
-// w / total, less the first n rejected rows' probabilities, each difference again
-// relative to what it left.
-template <class F>
-__device__ __forceinline__ double residual(double s, const double* left, int n, F q) {
-  for (int k = 0; k < n; ++k) {
-    const double d = s - q(k);
-    if (k == n - 1) return d > 0.0 ? d : 0.0;
-    if (left[k] > 0.0) s = (d > 0.0 ? d : 0.0) / left[k];
-  }
-  return s;
-}
 
 struct Shared {
-  Nodes n;
-  double scan[4];
+  int32_t rejected[SHARD_TREE_ROWS];                     // rows (Q) or tokens, in their order
+  double amount[SHARD_TREE_ROWS];                        // Q: what they left; weights of the tokens
+  double scan[kWalk / 64];
   State end;
-  int count, pick_part, found, last;
-  double before, target;
+  int count, pick_part, found, last, wants;
+  float u;
+  double target;
 };
 
-// The weights of a pair of granules of a row, 0 outside it.
+// s of a row's tokens four at a time, 0 outside it: quad i holds elements 4 i - mis ..
+// 4 i - mis + 3.  Q: the weights' shares, less the first n rejected rows'
+// probabilities, each difference again relative to what it left, the last one as it is.
 template <class T, bool Q>
 struct Weights {
-  static constexpr int VEC = Row<T>::VEC;
   const shard_verify_args& a;
-  const Row<T>& r;
+  const Row<T> r;
   const Shared& sh;
   const int64_t row0;
-  const double rate;
+  const Scale scale;
+  const double each;
   int n;          // rejected rows that count
-  __device__ __forceinline__ double pair(int64_t g, int64_t g1, double (&v)[2][VEC], int64_t (&e)[2]) const {
-    double sum = 0.0;
+  __device__ __forceinline__ Weights(const shard_verify_args& a, const Shared& sh, int64_t row0, int64_t row, double rate, int n)
+      : a(a), r((const T*)a.logits + row * a.row_stride, a.vocab), sh(sh), row0(row0), scale(sh.end.most, rate),
+        each(1.0 / sh.end.total), n(n) {}
+  struct Raw {
+    float x[4], q[4];   // q: of the first rejected row
+    int64_t e;          // the first element's index; all four lie in the row
+    bool whole;
+  };
+  __device__ __forceinline__ void probs(int j, const Raw& raw, float (&q)[4]) const {
+    const float* p = a.draft_probs + (row0 + sh.rejected[j]) * a.probs_stride + raw.e;
+    if (raw.whole) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float x[VEC];
+      for (int k = 0; k < 4; ++k) q[k] = p[k];
+    } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = -INFINITY;
-      e[u] = g + u < g1 ? r.load(g + u, x) : -VEC;
+      for (int k = 0; k < 4; ++k) q[k] = raw.e + k >= 0 && raw.e + k < r.n ? p[k] : 0.f;
+    }
+  }
+  __device__ __forceinline__ Raw fetch(int64_t i, int64_t end) const {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    Raw raw;
+    raw.e = i < end ? 4 * i - r.mis : -4;
+    raw.whole = raw.e >= 0 && raw.e + 4 <= r.n;
+    if (raw.whole) {
+      const vec4 v = *(const vec4*)(r.p + raw.e);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        double s = weight(x[k], sh.end.most, rate);
-        const int64_t i = e[u] + k;
-        if constexpr (Q) {
-          if (i >= 0 && i < a.vocab)
-            s = residual(s / sh.end.total, sh.n.amount, n,
-                         [&](int j) { return (double)a.draft_probs[(row0 + sh.n.rejected[j]) * a.probs_stride + i]; });
-        } else {
-          for (int j = 0; j < n; ++j)
-            if (sh.n.token[sh.n.rejected[j]] == i) s = 0.0;
-        }
-        v[u][k] = s;
-        sum += s;
+      for (int k = 0; k < 4; ++k) raw.x[k] = (float)v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) raw.x[k] = raw.e + k >= 0 && raw.e + k < r.n ? (float)r.p[raw.e + k] : -INFINITY;
+    }
+    if (Q && n > 0) probs(0, raw, raw.q);
+    return raw;
+  }
+  __device__ __forceinline__ double value(Raw& raw, double (&v)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = scale(raw.x[k]);
+    if constexpr (Q) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] *= each;
+      for (int j = 0; j < n; ++j) {
+        const double left = j == n - 1 ? 1.0 : sh.amount[j];
+        if (j) probs(j, raw, raw.q);
+        if (left > 0.0)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const double d = v[k] - (double)raw.q[k];
+            v[k] = d > 0.0 ? d : 0.0;
+            if (j < n - 1) v[k] /= left;
+          }
+      }
+    } else {
+      for (int j = 0; j < n; ++j) {
+        const int64_t gone = sh.rejected[j] - raw.e;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = gone == k ? 0.0 : v[k];
       }
     }
-    return sum;
+    return (v[0] + v[1]) + (v[2] + v[3]);
   }
 };
 
-// Sums over a workgroup: every thread's exclusive prefix, and the whole.
+// Sums over a workgroup of kWalk threads: every thread's exclusive prefix, and the whole.
 __device__ __forceinline__ double scan(double v, Shared& sh, double& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const double x = wave_scan(v);
   __syncthreads();
   if (lane == 63) sh.scan[wave] = x;
   __syncthreads();
-  double before = 0.0;
-  for (int k = 0; k < wave; ++k) before += sh.scan[k];
-  all = (sh.scan[0] + sh.scan[1]) + (sh.scan[2] + sh.scan[3]);
-  return before + (x - v);
+  const double waves = wave_scan(lane < kWalk / 64 ? sh.scan[lane] : 0.0);
+  all = lane_value(waves, kWalk / 64 - 1);
+  return (wave ? lane_value(waves, max(wave - 1, 0)) : 0.0) + (x - v);
 }
 
-// The walk.  Wave 0 decides; for Q, where sums over a row take the whole workgroup,
-// every wave decides, from the same numbers in the same way.  Leaves sh.end, the
-// rejected rows of the last row, and for Q what each but the last left.
+// The sum of a row's weights.
 template <class T, bool Q>
-__device__ void walk(const shard_verify_args& a, const VerifyWork& w, Shared& sh, int b, bool write) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ double sum_of(const Weights<T, Q>& weights, int64_t i0, int64_t i1, Shared& sh) {
+  double own = 0.0, all;
+#pragma unroll 1
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += kWalk) {
+    double v[4];
+    auto raw = weights.fetch(i, i1);
+    own += weights.value(raw, v);
+  }
+  scan(own, sh, all);
+  return all;
+}
+
+struct Rows {
+  int first, n;   // of a sequence that are looked at
+};
+__device__ __forceinline__ Rows rows_of(const shard_verify_args& a, int b) {
   int c0 = b, c1 = b + 1;
   if (a.cu_seqlens) {
     c0 = a.cu_seqlens[b];
@@ -296,101 +382,81 @@ __device__ void walk(const shard_verify_args& a, const VerifyWork& w, Shared& sh
   }
   c0 = min(max(c0, 0), a.n_tokens);
   c1 = min(max(c1, c0), a.n_tokens);
-  const int n = min(c1 - c0, min(a.width, SHARD_TREE_ROWS));
-  const double rate = rate_of(a, b);
-  const T* logits = (const T*)a.logits + c0 * a.row_stride;
-  for (int i = tid; i < n; i += kThreads) {
-    const int p = a.parents[c0 + i];
-    const int64_t t = a.tokens[c0 + i];
-    const bool ok = p >= 0 && p < i && t >= 0 && t < a.vocab;
-    sh.n.up[i] = p >= 0 && p < i ? p : -1;
-    sh.n.token[i] = ok ? (int32_t)t : -1;
-    sh.n.u[i] = a.uniforms[2 * (int64_t)(c0 + i)];
-    sh.n.logit[i] = ok ? (float)logits[p * a.row_stride + t] : -INFINITY;
+  return {c0, min(c1 - c0, min(a.width, SHARD_TREE_ROWS))};
+}
+
+template <class T>
+__device__ __forceinline__ void load_nodes(const shard_verify_args& a, Nodes& nodes, const Rows& rows, int tid, int threads) {
+  const T* logits = (const T*)a.logits + rows.first * a.row_stride;
+  for (int i = tid; i < rows.n; i += threads) {
+    const int64_t row = rows.first + i;
+    const int p = a.parents[row];
+    const int64_t t = a.tokens[row];
+    const float2 u = ((const float2*)a.uniforms)[row];
+    const bool child = p >= 0 && p < i, ok = child && t >= 0 && t < a.vocab;
+    nodes.up[i] = child ? p : -1;
+    nodes.token[i] = ok ? (int32_t)t : -1;
+    nodes.u[i] = u.x;
+    nodes.after[i] = u.y;
+    nodes.logit[i] = ok ? (float)logits[p * a.row_stride + t] : -INFINITY;
+    if (a.draft_probs) nodes.q[i] = ok ? a.draft_probs[row * a.probs_stride + t] : 0.f;
   }
-  __syncthreads();
-  int cur = 0, count = n > 0 ? 1 : 0, rejected = 0;
-  int32_t* path = a.path + (int64_t)b * a.width;
-  double total = 0.0;
-  float most = 0.f;
-  int at = -1;
-  bool none = n == 0;
-  // one row a turn; for Q a turn ends as well where a sum over the row is needed
-  while ((Q || wave == 0) && !none) {
-    const Joined j = join(w, c0 + cur, rate, lane);
-    most = j.most;
-    at = j.at;
-    total = j.sum;
-    rejected = 0;
-    if (most == -INFINITY || !(total >= 0.0) || total == INFINITY) {   // no distribution
-      none = true;
-      break;
-    }
-    if (count > a.max_depth) break;
-    double sum = total;     // of s; Q: of s / total, 1
-    if (Q) sum = 1.0;
-    int chosen = -1;
-    for (int base = (cur + 1) & ~63; base < n && chosen < 0; base += 64) {
-      const int i = base + lane;
-      const bool child = i < n && sh.n.up[i] == cur;
-      uint64_t todo = __builtin_amdgcn_ballot_w64(child);
-      const double e = child && sh.n.token[i] >= 0 ? weight(sh.n.logit[i], most, rate) : 0.0;
-      for (; todo && chosen < 0; todo &= todo - 1) {
-        const int bit = __builtin_ctzll(todo), c = base + bit;
-        const int token = sh.n.token[c];
-        const double mine = __shfl(e, bit), u = (double)sh.n.u[c];
-        if (token < 0) continue;
-        if (rate == 0.0) {
-          if (token == at) chosen = c;
-          continue;
-        }
-        if constexpr (Q) {
-          const auto q = [&](int k) {
-            return (double)a.draft_probs[(int64_t)(c0 + (k < rejected ? sh.n.rejected[k] : c)) * a.probs_stride + token];
-          };
-          if (rejected) {   // what the last rejection left, which nobody has summed yet
-            if (tid == 0) {
-              sh.end.total = total;
-              sh.end.most = most;
-            }
-            __syncthreads();
-            const Row<T> r(logits + (int64_t)cur * a.row_stride, a.vocab);
-            const Weights<T, Q> weights{a, r, sh, c0, rate, rejected};
-            double own = 0.0;
-            for (int64_t g = 2 * tid; g < r.count; g += 2 * kThreads) {
-              double v[2][Row<T>::VEC];
-              int64_t el[2];
-              own += weights.pair(g, r.count, v, el);
-            }
-            double all;
-            scan(own, sh, all);
-            __syncthreads();
-            if (tid == 0) sh.n.amount[rejected - 1] = all;
-            __syncthreads();
+}
+
+// A row's children in their order, until one is accepted: its row, or -1.  Leaves
+// the rejected ones in sh.  A whole wave.  Q: kSum where another child comes after
+// rejections of which only `known` have their sums in sh.amount.
+constexpr int kSum = -2;
+template <class T, bool Q>
+__device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nodes, Shared& sh, int c0, int n, int cur, const Joined& j,
+                                    double rate, int& rejected, int known = 0) {
+  const int lane = threadIdx.x & 63;
+  rejected = 0;
+  const Scale scale(j.most, rate);
+  double sum = j.sum;
+  int chosen = -1;
+  for (int base = (cur + 1) & ~63; base < n && chosen < 0; base += 64) {
+    const int i = base + lane;
+    const bool child = i < n && nodes.up[i] == cur;
+    uint64_t todo = __builtin_amdgcn_ballot_w64(child);
+    const int token_i = child ? nodes.token[i] : -1;
+    const float u_i = child ? nodes.u[i] : 0.f;
+    const double e = token_i >= 0 ? scale(nodes.logit[i]) : 0.0;
+    while (todo && chosen < 0) {
+      const int bit = __builtin_ctzll(todo), c = base + bit;
+      todo &= todo - 1;
+      const int token = __builtin_amdgcn_readlane(token_i, bit);
+      const double mine = lane_value(e, bit), u = (double)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u_i), bit));
+      if (rate == 0.0) {
+        if (token >= 0 && token == j.at) chosen = c;
+      } else if (token < 0) {
+        // passed over
+      } else if constexpr (Q) {
+        const auto q = [&](int k) { return (double)a.draft_probs[(int64_t)(c0 + sh.rejected[k]) * a.probs_stride + token]; };
+        if (rejected > known) return kSum;
+        double s = mine / j.sum;
+        for (int k = 0; k < rejected; ++k)
+          if (sh.amount[k] > 0.0) {
+            const double d = s - q(k);
+            s = (d > 0.0 ? d : 0.0) / sh.amount[k];
           }
-          double s = mine / total;
-          for (int k = 0; k < rejected; ++k)
-            if (sh.n.amount[k] > 0.0) {
-              const double d = s - q(k);
-              s = (d > 0.0 ? d : 0.0) / sh.n.amount[k];
-            }
-          if (u * q(rejected) < s) chosen = c;
-          else {
-            __syncthreads();
-            if (tid == 0) sh.n.rejected[rejected] = c;
-            ++rejected;
-            __syncthreads();
-          }
+        if (u * (double)nodes.q[c] < s) {
+          chosen = c;
         } else {
-          // a token that a sibling before has had rejected has nothing left
-          bool again = false;
-          for (int k = lane; k < rejected; k += 64) again |= sh.n.token[sh.n.rejected[k]] == token;
-          if (__builtin_amdgcn_ballot_w64(again)) continue;
-          if (u * sum < mine) chosen = c;
-          else {
+          if (lane == 0) sh.rejected[rejected] = c;
+          ++rejected;
+        }
+      } else {
+        // a token that a sibling before has had rejected has nothing left
+        bool again = false;
+        for (int k = lane; k < rejected; k += 64) again |= sh.rejected[k] == token;
+        if (!__builtin_amdgcn_ballot_w64(again)) {
+          if (u * sum < mine) {
+            chosen = c;
+          } else {
             if (lane == 0) {
-              sh.n.rejected[rejected] = c;
-              sh.n.amount[rejected] = mine;
+              sh.rejected[rejected] = token;
+              sh.amount[rejected] = mine;
             }
             ++rejected;
             sum -= mine;
@@ -398,111 +464,116 @@ __device__ void walk(const shard_verify_args& a, const VerifyWork& w, Shared& sh
         }
       }
     }
-    if (chosen < 0) break;
-    cur = chosen;
-    if (write && tid == 0 && count < a.width) path[count] = cur;
-    ++count;
   }
+  return chosen;
+}
+
+// What wave 0 found, for all, and the rest of the walk's outputs.
+__device__ __forceinline__ void ended(const shard_verify_args& a, const Nodes& nodes, Shared& sh, int b, const Rows& rows, const Joined& j,
+                                      bool none, int cur, int count, int rejected) {
+  const int tid = threadIdx.x;
+  int32_t* path = a.path + (int64_t)b * a.width;
   __syncthreads();
   if (tid == 0) {
-    sh.end.total = total;
-    sh.end.most = most;
-    sh.end.at = at;
-    sh.end.row = none ? -1 : c0 + cur;
+    sh.end.total = j.sum;
+    sh.end.most = j.most;
+    sh.end.at = j.at;
+    sh.end.row = none ? -1 : rows.first + cur;
     sh.end.rejected = rejected;
     sh.count = count;
-    if (write) {
-      a.counts[b] = count;
-      if (n > 0) path[0] = 0;
-    }
+    sh.u = rows.n > 0 ? nodes.after[cur] : 0.f;
+    a.counts[b] = count;
+    if (rows.n > 0) path[0] = 0;
   }
   __syncthreads();
-  if (write)
-    for (int i = sh.count + tid; i < a.width; i += kThreads) path[i] = -1;
+  for (int i = sh.count + tid; i < a.width; i += kWalk) path[i] = -1;
 }
 
-template <class T>
-__global__ __launch_bounds__(kThreads)
-void k_verify_rest(const shard_verify_args a, const VerifyWork w) {
-  __shared__ Shared sh;
-  const int tid = threadIdx.x, part = blockIdx.x, b = blockIdx.y;
-  walk<T, true>(a, w, sh, b, part == 0);
-  const State end = sh.end;
-  int c0 = a.cu_seqlens ? min(max(a.cu_seqlens[b], 0), a.n_tokens) : b;
-  if (part == 0) {
-    if (tid == 0) w.state[b] = end;
-    for (int k = tid; k < end.rejected; k += kThreads) {
-      w.rejected[c0 + k] = sh.n.rejected[k];
-      w.left[c0 + k] = k < end.rejected - 1 ? sh.n.amount[k] : 0.0;
-    }
-  }
-  const double rate = rate_of(a, b);
-  if (end.row < 0 || rate == 0.0) return;
-  const Row<T> r((const T*)a.logits + (int64_t)end.row * a.row_stride, a.vocab);
-  const Weights<T, true> weights{a, r, sh, c0, rate, end.rejected};
-  const int64_t g0 = part * w.granules, g1 = min(g0 + w.granules, r.count);
-  double own = 0.0;
-  for (int64_t g = g0 + 2 * tid; g < g1; g += 2 * kThreads) {
-    double v[2][Row<T>::VEC];
-    int64_t e[2];
-    own += weights.pair(g, g1, v, e);
-  }
-  double all;
-  scan(own, sh, all);
-  if (tid == 0) w.rest[(int64_t)b * w.parts + part] = all;
-}
-
-// The walk (Q: its state) and the answer.
+// The walk.  Wave 0 decides; for Q the whole workgroup sums what a rejection has
+// left where another child comes after it.  Leaves sh.end, the rejected rows (tokens)
+// of the last row, and for Q what each but the last left.  Returns the lane's part
+// of the last row (wave 0).
 template <class T, bool Q>
-__global__ __launch_bounds__(kThreads)
-void k_verify_walk(const shard_verify_args a, const VerifyWork w) {
-  constexpr int VEC = Row<T>::VEC;
-  __shared__ Shared sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
-  const int c0 = a.cu_seqlens ? min(max(a.cu_seqlens[b], 0), a.n_tokens) : b;
-  const double rate = rate_of(a, b);
-  if constexpr (Q) {
-    const State end = w.state[b];
-    if (tid == 0) sh.end = end;
-    for (int k = tid; k < end.rejected; k += kThreads) {
-      sh.n.rejected[k] = w.rejected[c0 + k];
-      sh.n.amount[k] = w.left[c0 + k];
+__device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyWork& w, Nodes& nodes, Shared& sh, Part (&held_stats)[kHeld],
+                                       int b, double rate) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Rows rows = rows_of(a, b);
+  const int c0 = rows.first, n = rows.n;
+  const Part* stats = w.stats + (int64_t)c0 * w.parts;
+  const bool held = n * w.parts <= kHeld;
+  if (held)
+#pragma unroll
+    for (int i = tid; i < kHeld; i += kWalk)
+      if (i < n * w.parts) held_stats[i] = stats[i];
+  load_nodes<T>(a, nodes, rows, tid, kWalk);
+  __syncthreads();
+  int cur = 0, count = n > 0 ? 1 : 0, rejected = 0;
+  int32_t* path = a.path + (int64_t)b * a.width;
+  Joined j{0.0, 0.0, 0.f, -1};
+  bool none = n == 0, wants = false;
+  int known = 0;                                        // Q: rejections of the row whose sums are known
+  do {
+    if (wave == 0) {
+      bool on = !none;
+      while (on) {                                      // one row a turn
+        if (known == 0) j = join((held ? held_stats : stats) + cur * w.parts, w.parts, rate, lane);
+        rejected = 0;
+        none = !has_answer(j.most, rate);
+        const int chosen = none || count > a.max_depth ? -1 : turn<T, Q>(a, nodes, sh, c0, n, cur, j, rate, rejected, known);
+        on = chosen >= 0;
+        wants = chosen == kSum;
+        if (on) {
+          cur = chosen;
+          if (lane == 0) path[count] = cur;
+          ++count;
+          known = 0;
+        }
+      }
+      if (Q && lane == 0) {
+        sh.end = State{j.sum, j.most, j.at, c0 + cur, rejected};
+        sh.wants = wants;
+      }
     }
-    __syncthreads();
-  } else {
-    walk<T, false>(a, w, sh, b, true);
-  }
+    if constexpr (Q) {
+      __syncthreads();
+      wants = sh.wants;
+      if (wants) {                                      // what the last rejection left, and the turn once more
+        known = sh.end.rejected;
+        const Weights<T, Q> weights(a, sh, c0, sh.end.row, rate, known);
+        const double all = sum_of(weights, 0, weights.r.count * (Row<T>::VEC / 4), sh);
+        if (tid == 0) sh.amount[known - 1] = all;
+        __syncthreads();
+      }
+    }
+  } while (Q && wants);
+  ended(a, nodes, sh, b, rows, j, none, cur, count, rejected);
+  return j.mine;
+}
+
+// The answer of a walk that has ended at sh.end: the part that it lies in from the
+// parts' sums, `part` in wave 0's lanes, then the token.
+template <class T, bool Q>
+__device__ __forceinline__ void answer(const shard_verify_args& a, const VerifyWork& w, Shared& sh, int b, int64_t c0, double rate,
+                                       double part) {
+  constexpr int kQuads = Row<T>::VEC / 4;   // of a granule
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const State end = sh.end;
   if (end.row < 0 || rate == 0.0) {
     if (tid == 0) a.next[b] = end.row < 0 ? -1 : end.at;
     return;
   }
-  const Row<T> r((const T*)a.logits + (int64_t)end.row * a.row_stride, a.vocab);
-  int rejected = end.rejected;
-  const float u = a.uniforms[2 * (int64_t)end.row + 1];
-  // the part that the answer lies in
+  Weights<T, Q> weights(a, sh, c0, end.row, rate, end.rejected);
   if (wave == 0) {
-    double v;
-    if constexpr (Q) {
-      v = lane < w.parts ? w.rest[(int64_t)b * w.parts + lane] : 0.0;
-    } else {
-      v = join(w, end.row, rate, lane).mine;
-      for (int k = 0; k < rejected; ++k) {
-        const int64_t g = (sh.n.token[sh.n.rejected[k]] + r.mis) / VEC;
-        if (g / w.granules == lane) v -= sh.n.amount[k];
-      }
-      v = v > 0.0 ? v : 0.0;
+    if constexpr (!Q) {
+      for (int k = 0; k < end.rejected; ++k)
+        if ((sh.rejected[k] + weights.r.mis) / Row<T>::VEC / w.granules == lane) part -= sh.amount[k];
+      part = part > 0.0 ? part : 0.0;
     }
-    double x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
-    const double total = __shfl(x, 63), target = (double)u * total;
-    const uint64_t over = __builtin_amdgcn_ballot_w64(x > target), some = __builtin_amdgcn_ballot_w64(v > 0.0);
+    const double x = wave_scan(part);
+    const double target = (double)sh.u * lane_value(x, 63);
+    const uint64_t over = __builtin_amdgcn_ballot_w64(x > target), some = __builtin_amdgcn_ballot_w64(part > 0.0);
     const int p = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
-    const double before = __shfl(x - v, max(p, 0));
+    const double before = lane_value(x - part, max(p, 0));
     if (lane == 0) {
       sh.pick_part = p;
       sh.target = target - before;
@@ -511,70 +582,226 @@ void k_verify_walk(const shard_verify_args a, const VerifyWork w) {
     }
   }
   __syncthreads();
-  int64_t g0 = sh.pick_part * w.granules, g1 = min(g0 + w.granules, r.count);
+  int64_t i0 = sh.pick_part * w.granules * kQuads, i1 = min((sh.pick_part + 1) * w.granules, weights.r.count) * kQuads;
   double target = sh.target;
-  if (sh.pick_part < 0) {   // nothing is left of s
-    if (!Q || rejected == 0) {
-      if (tid == 0) a.next[b] = end.at;
+  if (sh.pick_part < 0) {           // nothing is left of s
+    if (!Q || weights.n == 0) {     // of numbers that are not below 1
+      if (tid == 0) a.next[b] = -1;
       return;
     }
     // the last subtraction is not made; its row as a whole
-    do --rejected;
-    while (rejected && !(sh.n.amount[rejected - 1] > 0.0));
-    g0 = 0;
-    g1 = r.count;
-    const Weights<T, Q> weights{a, r, sh, c0, rate, rejected};
-    double own = 0.0, all;
-    for (int64_t g = g0 + 2 * tid; g < g1; g += 2 * kThreads) {
-      double v[2][VEC];
-      int64_t e[2];
-      own += weights.pair(g, g1, v, e);
-    }
-    scan(own, sh, all);
-    target = (double)u * all;
+    do --weights.n;
+    while (weights.n && !(sh.amount[weights.n - 1] > 0.0));
+    i0 = 0;
+    i1 = weights.r.count * kQuads;
+    target = (double)sh.u * sum_of(weights, i0, i1, sh);
   }
-  const Weights<T, Q> weights{a, r, sh, c0, rate, rejected};
   double base = 0.0;
-  for (int64_t at = g0; at < g1; at += 2 * kThreads) {
-    double v[2][VEC], all;
-    int64_t e[2];
-    const double own = weights.pair(at + 2 * tid, g1, v, e);
+#pragma unroll 1
+  for (int64_t at = i0; at < i1; at += kWalk) {
+    double v[4], all;
+    auto raw = weights.fetch(at + tid, i1);
+    const double own = weights.value(raw, v);
     double run = base + scan(own, sh, all);
     // the first element at which the running sum is above the target, else the last that has any
     int pick = -1, some = -1;
 #pragma unroll
-    for (int k = 0; k < 2 * VEC; ++k) {
-      const double s = v[k / VEC][k % VEC];
-      run += s;
-      if (s > 0.0) {
-        some = (int)(e[k / VEC] + k % VEC);
+    for (int k = 0; k < 4; ++k) {
+      run += v[k];
+      if (v[k] > 0.0) {
+        some = (int)(4 * (at + tid) - weights.r.mis + k);
         if (run > target && pick < 0) pick = some;
       }
     }
-    if (pick >= 0) atomicMin(&sh.found, pick);
-    if (some >= 0) atomicMax(&sh.last, some);
+    const uint64_t picks = __builtin_amdgcn_ballot_w64(pick >= 0), has = __builtin_amdgcn_ballot_w64(some >= 0);
+    if (picks) {
+      if (lane == __builtin_ctzll(picks)) atomicMin(&sh.found, pick);
+    } else if (has && lane == 63 - __builtin_clzll(has)) {
+      atomicMax(&sh.last, some);
+    }
     __syncthreads();
     if (sh.found != INT32_MAX) break;
     base += all;
     __syncthreads();
   }
+  if (tid == 0) a.next[b] = sh.found != INT32_MAX ? sh.found : sh.last;
+}
+
+// Many rows, few of them on a path: a launch a level.  Each workgroup takes its
+// sequence's turn at the row of the level before (all of them the same one), then its
+// parts of the row that this leads to.
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void k_verify_level(const shard_verify_args a, const VerifyWork w, int level) {
+  __shared__ Nodes nodes;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int b = blockIdx.y, part = blockIdx.x * (kThreads / 64) + wave;
+  const Rows rows = rows_of(a, b);
+  if (rows.n == 0) return;
+  Level s{0, 1, 0};
+  if (level > 0) {
+    s = w.level[(level - 1 & 1) * a.batch + b];
+    const double rate = rate_of(a, b);
+    if (s.done == 0) {
+      const Part* stats = w.stats + ((int64_t)(level - 1 & 1) * a.batch + b) * w.parts;
+      load_nodes<T>(a, nodes, rows, tid, kThreads);
+      __syncthreads();
+      if (wave == 0) {
+        const Joined j = join(stats, w.parts, rate, lane);
+        int rejected, chosen = -1;
+        if (has_answer(j.most, rate)) chosen = turn<T, false>(a, nodes, sh, rows.first, rows.n, s.row, j, rate, rejected);
+        if (lane == 0) sh.found = chosen;
+      }
+      __syncthreads();
+      if (sh.found < 0) {
+        s.done = level;                                // its last row's parts are those of the level before
+      } else {
+        s.row = sh.found;
+        if (tid == 0 && blockIdx.x == 0) a.path[(int64_t)b * a.width + s.count] = s.row;
+        ++s.count;
+      }
+    }
+  }
+  if (tid == 0 && blockIdx.x == 0) w.level[(level & 1) * a.batch + b] = s;
+  if (s.done == 0 && part < w.parts)
+    part_of<T>(a, w, rows.first + s.row, part, b, w.stats + ((int64_t)(level & 1) * a.batch + b) * w.parts + part);
+}
+
+// After `levels` of them: the last turn again, which leads nowhere, and the answer.
+template <class T>
+__global__ __launch_bounds__(kWalk)
+void k_verify_end(const shard_verify_args a, const VerifyWork w, int levels) {
+  __shared__ Nodes nodes;
+  __shared__ Shared sh;
+  const int b = blockIdx.x, last = levels - 1;
+  const double rate = rate_of(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Rows rows = rows_of(a, b);
+  Level s{0, 0, 0};
+  if (rows.n) s = w.level[(last & 1) * a.batch + b];
+  const int of = s.done ? s.done - 1 : last;            // the level that took its last row's parts
+  load_nodes<T>(a, nodes, rows, threadIdx.x, kWalk);
   __syncthreads();
-  if (tid == 0) a.next[b] = sh.found != INT32_MAX ? sh.found : sh.last >= 0 ? sh.last : end.at;
+  Joined j{0.0, 0.0, 0.f, -1};
+  int rejected = 0;
+  bool none = rows.n == 0;
+  if (wave == 0 && rows.n) {
+    j = join(w.stats + ((int64_t)(of & 1) * a.batch + b) * w.parts, w.parts, rate, lane);
+    none = !has_answer(j.most, rate);
+    if (!none && s.count <= a.max_depth) turn<T, false>(a, nodes, sh, rows.first, rows.n, s.row, j, rate, rejected);
+  }
+  ended(a, nodes, sh, b, rows, j, none, s.row, s.count, rejected);
+  const int c0 = rows.first;
+  const double mine = j.mine;
+  answer<T, false>(a, w, sh, b, c0, rate, mine);
+}
+
+template <class T, bool Q>
+__global__ __launch_bounds__(kWalk)
+void k_verify_walk(const shard_verify_args a, const VerifyWork w) {
+  __shared__ Part stats[kHeld];
+  __shared__ Nodes nodes;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, b = blockIdx.x;
+  const double rate = rate_of(a, b);
+  const double mine = walk<T, Q>(a, w, nodes, sh, stats, b, rate);
+  const int c0 = rows_of(a, b).first;
+  if constexpr (Q) {
+    const State end = sh.end;
+    if (tid == 0) w.state[b] = end;
+    if (tid < end.rejected) {
+      w.rejected[c0 + tid] = sh.rejected[tid];
+      w.left[c0 + tid] = tid < end.rejected - 1 ? sh.amount[tid] : 0.0;
+    }
+  } else {
+    answer<T, Q>(a, w, sh, b, c0, rate, mine);
+  }
+}
+
+// With draft_probs: a walk's end from its state.
+__device__ __forceinline__ void end_of(const shard_verify_args& a, const VerifyWork& w, Shared& sh, int b, int c0) {
+  const int tid = threadIdx.x;
+  const State end = w.state[b];
+  if (tid == 0) {
+    sh.end = end;
+    sh.u = end.row >= 0 ? a.uniforms[2 * (int64_t)end.row + 1] : 0.f;
+  }
+  for (int k = tid; k < end.rejected; k += blockDim.x) {
+    sh.rejected[k] = w.rejected[c0 + k];
+    sh.amount[k] = w.left[c0 + k];
+  }
+  __syncthreads();
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void k_verify_rest(const shard_verify_args a, const VerifyWork w) {
+  __shared__ Shared sh;
+  const int part = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int b = blockIdx.y, c0 = rows_of(a, b).first;
+  const double rate = rate_of(a, b);
+  end_of(a, w, sh, b, c0);
+  if (sh.end.row < 0 || rate == 0.0 || part >= w.parts) return;
+  const Weights<T, true> weights(a, sh, c0, sh.end.row, rate, sh.end.rejected);
+  constexpr int kQuads = Row<T>::VEC / 4;
+  const int64_t i1 = min((part + 1) * w.granules, weights.r.count) * kQuads;
+  double own = 0.0;
+  constexpr int U = 4;   // on their way together
+#pragma unroll 1
+  for (int64_t i = part * w.granules * kQuads; i < i1; i += 64 * U) {
+    typename Weights<T, true>::Raw raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = weights.fetch(i + 64 * u + lane, i1);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      double v[4];
+      own += weights.value(raw[u], v);
+    }
+  }
+  own = wave_sum(own);
+  if (lane == 0) w.rest[(int64_t)b * w.parts + part] = own;
+}
+
+template <class T>
+__global__ __launch_bounds__(kWalk)
+void k_verify_answer(const shard_verify_args a, const VerifyWork w) {
+  __shared__ Shared sh;
+  const int b = blockIdx.x, c0 = rows_of(a, b).first;
+  const double part = threadIdx.x < w.parts ? w.rest[(int64_t)b * w.parts + threadIdx.x] : 0.0;
+  const double rate = rate_of(a, b);
+  end_of(a, w, sh, b, c0);
+  answer<T, true>(a, w, sh, b, c0, rate, part);
 }
 
 // --------------------------------------------------------------------------
 // host side
 // --------------------------------------------------------------------------
+// Launches of a level each, or 0: all rows at once.  A row of 128,256 logits costs
+// 0.12 us of the chip (its exponentials in 64 bits), a level 2.3 us; about three
+// rows of a sequence are on its path.  All at once / by levels, us: 61 rows in 7
+// levels 17.8 / 24.3, 4 such trees 40.9 / 29.3, 64 chains of 5 46.3 / 33.0, 64 trees
+// of up to 26 134.5 / 47.2; 3,904 rows of 5,000 logits in 6 levels 47.4 / 39.4.
+int levels_of(const shard_verify_args* a) {
+  if (a->draft_probs) return 0;   // a turn may take sums over the row
+  const int64_t levels = (int64_t)(a->max_depth < a->width - 1 ? a->max_depth : a->width - 1) + 1;
+  return (a->n_tokens - 3 * (int64_t)a->batch) * a->vocab > 2500000 * levels ? (int)levels : 0;
+}
+
 bool plan(const shard_verify_args* a, VerifyWork& w, size_t& bytes) {
   if (a->n_tokens < 0 || a->n_tokens >= 1 << 24 || a->batch <= 0 || a->batch > 65535 || a->vocab <= 0 || a->vocab >= INT32_MAX - 64)
     return false;
   if (a->dtype != SHARD_FP16 && a->dtype != SHARD_BF16 && a->dtype != SHARD_FP32) return false;
   const int vec = a->dtype == SHARD_FP32 ? 4 : 8;
   const int64_t granules = (a->vocab + 2 * vec - 2) / vec;          // of the worst aligned row
-  const int64_t parts = (granules + 2 * kThreads - 1) / (2 * kThreads);
-  w.parts = (int)(parts < kMaxParts ? parts : kMaxParts);
-  w.granules = (granules + w.parts - 1) / w.parts;
-  w.granules += w.granules & 1;
+  w.granules = (granules + kMaxParts - 1) / kMaxParts;
+  if (w.granules < kTurn / 2) w.granules = kTurn / 2;
+  w.parts = (int)((granules + w.granules - 1) / w.granules);
+  w.levels = levels_of(a);
+  if (w.levels) {
+    bytes = (size_t)2 * a->batch * (w.parts * sizeof(Part) + sizeof(Level));
+    return true;
+  }
   bytes = (size_t)a->n_tokens * w.parts * sizeof(Part);
   if (a->draft_probs)
     bytes += (size_t)a->batch * (sizeof(State) + w.parts * sizeof(double)) + (size_t)a->n_tokens * (sizeof(double) + sizeof(int32_t));
@@ -588,12 +815,19 @@ using namespace shard;
 
 template <class T>
 static void launch_verify(const shard_verify_args& a, const VerifyWork& w, hipStream_t s) {
-  hipLaunchKernelGGL(k_verify_stats<T>, dim3((unsigned)a.n_tokens, w.parts), dim3(kThreads), 0, s, a, w);
+  const unsigned groups = (w.parts + kThreads / 64 - 1) / (kThreads / 64);
+  if (w.levels) {
+    for (int i = 0; i < w.levels; ++i) hipLaunchKernelGGL(k_verify_level<T>, dim3(groups, a.batch), dim3(kThreads), 0, s, a, w, i);
+    hipLaunchKernelGGL(k_verify_end<T>, dim3(a.batch), dim3(kWalk), 0, s, a, w, w.levels);
+    return;
+  }
+  hipLaunchKernelGGL(k_verify_stats<T>, dim3((unsigned)a.n_tokens, groups), dim3(kThreads), 0, s, a, w);
   if (a.draft_probs) {
-    hipLaunchKernelGGL(k_verify_rest<T>, dim3(w.parts, a.batch), dim3(kThreads), 0, s, a, w);
-    hipLaunchKernelGGL((k_verify_walk<T, true>), dim3(a.batch), dim3(kThreads), 0, s, a, w);
+    hipLaunchKernelGGL((k_verify_walk<T, true>), dim3(a.batch), dim3(kWalk), 0, s, a, w);
+    hipLaunchKernelGGL(k_verify_rest<T>, dim3(groups, a.batch), dim3(kThreads), 0, s, a, w);
+    hipLaunchKernelGGL(k_verify_answer<T>, dim3(a.batch), dim3(kWalk), 0, s, a, w);
   } else {
-    hipLaunchKernelGGL((k_verify_walk<T, false>), dim3(a.batch), dim3(kThreads), 0, s, a, w);
+    hipLaunchKernelGGL((k_verify_walk<T, false>), dim3(a.batch), dim3(kWalk), 0, s, a, w);
   }
 }
 
@@ -624,6 +858,7 @@ int shard_verify_drafts(const shard_verify_args* a, void* workspace, size_t work
     return SHARD_ERR_WORKSPACE;
   }
   w.stats = (Part*)workspace;
+  w.level = (Level*)(w.stats + (size_t)2 * a->batch * w.parts);
   if (a->draft_probs) {
     w.state = (State*)(w.stats + (size_t)a->n_tokens * w.parts);
     w.rest = (double*)(w.state + a->batch);
@@ -633,7 +868,7 @@ int shard_verify_drafts(const shard_verify_args* a, void* workspace, size_t work
   const hipStream_t s = (hipStream_t)stream;
   if (a->n_tokens == 0) {
     // sequences of no rows: nothing is read
-    hipLaunchKernelGGL((k_verify_walk<half_t, false>), dim3(a->batch), dim3(kThreads), 0, s, *a, w);
+    hipLaunchKernelGGL((k_verify_walk<half_t, false>), dim3(a->batch), dim3(kWalk), 0, s, *a, w);
   } else if (a->dtype == SHARD_FP16) {
     launch_verify<half_t>(*a, w, s);
   } else if (a->dtype == SHARD_BF16) {

@@ -176,6 +176,25 @@ def test_bounds(cuda, probs):
     assert c.run(max_new=3)[0].shape == (2, 3)
 
 
+@pytest.mark.parametrize("type", ["fp16", "bf16", "fp32"])
+def test_a_launch_a_level(cuda, type):
+    """Many rows, few of them on a path: the sizes that go level by level, with greedy and sampling sequences, empty
+    ones, walks that end early, at max_depth, at odd rows, and those that go to the end."""
+    for depth in (0, 2, 3):
+        Case([90], 128257, type, seed=depth, close=25.0).check(max_depth=depth)
+    new = [9, 0, 4, 1] * 20
+    temps = [[1.0, 0.5, 0.0, 0.8, 2.0][i % 5] for i in range(80)]
+    c = Case(new, 40009, type, temperature=temps, seed=7, close=25.0)
+    c.logits[0, 11], c.logits[15, 20000], c.logits[c.cu[16]] = torch.nan, torch.inf, -torch.inf
+    lengths = [len(p) for p, _ in c.check(max_depth=2)]
+    c.uniforms[:, 0] = 0.0
+    lengths += [len(p) for p, _ in c.check(max_depth=3)]
+    assert {0, 1, 2, 3, 4} <= set(lengths)
+    chain = Case([6] * 60, 40009, type, temperature=0.7, seed=8, width=1)
+    chain.uniforms[:, 0] = 0.0
+    assert max(len(p) for p, _ in chain.check(max_depth=3)) == 4
+
+
 @pytest.mark.parametrize("probs", [False, True], ids=["chosen", "drawn"])
 def test_the_answers_are_the_targets_own(cuda, probs):
     """The first token of 40,000 sequences is distributed as the target's, whatever is drafted, and so is the second
