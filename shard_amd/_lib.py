@@ -143,6 +143,7 @@ SIGNATURES = [
     ("shard_kv4_attn_workspace", c_size_t, [c_void_p]),
     ("shard_kv4_attn", c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
     ("shard_kv4_append_at", c_int32, [c_void_p, c_void_p, c_void_p]),
+    ("shard_kv4_tree_attn_workspace", c_size_t, [c_void_p]),
     ("shard_kv4_tree_attn", c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
     ("shard_kv4_keep", c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
     ("shard_draft_tree", c_int32, [c_void_p] * 3 + [c_int32] * 3 + [c_void_p] * 3),

@@ -458,6 +458,7 @@ struct AttnWork {
   int group, group_shift;       // query heads of a kv head; -1: no power of two
   int row_tiles;                // workgroups along a sequence's rows
   float sorted;                 // 16 / longest length where longer sequences go first, or 0
+  bool paired;                  // trees: row tiles side by side
   const uint64_t* mask;         // [row][words]: which rows of its sequence a row sees (trees)
   int words;
 };
@@ -602,9 +603,17 @@ void k_kv4_attn_rows(const shard_kv4_args a, const AttnWork w) {
   __shared__ float sh_m[WAVES][16 * NQ], sh_l[WAVES][16 * NQ];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
-  const int g = blockIdx.y;
-  const int split = blockIdx.x & (w.n_splits - 1), rt0 = blockIdx.x >> w.split_shift;
-  int b = blockIdx.z, len;
+  int g = blockIdx.y, split = blockIdx.x & (w.n_splits - 1), rt0 = blockIdx.x >> w.split_shift, b = blockIdx.z, len;
+  if (TREE && w.paired) {
+    // workgroups go to the XCDs in turn: the row tiles of the same pages one after
+    // the other on one of them, so that the second finds them in its L2
+    const int id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+    const int at = (id >> 3) / w.row_tiles, unit = at * 8 + (id & 7);
+    rt0 = (id >> 3) - at * w.row_tiles;
+    split = unit & (w.n_splits - 1);
+    b = (unit >> w.split_shift) / a.n_kv_heads;
+    g = (unit >> w.split_shift) - b * a.n_kv_heads;
+  }
   if (w.sorted != 0.f) b = by_length(a, w, b, lane, len);
   else len = a.seq_lens[b];
   const Seq s = seq_of(a, b, len);
@@ -1486,6 +1495,13 @@ struct AttnPlan {
   int row_tiles, n_splits, split_shift;
   float sorted;
 };
+// The number of splits nearest to sp, a power of two.
+void round_splits(AttnPlan& p, int64_t sp) {
+  p.split_shift = 0;
+  while ((int64_t)2 << p.split_shift <= kMaxSplits && (int64_t)2 << (2 * p.split_shift) < sp * sp) ++p.split_shift;
+  p.n_splits = 1 << p.split_shift;
+}
+
 AttnPlan plan_of(const shard_kv4_args* a) {
   AttnPlan p;
   const int group = a->n_q_heads / a->n_kv_heads;
@@ -1504,13 +1520,41 @@ AttnPlan plan_of(const shard_kv4_args* a) {
   if (sp > (tiles + kMinTiles - 1) / kMinTiles) sp = (tiles + kMinTiles - 1) / kMinTiles;
   if (sp > kMaxSplits) sp = kMaxSplits;
   if ((int64_t)a->n_tokens * a->n_q_heads >= 1 << 24) sp = 1;  // more rows than a launch of the join takes
-  // the nearest power of two
-  p.split_shift = 0;
-  while ((int64_t)2 << p.split_shift <= kMaxSplits && (int64_t)2 << (2 * p.split_shift) < sp * sp) ++p.split_shift;
-  p.n_splits = 1 << p.split_shift;
+  round_splits(p, sp);
   // several workgroups a CU: the longest first
   p.sorted = a->batch > 1 && wg * p.n_splits >= 1024 ? 16.f / len : 0.f;
   // few rows fold where a wave has more than a page (k_kv4_attn_rows)
+  if (rows <= 8 && tiles > kMinTiles * p.n_splits) p.rows = rows <= 4 ? 4 : 8;
+  return p;
+}
+
+// Trees have 8 to a few hundred rows a kv head: tiles of 32 of them a workgroup, the
+// workgroups of the same pages side by side (AttnWork::paired).  128-row tiles are
+// worth it where there is work for the whole chip at once and little of them stays
+// empty: 32 / 128 rows, us (32 heads on 8 of 128, one sequence): 61 nodes over 8K
+// 26.5 / 33.2, 128 over 4K 29.9 / 40.4, 256 over 4K 43.4 / 42.6, 256 over 16K 113.1 /
+// 96.5, 8 sequences of 64 over 8K 116.2 / 97.1.  Splits as in plan_of, but 32 pages
+// at most where that makes 1,152 workgroups or fewer: 18 uneven sequences of up to
+// 13,626 tokens 23.1, with 64 36.3; 16 x 16K, 2,048 workgroups, 126.7 and 118.0.
+AttnPlan tree_plan_of(const shard_kv4_args* a) {
+  AttnPlan p;
+  const int group = a->n_q_heads / a->n_kv_heads;
+  const int64_t n = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
+  const int64_t rows = (a->cu_seqlens ? n : 1) * group;
+  const int64_t cap = (int64_t)a->table_width * kPage;
+  const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
+  const int64_t tiles = (len + kPage - 1) / kPage;
+  const int64_t r32 = (rows + 31) / 32, r128 = (rows + kTileRows - 1) / kTileRows;
+  const bool whole = 100 * 4 * r128 <= 115 * r32 && a->batch * a->n_kv_heads * r128 * tiles > 6500;
+  p.rows = rows <= 16 ? 16 : whole ? kTileRows : 32;
+  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+  const int64_t wg = (int64_t)a->batch * a->n_kv_heads * p.row_tiles;
+  const int64_t most = wg * ((tiles + 31) / 32) <= 1152 ? 32 : 64;
+  int64_t sp = std::max((512 + wg - 1) / wg, (tiles + most - 1) / most);
+  sp = std::min(std::min(sp, (tiles + kMinTiles - 1) / kMinTiles), (int64_t)kMaxSplits);
+  if ((int64_t)a->n_tokens * a->n_q_heads >= 1 << 24) sp = 1;  // more rows than a launch of the join takes
+  round_splits(p, sp);
+  p.sorted = p.rows != kTileRows && a->batch > 1 && wg * p.n_splits >= 1024 ? 16.f / len : 0.f;
   if (rows <= 8 && tiles > kMinTiles * p.n_splits) p.rows = rows <= 4 ? 4 : 8;
   return p;
 }
@@ -1604,12 +1648,16 @@ int shard_kv4_read(const shard_kv4_args* a, void* stream) {
   return SHARD_OK;
 }
 
-size_t shard_kv4_attn_workspace(const shard_kv4_args* a) {
+static size_t attn_workspace(const shard_kv4_args* a, bool tree) {
   if (check_attn(a) || a->n_tokens == 0) return 0;
-  const AttnPlan p = plan_of(a);
+  const AttnPlan p = tree ? tree_plan_of(a) : plan_of(a);
   if (p.n_splits == 1) return 0;
   return (size_t)a->n_tokens * a->n_q_heads * p.n_splits * (a->head_dim + 2) * sizeof(float);
 }
+
+size_t shard_kv4_attn_workspace(const shard_kv4_args* a) { return attn_workspace(a, false); }
+
+size_t shard_kv4_tree_attn_workspace(const shard_kv4_args* a) { return attn_workspace(a, true); }
 
 static int launch_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t words, void* workspace, size_t workspace_bytes,
                        void* stream) {
@@ -1618,7 +1666,7 @@ static int launch_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t wo
   if (!rows_ok(a->q, a->q_stride, a->q_head_stride) || !a->out || (uintptr_t)a->out % 16) return SHARD_ERR_ARG;
   if (!(fabsf(a->scale) <= kMostScale)) return SHARD_ERR_ARG;  // NaN, or infinite times log2(e)
   if (a->n_tokens == 0) return SHARD_OK;
-  const AttnPlan p = plan_of(a);
+  const AttnPlan p = mask ? tree_plan_of(a) : plan_of(a);
   const int64_t rows = (int64_t)a->n_tokens * a->n_q_heads;
   AttnWork w{};
   w.n_splits = p.n_splits;
@@ -1627,11 +1675,13 @@ static int launch_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t wo
   w.group = a->n_q_heads / a->n_kv_heads;
   w.group_shift = w.group & (w.group - 1) ? -1 : __builtin_ctz(w.group);
   w.row_tiles = p.row_tiles;
+  const int64_t units = (int64_t)p.n_splits * a->n_kv_heads * a->batch;   // the kernel counts them in 32 bits
+  w.paired = mask && p.row_tiles > 1 && units % 8 == 0 && units * p.row_tiles <= INT32_MAX;
   w.mask = mask;
   w.words = words;
   if ((int64_t)w.n_splits * w.row_tiles * a->n_kv_heads > INT32_MAX) return SHARD_ERR_SHAPE;
   if (p.n_splits > 1) {
-    const size_t need = shard_kv4_attn_workspace(a);
+    const size_t need = attn_workspace(a, mask != nullptr);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) {
       char text[96];
       snprintf(text, sizeof(text), "shard_kv4_attn needs %zu bytes of workspace, 16-byte aligned", need);

@@ -1207,7 +1207,7 @@ def _kv4_attn(q, cache, block_table, seq_lens, mask, cu_seqlens, scale, out, max
     if T:
         args = _lib.KV4_PACK.pack(block_table.shape[0], T, H, G, D, code, *fields, *q_at, *(0,) * 6, 0, 0,
                                   scale, 0, 0, 0, out.data_ptr())
-        need = lib.shard_kv4_attn_workspace(args)
+        need = lib.shard_kv4_attn_workspace(args) if mask is None else lib.shard_kv4_tree_attn_workspace(args)
         ws = cache.new_empty(need) if need else None
         at = ws.data_ptr() if need else None
         if mask is None:

@@ -44,7 +44,7 @@ def test_refusals():
     for kw, code in ((dict(q=None), -1), (dict(n_q_heads=12), -2), (dict(scale=float("nan")), -1), (dict(out=P + 8), -1)):
         assert lib.shard_kv4_tree_attn(_args(**kw), P, 1, None, 0, None) == code
     wide = _args(table_width=512, table_stride=512)
-    assert lib.shard_kv4_tree_attn(wide, P, 1, None, lib.shard_kv4_attn_workspace(wide), None) == -4
+    assert lib.shard_kv4_tree_attn(wide, P, 1, None, lib.shard_kv4_tree_attn_workspace(wide), None) == -4
 
     page = 8 * 68 * 128
     keep = lambda layers=1, stride=0, rows=P, rows_stride=4, width=4, counts=P, **kw: \
