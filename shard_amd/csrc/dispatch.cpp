@@ -11,6 +11,7 @@
 #include <Python.h>
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include <ATen/ATen.h>
@@ -29,6 +30,14 @@ decltype(&shard_kv4_attn_workspace) p_attn_workspace;
 decltype(&shard_kv4_attn) p_attn;
 decltype(&shard_token_logprobs_workspace) p_logprobs_workspace;
 decltype(&shard_token_logprobs) p_logprobs;
+// null where the library has none of them: their calls go through ops.py
+decltype(&shard_kv4_append_at) p_append_at;
+decltype(&shard_kv4_tree_attn_workspace) p_tree_workspace;
+decltype(&shard_kv4_tree_attn) p_tree_attn;
+decltype(&shard_kv4_keep) p_keep;
+decltype(&shard_draft_tree) p_tree;
+decltype(&shard_verify_drafts_workspace) p_verify_workspace;
+decltype(&shard_verify_drafts) p_verify;
 
 // Uninitialized, on like's device (the current one); without the dispatcher's
 // share of at::empty (0.47 us against 0.71).
@@ -85,17 +94,23 @@ int half_code(const at::Tensor& t) {
   return t.scalar_type() == at::kHalf ? SHARD_FP16 : t.scalar_type() == at::kBFloat16 ? SHARD_BF16 : -1;
 }
 
-// The batch's part of an argument block (_kv4_batch of ops.py).
+// n whole numbers of 32 bits, one after the other.
+bool indexes(const at::Tensor& t, int64_t n) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+
+// The batch's part of an argument block (_kv4_batch of ops.py); `d`: the cache's
+// dimensions before the pages.
 bool batch(shard_kv4_args& a, int64_t n_tokens, const at::Tensor& cache, const at::Tensor& table, const at::Tensor& lens,
-           const at::Tensor* cu) {
-  if (cache.dim() != 3 || table.dim() != 2 || lens.dim() != 1 || cache.scalar_type() != at::kByte || table.scalar_type() != at::kInt ||
+           const at::Tensor* cu, int d = 0) {
+  if (cache.dim() != 3 + d || table.dim() != 2 || lens.dim() != 1 || cache.scalar_type() != at::kByte || table.scalar_type() != at::kInt ||
       lens.scalar_type() != at::kInt)
     return false;
-  const int64_t pages = cache.size(0), G = cache.size(1), width = cache.size(2), B = table.size(0), W = table.size(1);
+  const int64_t pages = cache.size(d), G = cache.size(d + 1), width = cache.size(d + 2), B = table.size(0), W = table.size(1);
   if ((width != 68 * 64 && width != 68 * 128) || lens.size(0) != B || !lens.is_contiguous()) return false;
-  if (cu ? cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) != B + 1 || !cu->is_contiguous() : n_tokens != B) return false;
-  if (cache.stride(2) != 1 || (cache.stride(1) != width && G > 1) || (table.stride(1) != 1 && W > 1)) return false;
-  const int64_t s0 = pages == 1 ? G * width : cache.stride(0), t0 = B == 1 ? W : table.stride(0);
+  if (cu ? !indexes(*cu, B + 1) : n_tokens != B) return false;
+  if (cache.stride(d + 2) != 1 || (cache.stride(d + 1) != width && G > 1) || (table.stride(1) != 1 && W > 1)) return false;
+  const int64_t s0 = pages == 1 ? G * width : cache.stride(d), t0 = B == 1 ? W : table.stride(0);
   if (pages <= 0 || G <= 0 || W <= 0 || B <= 0 || s0 < G * width || t0 < W || n_tokens <= 0) return false;
   if (pages > INT32_MAX || G > INT32_MAX || W > INT32_MAX || B > INT32_MAX || n_tokens > INT32_MAX) return false;
   a.batch = (int32_t)B;
@@ -122,17 +137,18 @@ bool rows(const at::Tensor& t, int64_t n_tokens, int64_t heads, int64_t D, const
   return t.stride(2) == 1 && ((*s0 | *s1) & 7) == 0 && ((uintptr_t)*p & 15) == 0;
 }
 
-// kv4_append(k, v, cache, block_table, seq_lens, phases, q, cu_seqlens, max_new, device, stream) -> rotated q, or True
+// kv4_append(k, v, cache, block_table, seq_lens, phases, q, cu_seqlens, max_new, [positions,] device, stream) -> rotated q, or True
 PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   int64_t device, stream;
-  const at::Tensor *k, *v, *cache, *table, *lens, *phases, *q, *cu;
+  const at::Tensor *k, *v, *cache, *table, *lens, *phases, *q, *cu, *at;
   shard_kv4_args a{};
-  if (n != 11 || !integer(o[9], &device) || !integer(o[10], &stream) || !tensor(o[0], device, &k) || !tensor(o[1], device, &v) ||
+  if ((n != 11 && n != 12) || !integer(o[n - 2], &device) || !integer(o[n - 1], &stream) || !tensor(o[0], device, &k) || !tensor(o[1], device, &v) ||
       !tensor(o[2], device, &cache) || !tensor(o[3], device, &table) || !tensor(o[4], device, &lens) || !tensor(o[5], device, &phases) ||
-      !tensor(o[6], device, &q, true) || !tensor(o[7], device, &cu, true) || !hint(o[8], &a.max_new))
+      !tensor(o[6], device, &q, true) || !tensor(o[7], device, &cu, true) || !hint(o[8], &a.max_new) ||
+      !tensor(n == 12 ? o[9] : Py_None, device, &at, true) || (at && !p_append_at))
     Py_RETURN_NONE;
-  if (k->dim() != 3 || !batch(a, k->size(0), *cache, *table, *lens, cu)) Py_RETURN_NONE;
+  if (k->dim() != 3 || !batch(a, k->size(0), *cache, *table, *lens, cu) || (at && !indexes(*at, a.n_tokens))) Py_RETURN_NONE;
   a.dtype = half_code(*k);
   const int64_t D = a.head_dim;
   if (a.dtype < 0 || v->scalar_type() != k->scalar_type() || (q && q->scalar_type() != k->scalar_type())) Py_RETURN_NONE;
@@ -157,7 +173,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
       out = make(q->sizes(), *q, q->scalar_type());
       a.q_out = out.data_ptr();
     }
-    rc = p_append(&a, (void*)stream);
+    rc = at ? p_append_at(&a, (const int32_t*)at->data_ptr(), (void*)stream) : p_append(&a, (void*)stream);
   }
   if (rc) Py_RETURN_NONE;
   if (!q) Py_RETURN_TRUE;
@@ -195,14 +211,15 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // kv4_attn(q, cache, block_table, seq_lens, cu_seqlens, scale, max_new, max_len, device, stream) -> out
+// kv4_tree_attn(q, cache, block_table, seq_lens, cu_seqlens, scale, max_new, max_len, mask, device, stream) -> out
 PyObject* attn(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   int64_t device, stream;
-  const at::Tensor *q, *cache, *table, *lens, *cu;
+  const at::Tensor *q, *cache, *table, *lens, *cu, *mask;
   shard_kv4_args a{};
-  if (n != 10 || !integer(o[8], &device) || !integer(o[9], &stream) || !tensor(o[0], device, &q) || !tensor(o[1], device, &cache) ||
+  if ((n != 10 && n != 11) || !integer(o[n - 2], &device) || !integer(o[n - 1], &stream) || !tensor(o[0], device, &q) || !tensor(o[1], device, &cache) ||
       !tensor(o[2], device, &table) || !tensor(o[3], device, &lens) || !tensor(o[4], device, &cu, true) || !hint(o[6], &a.max_new) ||
-      !hint(o[7], &a.max_len))
+      !hint(o[7], &a.max_len) || !tensor(n == 11 ? o[8] : Py_None, device, &mask, n == 10) || (mask && !p_tree_attn))
     Py_RETURN_NONE;
   if (q->dim() != 3 || !batch(a, q->size(0), *cache, *table, *lens, cu)) Py_RETURN_NONE;
   a.dtype = half_code(*q);
@@ -213,18 +230,150 @@ PyObject* attn(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (o[5] == Py_None) a.scale = (float)std::pow((double)a.head_dim, -0.5);
   else if (PyFloat_CheckExact(o[5])) a.scale = (float)PyFloat_AS_DOUBLE(o[5]);
   else Py_RETURN_NONE;
+  if (mask && (mask->scalar_type() != at::kLong || mask->dim() != 2 || mask->size(0) != a.n_tokens || mask->size(1) < 1 ||
+               mask->size(1) > INT32_MAX || !mask->is_contiguous()))
+    Py_RETURN_NONE;
   at::Tensor out;
   int rc;
   {
     const Unlocked unlocked;
     out = make(q->sizes(), *q, q->scalar_type());
     a.out = out.data_ptr();
-    const size_t need = p_attn_workspace(&a);
+    const size_t need = mask ? p_tree_workspace(&a) : p_attn_workspace(&a);
     const c10::DataPtr ws = scratch(need);
-    rc = p_attn(&a, ws.get(), need, (void*)stream);
+    rc = mask ? p_tree_attn(&a, (const uint64_t*)mask->data_ptr(), (int32_t)mask->size(1), ws.get(), need, (void*)stream)
+              : p_attn(&a, ws.get(), need, (void*)stream);
   }
   if (rc) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A tree's bound (_tree_width of ops.py).
+bool tree_width(PyObject* o, int64_t rows, int64_t* width) {
+  if (o == Py_None) *width = rows;
+  else if (!integer(o, width)) return false;
+  *width = std::min(*width, rows);
+  if (*width < 0 || *width > SHARD_TREE_ROWS) return false;
+  *width = std::max<int64_t>(*width, 1);
+  return true;
+}
+
+// draft_tree(parents, seq_lens, cu_seqlens, max_new, device, stream) -> mask, positions
+PyObject* tree(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t device, stream, width;
+  const at::Tensor *up, *lens, *cu;
+  if (!p_tree || n != 6 || !integer(o[4], &device) || !integer(o[5], &stream) || !tensor(o[0], device, &up) || !tensor(o[1], device, &lens) ||
+      !tensor(o[2], device, &cu, true) || up->dim() != 1 || lens->dim() != 1)
+    Py_RETURN_NONE;
+  const int64_t T = up->size(0), B = lens->size(0);
+  if (T <= 0 || T > INT32_MAX || B <= 0 || B > INT32_MAX || !indexes(*up, T) || !indexes(*lens, B) ||
+      (cu ? !indexes(*cu, B + 1) : T != B) || !tree_width(o[3], T, &width))
+    Py_RETURN_NONE;
+  const int64_t two[2] = {T, (width + 63) / 64}, one[1] = {T};
+  at::Tensor mask, positions;
+  int rc;
+  {
+    const Unlocked unlocked;
+    mask = make(two, *up, at::kLong);
+    positions = make(one, *up, at::kInt);
+    rc = p_tree((const int32_t*)up->data_ptr(), (const int32_t*)lens->data_ptr(), cu ? (const int32_t*)cu->data_ptr() : nullptr,
+                (int32_t)B, (int32_t)T, (int32_t)two[1], (uint64_t*)mask.data_ptr(), (int32_t*)positions.data_ptr(), (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
+  return Py_BuildValue("NN", THPVariable_Wrap(std::move(mask)), THPVariable_Wrap(std::move(positions)));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_keep(cache, block_table, seq_lens, rows, counts, cu_seqlens, device, stream) -> True
+PyObject* keep(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t device, stream;
+  const at::Tensor *cache, *table, *lens, *rows, *counts, *cu;
+  shard_kv4_args a{};
+  if (!p_keep || n != 8 || !integer(o[6], &device) || !integer(o[7], &stream) || !tensor(o[0], device, &cache) || !tensor(o[1], device, &table) ||
+      !tensor(o[2], device, &lens) || !tensor(o[3], device, &rows) || !tensor(o[4], device, &counts) || !tensor(o[5], device, &cu, true))
+    Py_RETURN_NONE;
+  const int d = cache->dim() == 4 ? 1 : 0;
+  if (table->dim() != 2 || !batch(a, cu ? INT32_MAX : table->size(0), *cache, *table, *lens, cu, d)) Py_RETURN_NONE;
+  const int64_t L = d ? cache->size(0) : 1;
+  if (L <= 0 || L > INT32_MAX || !indexes(*counts, a.batch) || rows->scalar_type() != at::kInt || rows->dim() != 2 ||
+      rows->size(0) != a.batch || rows->size(1) <= 0 || rows->size(1) > INT32_MAX || (rows->stride(1) != 1 && rows->size(1) > 1))
+    Py_RETURN_NONE;
+  const int64_t width = rows->size(1), stride = a.batch > 1 ? rows->stride(0) : width;
+  if (stride < width) Py_RETURN_NONE;
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = p_keep(&a, (int32_t)L, L > 1 ? cache->stride(0) : 0, (const int32_t*)rows->data_ptr(), stride, (int32_t)width,
+                (const int32_t*)counts->data_ptr(), (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(logits, tokens, parents, uniforms, cu_seqlens, draft_probs, temperature, max_new, max_depth, device, stream)
+// -> path, counts, next_tokens
+PyObject* verify(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t device, stream, width, depth = INT32_MAX;
+  const at::Tensor *x, *tokens, *up, *u, *cu, *probs, *temps = nullptr;
+  shard_verify_args a{};
+  if (!p_verify || n != 11 || !integer(o[9], &device) || !integer(o[10], &stream) || !tensor(o[0], device, &x) || !tensor(o[1], device, &tokens) ||
+      !tensor(o[2], device, &up) || !tensor(o[3], device, &u) || !tensor(o[4], device, &cu, true) || !tensor(o[5], device, &probs, true) ||
+      (o[8] != Py_None && !integer(o[8], &depth)) || depth < 0)
+    Py_RETURN_NONE;
+  const auto type = x->scalar_type();
+  const int code = type == at::kFloat ? SHARD_FP32 : half_code(*x);
+  if (code < 0 || x->dim() != 2 || x->size(0) <= 0 || x->size(0) > INT32_MAX || x->size(1) <= 0 || x->stride(1) != 1 || x->stride(0) < 0)
+    Py_RETURN_NONE;
+  const int64_t T = x->size(0), V = x->size(1);
+  if (tokens->scalar_type() != at::kLong || tokens->dim() != 1 || tokens->size(0) != T || !tokens->is_contiguous() || !indexes(*up, T) ||
+      u->scalar_type() != at::kFloat || u->dim() != 2 || u->size(0) != T || u->size(1) != 2 || !u->is_contiguous() ||
+      (cu && (cu->dim() != 1 || cu->size(0) < 2 || !indexes(*cu, cu->size(0)))) || !tree_width(o[7], T, &width))
+    Py_RETURN_NONE;
+  if (probs && (probs->scalar_type() != at::kFloat || probs->dim() != 2 || probs->size(0) != T || probs->size(1) != V ||
+                probs->stride(1) != 1 || probs->stride(0) < 0))
+    Py_RETURN_NONE;
+  const int64_t B = cu ? cu->size(0) - 1 : T;
+  if (B > INT32_MAX) Py_RETURN_NONE;
+  if (PyFloat_CheckExact(o[6])) a.temperature = (float)PyFloat_AS_DOUBLE(o[6]);
+  else if (!tensor(o[6], device, &temps) || temps->scalar_type() != at::kFloat || temps->dim() != 1 || temps->size(0) != B || !temps->is_contiguous())
+    Py_RETURN_NONE;
+  a.batch = (int32_t)B;
+  a.n_tokens = (int32_t)T;
+  a.vocab = V;
+  a.logits = x->data_ptr();
+  a.row_stride = x->stride(0);
+  a.dtype = code;
+  a.width = (int32_t)width;
+  a.tokens = (const int64_t*)tokens->data_ptr();
+  a.parents = (const int32_t*)up->data_ptr();
+  a.uniforms = (const float*)u->data_ptr();
+  a.cu_seqlens = cu ? (const int32_t*)cu->data_ptr() : nullptr;
+  a.draft_probs = probs ? (const float*)probs->data_ptr() : nullptr;
+  a.probs_stride = probs ? probs->stride(0) : 0;
+  a.temperatures = temps ? (const float*)temps->data_ptr() : nullptr;
+  a.max_depth = (int32_t)std::min<int64_t>(depth, INT32_MAX);
+  const int64_t one[1] = {B}, two[2] = {B, width};
+  at::Tensor path, counts, next;
+  int rc;
+  {
+    const Unlocked unlocked;
+    path = make(two, *x, at::kInt);
+    counts = make(one, *x, at::kInt);
+    next = make(one, *x, at::kLong);
+    a.path = (int32_t*)path.data_ptr();
+    a.counts = (int32_t*)counts.data_ptr();
+    a.next = (int64_t*)next.data_ptr();
+    const size_t need = p_verify_workspace(&a);
+    const c10::DataPtr ws = scratch(need);
+    rc = p_verify(&a, ws.get(), need, (void*)stream);
+  }
+  if (rc) Py_RETURN_NONE;
+  return Py_BuildValue("NNN", THPVariable_Wrap(std::move(path)), THPVariable_Wrap(std::move(counts)), THPVariable_Wrap(std::move(next)));
   END_HANDLE_TH_ERRORS
 }
 
@@ -288,6 +437,22 @@ PyObject* bind(PyObject*, PyObject* path) {
   p_attn = (decltype(p_attn))f[3];
   p_logprobs_workspace = (decltype(p_logprobs_workspace))f[4];
   p_logprobs = (decltype(p_logprobs))f[5];
+  // drafted tokens: all or none of them
+  const char* const more[] = {"shard_kv4_append_at", "shard_kv4_tree_attn_workspace", "shard_kv4_tree_attn", "shard_kv4_keep",
+                              "shard_draft_tree", "shard_verify_drafts_workspace", "shard_verify_drafts"};
+  constexpr int N = sizeof(more) / sizeof(more[0]);
+  void* g[N];
+  const auto verify_size = (decltype(&shard_verify_args_size))dlsym(lib, "shard_verify_args_size");
+  bool all = verify_size && verify_size() == sizeof(shard_verify_args);
+  for (int i = 0; i < N; ++i) all = (g[i] = dlsym(lib, more[i])) && all;
+  for (int i = 0; i < N && !all; ++i) g[i] = nullptr;
+  p_append_at = (decltype(p_append_at))g[0];
+  p_tree_workspace = (decltype(p_tree_workspace))g[1];
+  p_tree_attn = (decltype(p_tree_attn))g[2];
+  p_keep = (decltype(p_keep))g[3];
+  p_tree = (decltype(p_tree))g[4];
+  p_verify_workspace = (decltype(p_verify_workspace))g[5];
+  p_verify = (decltype(p_verify))g[6];
   Py_RETURN_NONE;
 }
 
@@ -296,6 +461,10 @@ PyMethodDef methods[] = {
     {"kv4_append", (PyCFunction)(void*)append, METH_FASTCALL, nullptr},
     {"kv4_read", (PyCFunction)(void*)read, METH_FASTCALL, nullptr},
     {"kv4_attn", (PyCFunction)(void*)attn, METH_FASTCALL, nullptr},
+    {"kv4_tree_attn", (PyCFunction)(void*)attn, METH_FASTCALL, nullptr},
+    {"draft_tree", (PyCFunction)(void*)tree, METH_FASTCALL, nullptr},
+    {"kv4_keep", (PyCFunction)(void*)keep, METH_FASTCALL, nullptr},
+    {"verify_drafts", (PyCFunction)(void*)verify, METH_FASTCALL, nullptr},
     {"token_logprobs", (PyCFunction)(void*)logprobs, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1099,9 +1099,9 @@ def kv4_append(k, v, cache, block_table, seq_lens, phases, q=None, cu_seqlens=No
     place (draft_tree's: drafted tokens that are siblings); a row whose position
     is negative or not below P is left out."""
     direct = _direct or _bind_direct()
-    if direct and positions is None and k.is_cuda:
+    if direct and k.is_cuda:
         dev = _current_device()
-        done = direct.kv4_append(k, v, cache, block_table, seq_lens, phases, q, cu_seqlens, max_new, dev, _raw_stream(dev))
+        done = direct.kv4_append(k, v, cache, block_table, seq_lens, phases, q, cu_seqlens, max_new, positions, dev, _raw_stream(dev))
         if done is not None:
             return None if q is None else done
     lib, T = _lib.load(), k.shape[0]
@@ -1251,6 +1251,12 @@ def draft_tree(parents, seq_lens, cu_seqlens=None, max_new=None):
     ancestors and itself.  Its position is its parent's + 1.  max_new, the most
     rows of a sequence (all rows where None; at most TREE_ROWS_MAX), is a bound: W
     holds as many, rows from 64 W on see no row and have position -1."""
+    direct = _direct or _bind_direct()
+    if direct and parents.is_cuda:
+        dev = _current_device()
+        done = direct.draft_tree(parents, seq_lens, cu_seqlens, max_new, dev, _raw_stream(dev))
+        if done is not None:
+            return done
     lib, T = _lib.load(), parents.shape[0] if parents.dim() else 0
     _require_gpu(parents, seq_lens, cu_seqlens)
     dev, B = parents.get_device(), seq_lens.shape[0] if seq_lens.dim() else 0
@@ -1273,6 +1279,12 @@ def kv4_tree_attn(q, cache, block_table, seq_lens, mask, cu_seqlens=None, scale=
     mask (T, W) int64 of draft_tree, or any bits: rows that a mask has no bit for
     are not seen, the row itself included.  Everything else as in kv4_attn; rows
     that see nothing are zeros."""
+    direct = _direct or _bind_direct()
+    if direct and out is None and mask is not None and q.is_cuda:
+        dev = _current_device()
+        done = direct.kv4_tree_attn(q, cache, block_table, seq_lens, cu_seqlens, scale, max_new, max_len, mask, dev, _raw_stream(dev))
+        if done is not None:
+            return done
     if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != q.shape[0] or mask.shape[1] < 1 or not mask.is_contiguous():
         raise TypeError(f"mask: expected ({q.shape[0]}, words) contiguous int64, got {tuple(mask.shape)} {mask.dtype}")
     return _kv4_attn(q, cache, block_table, seq_lens, mask, cu_seqlens, scale, out, max_new, max_len)
@@ -1292,6 +1304,11 @@ def kv4_keep(cache, block_table, seq_lens, rows, counts, cu_seqlens=None):
     seq_lens[b] less its rows, plus counts[b], tokens afterwards, and what lies
     behind them is no longer used.  Two sequences of one call must not share a
     page that holds rows of the step."""
+    direct = _direct or _bind_direct()
+    if direct and cache.is_cuda:
+        dev = _current_device()
+        if direct.kv4_keep(cache, block_table, seq_lens, rows, counts, cu_seqlens, dev, _raw_stream(dev)):
+            return
     layers = cache.unsqueeze(0) if cache.dim() == 3 else cache
     if layers.dim() != 4 or layers.shape[0] < 1:
         raise TypeError("cache: expected the (pages, kv heads, 68 * head_dim) uint8 of kv4_cache, or layers of them")
@@ -1343,6 +1360,13 @@ def verify_drafts(logits, tokens, parents, uniforms, cu_seqlens=None, draft_prob
     TREE_ROWS_MAX): those behind it are not looked at.  next_tokens is -1 where the
     walk ends at a row of NaN, +inf (unless greedy) or no logit above -inf, or a
     sequence has no rows.  Tokens outside the vocabulary are never accepted."""
+    direct = _direct or _bind_direct()
+    if direct and logits.is_cuda:
+        dev = _current_device()
+        done = direct.verify_drafts(logits, tokens, parents, uniforms, cu_seqlens, draft_probs, temperature, max_new, max_depth, dev,
+                                    _raw_stream(dev))
+        if done is not None:
+            return done
     lib = _lib.load()
     temps = temperature if isinstance(temperature, torch.Tensor) else None
     _require_gpu(logits, tokens, parents, uniforms, cu_seqlens, draft_probs, temps)

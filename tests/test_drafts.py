@@ -103,6 +103,25 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_compiled_dispatch_leaves_odd_calls():
+    """None (the way through ops.py) for operands that it does not take."""
+    from shard_amd import _lib, ops
+    _lib.load()
+    d = ops._bind_direct()
+    assert d
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    c, q = ops.kv4_cache(2, 2, 64, device="cpu"), torch.zeros(1, 2, 64, dtype=torch.float16)
+    for bad in ((), (None,) * 11, (q, c, i32(1, 2), i32(1), None, None, None, None, torch.ones(1, 1, dtype=torch.int64), 0, 0)):
+        assert d.kv4_tree_attn(*bad) is None
+    assert d.kv4_append(q, q, c, i32(1, 2), i32(1), torch.zeros(128, 32, 2), None, None, None, i32(1), 0, 0) is None
+    for bad in ((), (None,) * 6, (i32(1), i32(1), None, None, 0, 0)):
+        assert d.draft_tree(*bad) is None
+    for bad in ((), (None,) * 8, (c, i32(1, 2), i32(1), i32(1, 3), i32(1), None, 0, 0)):
+        assert d.kv4_keep(*bad) is None
+    for bad in ((), (None,) * 11, (torch.zeros(1, 5), torch.zeros(1, dtype=torch.int64), i32(1), torch.zeros(1, 2), None, None, 1.0, None, None, 0, 0)):
+        assert d.verify_drafts(*bad) is None
+
+
 # ---------------------------------------------------------------------------
 # PagedCache
 # ---------------------------------------------------------------------------

@@ -467,6 +467,39 @@ def test_a_step_captured(cuda):
         assert bool(torch.randn(64, device=cuda).isfinite().all())
 
 
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+def test_compiled_and_plain_dispatch_agree(cuda, type, monkeypatch):
+    """The compiled way and the one through Python give the same bits, and the compiled one takes plain calls."""
+    from shard_amd import ops
+    results = []
+    for direct in (ops._bind_direct(), False):
+        monkeypatch.setattr(ops, "_direct", direct)
+        b = Trees([300, 64, 90], [20, 1, 33], 8, 2, 128, type, seed=16).fill()
+        g = torch.Generator().manual_seed(1)
+        logits, tokens = torch.randn(54, 500, generator=g).to(b.type).to(cuda) * 3, torch.randint(0, 500, (54,), generator=g).to(cuda)
+        u, probs = torch.rand(54, 2, generator=g).to(cuda), torch.softmax(torch.randn(54, 600, generator=g), -1).to(cuda)[:, :500]
+        temps = torch.tensor([0.0, 1.0, 0.6], device=cuda)
+        verify = lambda **kw: ops.verify_drafts(logits, tokens, b.d_parents, u, cu_seqlens=b.d_cu, **kw)
+        b.plan()
+        q = b.append(q=b.d_q, positions=b.positions)
+        res = [b.mask, b.positions, *ops.draft_tree(b.d_parents, b.d_lens, cu_seqlens=b.d_cu), q, b.d_cache.clone(), b.tree_attn(),
+               b.tree_attn(scale=0.3, max_new=33), *verify(), *verify(temperature=temps, max_new=33), *verify(draft_probs=probs, max_depth=2)]
+        path, counts, _ = verify(temperature=0.0, max_new=33)
+        pool = torch.stack([b.d_cache, b.d_cache])
+        ops.kv4_keep(pool, b.d_table, b.d_lens, path, counts, cu_seqlens=b.d_cu)
+        ops.kv4_keep(b.d_cache, b.d_table, b.d_lens, path[:, :9], counts, cu_seqlens=b.d_cu)
+        results.append(res + [path, counts, pool, b.d_cache])
+        if direct:
+            dev, none = torch.cuda.current_device(), None
+            assert direct.kv4_tree_attn(b.d_q, b.d_cache, b.d_table, b.d_lens, b.d_cu, none, 33, 300, b.mask, dev, 0) is not None
+            assert direct.draft_tree(b.d_parents, b.d_lens, b.d_cu, 33, dev, 0) is not None
+            assert direct.verify_drafts(logits, tokens, b.d_parents, u, b.d_cu, none, 1.0, none, none, dev, 0) is not None
+            assert direct.kv4_keep(pool, b.d_table, b.d_lens, path, counts * 0, b.d_cu, dev, 0) is not None
+            torch.cuda.synchronize()
+    for x, y in zip(*results):
+        assert x.dtype == y.dtype and x.shape == y.shape and torch.equal(x, y)
+
+
 def test_refusals(cuda):
     from shard_amd import ops
     b = Trees([70, 40], [5, 4], 4, 2, 64, seed=1)
