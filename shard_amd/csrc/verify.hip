@@ -21,8 +21,9 @@
 //                    sum exp2((x - M) log2(e) / t)
 //   k_verify_walk    a sequence a workgroup: the walk, then the part that the
 //                    answer lies in from the parts' sums, and in it the token
-// With draft_probs s is another function of every token after a rejection, so two
-// more launches sum its parts (k_verify_rest) and answer (k_verify_answer).  Many
+// With draft_probs s is another function of every token after a rejection: the walk
+// leaves its sum to k_verify_rest, which has the whole chip, and goes on in the next
+// launch; k_verify_answer finds the token.  Many
 // rows, few of which are on a path, go a launch a level instead (k_verify_level,
 // k_verify_end), and only the rows on the paths are read.
 #include <math.h>
@@ -43,10 +44,11 @@ struct Part {
   float most;    // the largest logit, NaN where one is
   int32_t at;    // greedy: of the largest logit, the first of equal ones
 };
-struct State {   // of a sequence whose walk has ended
+struct State {   // of a sequence whose walk has ended, or wants a sum
   double total;  // sum of the last row's weights
   float most;
   int32_t at, row, rejected;   // row -1: nothing to answer
+  int32_t count, wants, round; // of the path; wants what its rejections have left; when it was written
 };
 
 struct Level {   // of a sequence's walk, a launch a level
@@ -141,10 +143,11 @@ struct OpMaxOf { __device__ float operator()(float a, float b) const { return ma
 // A row's largest logit says whether it has a distribution: a greedy one may be +inf.
 __device__ __forceinline__ bool has_answer(float most, double rate) { return most > -INFINITY && (most < INFINITY || rate == 0.0); }
 
-// log2(e) / temperature of a sequence; 0: greedy.
+// log2(e) / temperature of a sequence; 0: greedy.  An infinite temperature leaves a
+// rate that tells masked tokens from the others.
 __device__ __forceinline__ double rate_of(const shard_verify_args& a, int b) {
   const float t = a.temperatures ? a.temperatures[b] : a.temperature;
-  return t > 0.f ? kLog2e / (double)t : 0.0;
+  return t > 0.f ? fmax(kLog2e / (double)t, 1e-300) : 0.0;
 }
 
 // The sequence that row r belongs to (any, where it is nobody's).
@@ -266,7 +269,7 @@ struct Shared {
   double amount[SHARD_TREE_ROWS];                        // Q: what they left; weights of the tokens
   double scan[kWalk / 64];
   State end;
-  int count, pick_part, found, last, wants;
+  int count, pick_part, found, last;
   float u;
   double target;
 };
@@ -317,31 +320,59 @@ struct Weights {
     if (Q && n > 0) probs(0, raw, raw.q);
     return raw;
   }
-  __device__ __forceinline__ double value(Raw& raw, double (&v)[4]) const {
+  // s of U quads, a rejected row for all of them after the other
+  template <int U>
+  __device__ __forceinline__ double values(Raw (&raw)[U], double (&v)[U][4]) const {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = scale(raw.x[k]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[u][k] = scale(raw[u].x[k]);
     if constexpr (Q) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] *= each;
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[u][k] *= each;
       for (int j = 0; j < n; ++j) {
-        const double left = j == n - 1 ? 1.0 : sh.amount[j];
-        if (j) probs(j, raw, raw.q);
+        const double left = j == n - 1 ? 1.0 : sh.amount[j], part = 1.0 / left;
+        if (j)
+#pragma unroll
+          for (int u = 0; u < U; ++u) probs(j, raw[u], raw[u].q);
         if (left > 0.0)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const double d = v[k] - (double)raw.q[k];
-            v[k] = d > 0.0 ? d : 0.0;
-            if (j < n - 1) v[k] /= left;
-          }
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const double d = v[u][k] - (double)raw[u].q[k];
+              v[u][k] = (d > 0.0 ? d : 0.0) * part;
+            }
       }
     } else {
       for (int j = 0; j < n; ++j) {
-        const int64_t gone = sh.rejected[j] - raw.e;
+        const int64_t token = sh.rejected[j];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = gone == k ? 0.0 : v[k];
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[u][k] = token - raw[u].e == k ? 0.0 : v[u][k];
       }
     }
-    return (v[0] + v[1]) + (v[2] + v[3]);
+    double sum = 0.0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum += (v[u][0] + v[u][1]) + (v[u][2] + v[u][3]);
+    return sum;
+  }
+  // of quads i0 + `at`, i0 + at + stride, ..., U of them on their way together
+  template <int U>
+  __device__ __forceinline__ double sum(int64_t i0, int64_t i1, int at, int stride) const {
+    double own = 0.0;
+#pragma unroll 1
+    for (int64_t i = i0; i < i1; i += U * stride) {
+      Raw raw[U];
+      double v[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = fetch(i + u * stride + at, i1);
+      own += values(raw, v);
+    }
+    return own;
   }
 };
 
@@ -360,13 +391,8 @@ __device__ __forceinline__ double scan(double v, Shared& sh, double& all) {
 // The sum of a row's weights.
 template <class T, bool Q>
 __device__ __forceinline__ double sum_of(const Weights<T, Q>& weights, int64_t i0, int64_t i1, Shared& sh) {
-  double own = 0.0, all;
-#pragma unroll 1
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += kWalk) {
-    double v[4];
-    auto raw = weights.fetch(i, i1);
-    own += weights.value(raw, v);
-  }
+  double all;
+  const double own = weights.template sum<Q ? 3 : 4>(i0, i1, threadIdx.x, kWalk);   // 4 with Q: spills
   scan(own, sh, all);
   return all;
 }
@@ -480,6 +506,7 @@ __device__ __forceinline__ void ended(const shard_verify_args& a, const Nodes& n
     sh.end.at = j.at;
     sh.end.row = none ? -1 : rows.first + cur;
     sh.end.rejected = rejected;
+    sh.end.wants = 0;
     sh.count = count;
     sh.u = rows.n > 0 ? nodes.after[cur] : 0.f;
     a.counts[b] = count;
@@ -490,12 +517,13 @@ __device__ __forceinline__ void ended(const shard_verify_args& a, const Nodes& n
 }
 
 // The walk.  Wave 0 decides; for Q the whole workgroup sums what a rejection has
-// left where another child comes after it.  Leaves sh.end, the rejected rows (tokens)
-// of the last row, and for Q what each but the last left.  Returns the lane's part
-// of the last row (wave 0).
+// left where another child comes after it, or (not `last`) leaves that to another
+// launch and goes on `from` there.  Leaves sh.end, the rejected rows (tokens) of the
+// last row, and for Q what each but the last left.  Returns the lane's part of the
+// last row (wave 0).
 template <class T, bool Q>
 __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyWork& w, Nodes& nodes, Shared& sh, Part (&held_stats)[kHeld],
-                                       int b, double rate) {
+                                       int b, double rate, const State* from, bool last) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Rows rows = rows_of(a, b);
   const int c0 = rows.first, n = rows.n;
@@ -512,6 +540,18 @@ __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyW
   Joined j{0.0, 0.0, 0.f, -1};
   bool none = n == 0, wants = false;
   int known = 0;                                        // Q: rejections of the row whose sums are known
+  if (Q && from) {
+    cur = from->row - c0;
+    count = from->count;
+    known = from->rejected;
+    for (int k = tid; k < known; k += kWalk) sh.amount[k] = w.left[c0 + k];
+    if (wave == 0) {
+      j = join((held ? held_stats : stats) + cur * w.parts, w.parts, rate, lane);
+      const double left = wave_sum(lane < w.parts ? w.rest[(int64_t)b * w.parts + lane] : 0.0);
+      if (lane == 0) sh.amount[known - 1] = left;       // wave 0 has written it before, where it has
+    }
+    __syncthreads();
+  }
   do {
     if (wave == 0) {
       bool on = !none;
@@ -530,13 +570,13 @@ __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyW
         }
       }
       if (Q && lane == 0) {
-        sh.end = State{j.sum, j.most, j.at, c0 + cur, rejected};
-        sh.wants = wants;
+        sh.end = State{j.sum, j.most, j.at, c0 + cur, rejected, count, wants, 0};
       }
     }
     if constexpr (Q) {
       __syncthreads();
-      wants = sh.wants;
+      wants = sh.end.wants;
+      if (wants && !last) return j.mine;                // k_verify_rest sums it
       if (wants) {                                      // what the last rejection left, and the turn once more
         known = sh.end.rejected;
         const Weights<T, Q> weights(a, sh, c0, sh.end.row, rate, known);
@@ -599,16 +639,16 @@ __device__ __forceinline__ void answer(const shard_verify_args& a, const VerifyW
   double base = 0.0;
 #pragma unroll 1
   for (int64_t at = i0; at < i1; at += kWalk) {
-    double v[4], all;
-    auto raw = weights.fetch(at + tid, i1);
-    const double own = weights.value(raw, v);
+    double v[1][4], all;
+    typename Weights<T, Q>::Raw raw[1] = {weights.fetch(at + tid, i1)};
+    const double own = weights.values(raw, v);
     double run = base + scan(own, sh, all);
     // the first element at which the running sum is above the target, else the last that has any
     int pick = -1, some = -1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      run += v[k];
-      if (v[k] > 0.0) {
+      run += v[0][k];
+      if (v[0][k] > 0.0) {
         some = (int)(4 * (at + tid) - weights.r.mis + k);
         if (run > target && pick < 0) pick = some;
       }
@@ -699,22 +739,33 @@ void k_verify_end(const shard_verify_args a, const VerifyWork w, int levels) {
 
 template <class T, bool Q>
 __global__ __launch_bounds__(kWalk)
-void k_verify_walk(const shard_verify_args a, const VerifyWork w) {
+void k_verify_walk(const shard_verify_args a, const VerifyWork w, int round, bool last) {
   __shared__ Part stats[kHeld];
   __shared__ Nodes nodes;
   __shared__ Shared sh;
   const int tid = threadIdx.x, b = blockIdx.x;
   const double rate = rate_of(a, b);
-  const double mine = walk<T, Q>(a, w, nodes, sh, stats, b, rate);
   const int c0 = rows_of(a, b).first;
   if constexpr (Q) {
+    State from;
+    if (round) {
+      from = w.state[b];
+      if (!from.wants) return;
+    }
+    walk<T, Q>(a, w, nodes, sh, stats, b, rate, round ? &from : nullptr, last);
+    __syncthreads();
     const State end = sh.end;
-    if (tid == 0) w.state[b] = end;
-    if (tid < end.rejected) {
-      w.rejected[c0 + tid] = sh.rejected[tid];
-      w.left[c0 + tid] = tid < end.rejected - 1 ? sh.amount[tid] : 0.0;
+    if (tid == 0) {
+      sh.end.count = sh.end.wants ? end.count : sh.count;
+      sh.end.round = round;
+      w.state[b] = sh.end;
+    }
+    for (int k = tid; k < end.rejected; k += kWalk) {
+      w.rejected[c0 + k] = sh.rejected[k];
+      w.left[c0 + k] = k < end.rejected - 1 ? sh.amount[k] : 0.0;
     }
   } else {
+    const double mine = walk<T, Q>(a, w, nodes, sh, stats, b, rate, nullptr, true);
     answer<T, Q>(a, w, sh, b, c0, rate, mine);
   }
 }
@@ -736,29 +787,17 @@ __device__ __forceinline__ void end_of(const shard_verify_args& a, const VerifyW
 
 template <class T>
 __global__ __launch_bounds__(kThreads)
-void k_verify_rest(const shard_verify_args a, const VerifyWork w) {
+void k_verify_rest(const shard_verify_args a, const VerifyWork w, int round) {
   __shared__ Shared sh;
   const int part = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, c0 = rows_of(a, b).first;
   const double rate = rate_of(a, b);
   end_of(a, w, sh, b, c0);
-  if (sh.end.row < 0 || rate == 0.0 || part >= w.parts) return;
+  if (sh.end.round != round || sh.end.row < 0 || rate == 0.0 || part >= w.parts) return;
   const Weights<T, true> weights(a, sh, c0, sh.end.row, rate, sh.end.rejected);
   constexpr int kQuads = Row<T>::VEC / 4;
   const int64_t i1 = min((part + 1) * w.granules, weights.r.count) * kQuads;
-  double own = 0.0;
-  constexpr int U = 4;   // on their way together
-#pragma unroll 1
-  for (int64_t i = part * w.granules * kQuads; i < i1; i += 64 * U) {
-    typename Weights<T, true>::Raw raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = weights.fetch(i + 64 * u + lane, i1);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      double v[4];
-      own += weights.value(raw[u], v);
-    }
-  }
+  double own = weights.template sum<4>(part * w.granules * kQuads, i1, lane, 64);
   own = wave_sum(own);
   if (lane == 0) w.rest[(int64_t)b * w.parts + part] = own;
 }
@@ -786,6 +825,17 @@ int levels_of(const shard_verify_args* a) {
   if (a->draft_probs) return 0;   // a turn may take sums over the row
   const int64_t levels = (int64_t)(a->max_depth < a->width - 1 ? a->max_depth : a->width - 1) + 1;
   return (a->n_tokens - 3 * (int64_t)a->batch) * a->vocab > 2500000 * levels ? (int)levels : 0;
+}
+
+// With draft_probs: launches of the walk, each with one that sums what rejections
+// have left; a walk that wants more sums than they give takes them in its one
+// workgroup (50 us and more each, the launches 15, 5 where nobody wants them).  A
+// chain, whose depth is its rows, wants none; trees most often up to two.  128,256
+// tokens, the first of 4 children accepted / all 4 rejected, us: one sequence 23.6 / 154
+// with two launches, 28.5 / 126 with three; 16 sequences 37.1 / 191, 42.2 / 159.
+int rounds_of(const shard_verify_args* a) {
+  const int spare = a->width - 1 - (a->max_depth < a->width - 1 ? a->max_depth : a->width - 1);
+  return 1 + (spare < 2 ? spare : 2);
 }
 
 bool plan(const shard_verify_args* a, VerifyWork& w, size_t& bytes) {
@@ -823,11 +873,14 @@ static void launch_verify(const shard_verify_args& a, const VerifyWork& w, hipSt
   }
   hipLaunchKernelGGL(k_verify_stats<T>, dim3((unsigned)a.n_tokens, groups), dim3(kThreads), 0, s, a, w);
   if (a.draft_probs) {
-    hipLaunchKernelGGL((k_verify_walk<T, true>), dim3(a.batch), dim3(kWalk), 0, s, a, w);
-    hipLaunchKernelGGL(k_verify_rest<T>, dim3(groups, a.batch), dim3(kThreads), 0, s, a, w);
+    const int rounds = rounds_of(&a);
+    for (int i = 0; i < rounds; ++i) {
+      hipLaunchKernelGGL((k_verify_walk<T, true>), dim3(a.batch), dim3(kWalk), 0, s, a, w, i, i == rounds - 1);
+      hipLaunchKernelGGL(k_verify_rest<T>, dim3(groups, a.batch), dim3(kThreads), 0, s, a, w, i);
+    }
     hipLaunchKernelGGL(k_verify_answer<T>, dim3(a.batch), dim3(kWalk), 0, s, a, w);
   } else {
-    hipLaunchKernelGGL((k_verify_walk<T, false>), dim3(a.batch), dim3(kWalk), 0, s, a, w);
+    hipLaunchKernelGGL((k_verify_walk<T, false>), dim3(a.batch), dim3(kWalk), 0, s, a, w, 0, true);
   }
 }
 
@@ -868,7 +921,7 @@ int shard_verify_drafts(const shard_verify_args* a, void* workspace, size_t work
   const hipStream_t s = (hipStream_t)stream;
   if (a->n_tokens == 0) {
     // sequences of no rows: nothing is read
-    hipLaunchKernelGGL((k_verify_walk<half_t, false>), dim3(a->batch), dim3(kWalk), 0, s, *a, w);
+    hipLaunchKernelGGL((k_verify_walk<half_t, false>), dim3(a->batch), dim3(kWalk), 0, s, *a, w, 0, true);
   } else if (a->dtype == SHARD_FP16) {
     launch_verify<half_t>(*a, w, s);
   } else if (a->dtype == SHARD_BF16) {

@@ -105,6 +105,19 @@ def test_many_children(cuda):
     c.check()
 
 
+def test_extreme_temperatures(cuda):
+    """Nearly greedy, nearly uniform, and an infinite one: every token that is not masked alike."""
+    for probs in (False, True):
+        for t in (1e-3, 1e-30, 1e6, 1e30):
+            Case([6, 3], 200, "fp32", probs, t, seed=3).check()
+    c = Case([5] * 8, 200, "fp32", temperature=[float("inf")] * 8, seed=4)
+    c.logits[:, 50:] = -torch.inf
+    path, counts, following = c.run()
+    c.temperature, c.logits[:, :50] = [1.0] * 8, 0.0
+    want = c.check()
+    assert [(p[:n], t) for p, n, t in zip(path.tolist(), counts.tolist(), following.tolist())] == want
+
+
 def test_temperatures_of_each_sequence(cuda):
     """Greedy and sampling sequences in one call, more than a wave's lanes of them, empty ones among them."""
     new = [(3 * i) % 5 for i in range(150)]
@@ -193,6 +206,38 @@ def test_a_launch_a_level(cuda, type):
     chain = Case([6] * 60, 40009, type, temperature=0.7, seed=8, width=1)
     chain.uniforms[:, 0] = 0.0
     assert max(len(p) for p, _ in chain.check(max_depth=3)) == 4
+
+
+@pytest.mark.parametrize("what", ["rows", "levels", "probs"])
+def test_captured(cuda, what):
+    """All three ways, captured and replayed with other inputs in the same memory."""
+    from shard_amd import ops
+    V, new = (40009, [6] * 60) if what == "levels" else (3001, [9, 4, 0, 30])
+    B, T = len(new), sum(new)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    cu, g = i32([0] + np.cumsum(new).tolist()), torch.Generator(device="cuda").manual_seed(1)
+
+    def inputs(seed):
+        x = torch.randn(T, V, generator=g, device=cuda) * 4
+        return [x.bfloat16(), torch.randint(0, V, (T,), generator=g, device=cuda), i32(random_parents(new, seed)),
+                torch.rand(T, 2, generator=g, device=cuda) * 0.3, torch.softmax(x * 1.1, -1), torch.rand(B, generator=g, device=cuda)]
+    call = lambda x, tok, up, u, q, t: ops.verify_drafts(x, tok, up, u, cu_seqlens=cu, draft_probs=q if what == "probs" else None,
+                                                         temperature=t, max_new=30, max_depth=3)
+    held = inputs(0)
+    call(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call(*held)
+    for seed in range(1, 5):
+        new_in = inputs(seed)
+        want = call(*new_in)
+        for dst, src in zip(held, new_in):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert bool(torch.randn(64, device=cuda).isfinite().all())
 
 
 @pytest.mark.parametrize("probs", [False, True], ids=["chosen", "drawn"])
