@@ -7,7 +7,8 @@
 //
 // Host time of a call beside one MI355X, launches included, us, here / through
 // ops.py: kv4_append with q 4.8 / 10.1, kv4_read 5.3 / 8.4, kv4_attn (two launches)
-// 8.1 / 13.5, token_logprobs (two launches) 9.0 / 16.5.
+// 8.1 / 13.5, token_logprobs (two launches) 9.0 / 16.5, kv4_tree_attn 8.6 / 15.2,
+// verify_drafts 8.2 / 16.6, draft_tree, kv4_append and kv4_keep together 27-30 / 43.
 #include <Python.h>
 #include <dlfcn.h>
 

@@ -1313,7 +1313,8 @@ void k_kv4_merge(const shard_kv4_args a, const AttnWork w) {
 // --------------------------------------------------------------------------
 // A step's plan: which of its sequence's rows a drafted token sees, and where it
 // stands.  A row's ancestors have falling indices, so its words are written from
-// the last to the first as the walk up its parents passes them.
+// the last to the first as the walk up its parents passes them.  8 rows 1.5 us,
+// 1,196 rows of 64 sequences 4.6: a launch, and as many LDS reads as the tree is deep.
 // --------------------------------------------------------------------------
 struct TreeArgs {
   const int32_t* parents;
@@ -1361,6 +1362,8 @@ void k_draft_tree(const TreeArgs t) {
 // holds those of a channel (and 4 others), so it is read, merged and written once.
 // rows[j] >= j, so a place is read before or in the round that writes it, and what
 // a round writes of words that later ones read are the nibbles that were there.
+// 6,048 tokens (64 sequences in 32 layers, 8 heads of 128): 19 us for 13 MB, the
+// chain rows -> table -> words -> write of a workgroup with 3 tokens; one sequence 3.2.
 // --------------------------------------------------------------------------
 struct KeepArgs {
   int64_t layer_stride;
