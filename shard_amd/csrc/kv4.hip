@@ -134,6 +134,50 @@ __device__ __forceinline__ float to_odd(double d) {
   return __uint_as_float(u);
 }
 
+// 1 / s of a scale, rounded correctly: one Newton step, and 1 / 1.25, 1 / 1.5 and
+// 1 / 1.75 are far from the middle between two numbers.
+__device__ __forceinline__ float inverse(float s) {
+  const float r = __builtin_amdgcn_rcpf(s);
+  return fmaf(fmaf(-s, r, 1.0f), r, r);
+}
+
+// E2M1 codes of 8 numbers at scale s, r = 1 / s, as code4's, in 28 instructions (code4:
+// 14 each); neither infinities nor NaN, nor anything between 0 and 2^-133.  The quotient
+// is rounded correctly (Markstein: the remainder of x r is exact), and nothing is rounded
+// across a border, or onto it: borders and scales have 3 bits, so the quotient of the
+// number next to border s differs from the border by 4/7 of a step or more.  The
+// conversion rounds to the nearest, ties to the even code, and saturates.  x = -0: the
+// remainder is +0, and so is the quotient.
+__device__ __forceinline__ uint32_t codes8(const float (&x)[8], float s, float r) {
+  float q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float q0 = x[j] * r;
+    q[j] = fmaf(fmaf(-q0, s, x[j]), r, q0);
+  }
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.0f, 3);
+  return w;
+}
+// any other numbers
+__device__ __forceinline__ uint32_t codes8_any(const float (&x)[8], float s) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w |= code4(x[j], s) << (4 * j);
+  return w;
+}
+
+// Bit i of 8 as nibble i, all ones or 0.
+__device__ __forceinline__ uint32_t nibbles(uint32_t x) {
+  x = (x | x << 12) & 0x000f000fu;
+  x = (x | x << 6) & 0x03030303u;
+  x = (x | x << 3) & 0x11111111u;
+  return x * 15u;
+}
+
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, dpp_mov<kDppXor1>(v));
   return fmaxf(v, dpp_mov<kDppXor2>(v));
@@ -167,9 +211,8 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // come out as the formula's.  The products are exact there and the sum rounds
 // once, so nothing depends on contraction.
 // Measured (32 query heads on 8, head_dim 128, fp16): four prompts of 8,192
-// tokens 179 us, 4.0 TB/s of the 724 MB it reads and writes (a large copy: 4.75),
-// the vector pipe half busy with K's 64-bit rotation and the roundings; one token
-// 6 us.  That is not its chain of memory accesses (arguments, length, table, page,
+// tokens 168 us, 4.3 TB/s of the 724 MB it reads and writes (a large copy: 4.75 to
+// 5.0; 179 with code4 for every number); one token 5 to 6 us.  That is not its chain of memory accesses (arguments, length, table, page,
 // store): the read has the same and takes 3.2.  Most likely it is the serial work of
 // few lanes: 8 threads rotate, round and code 16 elements of K each, and 8 of a
 // query workgroup take 4 heads one after the other.
@@ -177,12 +220,16 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 constexpr int kHeadsQ = 4;
 
 // AT: a row is rotated at positions[row] instead of its own place (drafted tokens
-// of a tree: siblings have places of their own and one position).
+// of a tree: siblings have places of their own and one position).  64 trees of 13 to 26
+// tokens in 32 layers, 38,272 rows of 8 heads of 128: 177 us (code4: 217), of 25,600
+// workgroups with 12 rows each; a workgroup waits 3 us for the chain length ->
+// position -> phases and its store.  Not faster: dense rows, K and V apart (226 against 219),
+// more heads a workgroup (253), six waves a SIMD instead of four (spills, 314).
 template <class T, int D, bool AT>
 __global__ __launch_bounds__(256, 4)
 void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions) {
   constexpr int PB = D / 64;  // pairs of 32-channel blocks: (pb, pb + PB)
-  __shared__ __align__(4) uint8_t codes[32][D + 4];
+  __shared__ __align__(4) uint8_t codes[32][D / 2 + 4];  // of V, two channels a byte
   const int tid = threadIdx.x, b = blockIdx.z;
   const Seq s = seq_of(a, b);
   if (s.n == 0) return;
@@ -198,11 +245,14 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
     const bool mine = tok < 32 && i >= 0 && i < s.n;
     const int turn = AT ? (mine ? positions[s.row0 + i] : -1) : pos;
     const bool there = mine && pos >= 0 && pos < s.cap && turn >= 0 && turn < a.n_phases;
-    uint32_t new_bits = 0;                          // AT: of the group's tokens
+    uint32_t fresh;                                 // the group's new tokens
     if constexpr (AT) {
       const int bit = threadIdx.x & 31, row = t0 + bit - start;
       const int at = row >= 0 && row < s.n ? positions[s.row0 + row] : -1;
-      new_bits = (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0 && at < a.n_phases && t0 + bit >= 0);
+      fresh = (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0 && at < a.n_phases && t0 + bit >= 0);
+    } else {
+      const int from = min(max(start - t0, 0), 32), to = min(max(min(s.len, a.n_phases) - t0, from), 32);
+      fresh = (uint32_t)(((1ull << to) - 1) & ~((1ull << from) - 1));
     }
     float c[8], sn[8];
     if (there) {
@@ -241,15 +291,16 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
     if (page < 0) continue;
     uint8_t* base = head_of<D>(a, page, g);
     const int slot0 = t0 & 63, slot = slot0 + tok;
-    const auto is_new = [&](int t) {
-      return AT ? (bool)(new_bits >> t & 1) : (unsigned)(t0 + t - start) < (unsigned)s.n && t0 + t < a.n_phases;
-    };
     // all that the group reads, before anything waits: k, v, and the words of V
     // codes that earlier tokens share
-    constexpr int VU = D / 64;                        // 8-channel pieces of V a thread, words a thread
+    constexpr int VU = D / 64;                        // 8-channel pieces of V a thread
     typedef T vec8 __attribute__((ext_vector_type(8)));
     vec8 kx{}, ky{}, vx[VU];
-    uint32_t old[VU], keep[VU];
+    // a thread's words of V codes: 8 tokens of channels vc, vc + 1
+    const int kq = tid / (D / 2), vc2 = tid % (D / 2) * 2;
+    const uint32_t keep = ~nibbles((fresh >> (4 * kq) & 15u) | (fresh >> (16 + 4 * kq) & 15u) << 4);
+    const bool words = kq < 4 && keep != ~0u;
+    uint32_t old[2] = {};
     if (there) {
       const T* k = (const T*)a.k + (int64_t)(s.row0 + i) * a.k_stride + (int64_t)g * a.k_head_stride + ch;
       kx = *(const vec8*)k;
@@ -258,21 +309,14 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
 #pragma unroll
     for (int n = 0; n < VU; ++n) {
       const int u = tid + 256 * n, vt = u / (D / 8), vc = (u % (D / 8)) * 8;
-      if (is_new(vt))
+      if (fresh >> vt & 1)
         vx[n] = *(const vec8*)((const T*)a.v + (int64_t)(s.row0 + t0 + vt - start) * a.v_stride + (int64_t)g * a.v_head_stride + vc);
     }
+    if (words && keep != 0)
 #pragma unroll
-    for (int n = 0; n < VU; ++n) {
-      const int u = tid + 256 * n, kq = u / D, vc = u % D;
-      keep[n] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (!is_new(16 * (e >> 2) + 4 * kq + (e & 3))) keep[n] |= 15u << (4 * e);
-      old[n] = 0;
-      if (keep[n] != 0 && keep[n] != ~0u) old[n] = *(const uint32_t*)(base + v_word_at<D>(slot0 >> 5, kq, vc));
-    }
+      for (int n = 0; n < 2; ++n) old[n] = *(const uint32_t*)(base + v_word_at<D>(slot0 >> 5, kq, vc2 + n));
     if (there) {
-      float r[2][8];
+      float r[2][8], least = INFINITY, odd = 0.f;     // odd: NaN where r has an infinity
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const double x = (double)(float)kx[j], y = (double)(float)ky[j];
@@ -280,7 +324,10 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
         const double dh = y * c[j] + x * sn[j];
         r[0][j] = dl == dl ? to_odd(dl) : 0.f;
         r[1][j] = dh == dh ? to_odd(dh) : 0.f;
+        least = fminf(fminf(least, fabsf(r[0][j])), fabsf(r[1][j]));
+        odd = fmaf(r[0][j], 0.f, fmaf(r[1][j], 0.f, odd));
       }
+      const bool plain = least >= 0x1p-100f && odd == 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float m = 0.f;
@@ -288,9 +335,7 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
         for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(r[half][j]));
         const unsigned sb = scale_byte(quad_max(m));
         const float sc = e5m2(sb);
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w |= code4(r[half][j], sc) << (4 * j);
+        const uint32_t w = plain ? codes8(r[half], sc, inverse(sc)) : codes8_any(r[half], sc);
         const int cc = half * (D / 2) + ch;
         *(uint32_t*)(base + k_code_at<D>(slot, cc / (D / 4)) + (cc % (D / 4)) / 2) = w;
         if (lq == 0) base[k_scale_at<D>(slot, cc / 32)] = (uint8_t)sb;
@@ -300,33 +345,41 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
 #pragma unroll
     for (int n = 0; n < VU; ++n) {  // quads of lanes share a block of 32 channels
       const int u = tid + 256 * n, vt = u / (D / 8), vc = (u % (D / 8)) * 8;
-      if (is_new(vt)) {
-        float x[8], m = 0.f;
+      if (fresh >> vt & 1) {
+        float x[8], m = 0.f, odd = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           x[j] = (float)vx[n][j];
-          x[j] = x[j] == x[j] ? x[j] : 0.f;
-          m = fmaxf(m, fabsf(x[j]));
+          m = fmaxf(m, fabsf(x[j]));                  // without NaN
+          odd = fmaf(x[j], 0.f, odd);
         }
         const unsigned sb = scale_byte(quad_max(m));
         const float sc = e5m2(sb);
-        uint32_t w[2] = {};
+        uint32_t w;
+        if (odd == 0.f) {
+          w = codes8(x, sc, inverse(sc));
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= code4(x[j], sc) << (8 * (j & 3));
-        *(uint32_t*)&codes[vt][vc] = w[0];
-        *(uint32_t*)&codes[vt][vc + 4] = w[1];
+          for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? x[j] : 0.f;
+          w = codes8_any(x, sc);
+        }
+        *(uint32_t*)&codes[vt][vc / 2] = w;
         if ((vc & 31) == 0) base[v_scale_at<D>(slot0 + vt, vc / 32)] = (uint8_t)sb;
       }
     }
     __syncthreads();
+    if (words) {
+      uint32_t even = 0, uneven = 0;                  // tokens 0, 2, 4, 6 and 1, 3, 5, 7, a byte each; whatever lies in others
 #pragma unroll
-    for (int n = 0; n < VU; ++n) {
-      const int u = tid + 256 * n, kq = u / D, vc = u % D;
-      if (keep[n] == ~0u) continue;
-      uint32_t w = 0;
+      for (int e = 0; e < 8; e += 2) {
+        const int t = 16 * (e >> 2) + 4 * kq + (e & 3);
+        even |= (uint32_t)codes[t][vc2 / 2] << (4 * e);
+        uneven |= (uint32_t)codes[t + 1][vc2 / 2] << (4 * e);
+      }
+      const uint32_t w[2] = {(even & 0x0f0f0f0fu) | (uneven << 4 & 0xf0f0f0f0u), (even >> 4 & 0x0f0f0f0fu) | (uneven & 0xf0f0f0f0u)};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w |= (codes[16 * (e >> 2) + 4 * kq + (e & 3)][vc] & 15u) << (4 * e);  // whatever lies in the others
-      *(uint32_t*)(base + v_word_at<D>(slot0 >> 5, kq, vc)) = (old[n] & keep[n]) | (w & ~keep[n]);
+      for (int n = 0; n < 2; ++n)
+        *(uint32_t*)(base + v_word_at<D>(slot0 >> 5, kq, vc2 + n)) = (old[n] & keep) | (w[n] & ~keep);
     }
     __syncthreads();
   }

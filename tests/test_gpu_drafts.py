@@ -537,3 +537,37 @@ def test_refusals(cuda):
     same = b.d_cache.unsqueeze(0).expand(2, -1, -1, -1)            # layers on each other
     with pytest.raises(ops.ShardHipError):
         ops.kv4_keep(same, b.d_table, b.d_lens, rows, counts, cu_seqlens=b.d_cu)
+
+
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+def test_append_at_every_border(cuda, type):
+    """Codes at the borders of every scale, and next to them: numbers of the type (V, and K at an angle of 0), and products that
+    lie beside a border by a unit of 2^-23 or less (K at cosines next to 1)."""
+    from shard_amd import ops
+    D, dt = 64, {"fp16": torch.float16, "bf16": torch.bfloat16}[type]
+    marks = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0])
+    rows = []
+    for s in kv4.SCALES:
+        x = torch.tensor(np.concatenate([marks * s, -marks * s])).to(dt)
+        x = x.where(x.double().abs() <= 6.5 * s, 0)
+        bits16 = x.view(torch.int16)
+        near = [x] + [(bits16 + step).view(dt) for step in (-1, 1)]      # the next numbers of the type (of 0: NaN and subnormal)
+        x = torch.cat([n.where(n.double().abs() <= 6.5 * s, 0) for n in near])
+        x = torch.cat([x, x[:14]]).view(2, 31)
+        top = torch.tensor([[6.25 * s], [-6.25 * s]]).to(dt)               # 4 significant bits: the block's scale is s
+        rows.append(torch.cat([x, top], 1).reshape(1, D))
+    rows = torch.stack(rows)
+    n = len(rows)
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    table = torch.arange((n + 63) // 64, dtype=torch.int32, device=cuda)[None]
+    for cos in (1.0, 1 + 2.0 ** -23, 1 - 2.0 ** -24, -1.0, -1 - 2.0 ** -23):
+        phases = torch.zeros(128, D // 2, 2)
+        phases[..., 0] = cos
+        cache = ops.kv4_cache(table.shape[1], 1, D, device=cuda)
+        d = rows.to(cuda)
+        ops.kv4_append(d, d, cache, table, lens, phases.to(cuda), cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device=cuda))
+        K, V = (t.reshape(-1, D)[:n] for t in kv4.held(cache.cpu().numpy()))
+        x = rows[:, 0].double().numpy()
+        assert np.array_equal(V, kv4.round4(x.reshape(n, 2, 32)).reshape(n, D))
+        want = kv4.round4((x * np.float64(np.float32(cos))).reshape(n, 2, 32)).reshape(n, D)
+        assert np.array_equal(K, want), (cos, np.argwhere(K != want)[:4])
