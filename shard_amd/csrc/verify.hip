@@ -549,11 +549,11 @@ __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyW
     cur = from->row - c0;
     count = from->count;
     known = from->rejected;
-    for (int k = tid; k < known; k += kWalk) sh.amount[k] = w.left[c0 + k];
+    for (int k = tid; k < known - 1; k += kWalk) sh.amount[k] = w.left[c0 + k];
     if (wave == 0) {
       j = join((held ? held_stats : stats) + cur * w.parts, w.parts, rate, lane);
       const double left = wave_sum(lane < w.parts ? w.rest[(int64_t)b * w.parts + lane] : 0.0);
-      if (lane == 0) sh.amount[known - 1] = left;       // wave 0 has written it before, where it has
+      if (lane == 0) sh.amount[known - 1] = left;
     }
     __syncthreads();
   }
