@@ -423,12 +423,12 @@ __device__ __forceinline__ void load_nodes(const shard_verify_args& a, Nodes& no
     const int64_t row = rows.first + i;
     const int p = a.parents[row];
     const int64_t t = a.tokens[row];
-    const float2 u = ((const float2*)a.uniforms)[row];
+    const float* u = a.uniforms + 2 * row;          // 4-byte aligned
     const bool child = p >= 0 && p < i, ok = child && t >= 0 && t < a.vocab;
     nodes.up[i] = child ? p : -1;
     nodes.token[i] = ok ? (int32_t)t : -1;
-    nodes.u[i] = u.x;
-    nodes.after[i] = u.y;
+    nodes.u[i] = u[0];
+    nodes.after[i] = u[1];
     nodes.logit[i] = ok ? (float)logits[p * a.row_stride + t] : -INFINITY;
     if (a.draft_probs) nodes.q[i] = ok ? a.draft_probs[row * a.probs_stride + t] : 0.f;
   }

@@ -350,3 +350,19 @@ def test_refusals(cuda):
     none = torch.zeros(0, dtype=torch.int32, device=cuda)
     path, counts, following = call(x[:0], tok[:0], none, u[:0], torch.zeros(3, dtype=torch.int32, device=cuda))
     assert counts.tolist() == [0, 0] and following.tolist() == [-1, -1]
+
+
+@pytest.mark.parametrize("probs", [False, True], ids=["chosen", "drawn"])
+def test_operands_within_larger_ones(cuda, probs):
+    """Uniforms, parents, offsets, tokens, temperatures and logits that begin at any element of a larger tensor."""
+    from shard_amd import ops
+    c = Case([6, 9], 777, "fp16", probs, temperature=[0.7, 1.3], seed=21)
+    want = c.run()
+
+    def within(t, dtype=None):
+        t = torch.as_tensor(t, dtype=dtype)
+        return torch.cat([torch.zeros(1, dtype=t.dtype), t.flatten()]).cuda()[1:].view(t.shape)
+    got = ops.verify_drafts(within(c.logits), within(c.tokens), within(c.parents, torch.int32), within(c.uniforms),
+                            cu_seqlens=within(c.cu, torch.int32), draft_probs=within(c.probs) if probs else None,
+                            temperature=within([0.7, 1.3], torch.float32), max_new=9)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
