@@ -212,10 +212,11 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // once, so nothing depends on contraction.
 // Measured (32 query heads on 8, head_dim 128, fp16): four prompts of 8,192
 // tokens 164 us, 4.4 TB/s of the 724 MB it reads and writes (a large copy: 4.75 to
-// 5.0; 179 with code4 for every number); one token 5 us.  That is not its chain of memory accesses (arguments, length, table, page,
-// store): the read has the same and takes 3.2.  Most likely it is the serial work of
-// few lanes: 8 threads rotate, round and code 16 elements of K each, and 8 of a
-// query workgroup take 4 heads one after the other.
+// 5.0; 179 with code4 for every number); one token 5 us.  That is not its chain of
+// memory accesses (arguments, length, table, page, store): the read has the same and
+// takes 3.2.  Most likely it is the serial work of few lanes: 8 threads rotate, round
+// and code 16 elements of K each, and 8 of a query workgroup take 4 heads one after
+// the other.
 // --------------------------------------------------------------------------
 constexpr int kHeadsQ = 4;
 
