@@ -435,8 +435,9 @@ __device__ __forceinline__ void load_nodes(const shard_verify_args& a, Nodes& no
 }
 
 // A row's children in their order, until one is accepted: its row, or -1.  Leaves
-// the rejected ones in sh.  A whole wave.  Q: kSum where another child comes after
-// rejections of which only `known` have their sums in sh.amount.
+// the rejected ones in sh, stored by every lane: what a lane reads of them follows its
+// own store.  A whole wave.  Q: kSum where another child comes after rejections of
+// which only `known` have their sums in sh.amount.
 constexpr int kSum = -2;
 template <class T, bool Q>
 __device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nodes, Shared& sh, int c0, int n, int cur, const Joined& j,
@@ -474,7 +475,7 @@ __device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nod
         if (u * (double)nodes.q[c] < s) {
           chosen = c;
         } else {
-          if (lane == 0) sh.rejected[rejected] = c;
+          sh.rejected[rejected] = c;
           ++rejected;
         }
       } else {
@@ -485,10 +486,8 @@ __device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nod
           if (u * sum < mine) {
             chosen = c;
           } else {
-            if (lane == 0) {
-              sh.rejected[rejected] = token;
-              sh.amount[rejected] = mine;
-            }
+            sh.rejected[rejected] = token;
+            sh.amount[rejected] = mine;
             ++rejected;
             sum -= mine;
           }
