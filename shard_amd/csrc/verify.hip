@@ -271,7 +271,7 @@ struct Nodes {
 
 struct Shared {
   int32_t rejected[SHARD_TREE_ROWS];                     // rows (Q) or tokens, in their order
-  double amount[SHARD_TREE_ROWS];                        // Q: what they left; weights of the tokens
+  double amount[SHARD_TREE_ROWS];                        // Q: what they left
   double scan[kWalk / 64];
   State end;
   int count, pick_part, found, last;
@@ -291,9 +291,9 @@ struct Weights {
   const Scale scale;
   const double each;
   int n;          // rejected rows that count
-  __device__ __forceinline__ Weights(const shard_verify_args& a, const Shared& sh, int64_t row0, int64_t row, double rate, int n)
-      : a(a), r((const T*)a.logits + row * a.row_stride, a.vocab), sh(sh), row0(row0), scale(sh.end.most, rate),
-        each(1.0 / sh.end.total), n(n) {}
+  __device__ __forceinline__ Weights(const shard_verify_args& a, const Shared& sh, int64_t row0, int64_t row, float most, double total,
+                                     double rate, int n)
+      : a(a), r((const T*)a.logits + row * a.row_stride, a.vocab), sh(sh), row0(row0), scale(most, rate), each(1.0 / total), n(n) {}
   struct Raw {
     float x[4], q[4];   // q: of the first rejected row
     int64_t e;          // the first element's index; all four lie in the row
@@ -365,6 +365,11 @@ struct Weights {
     for (int u = 0; u < U; ++u) sum += (v[u][0] + v[u][1]) + (v[u][2] + v[u][3]);
     return sum;
   }
+  // a part's quads
+  __device__ __forceinline__ int64_t begin(const VerifyWork& w, int64_t part) const { return part * w.granules * (Row<T>::VEC / 4); }
+  __device__ __forceinline__ int64_t end(const VerifyWork& w, int64_t part) const {
+    return min((part + 1) * w.granules, r.count) * (Row<T>::VEC / 4);
+  }
   // of quads i0 + `at`, i0 + at + stride, ..., U of them on their way together
   template <int U>
   __device__ __forceinline__ double sum(int64_t i0, int64_t i1, int at, int stride) const {
@@ -434,19 +439,26 @@ __device__ __forceinline__ void load_nodes(const shard_verify_args& a, Nodes& no
   }
 }
 
+// A part's rejected weights are subtracted from its sum, which is off by some 2^-48 of
+// what it was: that may be all that is left of it, and a part that holds nothing must not
+// have the answer.  One of which less than this is left is summed again without them.
+constexpr double kVague = 0x1p-24;
+
 // A row's children in their order, until one is accepted: its row, or -1.  Leaves
 // the rejected ones in sh, stored by every lane: what a lane reads of them follows its
 // own store.  A whole wave.  Q: kSum where another child comes after rejections of
-// which only `known` have their sums in sh.amount.
+// which only `known` have their sums in sh.amount.  Otherwise j.mine is what the
+// rejections leave of the lane's part.
 constexpr int kSum = -2;
 template <class T, bool Q>
-__device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nodes, Shared& sh, int c0, int n, int cur, const Joined& j,
-                                    double rate, int& rejected, int known = 0) {
+__device__ __forceinline__ int turn(const shard_verify_args& a, const VerifyWork& w, const Nodes& nodes, Shared& sh, int c0, int n, int cur,
+                                    Joined& j, double rate, int& rejected, int known = 0) {
   const int lane = threadIdx.x & 63;
   rejected = 0;
   const Scale scale(j.most, rate);
-  double sum = j.sum;
+  double sum = j.sum, was = j.mine;                     // was: the lane's part when it was last summed
   int chosen = -1;
+  Weights<T, false> weights(a, sh, c0, c0 + cur, j.most, 1.0, rate, 0);
   for (int base = (cur + 1) & ~63; base < n && chosen < 0; base += 64) {
     const int i = base + lane;
     const bool child = i < n && nodes.up[i] == cur;
@@ -454,6 +466,7 @@ __device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nod
     const int token_i = child ? nodes.token[i] : -1;
     const float u_i = child ? nodes.u[i] : 0.f;
     const double e = token_i >= 0 ? scale(nodes.logit[i]) : 0.0;
+    const int part_i = (int)((uint32_t)(max(token_i, 0) + weights.r.mis) / Row<T>::VEC / (uint32_t)w.granules);
     while (todo && chosen < 0) {
       const int bit = __builtin_ctzll(todo), c = base + bit;
       todo &= todo - 1;
@@ -487,9 +500,15 @@ __device__ __forceinline__ int turn(const shard_verify_args& a, const Nodes& nod
             chosen = c;
           } else {
             sh.rejected[rejected] = token;
-            sh.amount[rejected] = mine;
             ++rejected;
             sum -= mine;
+            const int part = __builtin_amdgcn_readlane(part_i, bit);
+            if (lane == part) j.mine -= mine;
+            if (mine > 0.0 && lane_value(j.mine, part) < kVague * lane_value(was, part)) {
+              weights.n = rejected;
+              const double left = wave_sum(weights.template sum<4>(weights.begin(w, part), weights.end(w, part), lane, 64));
+              if (lane == part) j.mine = was = left;
+            }
           }
         }
       }
@@ -563,7 +582,7 @@ __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyW
         if (known == 0) j = join((held ? held_stats : stats) + cur * w.parts, w.parts, rate, lane);
         rejected = 0;
         none = !has_answer(j.most, rate);
-        const int chosen = none || count > a.max_depth ? -1 : turn<T, Q>(a, nodes, sh, c0, n, cur, j, rate, rejected, known);
+        const int chosen = none || count > a.max_depth ? -1 : turn<T, Q>(a, w, nodes, sh, c0, n, cur, j, rate, rejected, known);
         on = chosen >= 0;
         wants = chosen == kSum;
         if (on) {
@@ -583,7 +602,7 @@ __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyW
       if (wants && !last) return j.mine;                // k_verify_rest sums it
       if (wants) {                                      // what the last rejection left, and the turn once more
         known = sh.end.rejected;
-        const Weights<T, Q> weights(a, sh, c0, sh.end.row, rate, known);
+        const Weights<T, Q> weights(a, sh, c0, sh.end.row, sh.end.most, sh.end.total, rate, known);
         const double all = sum_of(weights, 0, weights.r.count * (Row<T>::VEC / 4), sh);
         if (tid == 0) sh.amount[known - 1] = all;
         __syncthreads();
@@ -595,24 +614,18 @@ __device__ __forceinline__ double walk(const shard_verify_args& a, const VerifyW
 }
 
 // The answer of a walk that has ended at sh.end: the part that it lies in from the
-// parts' sums, `part` in wave 0's lanes, then the token.
+// parts' sums of s, `part` in wave 0's lanes, then the token.
 template <class T, bool Q>
 __device__ __forceinline__ void answer(const shard_verify_args& a, const VerifyWork& w, Shared& sh, int b, int64_t c0, double rate,
                                        double part) {
-  constexpr int kQuads = Row<T>::VEC / 4;   // of a granule
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const State end = sh.end;
   if (end.row < 0 || rate == 0.0) {
     if (tid == 0) a.next[b] = end.row < 0 ? -1 : end.at;
     return;
   }
-  Weights<T, Q> weights(a, sh, c0, end.row, rate, end.rejected);
+  Weights<T, Q> weights(a, sh, c0, end.row, end.most, end.total, rate, end.rejected);
   if (wave == 0) {
-    if constexpr (!Q) {
-      for (int k = 0; k < end.rejected; ++k)
-        if ((sh.rejected[k] + weights.r.mis) / Row<T>::VEC / w.granules == lane) part -= sh.amount[k];
-      part = part > 0.0 ? part : 0.0;
-    }
     const double x = wave_scan(part);
     const double target = (double)sh.u * lane_value(x, 63);
     const uint64_t over = __builtin_amdgcn_ballot_w64(x > target), some = __builtin_amdgcn_ballot_w64(part > 0.0);
@@ -626,7 +639,7 @@ __device__ __forceinline__ void answer(const shard_verify_args& a, const VerifyW
     }
   }
   __syncthreads();
-  int64_t i0 = sh.pick_part * w.granules * kQuads, i1 = min((sh.pick_part + 1) * w.granules, weights.r.count) * kQuads;
+  int64_t i0 = weights.begin(w, sh.pick_part), i1 = weights.end(w, sh.pick_part);
   double target = sh.target;
   if (sh.pick_part < 0) {           // nothing is left of s
     if (!Q || weights.n == 0) {     // of numbers that are not below 1
@@ -637,7 +650,7 @@ __device__ __forceinline__ void answer(const shard_verify_args& a, const VerifyW
     do --weights.n;
     while (weights.n && !(sh.amount[weights.n - 1] > 0.0));
     i0 = 0;
-    i1 = weights.r.count * kQuads;
+    i1 = weights.r.count * (Row<T>::VEC / 4);
     target = (double)sh.u * sum_of(weights, i0, i1, sh);
   }
   double base = 0.0;
@@ -692,9 +705,9 @@ void k_verify_level(const shard_verify_args a, const VerifyWork w, int level) {
       load_nodes<T>(a, nodes, rows, tid, kThreads);
       __syncthreads();
       if (wave == 0) {
-        const Joined j = join(stats, w.parts, rate, lane);
+        Joined j = join(stats, w.parts, rate, lane);
         int rejected, chosen = -1;
-        if (has_answer(j.most, rate)) chosen = turn<T, false>(a, nodes, sh, rows.first, rows.n, s.row, j, rate, rejected);
+        if (has_answer(j.most, rate)) chosen = turn<T, false>(a, w, nodes, sh, rows.first, rows.n, s.row, j, rate, rejected);
         if (lane == 0) sh.found = chosen;
       }
       __syncthreads();
@@ -733,7 +746,7 @@ void k_verify_end(const shard_verify_args a, const VerifyWork w, int levels) {
   if (wave == 0 && rows.n) {
     j = join(w.stats + ((int64_t)(of & 1) * a.batch + b) * w.parts, w.parts, rate, lane);
     none = !has_answer(j.most, rate);
-    if (!none && s.count <= a.max_depth) turn<T, false>(a, nodes, sh, rows.first, rows.n, s.row, j, rate, rejected);
+    if (!none && s.count <= a.max_depth) turn<T, false>(a, w, nodes, sh, rows.first, rows.n, s.row, j, rate, rejected);
   }
   ended(a, nodes, sh, b, rows, j, none, s.row, s.count, rejected);
   const int c0 = rows.first;
@@ -798,10 +811,8 @@ void k_verify_rest(const shard_verify_args a, const VerifyWork w, int round) {
   const double rate = rate_of(a, b);
   end_of(a, w, sh, b, c0);
   if (sh.end.round != round || sh.end.row < 0 || rate == 0.0 || part >= w.parts) return;
-  const Weights<T, true> weights(a, sh, c0, sh.end.row, rate, sh.end.rejected);
-  constexpr int kQuads = Row<T>::VEC / 4;
-  const int64_t i1 = min((part + 1) * w.granules, weights.r.count) * kQuads;
-  double own = weights.template sum<4>(part * w.granules * kQuads, i1, lane, 64);
+  const Weights<T, true> weights(a, sh, c0, sh.end.row, sh.end.most, sh.end.total, rate, sh.end.rejected);
+  double own = weights.template sum<4>(weights.begin(w, part), weights.end(w, part), lane, 64);
   own = wave_sum(own);
   if (lane == 0) w.rest[(int64_t)b * w.parts + part] = own;
 }

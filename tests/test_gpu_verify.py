@@ -366,3 +366,58 @@ def test_operands_within_larger_ones(cuda, probs):
                             cu_seqlens=within(c.cu, torch.int32), draft_probs=within(c.probs) if probs else None,
                             temperature=within([0.7, 1.3], torch.float32), max_new=9)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _plan_is_by_levels(rows, batch, V, type, width, max_depth):
+    """Whether a call of these sizes goes a launch a level: its workspace holds two levels of every sequence then,
+    instead of every row's parts (16 bytes each)."""
+    import ctypes
+    from shard_amd import _lib
+    code, vec = {"fp16": (0, 8), "bf16": (1, 8), "fp32": (2, 4)}[type]
+    args = _lib.VerifyArgs(batch=batch, n_tokens=rows, vocab=V, dtype=code, width=width, max_depth=max_depth)
+    need = _lib.load().shard_verify_drafts_workspace(ctypes.byref(args))
+    granules = (V + 2 * vec - 2) // vec
+    parts = -(-granules // max(-(-granules // 64), 128))
+    assert need in (rows * parts * 16, 2 * batch * (parts * 16 + 12))
+    return need == 2 * batch * (parts * 16 + 12)
+
+
+def _siblings(levels, kept, tokens, u, after, V=10007):
+    """Sequences whose first row has logits at kept[b] ({token: logit}, -inf elsewhere) and children tokens[b] with
+    random numbers u[b], the answer's after[b]; by levels there are many more rows, which no walk reaches."""
+    B, n = len(kept), 40 if levels else 1 + max(map(len, tokens))
+    logits = torch.full((B, n, V), -torch.inf)
+    ids, uniforms, parents = torch.zeros(B, n, dtype=torch.int64), torch.zeros(B, n, 2), []
+    for b in range(B):
+        for t, x in kept[b].items():
+            logits[b, 0, t] = x
+        m = len(tokens[b])
+        ids[b, 1:1 + m], uniforms[b, 1:1 + m, 0], uniforms[b, 0, 1] = torch.tensor(tokens[b]), torch.tensor(u[b]), after[b]
+        parents += [-1] + [0] * m + [1] * (n - 1 - m)
+    assert _plan_is_by_levels(B * n, B, V, "fp32", n, 1) == levels
+    from shard_amd import ops
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    path, counts, following = ops.verify_drafts(logits.view(B * n, V).cuda(), ids.flatten().cuda(), i32(parents), uniforms.view(-1, 2).cuda(),
+                                                cu_seqlens=i32(list(range(0, B * n + 1, n))), max_new=n, max_depth=1)
+    return [path[b, :c].tolist() for b, c in enumerate(counts.tolist())], following.tolist()
+
+
+@pytest.mark.parametrize("levels", [False, True], ids=["rows", "levels"])
+def test_first_token_with_weight(cuda, levels):
+    """A random number of 0 gives the first token that has any weight: none of a part whose tokens were all rejected
+    (the rest masked, or too far below to have a weight), and a tiny one beside them where there is one."""
+    g = torch.Generator().manual_seed(31)
+    kept, tokens, u, want = [], [], [], []
+    for b in range(24):
+        x = (torch.randn(2, generator=g) * 2).tolist()
+        kept.append({100: x[0], 611: x[1], 9000: max(x) + 4.0, 9001: 0.0})
+        want.append(9000)
+        if b % 3 == 1:
+            kept[-1].update({7: -2000.0, 900: -1e30})              # exp(-2000) is 0 in 64 bits
+        elif b % 3 == 2:
+            kept[-1][300] = x[0] - 60.0
+            want[-1] = 300
+        tokens.append([100, 611])
+        u.append([0.999, 0.999])
+    paths, following = _siblings(levels, kept, tokens, u, [0.0] * 24)
+    assert paths == [[0]] * 24 and following == want
