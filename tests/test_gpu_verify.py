@@ -421,3 +421,34 @@ def test_first_token_with_weight(cuda, levels):
         u.append([0.999, 0.999])
     paths, following = _siblings(levels, kept, tokens, u, [0.0] * 24)
     assert paths == [[0]] * 24 and following == want
+
+
+@pytest.mark.parametrize("levels", [False, True], ids=["rows", "levels"])
+def test_what_rejections_leave(cuda, levels):
+    """After two rejected tokens of weights 1 and 2^-22 the third child, and the answer, are decided among weights of
+    2^-45, within a millionth of each border: a sum that is what subtraction leaves of the first one knows none of that."""
+    g = torch.Generator().manual_seed(32)
+    kept, tokens, u, after, paths, answers = [], [], [], [], [], []
+    for b in range(24):
+        # the small ones beside the large ones, and in parts of their own
+        ids = [40, 900, *torch.randperm(30 if b % 2 else 10007, generator=g)[:4].add(50).remainder(10007).tolist()]
+        ids[2:] = [t + 5000 if t in (40, 900) else t for t in ids[2:]]
+        x = [0.0, -22 * np.log(2.0), *(-45 * np.log(2.0) + torch.rand(4, generator=g).double().numpy())]
+        x = [float(np.float32(v)) for v in x]
+        w = np.exp(np.array(x))
+        left = w[2:].sum()                                        # after the first two; child 3 is ids[2]
+        accepted = b % 4 < 2
+        third = w[2] / left * (1 + (-1e-6 if accepted else 1e-6))
+        assert (1 - 2.0 ** -24) * w.sum() > w[0] and (1 - 2.0 ** -24) * w[1:].sum() > w[1]
+        kept.append(dict(zip(ids, x)))
+        tokens.append(ids[:3])
+        u.append([1 - 2.0 ** -24, 1 - 2.0 ** -24, third])
+        order = sorted(range(3, 6), key=lambda k: ids[k])         # where it is rejected: one of the other three
+        ends = np.cumsum([w[k] for k in order]) / w[3:].sum()
+        k = b // 4 % 2
+        above = b // 8 % 2
+        after.append(ends[k] * (1 + (1e-6 if above else -1e-6)))
+        paths.append([0, 3] if accepted else [0])
+        answers.append(-1 if accepted else ids[order[k + above]])
+    got, following = _siblings(levels, kept, tokens, u, after)
+    assert got == paths and following == answers
