@@ -298,9 +298,9 @@ void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions)
     typedef T vec8 __attribute__((ext_vector_type(8)));
     vec8 kx{}, ky{}, vx[VU];
     // a thread's words of V codes: 8 tokens of channels vc, vc + 1
-    const int kq = tid / (D / 2), vc2 = tid % (D / 2) * 2;
+    const int kq = tid / (D / 2) & 3, vc2 = tid % (D / 2) * 2;
     const uint32_t keep = ~nibbles((fresh >> (4 * kq) & 15u) | (fresh >> (16 + 4 * kq) & 15u) << 4);
-    const bool words = kq < 4 && keep != ~0u;
+    const bool words = tid < 2 * D && keep != ~0u;    // D = 64: half of the threads
     uint32_t old[2] = {};
     if (there) {
       const T* k = (const T*)a.k + (int64_t)(s.row0 + i) * a.k_stride + (int64_t)g * a.k_head_stride + ch;
