@@ -776,15 +776,16 @@ void k_verify_walk(const shard_verify_args a, const VerifyWork w, int round, boo
     }
     walk<T, Q>(a, w, nodes, sh, stats, b, rate, round ? &from : nullptr, last);
     __syncthreads();
-    const State end = sh.end;
+    const int rejected = sh.end.rejected;
     if (tid == 0) {
-      sh.end.count = sh.end.wants ? end.count : sh.count;
-      sh.end.round = round;
-      w.state[b] = sh.end;
+      State end = sh.end;
+      if (!end.wants) end.count = sh.count;
+      end.round = round;
+      w.state[b] = end;
     }
-    for (int k = tid; k < end.rejected; k += kWalk) {
+    for (int k = tid; k < rejected; k += kWalk) {
       w.rejected[c0 + k] = sh.rejected[k];
-      w.left[c0 + k] = k < end.rejected - 1 ? sh.amount[k] : 0.0;
+      w.left[c0 + k] = k < rejected - 1 ? sh.amount[k] : 0.0;
     }
   } else {
     const double mine = walk<T, Q>(a, w, nodes, sh, stats, b, rate, nullptr, true);
