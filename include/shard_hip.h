@@ -655,7 +655,8 @@ int shard_kv4_keep(const shard_kv4_args* args, int32_t n_layers, int64_t layer_s
  *
  * A sequence's rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (null: row b alone),
  * parents as in shard_draft_tree; width, up to SHARD_TREE_ROWS, bounds the rows
- * of a sequence that are looked at.  A child whose token is not of the vocabulary
+ * of a sequence that are looked at.  Sequences that share rows: with draft_probs any
+ * path and token may be theirs.  A child whose token is not of the vocabulary
  * is passed over.  A row of NaN, +inf (temperature above 0) or without a logit
  * above -inf has no answer: the walk ends there, next -1.  A sequence without rows:
  * count 0, next -1.  A child tried after a rejected one with draft_probs takes a

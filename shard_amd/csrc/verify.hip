@@ -793,16 +793,17 @@ void k_verify_walk(const shard_verify_args a, const VerifyWork w, int round, boo
   }
 }
 
-// With draft_probs: a walk's end from its state.
-__device__ __forceinline__ void end_of(const shard_verify_args& a, const VerifyWork& w, Shared& sh, int b, int c0) {
-  const int tid = threadIdx.x;
+// With draft_probs: a walk's end from its state.  Sequences that share rows (offsets that
+// do not ascend) write over each other's rejected rows: none of them leaves the sequence.
+__device__ __forceinline__ void end_of(const shard_verify_args& a, const VerifyWork& w, Shared& sh, int b, const Rows& rows) {
+  const int tid = threadIdx.x, c0 = rows.first;
   const State end = w.state[b];
   if (tid == 0) {
     sh.end = end;
     sh.u = end.row >= 0 ? a.uniforms[2 * (int64_t)end.row + 1] : 0.f;
   }
   for (int k = tid; k < end.rejected; k += blockDim.x) {
-    sh.rejected[k] = w.rejected[c0 + k];
+    sh.rejected[k] = min(w.rejected[c0 + k], rows.n - 1);
     sh.amount[k] = w.left[c0 + k];
   }
   __syncthreads();
@@ -813,9 +814,11 @@ __global__ __launch_bounds__(kThreads)
 void k_verify_rest(const shard_verify_args a, const VerifyWork w, int round) {
   __shared__ Shared sh;
   const int part = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int b = blockIdx.y, c0 = rows_of(a, b).first;
+  const int b = blockIdx.y;
+  const Rows rows = rows_of(a, b);
+  const int c0 = rows.first;
   const double rate = rate_of(a, b);
-  end_of(a, w, sh, b, c0);
+  end_of(a, w, sh, b, rows);
   if (sh.end.round != round || sh.end.row < 0 || rate == 0.0 || part >= w.parts) return;
   const Weights<T, true> weights(a, sh, c0, sh.end.row, sh.end.most, sh.end.total, rate, sh.end.rejected);
   double own = weights.template sum<4>(weights.begin(w, part), weights.end(w, part), lane, 64);
@@ -827,11 +830,12 @@ template <class T>
 __global__ __launch_bounds__(kWalk)
 void k_verify_answer(const shard_verify_args a, const VerifyWork w) {
   __shared__ Shared sh;
-  const int b = blockIdx.x, c0 = rows_of(a, b).first;
+  const int b = blockIdx.x;
+  const Rows rows = rows_of(a, b);
   const double part = threadIdx.x < w.parts ? w.rest[(int64_t)b * w.parts + threadIdx.x] : 0.0;
   const double rate = rate_of(a, b);
-  end_of(a, w, sh, b, c0);
-  answer<T, true>(a, w, sh, b, c0, rate, part);
+  end_of(a, w, sh, b, rows);
+  answer<T, true>(a, w, sh, b, rows.first, rate, part);
 }
 
 // --------------------------------------------------------------------------

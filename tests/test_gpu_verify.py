@@ -452,3 +452,22 @@ def test_what_rejections_leave(cuda, levels):
         answers.append(-1 if accepted else ids[order[k + above]])
     got, following = _siblings(levels, kept, tokens, u, after)
     assert got == paths and following == answers
+
+
+def test_offsets_that_do_not_ascend(cuda):
+    """Sequences that share rows, with draft_probs: whatever is theirs, their answers are rows and tokens, and the other
+    sequences' are right.  600 rejected rows of the first lie where the third keeps its own."""
+    c = Case([600, 100], 200, "fp32", True, seed=41)
+    c.parents = [-1] + [0] * 599 + random_parents([100], 3)
+    c.uniforms[:, 0] = 1 - 2.0 ** -24
+    c.uniforms[640:, 0] *= 0.3
+    c.parents[640:] = random_parents([60], 4)
+    path, counts, following = c.run(cu_seqlens=torch.tensor([0, 600, 590, 640, 700], dtype=torch.int32, device=cuda), max_new=600)
+    n, path = counts.tolist(), path.tolist()
+    assert n[1] == 0 and int(following[1]) == -1
+    for b, rows in ((0, 600), (2, 50)):
+        assert 1 <= n[b] <= rows and all(0 <= r < rows for r in path[b][:n[b]]) and -1 <= int(following[b]) < 200
+    want, margin = plain.verify(c.logits[640:].numpy(), c.tokens[640:].tolist(), c.parents[640:], c.uniforms[640:].numpy(), [0, 60],
+                                c.probs[640:].numpy(), [1.0])
+    assert margin > 200 * 2.0 ** -48
+    assert (path[3][:n[3]], int(following[3])) == want[0]
