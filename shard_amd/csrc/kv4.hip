@@ -1688,7 +1688,7 @@ int shard_kv4_append_at(const shard_kv4_args* a, const int32_t* positions, void*
   const dim3 grid(groups_of(a), a->n_kv_heads + q_groups, a->batch);
   if (positions) KV4_DISPATCH_N(k_kv4_append, true, grid, (hipStream_t)stream, *a, positions);
   else KV4_DISPATCH_N(k_kv4_append, false, grid, (hipStream_t)stream, *a, positions);
-  SHARD_LAUNCH_CHECK("shard_kv4_append");
+  SHARD_LAUNCH_CHECK(positions ? "shard_kv4_append_at" : "shard_kv4_append");
   return SHARD_OK;
 }
 
@@ -1741,7 +1741,7 @@ static int launch_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t wo
     const size_t need = attn_workspace(a, mask != nullptr);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) {
       char text[96];
-      snprintf(text, sizeof(text), "shard_kv4_attn needs %zu bytes of workspace, 16-byte aligned", need);
+      snprintf(text, sizeof(text), "shard_kv4_%sattn needs %zu bytes of workspace, 16-byte aligned", mask ? "tree_" : "", need);
       set_last_text(text);
       return SHARD_ERR_WORKSPACE;
     }
@@ -1765,12 +1765,12 @@ static int launch_attn(const shard_kv4_args* a, const uint64_t* mask, int32_t wo
     else if (p.rows == 32) KV4_DISPATCH_NM(k_kv4_attn_rows, 32, false, rows_grid, s, *a, w);
     else KV4_DISPATCH_N(k_kv4_attn_tile, false, tile_grid, s, *a, w);
   }
-  SHARD_LAUNCH_CHECK("shard_kv4_attn");
+  SHARD_LAUNCH_CHECK(mask ? "shard_kv4_tree_attn" : "shard_kv4_attn");
   if (p.n_splits > 1) {
     // up to 8 splits of a row are one load's; more, and few rows, spread over waves
     if (p.n_splits > 8) KV4_DISPATCH_N(k_kv4_merge, 4, dim3((unsigned)rows), s, *a, w);
     else KV4_DISPATCH_N(k_kv4_merge, 1, dim3((unsigned)((rows + 3) / 4)), s, *a, w);
-    SHARD_LAUNCH_CHECK("shard_kv4_attn merge");
+    SHARD_LAUNCH_CHECK(mask ? "shard_kv4_tree_attn merge" : "shard_kv4_attn merge");
   }
   return SHARD_OK;
 }

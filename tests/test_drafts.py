@@ -240,3 +240,12 @@ def test_a_verification_that_fails_undoes_the_step(paged, monkeypatch):
                 paged.speculate(Model(), [a], [[5, 6, 1]], [[-1, 0, 1]], temperature=0.5)
         assert paged.length(a) == 2 and paged.free_pages() == 7 and not paged._drafted()
     assert paged.begin([a], [1]).tolist() == [[2]]
+
+
+def test_errors_name_their_entry_point():
+    from shard_amd import _lib
+    lib = _lib.load()
+    wide = _args(table_width=512, table_stride=512)
+    for call, need, name in ((lambda a: lib.shard_kv4_tree_attn(a, P, 1, None, 0, None), lib.shard_kv4_tree_attn_workspace(wide), b"shard_kv4_tree_attn"),
+                             (lambda a: lib.shard_kv4_attn(a, None, 0, None), lib.shard_kv4_attn_workspace(wide), b"shard_kv4_attn")):
+        assert call(wide) == -4 and lib.shard_last_error().startswith(name + b" needs %d bytes" % need)
