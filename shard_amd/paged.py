@@ -200,7 +200,7 @@ class PagedCache(HFCache):
             self._pages[s], self._lens[s] = p, t
         self._step = dict(table=table, lens=lens, cu=None if max(new) == min(new) == 1 else cu_dev, rows=cu[-1],
                           max_new=max(new), max_len=max(total), undo=list(zip(seqs, new, want)),
-                          left=set(range(len(self.layers))), tree=tree, depth=depth)
+                          left=set(range(len(self.layers))), tree=tree, depth=depth, parents=trees)
         return pos
 
     def cancel(self):
@@ -214,13 +214,18 @@ class PagedCache(HFCache):
         """Settle a step of trees: of each of its sequences, in the step's order, the
         rows path[i, :counts[i]] stay (path (B, P) and counts (B,) int32 on the
         device, of ops.verify_drafts), moved to where the sequence goes on; its other
-        rows leave the cache.  Returns the counts as a list."""
+        rows leave the cache.  They are row 0 and then a child of the row before each;
+        ValueError where they are not, and nothing changes.  Returns the counts as a
+        list."""
         step = self._drafted()
         if step is None or self._open():
             raise ValueError("no drafted tokens to accept: a step of trees that every layer has stored comes first")
         n = counts.tolist()
         if len(n) != len(step["undo"]) or any(not 0 <= c <= min(new, path.shape[1]) for c, (_, new, _) in zip(n, step["undo"])):
             raise ValueError("counts: expected one for each sequence of the step, at most its rows and the path's length")
+        for c, rows, up in zip(n, path.tolist(), step["parents"]):
+            if any(not 0 <= r < len(up) or up[r] != at for r, at in zip(rows[:c], [-1] + rows)):
+                raise ValueError(f"path: {rows[:c]} are not row 0 and a child of the row before each")
         ops.kv4_keep(self.pool, step["table"], step["lens"], path, counts, cu_seqlens=step["cu"])
         step["tree"] = None
         for c, (seq, new, _) in zip(n, step["undo"]):

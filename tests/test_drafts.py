@@ -249,3 +249,18 @@ def test_errors_name_their_entry_point():
     for call, need, name in ((lambda a: lib.shard_kv4_tree_attn(a, P, 1, None, 0, None), lib.shard_kv4_tree_attn_workspace(wide), b"shard_kv4_tree_attn"),
                              (lambda a: lib.shard_kv4_attn(a, None, 0, None), lib.shard_kv4_attn_workspace(wide), b"shard_kv4_attn")):
         assert call(wide) == -4 and lib.shard_last_error().startswith(name + b" needs %d bytes" % need)
+
+
+def test_rows_that_are_no_path_are_refused(paged):
+    """accept() takes a path from row 0 down each row's child: other rows' keys are rotated at other positions, and ones
+    out of order, of another sequence or -1 would leave the cache without the tokens that the lengths count."""
+    a, b = paged.add(), paged.add()
+    paged.begin([a, b], [5, 2], parents=[[-1, 0, 0, 2, 3], [-1, 0]])
+    _store(paged, 7)
+    for path in ([[0, 3, -1], [0, 1, -1]], [[0, 2, 2], [0, 1, -1]], [[2, 3, 4], [0, 1, -1]], [[0, 2, -1], [0, 1, -1]], [[0, 2, 5], [0, 1, -1]],
+                 [[0, 2, 3], [1, 0, -1]], [[0, 2, 3], [0, 2, -1]], [[0, 1, 2], [0, 1, -1]], [[0, -2, -1], [0, 1, -1]]):
+        with pytest.raises(ValueError, match="path"):
+            paged.accept(_i32(*path), _i32(3, 2))
+    assert paged._drafted() and paged.length(a) == 5 and not [c for c in paged.calls if isinstance(c, tuple)]
+    assert paged.accept(_i32([0, 2, 3], [0, -1, 7]), _i32(3, 1)) == [3, 1]
+    assert paged.length(a) == 3 and paged.length(b) == 1
