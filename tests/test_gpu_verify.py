@@ -471,3 +471,83 @@ def test_offsets_that_do_not_ascend(cuda):
                                 c.probs[640:].numpy(), [1.0])
     assert margin > 200 * 2.0 ** -48
     assert (path[3][:n[3]], int(following[3])) == want[0]
+
+
+class ByLevels(Case):
+    """A case whose sizes go a launch a level."""
+
+    def check(self, max_depth):
+        type = {v: k for k, v in TYPES.items()}[self.logits.dtype]
+        assert _plan_is_by_levels(len(self.parents), len(self.new), self.V, type, max(self.new), max_depth)
+        return super().check(max_depth=max_depth)
+
+
+@pytest.mark.parametrize("type", ["fp16", "bf16", "fp32"])
+def test_levels_of_uneven_trees(cuda, type):
+    """By levels: sequences of their own temperatures, greedy ones among them, empty ones, rows of NaN, +inf and nothing,
+    walks that end at every level from the first to the last and at max_depth."""
+    new = [33, 0, 9, 1, 20, 40] * 7
+    temps = [[1.0, 0.5, 0.0, 0.8, 2.0][i % 5] for i in range(len(new))]
+    c = ByLevels(new, 28001, type, temperature=temps, seed=17, close=25.0)
+    first = c.cu
+    c.logits[first[0], 11], c.logits[first[6], 20000], c.logits[first[12]] = torch.nan, torch.inf, -torch.inf
+    lengths = [len(p) for p, _ in c.check(max_depth=5)]
+    c.uniforms[:, 0] = 0.0
+    lengths += [len(p) for p, _ in c.check(max_depth=4)]
+    assert {0, 1, 2, 3, 4, 5} <= set(lengths)
+    chain = ByLevels([10] * 45, 40009, type, temperature=0.7, seed=18, width=1, close=25.0)
+    lengths = {len(p) for p, _ in chain.check(max_depth=4)}
+    chain.uniforms[:, 0] = 0.0
+    lengths |= {len(p) for p, _ in chain.check(max_depth=3)}
+    assert {1, 2, 4} <= lengths
+
+
+def test_levels_to_the_last_row(cuda):
+    """By levels where max_depth is the most that a tree of so many rows can have: the walk ends as no row is left."""
+    c = ByLevels([5] * 90, 70001, "fp16", temperature=0.9, seed=19, width=1, close=30.0)
+    for u in (None, 0.0):
+        if u is not None:
+            c.uniforms[:, 0] = u
+        lengths = [len(p) for p, _ in c.check(max_depth=4)]
+    assert max(lengths) == 5
+
+
+def test_levels_captured(cuda):
+    """By levels in a graph, replayed with other inputs in the same memory and eager work between."""
+    from shard_amd import ops
+    V, new = 40009, [20] * 20
+    B, T = len(new), sum(new)
+    assert _plan_is_by_levels(T, B, V, "bf16", 20, 3)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    cu, g = i32([0] + np.cumsum(new).tolist()), torch.Generator(device="cuda").manual_seed(1)
+
+    def inputs(seed):
+        tokens, parents = torch.randint(0, V, (T,), generator=g, device=cuda), i32(random_parents(new, seed))
+        x = torch.randn(T, V, generator=g, device=cuda) * 2
+        at = (torch.arange(T, device=cuda) // 20 * 20 + parents.clamp(min=0)).long()
+        x.index_put_((at, tokens), torch.rand(T, generator=g, device=cuda) * 20, accumulate=True)
+        return [x.bfloat16(), tokens, parents, torch.rand(T, 2, generator=g, device=cuda), torch.rand(B, generator=g, device=cuda) - 0.2]
+    call = lambda x, tok, up, u, t: ops.verify_drafts(x, tok, up, u, cu_seqlens=cu, temperature=t, max_new=20, max_depth=3)
+    held = inputs(0)
+    call(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call(*held)
+    seen = set()
+    for seed in range(1, 5):
+        new_in = inputs(seed)
+        want = call(*new_in)
+        for dst, src in zip(held, new_in):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        seen |= set(want[1].tolist())
+        temps = new_in[4].tolist()
+        answers, margin = plain.verify(new_in[0].float().cpu().numpy(), new_in[1].tolist(), new_in[2].tolist(), new_in[3].cpu().numpy(),
+                                       cu.tolist(), None, temps, 3, 20)
+        assert margin > V * 2.0 ** -48
+        assert [(p[:n], t) for p, n, t in zip(want[0].tolist(), want[1].tolist(), want[2].tolist())] == answers
+        assert bool(torch.randn(64, device=cuda).isfinite().all())
+    assert {1, 2, 3, 4} <= seen
