@@ -571,3 +571,117 @@ def test_append_at_every_border(cuda, type):
         assert np.array_equal(V, kv4.round4(x.reshape(n, 2, 32)).reshape(n, D))
         want = kv4.round4((x * np.float64(np.float32(cos))).reshape(n, 2, 32)).reshape(n, D)
         assert np.array_equal(K, want), (cos, np.argwhere(K != want)[:4])
+
+
+# ---------------------------------------------------------------------------
+# the plans that large calls get
+# ---------------------------------------------------------------------------
+def _plan(b):
+    """(rows of a tile, row tiles, splits, longest first, tiles of the same pages side by side) of a call with its
+    launch hints, restated; the splits are those that its workspace is for."""
+    import ctypes
+    from shard_amd import _lib
+    B, T, most, length = len(b.total), sum(b.new), max(b.new), max(b.total)
+    args = _lib.KV4Args(batch=B, n_tokens=T, n_q_heads=b.H, n_kv_heads=b.G, head_dim=b.D, dtype=0, n_pages=b.n_pages,
+                        table_width=b.table.shape[1], cache=4096, page_stride=b.G * 68 * b.D, block_table=4096,
+                        table_stride=b.table.shape[1], seq_lens=4096, cu_seqlens=4096, max_new=most, max_len=length)
+    need = _lib.load().shard_kv4_tree_attn_workspace(ctypes.byref(args))
+    splits, left = divmod(need, T * b.H * (b.D + 2) * 4)
+    splits = max(splits, 1)
+    assert left == 0
+    up = lambda n, d: -(-n // d)
+    rows, pages = most * (b.H // b.G), up(length, 64)
+    whole = 400 * up(rows, 128) <= 115 * up(rows, 32) and B * b.G * up(rows, 128) * pages > 6500
+    tile = 16 if rows <= 16 else 128 if whole else 32
+    tiles = up(rows, tile)
+    groups = B * b.G * tiles
+    want = max(up(512, groups), up(pages, 32 if groups * up(pages, 32) <= 1152 else 64))
+    want = min(want, up(pages, 4), 128)
+    assert splits == max(2 ** k for k in range(8) if k == 0 or 2 ** (2 * k - 1) < want * want)
+    return tile, tiles, splits, tile != 128 and B > 1 and groups * splits >= 1024, tiles > 1 and B * b.G * splits % 8 == 0
+
+
+class Large(Trees):
+    """Trees with the reference by matrix products."""
+
+    def reference(self, scale, mask):
+        k, v = kv4.held(self.d_cache.cpu().numpy())
+        T, group = sum(self.new), self.H // self.G
+        want, a, d = np.zeros((T, self.H, self.D)), np.zeros((T, self.H, self.D)), np.zeros((T, self.H))
+        words = mask.cpu().numpy().view(np.uint64)
+        for b, (n, m) in enumerate(zip(self.total, self.new)):
+            r0, t = int(self.cu[b]), np.arange(n)
+            page = self.table[b].numpy()[t // 64]
+            K, V = k[page, t % 64], v[page, t % 64]
+            bits = (words[r0:r0 + m, :, None] >> np.arange(64, dtype=np.uint64) & np.uint64(1)).reshape(m, 64 * words.shape[1]).astype(bool)
+            bits = np.pad(bits, ((0, 0), (0, max(0, m - bits.shape[1]))))[:, :m]
+            seen = np.concatenate([np.ones((m, n - m), bool), bits], 1)
+            seen, some = np.repeat(seen, group, 0), np.repeat(seen.any(1), group)
+            for g in range(self.G):
+                q = self.q[r0:r0 + m, g * group:(g + 1) * group].double().numpy().reshape(m * group, self.D)[some]
+                s = np.where(seen[some], q @ K[:, g].T * scale, -np.inf)
+                w = np.exp(s - s.max(1, keepdims=True, initial=-1e300))
+                w /= w.sum(1, keepdims=True)
+                size = np.where(seen[some], np.abs(q) @ np.abs(K[:, g]).T * abs(scale), 0).max(1, initial=0)
+                for out, x in ((want, w @ V[:, g]), (a, w @ np.abs(V[:, g])), (d[..., None], size[:, None])):
+                    of = np.zeros((m * group, x.shape[1]))
+                    of[some] = x
+                    out[r0:r0 + m, g * group:(g + 1) * group] = of.reshape(m, group, x.shape[1])
+        return want, a, d
+
+    def check(self, out, mask=None):
+        want, a, d = self.reference(self.D ** -0.5, self.mask if mask is None else mask)
+        d, n = d[:, :, None], max(self.total) + 64
+        # as Trees.check
+        weight = 2 * (self.D + 4) * 2.0 ** -24 * d + (2 * self.D * 2.0 ** -26 * d if self.type == torch.bfloat16 else 0)
+        weight = weight + 2.0 ** -11 + n * 2.0 ** -25 + (n + 200) * 2.0 ** -24
+        err = weight * 2 * a
+        tol = err + torch.finfo(self.type).eps / 2 * (np.abs(want) + err) + 2.0 ** -25
+        off = np.abs(out.cpu().double().numpy() - want)
+        assert (off <= tol).all(), (off.max(), (off / tol).max())
+
+    def check_all(self):
+        """Trees; any bits; fewer words than rows, of which most rows see none; the same bits again on another stream."""
+        hints = dict(max_new=max(self.new), max_len=max(self.total))
+        self.plan()
+        out = self.tree_attn(**hints)
+        self.check(out)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = self.tree_attn(**hints)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(again, out)
+        g = torch.Generator().manual_seed(7)
+        any_bits = lambda words: torch.randint(-2 ** 63, 2 ** 63 - 1, (sum(self.new), words), generator=g)
+        for mask in (any_bits(self.mask.shape[1]), any_bits(1) & any_bits(1) & any_bits(1) & any_bits(1) & any_bits(1) & any_bits(1)):
+            mask[::5] = 0
+            mask[1::5, :-1] = 0                                   # of a tree without tokens before it: no key of the first page
+            self.check(self.tree_attn(mask=mask.to("cuda"), **hints), mask=mask)
+
+
+TILES = [  # total, new, H, G, splits
+    ([26100], [256], 8, 2, 32), ([8800, 70, 170, 300], [170, 0, 170, 128], 9, 3, 8),
+    ([900 - 7 * i for i in range(30)] + [128, 60], [128, 128, 77, 0, 1] * 6 + [128, 60], 16, 4, 1),
+]
+
+
+@pytest.mark.parametrize("type,D", [("fp16", 128), ("bf16", 64), ("fp16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("total,new,H,G,splits", TILES, ids=["one", "uneven", "whole"])
+def test_tree_attention_by_tiles_of_128_rows(cuda, total, new, H, G, splits, type, D):
+    b = Large(total, new, H, G, D, type, seed=len(total), wide=2)
+    tile, _, n, *_ = _plan(b)
+    assert (tile, n) == (128, splits)
+    b.fill().check_all()
+
+
+@pytest.mark.parametrize("type,D", [("fp16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("B,longest,most", [(32, 8300, 16), (70, 2000, 13)])
+def test_tree_attention_longest_first_and_side_by_side(cuda, B, longest, most, type, D):
+    rng = random.Random(B)
+    total = [longest] + [min(longest - 1, int(40 * 1.2 ** rng.uniform(0, 20))) for _ in range(B - 1)]
+    new = [most] + [rng.choice([0, 1, 5, most, most]) for _ in range(B - 1)]
+    b = Large(total, new, 32, 8, D, type, seed=B, wide=1)
+    tile, tiles, _, by_length, paired = _plan(b)
+    assert tile == 32 and tiles == 2 and by_length and paired
+    b.fill().check_all()
