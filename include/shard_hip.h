@@ -649,7 +649,8 @@ int shard_kv4_keep(const shard_kv4_args* args, int32_t n_layers, int64_t layer_s
  * children have been.  path[b] (batch, width) are the rows it went through from
  * row 0 on, -1 behind them, counts[b] their number; next[b] is the first token at
  * which the running sum of s exceeds uniforms[row][1] sum(s), row the last one.
- * Weights and sums in 64 bits.  A temperature (temperatures[b], or temperature where
+ * Weights and sums in 64 bits, what rejections leave summed anew where subtraction
+ * would not tell.  A temperature (temperatures[b], or temperature where
  * that is null) of 0 or below: p is 1 at the largest logit, the first of equal ones,
  * and no random number counts.  Numbers are in [0, 1) (others: any token, or -1).
  *
@@ -660,8 +661,9 @@ int shard_kv4_keep(const shard_kv4_args* args, int32_t n_layers, int64_t layer_s
  * is passed over.  A row of NaN, +inf (temperature above 0) or without a logit
  * above -inf has no answer: the walk ends there, next -1.  A sequence without rows:
  * count 0, next -1.  A child tried after a rejected one with draft_probs takes a
- * pass over the row, all but a sequence's first two in one workgroup (128,256
- * tokens: 16 and 19 us, then 70 to 100 each).
+ * pass over the row.  A sequence's first min(2, width - 1 - max_depth) such passes use
+ * the whole chip (128,256 tokens: 16 and 19 us), the others one workgroup (40 to 60
+ * each): tell max_depth where trees are no chains.
  *
  * Workspace: shard_verify_drafts_workspace(args) bytes, 16-byte aligned; nothing in
  * it needs clearing. */

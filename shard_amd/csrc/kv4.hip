@@ -214,9 +214,9 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // tokens 164 us, 4.4 TB/s of the 724 MB it reads and writes (a large copy: 4.75 to
 // 5.0; 179 with code4 for every number); one token 5 us.  That is not its chain of
 // memory accesses (arguments, length, table, page, store): the read has the same and
-// takes 3.2.  Most likely it is the serial work of few lanes: 8 threads rotate, round
-// and code 16 elements of K each, and 8 of a query workgroup take 4 heads one after
-// the other.
+// takes 3.2.  What is left is the serial work of few lanes, not measured apart: 8 threads
+// rotate, round and code 16 elements of K each, and 8 of a query workgroup take 4 heads
+// one after the other.
 // --------------------------------------------------------------------------
 constexpr int kHeadsQ = 4;
 
@@ -224,8 +224,9 @@ constexpr int kHeadsQ = 4;
 // of a tree: siblings have places of their own and one position).  64 trees of 13 to 26
 // tokens in 32 layers, 38,272 rows of 8 heads of 128: 177 us (code4: 217), of 25,600
 // workgroups with 12 rows each; a workgroup waits 3 us for the chain length ->
-// position -> phases and its store.  Not faster: dense rows, K and V apart (226 against 219),
-// more heads a workgroup (253), six waves a SIMD instead of four (spills, 314).
+// position -> phases and its store.  Not faster, all of them with code4 still, whose 71.9
+// million instructions are 43.6 now: dense rows, K and V apart (226 against 219 then), more
+// heads a workgroup (253), six waves a SIMD instead of four (spills, 314).
 template <class T, int D, bool AT>
 __global__ __launch_bounds__(256, 4)
 void k_kv4_append(const shard_kv4_args a, const int32_t* __restrict__ positions) {
@@ -1589,10 +1590,15 @@ AttnPlan plan_of(const shard_kv4_args* a) {
 // workgroups of the same pages side by side (AttnWork::paired).  128-row tiles are
 // worth it where there is work for the whole chip at once and little of them stays
 // empty: 32 / 128 rows, us (32 heads on 8 of 128, one sequence): 61 nodes over 8K
-// 26.5 / 33.2, 128 over 4K 29.9 / 40.4, 256 over 4K 43.4 / 42.6, 256 over 16K 113.1 /
-// 96.5, 8 sequences of 64 over 8K 116.2 / 97.1.  Splits as in plan_of, but 32 pages
-// at most where that makes 1,152 workgroups or fewer: 18 uneven sequences of up to
-// 13,626 tokens 23.1, with 64 36.3; 16 x 16K, 2,048 workgroups, 126.7 and 118.0.
+// 26.5 / 33.2, 128 over 4K 29.9 / 40.4, 256 over 16K 113.1 / 96.5, 8 sequences of 64 over
+// 8K 116.2 / 97.1.  Near the border, in page units of 128 rows and a kv head: at 4,096
+// 128 nodes over 8K 38.8 / 43.8, 256 over 4K 39.1 / 38.6; at 6,144 128 over 12K 51.2 /
+// 48.4, 256 over 6K 52.3 / 45.4, 4 sequences of 64 51 / 45.5 (head_dim 64, 128 and 256
+// nodes: 34.5 / 37.4, 34.4 / 30.5); at 6,320 2 of 200 nodes, 3 heads a kv head, with a
+// tile that is two thirds full 55.5 / 57.2; at 8,192 61 / 54.  So 64 and 256 nodes gain
+// a tenth from 5,000 on already, where the others lose up to 8%.  Splits as in plan_of,
+// but 32 pages at most where that makes 1,152 workgroups or fewer: 18 uneven sequences
+// of up to 13,626 tokens 23.1, with 64 36.3; 16 x 16K, 2,048 workgroups, 126.7 and 118.0.
 AttnPlan tree_plan_of(const shard_kv4_args* a) {
   AttnPlan p;
   const int group = a->n_q_heads / a->n_kv_heads;

@@ -19,8 +19,9 @@
 // Rows are cut into at most 64 parts.
 //   k_verify_stats   a part of a row a wave: its largest logit M and
 //                    sum exp2((x - M) log2(e) / t)
-//   k_verify_walk    a sequence a workgroup: the walk, then the part that the
-//                    answer lies in from the parts' sums, and in it the token
+//   k_verify_walk    a sequence a workgroup: the walk, which takes rejected tokens
+//                    out of the parts' sums (kVague), then the part that the
+//                    answer lies in from those sums, and in it the token
 // With draft_probs s is another function of every token after a rejection: the walk
 // leaves its sum to k_verify_rest, which has the whole chip, and goes on in the next
 // launch; k_verify_answer finds the token.  Many
@@ -164,8 +165,11 @@ __device__ __forceinline__ int sequence_of(const shard_verify_args& a, int r, in
   return max(before - 1, 0);
 }
 
-// A part a wave: no barrier, nothing in LDS.  kTurn granules a turn, all on their way
-// before the first is looked at.
+// A part a wave: no barrier, nothing in LDS.  kTurn granules a turn; one that lies wholly
+// within the part and the row is on its way before the first is looked at.  Any other
+// (every one of half-precision rows below 131,072 logits: a part has 251 granules at 128,256)
+// is loaded granule by granule and filled up with -inf, whose weights take as long as
+// others: 2% more at 128,256, twice as many between 32,000 and 65,536, 1.7 times at 151,936.
 constexpr int kTurn = 256;
 
 template <class T>
@@ -854,8 +858,12 @@ int levels_of(const shard_verify_args* a) {
 
 // With draft_probs: launches of the walk, each with one that sums what rejections
 // have left; a walk that wants more sums than they give takes them in its one
-// workgroup (50 us and more each, the launches 15, 5 where nobody wants them).  A
-// chain, whose depth is its rows, wants none; trees most often up to two.  128,256
+// workgroup (40 to 60 us each, the launches 15, 5 where nobody wants them).  A
+// chain, whose depth is its rows, wants none; trees most often up to two.  Trees whose
+// max_depth is not told pass for chains, and so does a batch with a chain as long as its
+// largest tree: 2 / 3 / 4 children of one row rejected, us, told and not, one sequence
+// 36.8 and 60.4 / 55.7 and 110 / 117 and 172, 16 sequences 51.9 and 81.5 / 77 and 140 /
+// 158 and 214.  128,256
 // tokens, the first of 4 children accepted / all 4 rejected, us: one sequence 23.6 / 154
 // with two launches, 28.5 / 126 with three; 16 sequences 37.1 / 191, 42.2 / 159.
 int rounds_of(const shard_verify_args* a) {
