@@ -28,10 +28,10 @@
 // rows, few of which are on a path, go a launch a level instead (k_verify_level,
 // k_verify_end), and only the rows on the paths are read.
 //
-// Measured, 128,256 logits a row, us: 5 rows of one sequence 4.9 + 5.7 (a chain of
-// loads and reductions), 61 rows 10.6 + 6.9; 192 rows of 32 sequences with draft_probs
-// 25 (vector issue: 20 64-bit instructions a weight) + 9 + 12 + 5; 1,190 rows of 64
-// trees, 7 levels 1.8 to 7 each, the end 7.6.
+// Measured, 128,256 logits a row, us: 5 rows of one sequence 4.9 + 5.8 (a chain of
+// loads and reductions), 61 rows 10.3 + 7.0; 192 rows of 32 sequences with draft_probs
+// 26 (vector issue: 20 64-bit instructions a weight) + 9 + 12 + 5; 1,190 rows of 64
+// trees, 7 levels 1.7 to 7 each, the end 7.7.
 #include <math.h>
 #include <stdio.h>
 
